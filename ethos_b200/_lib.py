@@ -94,6 +94,18 @@ EXPORTS = {
     # save_hacc, save_dot, save_qpre, save_bn, save_qhat, htab, gtab, dx, d_latents, d_w1, d_w2,
     # d_wq, d_bn, d_keys, workspace, workspace_bytes, dev_err, stage_events, stream
     "ethos_layer_backward_f32": (_I, [_DIMS, _I, _F] + [_P] * 26 + [_SZ, _P, _P, _P]),
+    # ids, ids_i64, weight, ldw, dtype, tokens, vocab, dim, scale, out, dev_err, stream
+    "ethos_embedding_forward": (_I, [_P, _I, _P, _I64, _I, _I64, _I64, _I64, _F, _P, _P, _P]),
+    "ethos_embedding_backward_workspace_size": (_SZ, [_I64, _I64, _I64]),
+    # ids, ids_i64, dy, dtype, tokens, vocab, dim, padding, scale, d_weight, workspace,
+    # workspace_bytes, dev_err, stream
+    "ethos_embedding_backward": (_I, [_P, _I, _P, _I, _I64, _I64, _I64, _I64, _F, _P, _P, _SZ, _P, _P]),
+    "ethos_balance_scratch_size": (_SZ, []),
+    # ids, ids_i64, weights, dtype, mask, tokens, heads, k, experts, counts, loss, scratch, dev_err,
+    # stream
+    "ethos_balance_forward": (_I, [_P, _I, _P, _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
+    # ids, ids_i64, dtype, mask, tokens, heads, k, experts, counts, scratch, grad, d_weights, stream
+    "ethos_balance_backward": (_I, [_P, _I, _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     "ethos_test_gemm_withhold": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _P]),
 }
 

@@ -55,7 +55,7 @@ def build(force=False, verbose=False, extra_flags=()):
     tmp = LIB_PATH + ".tmp"
     cmd = [nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "--shared",
            "-Xcompiler", "-fPIC,-O3", "-I", INCLUDE, "-I", CSRC,
-           "--expt-relaxed-constexpr", *extra_flags, "-o", tmp, *srcs]
+           "--expt-relaxed-constexpr", "--threads", "0", *extra_flags, "-o", tmp, *srcs]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

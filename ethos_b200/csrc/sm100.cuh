@@ -19,10 +19,10 @@ namespace ethos {
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s: no legitimate wait comes close
 
-// Per-device wait limit read by mbar_wait once it starts checking the clock
+// Per-device wait limit (one copy per translation unit) read by mbar_wait once it starts checking the clock
 // (ethos_set_wait_limit_ns; a test shortens it to make a withheld stage time
 // out quickly).  Only the slow path of a wait reads it.
-__device__ unsigned long long g_wait_limit_ns = kWaitLimitNs;
+static __device__ unsigned long long g_wait_limit_ns = kWaitLimitNs;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -84,7 +84,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // flag: once any role gives up, every other wait returns false promptly.  A
 // null `abort` makes a drain wait (used on the abort path itself): it only
 // ends on completion or on the time limit.
-__device__ __noinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err,
+static __device__ __noinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err,
                                        int site) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();

@@ -1,0 +1,74 @@
+"""Differentiable training operators around the expert layers, as functions of
+tensors: the decoder's token embedding and the balance of the routing.
+
+All run in ``libethos_b200.so`` on CUDA tensors (there is no CPU path), on the
+current stream, and without a host synchronisation: an id outside its range is
+recorded in the device error word (``ops.check_device_error``).
+"""
+
+import torch
+
+from . import ops
+
+__all__ = ["embedding", "balance_loss"]
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.padding_idx, ctx.vocab, ctx.dtype = scale, padding_idx, weight.shape[0], weight.dtype
+        return ops.embedding_forward(ids, weight, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ids, = ctx.saved_tensors
+        return None, ops.embedding_backward(ids, dy, ctx.vocab, ctx.scale, ctx.padding_idx), None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """``scale * weight[ids]``: rows of the table ``weight [V, d]`` (fp32 or
+    bf16) for token ids of any shape, each value rounded once.
+
+    The gradient with respect to ``weight`` is dense, in its dtype: every
+    token's ``scale * dy`` summed in fp32 in token order (the same bits in
+    every run) and rounded once; rows no token holds are zero.  The row of
+    ``padding_idx`` (None: no such row) gets no gradient; a negative index
+    counts from the end, as in ``torch.nn.Embedding``."""
+    if padding_idx is not None:
+        V = weight.shape[0]
+        if not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx {padding_idx} is not in the table of {V} rows")
+        padding_idx = padding_idx % V
+    return _Embedding.apply(ids, weight, float(scale), padding_idx)
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weights, ids, num_experts, mask):
+        loss, counts, scratch = ops.balance_forward(weights, ids, num_experts, mask)
+        ctx.save_for_backward(ids, mask, counts, scratch)
+        ctx.dtype = weights.dtype
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    def backward(ctx, grad, _):
+        ids, mask, counts, scratch = ctx.saved_tensors
+        return ops.balance_backward(grad, ids, counts, scratch, ctx.dtype, mask), None, None, None
+
+
+def balance_loss(weights, ids, num_experts, mask=None):
+    """Balance loss of the router's choices, and how often each expert was
+    chosen: ``(loss, counts)`` from routing ``weights [T, H, k]`` (fp32 or
+    bf16) and ``ids [T, H, k]`` (int32 or int64).
+
+    With ``c[e]`` the selections of expert e and n tokens::
+
+        loss = N * sum_e (c[e] / (n H k)) * (sum of e's weights / (n H))
+
+    which is 1 when all N experts are chosen evenly and grows as the choices
+    crowd; counts are constants in the gradient.  ``mask`` (bool ``[T]``)
+    leaves tokens out; without any token the loss and the gradient are 0.
+    ``counts`` is int32 ``[N]``."""
+    return _BalanceLoss.apply(weights, ids, int(num_experts), mask)

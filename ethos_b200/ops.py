@@ -14,7 +14,8 @@ from ._lib import EthosDims, EthosError, check, lib
 __all__ = [
     "make_dims", "gemm_bf16", "gemm_ex", "product_key_topk", "expert_forward", "router_forward", "layer_forward",
     "device_error_word", "check_device_error", "PackedWeights", "layer_backward", "layer_forward_f32",
-    "router_forward_f32", "layer_backward_f32",
+    "router_forward_f32", "layer_backward_f32", "embedding_forward", "embedding_backward", "balance_forward",
+    "balance_backward",
 ]
 
 _ERR_WORDS = {}
@@ -526,3 +527,117 @@ def layer_backward_f32(dy, x32, pw, saved, bn_training, eps, stage_events=None):
                                      ws_bytes, _vp(err), _events(stage_events), _stream(dev)),
           "ethos_layer_backward_f32")
     return g
+
+
+# ------------------------------------------- training: the model's ends --
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}  # ETHOS_F32, ETHOS_BF16
+
+
+def _dtype_code(t, name):
+    code = _DTYPE_CODE.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: fp32 or bf16, not {t.dtype}")
+    return code
+
+
+def _ids_i64(t, name):
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: int32 or int64, not {t.dtype}")
+    return 1 if t.dtype == torch.int64 else 0
+
+
+def _same_device(ref, *named):
+    for t, name in named:
+        if t is None:
+            continue
+        _require_cuda(t, name)
+        if t.device != ref.device:
+            raise ValueError(f"{name} is on {t.device}, not on {ref.device}")
+
+
+def embedding_forward(ids, weight, scale=1.0):
+    """``scale * weight[ids]`` (ethos_embedding_forward): ids of any shape,
+    int32 or int64; ``weight`` ``[V, d]`` fp32 or bf16 with unit column stride.
+    An id outside ``[0, V)`` sets the device error word and gives zeros."""
+    _require_cuda(weight, "weight")
+    _same_device(weight, (ids, "ids"))
+    if weight.dim() != 2:
+        raise ValueError("weight: [vocab, dim]")
+    code, i64 = _dtype_code(weight, "weight"), _ids_i64(ids, "ids")
+    V, d = weight.shape
+    if weight.stride(1) != 1 or (V > 1 and weight.stride(0) < d):
+        weight = weight.contiguous()
+    ids = ids.contiguous()
+    out = torch.empty((*ids.shape, d), dtype=weight.dtype, device=weight.device)
+    err = device_error_word(weight.device)
+    check(lib().ethos_embedding_forward(_vp(ids), i64, _vp(weight), max(weight.stride(0), d), code, ids.numel(), V, d,
+                                        float(scale), _vp(out), _vp(err), _stream(weight.device)),
+          "ethos_embedding_forward")
+    return out
+
+
+def embedding_backward(ids, dy, vocab, scale=1.0, padding_idx=None):
+    """Gradient of ``embedding_forward`` with respect to the table
+    (ethos_embedding_backward): dense ``[vocab, d]`` in ``dy``'s dtype, summed
+    in fp32 in token order, the same in every run.  Tokens equal to
+    ``padding_idx`` contribute nothing."""
+    _require_cuda(dy, "dy")
+    _same_device(dy, (ids, "ids"))
+    code, i64 = _dtype_code(dy, "dy"), _ids_i64(ids, "ids")
+    d = dy.shape[-1]
+    if tuple(dy.shape[:-1]) != tuple(ids.shape):
+        raise ValueError(f"dy {tuple(dy.shape)} does not belong to ids {tuple(ids.shape)}")
+    ids, dy = ids.contiguous(), dy.contiguous()
+    L = lib()
+    T = ids.numel()
+    dw = torch.empty((vocab, d), dtype=dy.dtype, device=dy.device)
+    ws_bytes = L.ethos_embedding_backward_workspace_size(T, vocab, d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
+    err = device_error_word(dy.device)
+    check(L.ethos_embedding_backward(_vp(ids), i64, _vp(dy), code, T, vocab, d,
+                                     -1 if padding_idx is None else int(padding_idx), float(scale), _vp(dw), _vp(ws),
+                                     ws_bytes, _vp(err), _stream(dy.device)), "ethos_embedding_backward")
+    return dw
+
+
+def balance_forward(weights, ids, num_experts, mask=None):
+    """Balance loss and per-expert counts (ethos_balance_forward): routing
+    ``weights`` and ``ids`` ``[T, H, k]``, ``mask`` bool ``[T]`` (False: leave
+    the token out).  Returns ``(loss fp32 scalar, counts int32 [N], scratch)``;
+    the scratch goes to ``balance_backward``."""
+    _require_cuda(weights, "weights")
+    _same_device(weights, (ids, "ids"), (mask, "mask"))
+    code, i64 = _dtype_code(weights, "weights"), _ids_i64(ids, "ids")
+    if weights.dim() != 3 or ids.shape != weights.shape:
+        raise ValueError("weights and ids: [tokens, heads, k], of one shape")
+    T, H, k = weights.shape
+    if mask is not None:
+        if mask.dtype != torch.bool or tuple(mask.shape) != (T,):
+            raise ValueError("mask: bool [tokens]")
+        mask = mask.contiguous()
+    weights, ids = weights.contiguous(), ids.contiguous()
+    L = lib()
+    dev = weights.device
+    counts = torch.empty((num_experts,), dtype=torch.int32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    scratch = torch.empty(L.ethos_balance_scratch_size(), dtype=torch.uint8, device=dev)
+    err = device_error_word(dev)
+    check(L.ethos_balance_forward(_vp(ids), i64, _vp(weights), code, _vp(mask), T, H, k, num_experts, _vp(counts),
+                                  _vp(loss), _vp(scratch), _vp(err), _stream(dev)), "ethos_balance_forward")
+    return loss, counts, scratch
+
+
+def balance_backward(grad, ids, counts, scratch, dtype, mask=None):
+    """``grad * dloss/dweights`` of ``balance_forward`` in ``dtype``; ``grad`` is
+    a fp32 device scalar, ``counts`` and ``scratch`` the forward's."""
+    _require_cuda(ids, "ids")
+    T, H, k = ids.shape
+    dev = ids.device
+    dw = torch.empty((T, H, k), dtype=dtype, device=dev)
+    ids = ids.contiguous()
+    mask = mask.contiguous() if mask is not None else None
+    grad = grad.to(torch.float32)
+    check(lib().ethos_balance_backward(_vp(ids), _ids_i64(ids, "ids"), _dtype_code(dw, "weights"), _vp(mask), T, H, k,
+                                       counts.numel(), _vp(counts), _vp(scratch), _vp(grad), _vp(dw), _stream(dev)),
+          "ethos_balance_backward")
+    return dw

@@ -45,7 +45,7 @@ extern "C" {
 #define ETHOS_ERR_NO_DEVICE 7         /* no sm_100 device current             */
 #define ETHOS_ERR_SCRATCH_LIMIT 8     /* request exceeds the static scratch   */
 /* device-side codes (reported through dev_err) */
-#define ETHOS_ERR_ID_OUT_OF_RANGE 16  /* an expert id outside [0, N)          */
+#define ETHOS_ERR_ID_OUT_OF_RANGE 16  /* an expert id, token id or label outside its range */
 #define ETHOS_ERR_TIMEOUT_BASE 1000   /* + site: a bounded wait gave up       */
 
 /* Layer dimensions (names follow the reference config, train.py:33-48). */
@@ -449,6 +449,47 @@ int ethos_adamw_step(const ethos_adam_tensor* tensors, int num_tensors, int64_t 
 size_t ethos_grad_clip_workspace_size(void);
 int ethos_grad_clip_coef(const ethos_adam_tensor* tensors, int num_tensors, float max_norm, void* workspace,
                          size_t workspace_bytes, float* out, int* dev_err, void* stream);
+
+/* ------------------------------------------- training: the model's ends --
+ * Operators of a training step around the expert layers: the token embedding
+ * (model.py:374), the balance of the routing, and the cross entropy of the
+ * output head (model.py:385, train.py:200).  dtype arguments take the codes
+ * below; ids and labels are int32 (ids_i64 = 0) or int64 (1). */
+#define ETHOS_F32 0
+#define ETHOS_BF16 1
+
+/* out[t] = scale * weight[ids[t]], rounded once to dtype.  weight [vocab, dim]
+ * with row pitch ldw (elements), out [tokens, dim].  An id outside [0, vocab)
+ * sets ETHOS_ERR_ID_OUT_OF_RANGE in dev_err and gives a zero row. */
+int ethos_embedding_forward(const void* ids, int ids_i64, const void* weight, int64_t ldw, int dtype, int64_t tokens,
+                            int64_t vocab, int64_t dim, float scale, void* out, int* dev_err, void* stream);
+
+size_t ethos_embedding_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim);
+
+/* d_weight[v] = scale * (sum of dy[t] over the tokens with ids[t] == v), every
+ * row of [vocab, dim] written, fp32 sums in token order (the same result in
+ * every run), rounded once.  Tokens equal to `padding` (-1: none) and ids out
+ * of range contribute nothing.  tokens < 2^30, vocab < 2^30. */
+int ethos_embedding_backward(const void* ids, int ids_i64, const void* dy, int dtype, int64_t tokens, int64_t vocab,
+                             int64_t dim, int64_t padding, float scale, void* d_weight, void* workspace,
+                             size_t workspace_bytes, int* dev_err, void* stream);
+
+/* Balance loss of the router's choices and per-expert counts.  ids and
+ * weights (dtype) [tokens, heads, k]; mask (may be NULL) one byte per token,
+ * 0 = leave the token out.  With c[e] the selections of expert e and n tokens
+ * left: loss = experts * sum_e (c[e] / (n heads k)) * (weights of e / (n
+ * heads)), 1 for an even choice, 0 without tokens.  counts int32 [experts];
+ * scratch (ethos_balance_scratch_size bytes) is kept for the backward. */
+size_t ethos_balance_scratch_size(void);
+int ethos_balance_forward(const void* ids, int ids_i64, const void* weights, int dtype, const uint8_t* mask,
+                          int64_t tokens, int64_t heads, int64_t k, int64_t experts, int32_t* counts, float* loss,
+                          void* scratch, int* dev_err, void* stream);
+
+/* d_weights = grad * dloss/dweights (counts constant), in dtype; grad is a
+ * device fp32 scalar, counts and scratch are the forward's. */
+int ethos_balance_backward(const void* ids, int ids_i64, int dtype, const uint8_t* mask, int64_t tokens,
+                           int64_t heads, int64_t k, int64_t experts, const int32_t* counts, const void* scratch,
+                           const float* grad, void* d_weights, void* stream);
 
 #ifdef __cplusplus
 }
