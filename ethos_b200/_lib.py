@@ -106,6 +106,17 @@ EXPORTS = {
     "ethos_balance_forward": (_I, [_P, _I, _P, _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     # ids, ids_i64, dtype, mask, tokens, heads, k, experts, counts, scratch, grad, d_weights, stream
     "ethos_balance_backward": (_I, [_P, _I, _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
+    "ethos_xent_save_size": (_SZ, [_I64, _I64, _I64, _I]),
+    "ethos_xent_forward_workspace_size": (_SZ, [_I64, _I64, _I64, _I]),
+    # hidden, ldh, weight, ldw, dtype, labels, labels_i64, ignore_index, reduction, tokens, vocab, dim,
+    # loss, save, save_bytes, workspace, workspace_bytes, dev_err, stream
+    "ethos_xent_forward": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _I64, _I, _I64, _I64, _I64, _P, _P, _SZ, _P, _SZ,
+                                _P, _P]),
+    "ethos_xent_backward_workspace_size": (_SZ, [_I64, _I64, _I64, _I]),
+    # hidden, ldh, weight, ldw, dtype, reduction, tokens, vocab, dim, grad, save, save_bytes, d_hidden,
+    # d_weight, workspace, workspace_bytes, dev_err, stream
+    "ethos_xent_backward": (_I, [_P, _I64, _P, _I64, _I, _I, _I64, _I64, _I64, _P, _P, _SZ, _P, _P, _P, _SZ, _P,
+                                 _P]),
     "ethos_test_gemm_withhold": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _P]),
 }
 

@@ -1,5 +1,6 @@
 // C ABI of the training operators around the expert layers (declared in
-// include/ethos_b200.h): token embedding, routing balance loss.
+// include/ethos_b200.h): token embedding, routing balance loss, cross
+// entropy of the output head.
 // Host-side orchestration only, as in capi.cu.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -8,6 +9,7 @@
 #include "host.cuh"
 #include "balance.cuh"
 #include "embed.cuh"
+#include "xent.cuh"
 
 using namespace ethos;
 
@@ -137,6 +139,168 @@ int balance_check(const void* ids, int dtype, int64_t tokens, int64_t heads, int
   return ETHOS_OK;
 }
 
+// ---------------------------------------------------------- cross entropy --
+// Layout of one problem.  The unit counts assume 74 SM pairs (a B200); the
+// kernels are right for any number.
+constexpr int64_t kPairs = 74;
+// one piece's gradient of the logits; at least XE_MIN_PIECE columns
+constexpr int64_t kPieceBytes = int64_t(1) << 30;
+constexpr int64_t kMinPiece = 8192;
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+struct XentPlan {
+  int64_t T, V, d;
+  int planes;
+  bool pack_w;             // the table is read through bf16 planes
+  int64_t ldd;             // columns of a plane
+  int64_t t_pad, v_pad;    // rows of a plane
+  int run, runs;           // STATS: column tiles per unit, units along the vocabulary
+  int64_t piece;           // DLOGITS, GRADS: columns of a piece
+  int slots;               // K slices of dh
+  int64_t dh_ld;
+};
+
+XentPlan xent_plan(int64_t T, int64_t V, int64_t d, int dtype) {
+  XentPlan p;
+  p.T = T;
+  p.V = V;
+  p.d = d;
+  p.planes = dtype == ETHOS_F32 ? 3 : 1;
+  p.pack_w = dtype == ETHOS_F32 || d % 8 != 0;
+  p.ldd = up(d, 8);
+  p.t_pad = up(T, XE_TILE);
+  p.v_pad = up(V, XE_TILE);
+  const int64_t num_m = p.t_pad / XE_TILE, num_n = p.v_pad / XE_TILE;
+  int64_t run = num_m * num_n / (kPairs * 6);
+  p.run = static_cast<int>(run < 1 ? 1 : (run > 16 ? 16 : run));
+  p.runs = static_cast<int>((num_n + p.run - 1) / p.run);
+  int64_t most = kPieceBytes / (p.t_pad * 2 * p.planes) / XE_TILE * XE_TILE;
+  if (most < kMinPiece) most = kMinPiece;
+  const int64_t pieces = (V + most - 1) / most;
+  p.piece = up((V + pieces - 1) / pieces, XE_TILE);
+  p.dh_ld = up(d, 8);
+  p.slots = 1;
+  if (pieces == 1) {
+    // few row tiles and a long contraction: cut dh's K so that a slice is no
+    // longer than a dW tile's or than a third of a pair's share of the work
+    const int64_t nt = (d + XE_TILE - 1) / XE_TILE;
+    const int64_t kb_h = p.piece / G2_BK, kb_w = (T + G2_BK - 1) / G2_BK;
+    const int64_t share = (num_m * nt * kb_h + num_n * nt * kb_w) / (kPairs * 3);
+    const int64_t target = kb_w > share ? kb_w : share;
+    int64_t s = (kb_h + target - 1) / target;
+    if (s > 64) s = 64;
+    const int64_t per = (kb_h + s - 1) / s;
+    p.slots = static_cast<int>((kb_h + per - 1) / per);
+  }
+  return p;
+}
+
+struct XentSave {
+  XeRows rw;
+  __nv_bfloat16* hp;  // packed rows of hidden, [planes][t_pad][ldd]
+};
+void carve_save(Carve& c, const XentPlan& p, XentSave* s) {
+  s->rw.meta = c.take<XeMeta>(1);
+  s->rw.pos = c.take<int>(static_cast<size_t>(p.T));
+  s->rw.idx = c.take<int>(static_cast<size_t>(p.t_pad));
+  s->rw.yc = c.take<int>(static_cast<size_t>(p.t_pad));
+  s->rw.lse = c.take<float>(static_cast<size_t>(p.t_pad));
+  s->rw.lab = c.take<float>(static_cast<size_t>(p.t_pad));
+  s->hp = c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.t_pad * p.ldd));
+}
+struct XentFwd {
+  __nv_bfloat16* wp;
+  float2* part;
+  double* block_sum;
+};
+void carve_xent_fwd(Carve& c, const XentPlan& p, XentFwd* s) {
+  s->wp = p.pack_w ? c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.v_pad * p.ldd)) : nullptr;
+  s->part = c.take<float2>(static_cast<size_t>(2 * p.runs * p.t_pad));
+  s->block_sum = c.take<double>(static_cast<size_t>((p.T + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS));
+}
+struct XentBwd {
+  __nv_bfloat16* wp;
+  __nv_bfloat16* dl;
+  float* dh;
+};
+void carve_xent_bwd(Carve& c, const XentPlan& p, XentBwd* s) {
+  s->wp = p.pack_w ? c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.v_pad * p.ldd)) : nullptr;
+  s->dl = c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.t_pad * p.piece));
+  s->dh = c.take<float>(static_cast<size_t>(p.slots * p.t_pad * p.dh_ld));
+}
+
+template <class S, int PLANES>
+int xent_pack(const void* src, int64_t lds, int64_t d, const int* idx, const int* rows, int64_t count,
+              __nv_bfloat16* dst, int64_t plane_rows, int64_t ldd, cudaStream_t sm, const DeviceInfo& dev) {
+  int64_t blocks = (plane_rows * (ldd / 8) + 255) / 256;
+  if (blocks > 16ll * dev.sm_count) blocks = 16ll * dev.sm_count;
+  return launch_pdl(k_xent_pack<S, PLANES>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
+                    static_cast<const S*>(src), lds, static_cast<int>(d), idx, rows, count, dst, plane_rows,
+                    static_cast<int>(ldd));
+}
+int xent_pack_any(int dtype, const void* src, int64_t lds, int64_t d, const int* idx, const int* rows, int64_t count,
+                  __nv_bfloat16* dst, int64_t plane_rows, int64_t ldd, cudaStream_t sm, const DeviceInfo& dev) {
+  return dtype == ETHOS_BF16
+             ? xent_pack<__nv_bfloat16, 1>(src, lds, d, idx, rows, count, dst, plane_rows, ldd, sm, dev)
+             : xent_pack<float, 3>(src, lds, d, idx, rows, count, dst, plane_rows, ldd, sm, dev);
+}
+
+template <int MODE, int PLANES>
+int launch_xent(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1, const CUtensorMap& b1,
+                const XeArgs& args, int64_t units, int* err, cudaStream_t sm, const DeviceInfo& dev) {
+  auto kern = k_xent_gemm<MODE, PLANES>;
+  int st = smem_attr_once(reinterpret_cast<const void*>(kern), XE_SMEM);
+  if (st != ETHOS_OK) return st;
+  int64_t pairs = max_pair_clusters(reinterpret_cast<const void*>(kern), XE_THREADS, XE_SMEM, dev);
+  if (pairs <= 0) return ETHOS_ERR_CUDA;
+  if (pairs > units) pairs = units;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(static_cast<unsigned>(XE_THREADS));
+  cfg.dynamicSmemBytes = static_cast<size_t>(XE_SMEM);
+  cfg.stream = sm;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  count_launch();
+  if (cudaLaunchKernelEx(&cfg, kern, a0, b0, a1, b1, args, err) != cudaSuccess) return ETHOS_ERR_CUDA;
+  return launch_status();
+}
+template <int MODE>
+int launch_xent_planes(int planes, const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
+                       const CUtensorMap& b1, const XeArgs& args, int64_t units, int* err, cudaStream_t sm,
+                       const DeviceInfo& dev) {
+  return planes == 1 ? launch_xent<MODE, 1>(a0, b0, a1, b1, args, units, err, sm, dev)
+                     : launch_xent<MODE, 3>(a0, b0, a1, b1, args, units, err, sm, dev);
+}
+
+// The rows of hidden that the products read: hidden itself (bf16, aligned, no
+// more than XE_ROWS_DIRECT tokens) or the packed rows in the save buffer.
+struct XentRowsOperand {
+  const void* ptr;
+  int64_t rows, cols, ld, plane_rows;
+  bool direct;
+};
+XentRowsOperand xent_rows(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, int dtype) {
+  const bool direct = dtype == ETHOS_BF16 && p.T <= XE_ROWS_DIRECT && p.d % 8 == 0 && ldh % 8 == 0 && aligned16(hidden);
+  if (direct) return XentRowsOperand{hidden, p.T, p.d, ldh, 0, true};
+  return XentRowsOperand{sv.hp, p.planes * p.t_pad, p.ldd, p.ldd, p.t_pad, false};
+}
+
+int xent_check(int64_t tokens, int64_t vocab, int64_t dim, int64_t ldh, int64_t ldw, int dtype, int reduction) {
+  if (tokens < 1 || vocab < 1 || dim < 1 || ldh < dim || ldw < dim || !known_dtype(dtype)) return ETHOS_ERR_INVALID_ARG;
+  if (reduction < XE_NONE || reduction > XE_MEAN) return ETHOS_ERR_INVALID_ARG;
+  if (tokens > (1 << 24) || vocab > (1 << 24) || dim > (1 << 16)) return ETHOS_ERR_UNSUPPORTED_SHAPE;
+  return ETHOS_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -249,6 +413,170 @@ int ethos_balance_backward(const void* ids, int ids_i64, int dtype, const uint8_
                                                                         grad, d_weights, sm, *dev)
                              : balance_backward<int32_t, float>(ids, mask, tokens, H, K, experts, counts, s, grad,
                                                                 d_weights, sm, *dev);
+}
+
+size_t ethos_xent_save_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype) {
+  if (xent_check(tokens, vocab, dim, dim, dim, dtype, 0) != ETHOS_OK) return 0;
+  Carve c{nullptr, 0, 0};
+  XentSave s;
+  carve_save(c, xent_plan(tokens, vocab, dim, dtype), &s);
+  return c.off + 256;
+}
+
+size_t ethos_xent_forward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype) {
+  if (xent_check(tokens, vocab, dim, dim, dim, dtype, 0) != ETHOS_OK) return 0;
+  Carve c{nullptr, 0, 0};
+  XentFwd s;
+  carve_xent_fwd(c, xent_plan(tokens, vocab, dim, dtype), &s);
+  return c.off + 256;
+}
+
+size_t ethos_xent_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype) {
+  if (xent_check(tokens, vocab, dim, dim, dim, dtype, 0) != ETHOS_OK) return 0;
+  Carve c{nullptr, 0, 0};
+  XentBwd s;
+  carve_xent_bwd(c, xent_plan(tokens, vocab, dim, dtype), &s);
+  return c.off + 256;
+}
+
+int ethos_xent_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype,
+                       const void* labels, int labels_i64, int64_t ignore_index, int reduction, int64_t tokens,
+                       int64_t vocab, int64_t dim, float* loss, void* save, size_t save_bytes, void* workspace,
+                       size_t workspace_bytes, int* dev_err, void* stream) {
+  int st = xent_check(tokens, vocab, dim, ldh, ldw, dtype, reduction);
+  if (st != ETHOS_OK) return st;
+  if (!hidden || !weight || !labels || !loss || !dev_err) return ETHOS_ERR_INVALID_ARG;
+  const XentPlan p = xent_plan(tokens, vocab, dim, dtype);
+  Carve cs{static_cast<char*>(save), 0, save_bytes}, cw{static_cast<char*>(workspace), 0, workspace_bytes};
+  XentSave sv;
+  XentFwd ws;
+  carve_save(cs, p, &sv);
+  carve_xent_fwd(cw, p, &ws);
+  if (!save || !workspace || cs.off > save_bytes || cw.off > workspace_bytes) return ETHOS_ERR_WORKSPACE;
+  if (!aligned16(save) || !aligned16(workspace)) return ETHOS_ERR_ALIGNMENT;
+  if (!p.pack_w && (ldw % 8 != 0 || !aligned16(weight))) return ETHOS_ERR_ALIGNMENT;
+  DeviceInfo* dev = nullptr;
+  if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
+  cudaStream_t sm = static_cast<cudaStream_t>(stream);
+  const bool compact = tokens > XE_ROWS_DIRECT;
+  float* loss_rows = reduction == XE_NONE ? loss : nullptr;
+  const int T = static_cast<int>(tokens);
+  st = labels_i64 ? launch_pdl(k_xent_index<int64_t>, dim3(1), dim3(1024), 0, sm, static_cast<const int64_t*>(labels),
+                               T, vocab, ignore_index, compact, sv.rw, loss_rows, dev_err)
+                  : launch_pdl(k_xent_index<int32_t>, dim3(1), dim3(1024), 0, sm, static_cast<const int32_t*>(labels),
+                               T, vocab, ignore_index, compact, sv.rw, loss_rows, dev_err);
+  if (st != ETHOS_OK) return st;
+  const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype);
+  if (!h.direct &&
+      (st = xent_pack_any(dtype, hidden, ldh, dim, sv.rw.idx, &sv.rw.meta->rows, 0, sv.hp, p.t_pad, p.ldd, sm,
+                          *dev)) != ETHOS_OK)
+    return st;
+  if (p.pack_w && (st = xent_pack_any(dtype, weight, ldw, dim, nullptr, nullptr, vocab, ws.wp, p.v_pad, p.ldd, sm,
+                                      *dev)) != ETHOS_OK)
+    return st;
+  CUtensorMap ta, tb;
+  if ((st = make_tmap_bf16(&ta, h.ptr, h.rows, h.cols, G2_BM, h.ld)) != ETHOS_OK) return st;
+  st = p.pack_w ? make_tmap_bf16(&tb, ws.wp, p.planes * p.v_pad, p.ldd, G2_BM, p.ldd)
+                : make_tmap_bf16(&tb, weight, vocab, dim, G2_BM, ldw);
+  if (st != ETHOS_OK) return st;
+  XeArgs a = {};
+  a.rw = sv.rw;
+  a.p[0] = XeProduct{static_cast<int>(h.plane_rows), static_cast<int>(p.v_pad), T, static_cast<int>(vocab),
+                     static_cast<int>(dim)};
+  a.run = p.run;
+  a.part = ws.part;
+  a.part_ld = p.t_pad;
+  if ((st = launch_xent_planes<XE_STATS>(p.planes, ta, tb, ta, tb, a, p.t_pad / XE_TILE * p.runs, dev_err, sm,
+                                         *dev)) != ETHOS_OK)
+    return st;
+  return launch_pdl(k_xent_loss, dim3(static_cast<unsigned>((tokens + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS)), dim3(256), 0,
+                    sm, sv.rw, static_cast<const float2*>(ws.part), 2 * p.runs, p.t_pad, reduction, loss,
+                    ws.block_sum);
+}
+
+int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype, int reduction,
+                        int64_t tokens, int64_t vocab, int64_t dim, const float* grad, const void* save,
+                        size_t save_bytes, void* d_hidden, void* d_weight, void* workspace, size_t workspace_bytes,
+                        int* dev_err, void* stream) {
+  int st = xent_check(tokens, vocab, dim, ldh, ldw, dtype, reduction);
+  if (st != ETHOS_OK) return st;
+  if (!hidden || !weight || !grad || !dev_err) return ETHOS_ERR_INVALID_ARG;
+  const XentPlan p = xent_plan(tokens, vocab, dim, dtype);
+  Carve cs{static_cast<char*>(const_cast<void*>(save)), 0, save_bytes},
+      cw{static_cast<char*>(workspace), 0, workspace_bytes};
+  XentSave sv;
+  XentBwd ws;
+  carve_save(cs, p, &sv);
+  carve_xent_bwd(cw, p, &ws);
+  if (!save || !workspace || cs.off > save_bytes || cw.off > workspace_bytes) return ETHOS_ERR_WORKSPACE;
+  if (!aligned16(save) || !aligned16(workspace)) return ETHOS_ERR_ALIGNMENT;
+  if (!p.pack_w && (ldw % 8 != 0 || !aligned16(weight))) return ETHOS_ERR_ALIGNMENT;
+  if (!d_hidden && !d_weight) return ETHOS_OK;
+  DeviceInfo* dev = nullptr;
+  if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
+  cudaStream_t sm = static_cast<cudaStream_t>(stream);
+  const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype);
+  if (p.pack_w && (st = xent_pack_any(dtype, weight, ldw, dim, nullptr, nullptr, vocab, ws.wp, p.v_pad, p.ldd, sm,
+                                      *dev)) != ETHOS_OK)
+    return st;
+  const int T = static_cast<int>(tokens), D = static_cast<int>(dim);
+  const int64_t num_m = p.t_pad / XE_TILE, nt = (dim + XE_TILE - 1) / XE_TILE;
+  const int esz = dtype == ETHOS_BF16 ? 2 : 4;
+  CUtensorMap ha, hb;  // rows of hidden, K-major (A of the logits) and MN-major (B of dW)
+  if ((st = make_tmap_bf16(&ha, h.ptr, h.rows, h.cols, G2_BM, h.ld)) != ETHOS_OK) return st;
+  if ((st = make_tmap_bf16(&hb, h.ptr, h.rows, h.cols, G2_BK, h.ld)) != ETHOS_OK) return st;
+  for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
+    const int64_t n = vocab - v0 < p.piece ? vocab - v0 : p.piece;
+    const void* wptr = p.pack_w ? static_cast<const void*>(ws.wp + v0 * p.ldd)
+                                : static_cast<const void*>(static_cast<const __nv_bfloat16*>(weight) + v0 * ldw);
+    const int64_t wrows = p.pack_w ? p.planes * p.v_pad - v0 : n;
+    const int64_t wcols = p.pack_w ? p.ldd : dim, wld = p.pack_w ? p.ldd : ldw;
+    CUtensorMap wb, wk, dk, dm;
+    if ((st = make_tmap_bf16(&wb, wptr, wrows, wcols, G2_BM, wld)) != ETHOS_OK) return st;
+    if ((st = make_tmap_bf16(&wk, wptr, wrows, wcols, G2_BK, wld)) != ETHOS_OK) return st;
+    if ((st = make_tmap_bf16(&dk, ws.dl, p.planes * p.t_pad, p.piece, G2_BM, p.piece)) != ETHOS_OK) return st;
+    if ((st = make_tmap_bf16(&dm, ws.dl, p.planes * p.t_pad, p.piece, G2_BK, p.piece)) != ETHOS_OK) return st;
+    XeArgs a = {};
+    a.rw = sv.rw;
+    a.p[0] = XeProduct{static_cast<int>(h.plane_rows), static_cast<int>(p.v_pad), T, static_cast<int>(n), D};
+    a.v0 = static_cast<int>(v0);
+    a.grad = grad;
+    a.reduction = reduction;
+    a.dl = ws.dl;
+    a.dl_plane_rows = p.t_pad;
+    a.ldl = p.piece;
+    if ((st = launch_xent_planes<XE_DLOGITS>(p.planes, ha, wb, ha, wb, a, num_m * ((n + XE_TILE - 1) / XE_TILE),
+                                             dev_err, sm, *dev)) != ETHOS_OK)
+      return st;
+    XeArgs g = {};
+    g.rw = sv.rw;
+    g.grad = grad;
+    g.reduction = reduction;
+    g.p[0] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(p.v_pad), T, D, static_cast<int>(n)};
+    g.p[1] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(h.plane_rows), static_cast<int>(n), D, T};
+    g.dh_slots = p.slots;
+    g.dh_accumulate = v0 > 0;
+    g.dh_acc = ws.dh;
+    g.dh_slot_size = p.t_pad * p.dh_ld;
+    g.dh_ld = p.dh_ld;
+    g.dw = d_weight ? static_cast<char*>(d_weight) + v0 * dim * esz : nullptr;
+    g.dw_bf16 = dtype == ETHOS_BF16;
+    g.do_dh = d_hidden != nullptr;
+    g.do_dw = d_weight != nullptr;
+    const int64_t units = (g.do_dh ? num_m * nt * p.slots : 0) + (g.do_dw ? (n + XE_TILE - 1) / XE_TILE * nt : 0);
+    if ((st = launch_xent_planes<XE_GRADS>(p.planes, dk, wk, dm, hb, g, units, dev_err, sm, *dev)) != ETHOS_OK)
+      return st;
+  }
+  if (!d_hidden) return ETHOS_OK;
+  int64_t blocks = (tokens * ((dim + 3) / 4) + 255) / 256;
+  if (blocks > 16ll * dev->sm_count) blocks = 16ll * dev->sm_count;
+  return dtype == ETHOS_BF16
+             ? launch_pdl(k_xent_dhidden<__nv_bfloat16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
+                          static_cast<const float*>(ws.dh), p.slots, p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad,
+                          reduction, tokens, D, static_cast<__nv_bfloat16*>(d_hidden))
+             : launch_pdl(k_xent_dhidden<float>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
+                          static_cast<const float*>(ws.dh), p.slots, p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad,
+                          reduction, tokens, D, static_cast<float*>(d_hidden));
 }
 
 }  // extern "C"

@@ -1,5 +1,6 @@
 """Differentiable training operators around the expert layers, as functions of
-tensors: the decoder's token embedding and the balance of the routing.
+tensors: the decoder's token embedding, the balance of the routing, and the
+cross entropy of the output head.
 
 All run in ``libethos_b200.so`` on CUDA tensors (there is no CPU path), on the
 current stream, and without a host synchronisation: an id outside its range is
@@ -10,7 +11,7 @@ import torch
 
 from . import ops
 
-__all__ = ["embedding", "balance_loss"]
+__all__ = ["embedding", "balance_loss", "linear_cross_entropy"]
 
 
 class _Embedding(torch.autograd.Function):
@@ -72,3 +73,36 @@ def balance_loss(weights, ids, num_experts, mask=None):
     leaves tokens out; without any token the loss and the gradient are 0.
     ``counts`` is int32 ``[N]``."""
     return _BalanceLoss.apply(weights, ids, int(num_experts), mask)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, ignore_index, reduction):
+        loss, save = ops.linear_cross_entropy_forward(hidden, weight, labels, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, save)
+        ctx.reduction = reduction
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        hidden, weight, save = ctx.saved_tensors
+        dh, dw = ops.linear_cross_entropy_backward(grad, hidden, weight, save, ctx.reduction,
+                                                   ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dh, dw, None, None, None
+
+
+def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="mean"):
+    """``torch.nn.functional.cross_entropy(hidden @ weight.T, labels)`` without
+    the logits: ``hidden [..., d]`` against the vocabulary's rows ``weight [V,
+    d]`` (one dtype, fp32 or bf16), ``labels [...]`` int32 or int64.
+
+    The loss is fp32: per token, or summed or averaged over the tokens whose
+    label is not ``ignore_index`` (the mean over none is NaN, as torch has
+    it).  Ignored tokens take no part in the products.  The backward forms the
+    logits again, a piece of the vocabulary at a time, so memory does not grow
+    with ``T * V``; gradients have the operands' dtype."""
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"labels {tuple(labels.shape)} do not belong to hidden {tuple(hidden.shape)}")
+    flat = hidden.reshape(-1, hidden.shape[-1]) if hidden.dim() != 2 else hidden
+    loss = _LinearCrossEntropy.apply(flat, weight, labels.reshape(-1), ignore_index, reduction)
+    return loss.view(labels.shape) if reduction == "none" else loss

@@ -15,7 +15,7 @@ __all__ = [
     "make_dims", "gemm_bf16", "gemm_ex", "product_key_topk", "expert_forward", "router_forward", "layer_forward",
     "device_error_word", "check_device_error", "PackedWeights", "layer_backward", "layer_forward_f32",
     "router_forward_f32", "layer_backward_f32", "embedding_forward", "embedding_backward", "balance_forward",
-    "balance_backward",
+    "balance_backward", "linear_cross_entropy_forward", "linear_cross_entropy_backward",
 ]
 
 _ERR_WORDS = {}
@@ -641,3 +641,77 @@ def balance_backward(grad, ids, counts, scratch, dtype, mask=None):
                                        counts.numel(), _vp(counts), _vp(scratch), _vp(grad), _vp(dw), _stream(dev)),
           "ethos_balance_backward")
     return dw
+
+
+_XENT_REDUCTION = {"none": 0, "sum": 1, "mean": 2}  # ETHOS_XENT_*
+
+
+def _xent_rows(t):
+    """Unit column stride and a row pitch of at least the width."""
+    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _xent_weight(w):
+    """What the products can read in place: rows of 16-byte pieces (other
+    widths go through packed copies in the workspace)."""
+    w = _xent_rows(w)
+    if w.dtype == torch.bfloat16 and w.shape[1] % 8 == 0 and (w.data_ptr() % 16 or w.stride(0) % 8):
+        w = w.clone(memory_format=torch.contiguous_format)
+    return w
+
+
+def linear_cross_entropy_forward(hidden, weight, labels, ignore_index=-100, reduction="mean"):
+    """Cross entropy of the logits ``hidden @ weight.T`` without keeping them
+    (ethos_xent_forward): ``hidden [T, d]``, ``weight [V, d]`` of one dtype
+    (fp32 or bf16), ``labels [T]`` int32 or int64.  Returns ``(loss fp32 [T]
+    or scalar, save)``; ``save`` goes to ``linear_cross_entropy_backward``."""
+    _require_cuda(hidden, "hidden")
+    _same_device(hidden, (weight, "weight"), (labels, "labels"))
+    code, i64 = _dtype_code(hidden, "hidden"), _ids_i64(labels, "labels")
+    if reduction not in _XENT_REDUCTION:
+        raise ValueError(f"reduction: none, sum or mean, not {reduction!r}")
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"hidden [T, d] and weight [V, d]: got {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if weight.dtype != hidden.dtype:
+        raise ValueError(f"hidden is {hidden.dtype}, weight {weight.dtype}")
+    if tuple(labels.shape) != (hidden.shape[0],):
+        raise ValueError(f"labels: [{hidden.shape[0]}], got {tuple(labels.shape)}")
+    (T, d), V, dev = hidden.shape, weight.shape[0], hidden.device
+    hidden, weight, labels = _xent_rows(hidden), _xent_weight(weight), labels.contiguous()
+    red = _XENT_REDUCTION[reduction]
+    L = lib()
+    loss = torch.empty((T,) if red == 0 else (), dtype=torch.float32, device=dev)
+    if T == 0:  # as torch: nothing, 0, and the mean of nothing
+        return (loss if red == 0 else loss.fill_(0.0 if red == 1 else float("nan"))), None
+    save = torch.empty(L.ethos_xent_save_size(T, V, d, code), dtype=torch.uint8, device=dev)
+    ws = torch.empty(L.ethos_xent_forward_workspace_size(T, V, d, code), dtype=torch.uint8, device=dev)
+    err = device_error_word(dev)
+    check(L.ethos_xent_forward(_vp(hidden), max(hidden.stride(0), d), _vp(weight), max(weight.stride(0), d), code,
+                               _vp(labels), i64, int(ignore_index), red, T, V, d, _vp(loss), _vp(save), save.numel(),
+                               _vp(ws), ws.numel(), _vp(err), _stream(dev)), "ethos_xent_forward")
+    return loss, save
+
+
+def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", need_hidden=True, need_weight=True):
+    """``(d_hidden, d_weight)`` in the operands' dtype (None where not needed)
+    from the loss's gradient ``grad`` (fp32, ``[T]`` for reduction "none",
+    else a scalar) and ``linear_cross_entropy_forward``'s ``save``."""
+    _require_cuda(hidden, "hidden")
+    _same_device(hidden, (weight, "weight"), (grad, "grad"))
+    (T, d), V, dev = hidden.shape, weight.shape[0], hidden.device
+    dh = torch.empty((T, d), dtype=hidden.dtype, device=dev) if need_hidden else None
+    dw = torch.empty((V, d), dtype=weight.dtype, device=dev) if need_weight else None
+    if T == 0:
+        return dh, dw.zero_() if dw is not None else None
+    code, red = _dtype_code(hidden, "hidden"), _XENT_REDUCTION[reduction]
+    hidden, weight = _xent_rows(hidden), _xent_weight(weight)
+    grad = grad.to(torch.float32).contiguous()
+    if grad.numel() != (T if red == 0 else 1):
+        raise ValueError(f"grad of {grad.numel()} values for reduction {reduction!r}")
+    L = lib()
+    ws = torch.empty(L.ethos_xent_backward_workspace_size(T, V, d, code), dtype=torch.uint8, device=dev)
+    err = device_error_word(dev)
+    check(L.ethos_xent_backward(_vp(hidden), max(hidden.stride(0), d), _vp(weight), max(weight.stride(0), d), code, red,
+                                T, V, d, _vp(grad), _vp(save), save.numel(), _vp(dh), _vp(dw), _vp(ws), ws.numel(),
+                                _vp(err), _stream(dev)), "ethos_xent_backward")
+    return dh, dw

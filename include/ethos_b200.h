@@ -491,6 +491,40 @@ int ethos_balance_backward(const void* ids, int ids_i64, int dtype, const uint8_
                            int64_t heads, int64_t k, int64_t experts, const int32_t* counts, const void* scratch,
                            const float* grad, void* d_weights, void* stream);
 
+/* Cross entropy of the output head without its logits in memory:
+ *   l = hidden weight^T,  loss[t] = logsumexp(l[t]) - l[t, labels[t]],
+ * hidden [tokens, dim] (row pitch ldh), weight [vocab, dim] (row pitch ldw),
+ * both dtype; fp32 sums (fp32 operands as sums of bf16 parts, the products to
+ * fp32 accuracy).  Tokens whose label is ignore_index are left out (loss 0,
+ * no gradient); a label outside [0, vocab) sets ETHOS_ERR_ID_OUT_OF_RANGE in
+ * dev_err and its token is left out too.  reduction: NONE (loss fp32
+ * [tokens]), SUM or MEAN over the tokens not left out (loss one fp32; MEAN
+ * without a token is NaN).  For bf16 with dim % 8 == 0, weight must be 16-byte
+ * aligned with ldw % 8 == 0 (else ETHOS_ERR_ALIGNMENT).  `save` receives what
+ * the backward needs (row numbers, logsumexps, packed rows of hidden).
+ * tokens, vocab <= 2^24, dim <= 2^16. */
+#define ETHOS_XENT_NONE 0
+#define ETHOS_XENT_SUM 1
+#define ETHOS_XENT_MEAN 2
+size_t ethos_xent_save_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype);
+size_t ethos_xent_forward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype);
+int ethos_xent_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype,
+                       const void* labels, int labels_i64, int64_t ignore_index, int reduction, int64_t tokens,
+                       int64_t vocab, int64_t dim, float* loss, void* save, size_t save_bytes, void* workspace,
+                       size_t workspace_bytes, int* dev_err, void* stream);
+
+/* Gradients with respect to hidden [tokens, dim] and weight [vocab, dim]
+ * (dtype, contiguous; either may be NULL: not computed), given grad, the
+ * loss's gradient on the device (fp32, [tokens] for NONE, else one).  The
+ * logits are formed again, one piece of the vocabulary at a time (a piece's
+ * gradient takes about 1 GiB of the workspace, or 8192 columns).  hidden,
+ * weight and the sizes are the forward's. */
+size_t ethos_xent_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype);
+int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype, int reduction,
+                        int64_t tokens, int64_t vocab, int64_t dim, const float* grad, const void* save,
+                        size_t save_bytes, void* d_hidden, void* d_weight, void* workspace, size_t workspace_bytes,
+                        int* dev_err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
