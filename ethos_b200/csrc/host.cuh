@@ -41,6 +41,14 @@ inline int base_device_info(DeviceInfo** out) {
     d.major = major;
   }
   if (d.major != 10) return ETHOS_ERR_NO_DEVICE;
+  // cuTensorMapEncodeTiled needs a current context, and a thread that has made
+  // no runtime call that binds one (an autograd worker whose allocations all
+  // came from the cache) has none
+  static thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return ETHOS_ERR_CUDA;
+    bound = dev;
+  }
   *out = &d;
   return ETHOS_OK;
 }

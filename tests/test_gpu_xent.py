@@ -305,6 +305,26 @@ def test_one_gradient_only_and_no_tokens():
 
 
 @pytest.mark.gpu
+def test_backward_in_a_thread_without_a_context():
+    """A thread's first CUDA work is the backward, and its memory comes from
+    the caching allocator (as in autograd's worker)."""
+    import threading
+    h, W, y = (t.cuda() for t in _inputs(300, 2000, 64, torch.bfloat16, seed=11, ignored=0.5))
+    loss, save = ops.linear_cross_entropy_forward(h, W, y)
+    one = torch.ones((), device="cuda")
+    want = ops.linear_cross_entropy_backward(one, h, W, save)
+    del loss
+    again = [t.clone() for t in want]
+    del want  # its blocks, and the workspace's, are in the cache now
+    got = []
+    t = threading.Thread(target=lambda: got.extend(ops.linear_cross_entropy_backward(one, h, W, save)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 2 and all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.gpu
 def test_refusals():
     h, W, y = (t.cuda() for t in _inputs(10, 20, 8, torch.float32, seed=10))
     with pytest.raises(RuntimeError, match="no CPU path"):
