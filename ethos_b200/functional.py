@@ -51,10 +51,13 @@ class _BalanceLoss(torch.autograd.Function):
         ctx.save_for_backward(ids, mask, counts, scratch)
         ctx.dtype = weights.dtype
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)  # no zeros for the counts
         return loss, counts
 
     @staticmethod
     def backward(ctx, grad, _):
+        if grad is None:
+            return None, None, None, None
         ids, mask, counts, scratch = ctx.saved_tensors
         return ops.balance_backward(grad, ids, counts, scratch, ctx.dtype, mask), None, None, None
 

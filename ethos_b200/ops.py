@@ -6,6 +6,7 @@ CUDA device: there is no CPU path.
 """
 
 import ctypes
+import functools
 
 import torch
 
@@ -52,12 +53,16 @@ def _require_cuda(t, name):
 
 def device_error_word(device):
     """The per-device int32 word where kernels record bounds/timeout errors."""
+    w = _ERR_WORDS.get(device)  # a torch.device with an index: the common call
+    if w is not None:
+        return w
     device = torch.device(device)
     key = (device.type, device.index if device.index is not None else torch.cuda.current_device())
     w = _ERR_WORDS.get(key)
     if w is None:
         w = torch.zeros(4, dtype=torch.int32, device=device)
         _ERR_WORDS[key] = w
+    _ERR_WORDS[torch.device(*key)] = w
     return w
 
 
@@ -531,6 +536,10 @@ def layer_backward_f32(dy, x32, pw, saved, bn_training, eps, stage_events=None):
 
 # ------------------------------------------- training: the model's ends --
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1}  # ETHOS_F32, ETHOS_BF16
+_INT_CODE = {torch.int32: 0, torch.int64: 1}
+# current stream handle of a device index, without building a Stream object:
+# these calls are short, and a step makes several (2.4 -> 0.1 us)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _dtype_code(t, name):
@@ -541,18 +550,26 @@ def _dtype_code(t, name):
 
 
 def _ids_i64(t, name):
-    if t.dtype not in (torch.int32, torch.int64):
+    code = _INT_CODE.get(t.dtype)
+    if code is None:
         raise ValueError(f"{name}: int32 or int64, not {t.dtype}")
-    return 1 if t.dtype == torch.int64 else 0
+    return code
 
 
-def _same_device(ref, *named):
-    for t, name in named:
-        if t is None:
-            continue
+def _on(dev, t, name):
+    if t.device != dev:
         _require_cuda(t, name)
-        if t.device != ref.device:
-            raise ValueError(f"{name} is on {t.device}, not on {ref.device}")
+        raise ValueError(f"{name} is on {t.device}, not on {dev}")
+
+
+@functools.lru_cache(maxsize=256)
+def _size(name, *dims):
+    """A workspace size of the library, which depends on the sizes only."""
+    return getattr(lib(), name)(*dims)
+
+
+def _bytes(n, dev):
+    return torch.empty(n, dtype=torch.uint8, device=dev)
 
 
 def embedding_forward(ids, weight, scale=1.0):
@@ -560,18 +577,20 @@ def embedding_forward(ids, weight, scale=1.0):
     int32 or int64; ``weight`` ``[V, d]`` fp32 or bf16 with unit column stride.
     An id outside ``[0, V)`` sets the device error word and gives zeros."""
     _require_cuda(weight, "weight")
-    _same_device(weight, (ids, "ids"))
+    dev = weight.device
+    _on(dev, ids, "ids")
     if weight.dim() != 2:
         raise ValueError("weight: [vocab, dim]")
     code, i64 = _dtype_code(weight, "weight"), _ids_i64(ids, "ids")
     V, d = weight.shape
-    if weight.stride(1) != 1 or (V > 1 and weight.stride(0) < d):
+    ldw = weight.stride(0)
+    if weight.stride(1) != 1 or ldw < d:
         weight = weight.contiguous()
+        ldw = d
     ids = ids.contiguous()
-    out = torch.empty((*ids.shape, d), dtype=weight.dtype, device=weight.device)
-    err = device_error_word(weight.device)
-    check(lib().ethos_embedding_forward(_vp(ids), i64, _vp(weight), max(weight.stride(0), d), code, ids.numel(), V, d,
-                                        float(scale), _vp(out), _vp(err), _stream(weight.device)),
+    out = weight.new_empty((*ids.shape, d))
+    check(lib().ethos_embedding_forward(ids.data_ptr(), i64, weight.data_ptr(), ldw, code, ids.numel(), V, d, scale,
+                                        out.data_ptr(), device_error_word(dev).data_ptr(), _raw_stream(dev.index)),
           "ethos_embedding_forward")
     return out
 
@@ -582,21 +601,20 @@ def embedding_backward(ids, dy, vocab, scale=1.0, padding_idx=None):
     in fp32 in token order, the same in every run.  Tokens equal to
     ``padding_idx`` contribute nothing."""
     _require_cuda(dy, "dy")
-    _same_device(dy, (ids, "ids"))
+    dev = dy.device
+    _on(dev, ids, "ids")
     code, i64 = _dtype_code(dy, "dy"), _ids_i64(ids, "ids")
     d = dy.shape[-1]
-    if tuple(dy.shape[:-1]) != tuple(ids.shape):
+    if dy.shape[:-1] != ids.shape:
         raise ValueError(f"dy {tuple(dy.shape)} does not belong to ids {tuple(ids.shape)}")
     ids, dy = ids.contiguous(), dy.contiguous()
-    L = lib()
     T = ids.numel()
-    dw = torch.empty((vocab, d), dtype=dy.dtype, device=dy.device)
-    ws_bytes = L.ethos_embedding_backward_workspace_size(T, vocab, d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
-    err = device_error_word(dy.device)
-    check(L.ethos_embedding_backward(_vp(ids), i64, _vp(dy), code, T, vocab, d,
-                                     -1 if padding_idx is None else int(padding_idx), float(scale), _vp(dw), _vp(ws),
-                                     ws_bytes, _vp(err), _stream(dy.device)), "ethos_embedding_backward")
+    dw = dy.new_empty((vocab, d))
+    ws = _bytes(_size("ethos_embedding_backward_workspace_size", T, vocab, d), dev)
+    check(lib().ethos_embedding_backward(ids.data_ptr(), i64, dy.data_ptr(), code, T, vocab, d,
+                                         -1 if padding_idx is None else padding_idx, scale, dw.data_ptr(),
+                                         ws.data_ptr(), ws.numel(), device_error_word(dev).data_ptr(),
+                                         _raw_stream(dev.index)), "ethos_embedding_backward")
     return dw
 
 
@@ -606,24 +624,27 @@ def balance_forward(weights, ids, num_experts, mask=None):
     the token out).  Returns ``(loss fp32 scalar, counts int32 [N], scratch)``;
     the scratch goes to ``balance_backward``."""
     _require_cuda(weights, "weights")
-    _same_device(weights, (ids, "ids"), (mask, "mask"))
+    dev = weights.device
+    _on(dev, ids, "ids")
     code, i64 = _dtype_code(weights, "weights"), _ids_i64(ids, "ids")
     if weights.dim() != 3 or ids.shape != weights.shape:
         raise ValueError("weights and ids: [tokens, heads, k], of one shape")
     T, H, k = weights.shape
+    mptr = 0
     if mask is not None:
+        _on(dev, mask, "mask")
         if mask.dtype != torch.bool or tuple(mask.shape) != (T,):
             raise ValueError("mask: bool [tokens]")
         mask = mask.contiguous()
+        mptr = mask.data_ptr()
     weights, ids = weights.contiguous(), ids.contiguous()
-    L = lib()
-    dev = weights.device
     counts = torch.empty((num_experts,), dtype=torch.int32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    scratch = torch.empty(L.ethos_balance_scratch_size(), dtype=torch.uint8, device=dev)
-    err = device_error_word(dev)
-    check(L.ethos_balance_forward(_vp(ids), i64, _vp(weights), code, _vp(mask), T, H, k, num_experts, _vp(counts),
-                                  _vp(loss), _vp(scratch), _vp(err), _stream(dev)), "ethos_balance_forward")
+    scratch = _bytes(_size("ethos_balance_scratch_size"), dev)
+    check(lib().ethos_balance_forward(ids.data_ptr(), i64, weights.data_ptr(), code, mptr, T, H, k, num_experts,
+                                      counts.data_ptr(), loss.data_ptr(), scratch.data_ptr(),
+                                      device_error_word(dev).data_ptr(), _raw_stream(dev.index)),
+          "ethos_balance_forward")
     return loss, counts, scratch
 
 
@@ -637,9 +658,10 @@ def balance_backward(grad, ids, counts, scratch, dtype, mask=None):
     ids = ids.contiguous()
     mask = mask.contiguous() if mask is not None else None
     grad = grad.to(torch.float32)
-    check(lib().ethos_balance_backward(_vp(ids), _ids_i64(ids, "ids"), _dtype_code(dw, "weights"), _vp(mask), T, H, k,
-                                       counts.numel(), _vp(counts), _vp(scratch), _vp(grad), _vp(dw), _stream(dev)),
-          "ethos_balance_backward")
+    check(lib().ethos_balance_backward(ids.data_ptr(), _ids_i64(ids, "ids"), _dtype_code(dw, "weights"),
+                                       0 if mask is None else mask.data_ptr(), T, H, k, counts.numel(),
+                                       counts.data_ptr(), scratch.data_ptr(), grad.data_ptr(), dw.data_ptr(),
+                                       _raw_stream(dev.index)), "ethos_balance_backward")
     return dw
 
 
@@ -648,14 +670,19 @@ _XENT_REDUCTION = {"none": 0, "sum": 1, "mean": 2}  # ETHOS_XENT_*
 
 def _xent_rows(t):
     """Unit column stride and a row pitch of at least the width."""
-    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _pitch(t):
+    """Row pitch (a single row may carry any stride)."""
+    return max(t.stride(0), t.shape[1])
 
 
 def _xent_weight(w):
     """What the products can read in place: rows of 16-byte pieces (other
     widths go through packed copies in the workspace)."""
     w = _xent_rows(w)
-    if w.dtype == torch.bfloat16 and w.shape[1] % 8 == 0 and (w.data_ptr() % 16 or w.stride(0) % 8):
+    if w.dtype == torch.bfloat16 and w.shape[1] % 8 == 0 and (w.data_ptr() % 16 or _pitch(w) % 8):
         w = w.clone(memory_format=torch.contiguous_format)
     return w
 
@@ -666,29 +693,30 @@ def linear_cross_entropy_forward(hidden, weight, labels, ignore_index=-100, redu
     (fp32 or bf16), ``labels [T]`` int32 or int64.  Returns ``(loss fp32 [T]
     or scalar, save)``; ``save`` goes to ``linear_cross_entropy_backward``."""
     _require_cuda(hidden, "hidden")
-    _same_device(hidden, (weight, "weight"), (labels, "labels"))
+    dev = hidden.device
+    _on(dev, weight, "weight")
+    _on(dev, labels, "labels")
     code, i64 = _dtype_code(hidden, "hidden"), _ids_i64(labels, "labels")
-    if reduction not in _XENT_REDUCTION:
+    red = _XENT_REDUCTION.get(reduction)
+    if red is None:
         raise ValueError(f"reduction: none, sum or mean, not {reduction!r}")
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"hidden [T, d] and weight [V, d]: got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if weight.dtype != hidden.dtype:
         raise ValueError(f"hidden is {hidden.dtype}, weight {weight.dtype}")
-    if tuple(labels.shape) != (hidden.shape[0],):
-        raise ValueError(f"labels: [{hidden.shape[0]}], got {tuple(labels.shape)}")
-    (T, d), V, dev = hidden.shape, weight.shape[0], hidden.device
-    hidden, weight, labels = _xent_rows(hidden), _xent_weight(weight), labels.contiguous()
-    red = _XENT_REDUCTION[reduction]
-    L = lib()
+    (T, d), V = hidden.shape, weight.shape[0]
+    if tuple(labels.shape) != (T,):
+        raise ValueError(f"labels: [{T}], got {tuple(labels.shape)}")
     loss = torch.empty((T,) if red == 0 else (), dtype=torch.float32, device=dev)
     if T == 0:  # as torch: nothing, 0, and the mean of nothing
         return (loss if red == 0 else loss.fill_(0.0 if red == 1 else float("nan"))), None
-    save = torch.empty(L.ethos_xent_save_size(T, V, d, code), dtype=torch.uint8, device=dev)
-    ws = torch.empty(L.ethos_xent_forward_workspace_size(T, V, d, code), dtype=torch.uint8, device=dev)
-    err = device_error_word(dev)
-    check(L.ethos_xent_forward(_vp(hidden), max(hidden.stride(0), d), _vp(weight), max(weight.stride(0), d), code,
-                               _vp(labels), i64, int(ignore_index), red, T, V, d, _vp(loss), _vp(save), save.numel(),
-                               _vp(ws), ws.numel(), _vp(err), _stream(dev)), "ethos_xent_forward")
+    hidden, weight, labels = _xent_rows(hidden), _xent_weight(weight), labels.contiguous()
+    save = _bytes(_size("ethos_xent_save_size", T, V, d, code), dev)
+    ws = _bytes(_size("ethos_xent_forward_workspace_size", T, V, d, code), dev)
+    check(lib().ethos_xent_forward(hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), code,
+                                   labels.data_ptr(), i64, ignore_index, red, T, V, d, loss.data_ptr(),
+                                   save.data_ptr(), save.numel(), ws.data_ptr(), ws.numel(),
+                                   device_error_word(dev).data_ptr(), _raw_stream(dev.index)), "ethos_xent_forward")
     return loss, save
 
 
@@ -697,10 +725,12 @@ def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", 
     from the loss's gradient ``grad`` (fp32, ``[T]`` for reduction "none",
     else a scalar) and ``linear_cross_entropy_forward``'s ``save``."""
     _require_cuda(hidden, "hidden")
-    _same_device(hidden, (weight, "weight"), (grad, "grad"))
-    (T, d), V, dev = hidden.shape, weight.shape[0], hidden.device
-    dh = torch.empty((T, d), dtype=hidden.dtype, device=dev) if need_hidden else None
-    dw = torch.empty((V, d), dtype=weight.dtype, device=dev) if need_weight else None
+    dev = hidden.device
+    _on(dev, weight, "weight")
+    _on(dev, grad, "grad")
+    (T, d), V = hidden.shape, weight.shape[0]
+    dh = hidden.new_empty((T, d)) if need_hidden else None
+    dw = weight.new_empty((V, d)) if need_weight else None
     if T == 0:
         return dh, dw.zero_() if dw is not None else None
     code, red = _dtype_code(hidden, "hidden"), _XENT_REDUCTION[reduction]
@@ -708,10 +738,10 @@ def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", 
     grad = grad.to(torch.float32).contiguous()
     if grad.numel() != (T if red == 0 else 1):
         raise ValueError(f"grad of {grad.numel()} values for reduction {reduction!r}")
-    L = lib()
-    ws = torch.empty(L.ethos_xent_backward_workspace_size(T, V, d, code), dtype=torch.uint8, device=dev)
-    err = device_error_word(dev)
-    check(L.ethos_xent_backward(_vp(hidden), max(hidden.stride(0), d), _vp(weight), max(weight.stride(0), d), code, red,
-                                T, V, d, _vp(grad), _vp(save), save.numel(), _vp(dh), _vp(dw), _vp(ws), ws.numel(),
-                                _vp(err), _stream(dev)), "ethos_xent_backward")
+    ws = _bytes(_size("ethos_xent_backward_workspace_size", T, V, d, code), dev)
+    check(lib().ethos_xent_backward(hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), code, red,
+                                    T, V, d, grad.data_ptr(), save.data_ptr(), save.numel(),
+                                    dh.data_ptr() if need_hidden else 0, dw.data_ptr() if need_weight else 0,
+                                    ws.data_ptr(), ws.numel(), device_error_word(dev).data_ptr(),
+                                    _raw_stream(dev.index)), "ethos_xent_backward")
     return dh, dw
