@@ -112,6 +112,12 @@ EXPORTS = {
     # loss, save, save_bytes, workspace, workspace_bytes, dev_err, stream
     "ethos_xent_forward": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _I64, _I, _I64, _I64, _I64, _P, _P, _SZ, _P, _SZ,
                                 _P, _P]),
+    "ethos_xent_forward_backward_workspace_size": (_SZ, [_I64, _I64, _I64, _I]),
+    # hidden, ldh, weight, ldw, dtype, labels, labels_i64, ignore_index, reduction, tokens, vocab, dim,
+    # loss, save, save_bytes, d_hidden, d_weight, workspace, workspace_bytes, dev_err, stream
+    "ethos_xent_forward_backward": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _I64, _I, _I64, _I64, _I64, _P, _P, _SZ, _P,
+                                         _P, _P, _SZ, _P, _P]),
+    "ethos_xent_scale": (_I, [_P, _P, _I, _I64, _P]),
     "ethos_xent_backward_workspace_size": (_SZ, [_I64, _I64, _I64, _I]),
     # hidden, ldh, weight, ldw, dtype, reduction, tokens, vocab, dim, grad, save, save_bytes, d_hidden,
     # d_weight, workspace, workspace_bytes, dev_err, stream

@@ -24,6 +24,7 @@ constexpr int EMB_SORT_THREADS = 512;
 constexpr int EMB_SORT_WARPS = EMB_SORT_THREADS / 32;
 constexpr int EMB_MAX_RANGE = 1024;  // ids owned by one block of the sort
 constexpr int EMB_CHUNK = 32;        // sorted tokens summed by one unit
+constexpr int64_t EMB_NO_PADDING = INT64_MIN;
 
 template <class T>
 struct Vec16;  // 16-byte vector of T as fp32 values
@@ -119,11 +120,14 @@ __global__ void __launch_bounds__(256) k_embed_fwd(const I* __restrict__ ids, co
 // list begins, so that blocks need nothing from one another.  Within the
 // block, warp w takes the w-th contiguous part of the tokens, counts its ids,
 // and after a scan over (id, warp) places its tokens in order.  Ids that are
-// out of range, or equal to `padding` (no gradient), take no place.
+// out of range, or equal to `padding` (no gradient; EMB_NO_PADDING: no such
+// id), take no place.  `count`, if given, is the number of tokens on the device
+// (at most `tokens`).
 //   offs [V + 1]  first place of each id (offs[V] = places in use)
 //   perm [tokens] token at each place;  sid [tokens] its id
 template <class I>
-__global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __restrict__ ids, int tokens, int64_t vocab,
+__global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __restrict__ ids, int tokens,
+                                                                 const int* __restrict__ count, int64_t vocab,
                                                                  int64_t padding, int range, int* __restrict__ offs,
                                                                  int* __restrict__ perm, int* __restrict__ sid,
                                                                  int* err) {
@@ -133,6 +137,7 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __rest
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (count != nullptr) tokens = min(tokens, *count);
   const int64_t lo = static_cast<int64_t>(blockIdx.x) * range;
   const int n = static_cast<int>(lo + range < vocab ? range : vocab - lo);  // ids owned
   for (int i = threadIdx.x; i < EMB_SORT_WARPS * range; i += EMB_SORT_THREADS) cnt[i] = 0;
@@ -145,11 +150,13 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __rest
 #pragma unroll 4
   for (int64_t t = t0 + lane; t < t1; t += 32) {
     const int64_t id = static_cast<int64_t>(__ldg(ids + t));
+    if (id == padding) continue;
     if (id < 0 || id >= vocab) {
       if (blockIdx.x == 0) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
-    } else if (id != padding) {
-      if (id < lo) ++below;
-      else if (id < lo + n) atomicAdd(mine + static_cast<int>(id - lo), 1);
+    } else if (id < lo) {
+      ++below;
+    } else if (id < lo + n) {
+      atomicAdd(mine + static_cast<int>(id - lo), 1);
     }
   }
 #pragma unroll
@@ -218,16 +225,34 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __rest
 }
 
 // --------------------------------------------------------------- row sums --
+// N fp32 values to N elements of O (16-byte stores with kVec)
+template <class O, bool kVec, int N>
+__device__ __forceinline__ void store_row(O* p, const float (&v)[N]) {
+  if constexpr (!kVec) {
+    RowAccess<O, false>::store(p, v);
+  } else if constexpr (std::is_same<O, float>::value) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  } else {
+    Vec16<O>::store(p, v);
+  }
+}
+
 // Blocks [0, sum_blocks): chunks of EMB_CHUNK places, `ty` chunks per block,
-// tx threads along the columns.  part [chunks][2][d] fp32 receives the piece
+// tx threads along the columns.  Token t contributes row t of dy (pitch ldy)
+// times row_scale[t], if given.  part [chunks][2][d] fp32 receives the piece
 // of the row that continues from the previous chunk (0) and of the row that
 // continues into the next (1); a chunk inside one row uses slot 0.
-// Remaining blocks: zero rows of ids that no token holds.
-template <class T, bool kVec>
-__global__ void __launch_bounds__(256) k_embed_rows(const T* __restrict__ dy, int d, int64_t vocab, float scale,
-                                                    const int* __restrict__ offs, const int* __restrict__ perm,
-                                                    const int* __restrict__ sid, int chunk_blocks, int col_blocks,
-                                                    float* __restrict__ part, T* __restrict__ dw) {
+// Sums go to row id of dw, or (kByPlace) to row offs[id]: the rows of ids in
+// use, without the others.  Remaining blocks: zero rows of ids that no token
+// holds.
+template <class T, bool kVec, class O, bool kByPlace>
+__global__ void __launch_bounds__(256) k_embed_rows(const T* __restrict__ dy, int64_t ldy,
+                                                    const float* __restrict__ row_scale, int d, int64_t vocab,
+                                                    float scale, const int* __restrict__ offs,
+                                                    const int* __restrict__ perm, const int* __restrict__ sid,
+                                                    int chunk_blocks, int col_blocks, float* __restrict__ part,
+                                                    O* __restrict__ dw) {
   using A = RowAccess<T, kVec>;
   constexpr int N = A::N;
   constexpr int U = 4;  // rows in flight per thread
@@ -256,8 +281,14 @@ __global__ void __launch_bounds__(256) k_embed_rows(const T* __restrict__ dy, in
       for (int u = 0; u < U; ++u) {
         id[u] = -1;
         if (p + u < p1) {
+          const int t = perm[p + u];
           id[u] = sid[p + u];
-          A::load(dy + static_cast<int64_t>(perm[p + u]) * d + c, v[u]);
+          A::load(dy + t * ldy + c, v[u]);
+          if (row_scale != nullptr) {
+            const float f = row_scale[t];
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[u][j] *= f;
+          }
         }
       }
 #pragma unroll
@@ -270,7 +301,7 @@ __global__ void __launch_bounds__(256) k_embed_rows(const T* __restrict__ dy, in
           } else {
 #pragma unroll
             for (int j = 0; j < N; ++j) acc[j] *= scale;
-            A::store(dw + static_cast<int64_t>(cur) * d + c, acc);
+            store_row<O, kVec>(dw + static_cast<int64_t>(kByPlace ? offs[cur] : cur) * d + c, acc);
           }
           first = false;
           cur = id[u];
@@ -288,7 +319,7 @@ __global__ void __launch_bounds__(256) k_embed_rows(const T* __restrict__ dy, in
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] *= scale;
-      A::store(dw + static_cast<int64_t>(cur) * d + c, acc);
+      store_row<O, kVec>(dw + static_cast<int64_t>(kByPlace ? offs[cur] : cur) * d + c, acc);
     }
     return;
   }
@@ -301,18 +332,17 @@ __global__ void __launch_bounds__(256) k_embed_rows(const T* __restrict__ dy, in
   for (int j = 0; j < N; ++j) z[j] = 0.0f;
   for (int64_t v = static_cast<int64_t>(blockIdx.x - sum_blocks) * 8 + (tid >> 5); v < vocab; v += nw) {
     if (offs[v] != offs[v + 1]) continue;
-    for (int c = lane * N; c < d; c += 32 * N) A::store(dw + v * d + c, z);
+    for (int c = lane * N; c < d; c += 32 * N) store_row<O, kVec>(dw + v * d + c, z);
   }
 }
 
 // Rows that cross chunks: the chunk in which such a row begins adds its own
 // piece and the pieces of the following chunks, in order, and writes the row.
-template <class T, bool kVec>
+template <class T, bool kVec, class O, bool kByPlace>
 __global__ void __launch_bounds__(256) k_embed_join(int d, int64_t vocab, float scale, const int* __restrict__ offs,
                                                     const int* __restrict__ sid, int col_blocks,
-                                                    const float* __restrict__ part, T* __restrict__ dw) {
-  using A = RowAccess<T, kVec>;
-  constexpr int N = A::N;
+                                                    const float* __restrict__ part, O* __restrict__ dw) {
+  constexpr int N = RowAccess<T, kVec>::N;
   pdl_launch_dependents();
   pdl_wait();
   const int places = offs[vocab];
@@ -335,7 +365,7 @@ __global__ void __launch_bounds__(256) k_embed_join(int d, int64_t vocab, float 
   }
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] *= scale;
-  A::store(dw + static_cast<int64_t>(cur) * d + c, acc);
+  store_row<O, kVec>(dw + static_cast<int64_t>(kByPlace ? offs[cur] : cur) * d + c, acc);
 }
 
 }  // namespace ethos

@@ -59,9 +59,11 @@ void carve_embed(Carve& c, int64_t tokens, int64_t vocab, int64_t dim, EmbedScra
   s->part = c.take<float>(static_cast<size_t>((tokens + EMB_CHUNK - 1) / EMB_CHUNK * 2 * dim));
 }
 
-template <class T, bool kVec>
-int embed_rows(const EmbedScratch& s, const void* dy, int64_t tokens, int64_t vocab, int d, float scale, void* dw,
-               cudaStream_t sm, const DeviceInfo& dev) {
+// Row sums of the sorted tokens (k_embed_rows, k_embed_join).  kByPlace: the
+// rows in use only; otherwise every row of the table.
+template <class T, bool kVec, class O, bool kByPlace>
+int embed_rows(const EmbedScratch& s, const void* dy, int64_t ldy, const float* row_scale, int64_t tokens,
+               int64_t vocab, int d, float scale, O* dw, cudaStream_t sm, const DeviceInfo& dev) {
   const int pieces = d / RowAccess<T, kVec>::N;
   int tx = 8;
   while (tx < pieces && tx < 256) tx *= 2;
@@ -69,23 +71,23 @@ int embed_rows(const EmbedScratch& s, const void* dy, int64_t tokens, int64_t vo
   const int col_blocks = (pieces + tx - 1) / tx;
   const int chunks = static_cast<int>((tokens + EMB_CHUNK - 1) / EMB_CHUNK);
   const int chunk_blocks = (chunks + ty - 1) / ty;
-  const int64_t fill_most = (vocab + 7) / 8;
+  const int64_t fill_most = kByPlace ? 0 : (vocab + 7) / 8;
   const int fill = static_cast<int>(fill_most < 4 * dev.sm_count ? fill_most : 4 * dev.sm_count);
   const int64_t grid = static_cast<int64_t>(chunk_blocks) * col_blocks;
   if (grid + fill > (int64_t(1) << 31) - 1) return ETHOS_ERR_UNSUPPORTED_SHAPE;
-  int st = launch_pdl(k_embed_rows<T, kVec>, dim3(static_cast<unsigned>(grid + fill)), dim3(tx, ty), 0, sm,
-                      static_cast<const T*>(dy), d, vocab, scale, static_cast<const int*>(s.offs),
+  int st = launch_pdl(k_embed_rows<T, kVec, O, kByPlace>, dim3(static_cast<unsigned>(grid + fill)), dim3(tx, ty), 0,
+                      sm, static_cast<const T*>(dy), ldy, row_scale, d, vocab, scale, static_cast<const int*>(s.offs),
                       static_cast<const int*>(s.perm), static_cast<const int*>(s.sid), chunk_blocks, col_blocks,
-                      s.part, static_cast<T*>(dw));
+                      s.part, dw);
   if (st != ETHOS_OK || chunks < 2) return st;
-  return launch_pdl(k_embed_join<T, kVec>, dim3(static_cast<unsigned>(grid)), dim3(tx, ty), 0, sm, d, vocab, scale,
-                    static_cast<const int*>(s.offs), static_cast<const int*>(s.sid), col_blocks,
-                    static_cast<const float*>(s.part), static_cast<T*>(dw));
+  return launch_pdl(k_embed_join<T, kVec, O, kByPlace>, dim3(static_cast<unsigned>(grid)), dim3(tx, ty), 0, sm, d,
+                    vocab, scale, static_cast<const int*>(s.offs), static_cast<const int*>(s.sid), col_blocks,
+                    static_cast<const float*>(s.part), dw);
 }
 
 template <class I>
-int embed_sort(const EmbedScratch& s, const void* ids, int64_t tokens, int64_t vocab, int64_t padding, int* err,
-               cudaStream_t sm, const DeviceInfo& dev) {
+int embed_sort(const EmbedScratch& s, const void* ids, int64_t tokens, const int* count, int64_t vocab,
+               int64_t padding, int* err, cudaStream_t sm, const DeviceInfo& dev) {
   // one block per SM, more when a block would own over EMB_MAX_RANGE ids
   int64_t blocks = dev.sm_count;
   if (blocks * EMB_MAX_RANGE < vocab) blocks = (vocab + EMB_MAX_RANGE - 1) / EMB_MAX_RANGE;
@@ -97,8 +99,17 @@ int embed_sort(const EmbedScratch& s, const void* ids, int64_t tokens, int64_t v
                                 EMB_SORT_WARPS * EMB_MAX_RANGE * static_cast<int>(sizeof(int)));
   if (st != ETHOS_OK) return st;
   return launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(EMB_SORT_THREADS), static_cast<size_t>(smem), sm,
-                    static_cast<const I*>(ids), static_cast<int>(tokens), vocab, padding, range, s.offs, s.perm,
-                    s.sid, err);
+                    static_cast<const I*>(ids), static_cast<int>(tokens), count, vocab, padding, range, s.offs,
+                    s.perm, s.sid, err);
+}
+
+template <class T>
+int embed_table_grad(const EmbedScratch& s, const void* dy, int64_t tokens, int64_t vocab, int d, float scale,
+                     void* dw, cudaStream_t sm, const DeviceInfo& dev) {
+  T* o = static_cast<T*>(dw);
+  return d % Vec16<T>::N == 0 && aligned16(dy) && aligned16(dw)
+             ? embed_rows<T, true, T, false>(s, dy, d, nullptr, tokens, vocab, d, scale, o, sm, dev)
+             : embed_rows<T, false, T, false>(s, dy, d, nullptr, tokens, vocab, d, scale, o, sm, dev);
 }
 
 // ---------------------------------------------------------------- balance --
@@ -146,18 +157,23 @@ constexpr int64_t kPairs = 74;
 // one piece's gradient of the logits; at least XE_MIN_PIECE columns
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
 constexpr int64_t kMinPiece = 8192;
+// largest E of the keep way: 16 384 tokens of a 100 277-word vocabulary take
+// 3.3 GB of the GPU's 180 for the length of the call
+constexpr int64_t kKeepBytes = int64_t(4) << 30;
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 struct XentPlan {
   int64_t T, V, d;
   int planes;
+  int tile_n;              // columns of a GEMM tile
+  bool keep;               // the keep way is open
   bool pack_w;             // the table is read through bf16 planes
   int64_t ldd;             // columns of a plane
   int64_t t_pad, v_pad;    // rows of a plane
   int run, runs;           // STATS: column tiles per unit, units along the vocabulary
   int64_t piece;           // DLOGITS, GRADS: columns of a piece
-  int slots;               // K slices of dh
+  int slots, slots_piece;  // K slices of dh: keep way, piece way
   int64_t dh_ld;
 };
 
@@ -167,32 +183,39 @@ XentPlan xent_plan(int64_t T, int64_t V, int64_t d, int dtype) {
   p.V = V;
   p.d = d;
   p.planes = dtype == ETHOS_F32 ? 3 : 1;
+  p.tile_n = p.planes == 1 ? XeCfg<1>::kTileN : XeCfg<3>::kTileN;
   p.pack_w = dtype == ETHOS_F32 || d % 8 != 0;
   p.ldd = up(d, 8);
   p.t_pad = up(T, XE_TILE);
   p.v_pad = up(V, XE_TILE);
-  const int64_t num_m = p.t_pad / XE_TILE, num_n = p.v_pad / XE_TILE;
+  p.keep = p.planes == 1 && p.t_pad * up(V, 64) * 2 <= kKeepBytes;
+  const int64_t num_m = p.t_pad / XE_TILE, num_n = (V + p.tile_n - 1) / p.tile_n;
+  // a unit's columns: long enough to make few pieces of each row, short enough
+  // for six units a pair
   int64_t run = num_m * num_n / (kPairs * 6);
-  p.run = static_cast<int>(run < 1 ? 1 : (run > 16 ? 16 : run));
+  const int64_t most_run = 4096 / p.tile_n;
+  p.run = static_cast<int>(run < 1 ? 1 : (run > most_run ? most_run : run));
   p.runs = static_cast<int>((num_n + p.run - 1) / p.run);
   int64_t most = kPieceBytes / (p.t_pad * 2 * p.planes) / XE_TILE * XE_TILE;
   if (most < kMinPiece) most = kMinPiece;
   const int64_t pieces = (V + most - 1) / most;
   p.piece = up((V + pieces - 1) / pieces, XE_TILE);
   p.dh_ld = up(d, 8);
-  p.slots = 1;
-  if (pieces == 1) {
-    // few row tiles and a long contraction: cut dh's K so that a slice is no
-    // longer than a dW tile's or than a third of a pair's share of the work
-    const int64_t nt = (d + XE_TILE - 1) / XE_TILE;
-    const int64_t kb_h = p.piece / G2_BK, kb_w = (T + G2_BK - 1) / G2_BK;
-    const int64_t share = (num_m * nt * kb_h + num_n * nt * kb_w) / (kPairs * 3);
-    const int64_t target = kb_w > share ? kb_w : share;
+  if (pieces > 1 && !p.keep) {
+    p.slots = 1;
+  } else {
+    // few row tiles and a long contraction: cut dh's K so that a tile's slice
+    // is at most about a third of a pair's share of the whole work
+    const int64_t nt = (d + p.tile_n - 1) / p.tile_n;
+    const int64_t kb_h = (V + G2_BK - 1) / G2_BK, kb_w = (T + G2_BK - 1) / G2_BK;
+    const int64_t share = (num_m * nt * kb_h + p.v_pad / XE_TILE * nt * kb_w) / (kPairs * 3);
+    const int64_t target = share > 8 ? share : 8;
     int64_t s = (kb_h + target - 1) / target;
     if (s > 64) s = 64;
     const int64_t per = (kb_h + s - 1) / s;
     p.slots = static_cast<int>((kb_h + per - 1) / per);
   }
+  p.slots_piece = pieces == 1 ? p.slots : 1;
   return p;
 }
 
@@ -205,8 +228,11 @@ void carve_save(Carve& c, const XentPlan& p, XentSave* s) {
   s->rw.pos = c.take<int>(static_cast<size_t>(p.T));
   s->rw.idx = c.take<int>(static_cast<size_t>(p.t_pad));
   s->rw.yc = c.take<int>(static_cast<size_t>(p.t_pad));
-  s->rw.lse = c.take<float>(static_cast<size_t>(p.t_pad));
   s->rw.lab = c.take<float>(static_cast<size_t>(p.t_pad));
+  s->rw.c = c.take<float>(static_cast<size_t>(p.t_pad));
+  s->rw.lse = c.take<float>(static_cast<size_t>(p.t_pad));
+  s->rw.q = c.take<float>(static_cast<size_t>(p.t_pad));
+  s->rw.r = c.take<float>(static_cast<size_t>(p.t_pad));
   s->hp = c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.t_pad * p.ldd));
 }
 struct XentFwd {
@@ -227,38 +253,83 @@ struct XentBwd {
 void carve_xent_bwd(Carve& c, const XentPlan& p, XentBwd* s) {
   s->wp = p.pack_w ? c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.v_pad * p.ldd)) : nullptr;
   s->dl = c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.t_pad * p.piece));
+  s->dh = c.take<float>(static_cast<size_t>(p.slots_piece * p.t_pad * p.dh_ld));
+}
+struct XentKeep {
+  XentFwd f;
+  int* redo_tile;
+  __nv_bfloat16* e;     // [t_pad][lde]
+  int64_t lde;
+  __nv_bfloat16* hr;    // rows r h
+  float* dh;
+  EmbedScratch sort;
+  float* label_rows;
+};
+void carve_xent_keep(Carve& c, const XentPlan& p, XentKeep* s) {
+  carve_xent_fwd(c, p, &s->f);
+  s->lde = up(p.V, 64);
+  s->redo_tile = c.take<int>(static_cast<size_t>(p.t_pad / XE_TILE));
+  s->e = c.take<__nv_bfloat16>(static_cast<size_t>(p.t_pad * s->lde));
+  s->hr = c.take<__nv_bfloat16>(static_cast<size_t>(p.t_pad * p.ldd));
   s->dh = c.take<float>(static_cast<size_t>(p.slots * p.t_pad * p.dh_ld));
+  carve_embed(c, p.t_pad, p.V, p.d, &s->sort);
+  s->label_rows = c.take<float>(static_cast<size_t>(p.t_pad * p.d));
 }
 
-template <class S, int PLANES>
-int xent_pack(const void* src, int64_t lds, int64_t d, const int* idx, const int* rows, int64_t count,
-              __nv_bfloat16* dst, int64_t plane_rows, int64_t ldd, cudaStream_t sm, const DeviceInfo& dev) {
-  int64_t blocks = (plane_rows * (ldd / 8) + 255) / 256;
+int xent_pack_w(const XentPlan& p, int dtype, const void* weight, int64_t ldw, __nv_bfloat16* wp, cudaStream_t sm,
+                const DeviceInfo& dev) {
+  int64_t blocks = (p.v_pad * (p.ldd / 8) + 255) / 256;
   if (blocks > 16ll * dev.sm_count) blocks = 16ll * dev.sm_count;
-  return launch_pdl(k_xent_pack<S, PLANES>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
-                    static_cast<const S*>(src), lds, static_cast<int>(d), idx, rows, count, dst, plane_rows,
-                    static_cast<int>(ldd));
-}
-int xent_pack_any(int dtype, const void* src, int64_t lds, int64_t d, const int* idx, const int* rows, int64_t count,
-                  __nv_bfloat16* dst, int64_t plane_rows, int64_t ldd, cudaStream_t sm, const DeviceInfo& dev) {
+  const dim3 grid(static_cast<unsigned>(blocks));
+  const int d = static_cast<int>(p.d), ldd = static_cast<int>(p.ldd);
   return dtype == ETHOS_BF16
-             ? xent_pack<__nv_bfloat16, 1>(src, lds, d, idx, rows, count, dst, plane_rows, ldd, sm, dev)
-             : xent_pack<float, 3>(src, lds, d, idx, rows, count, dst, plane_rows, ldd, sm, dev);
+             ? launch_pdl(k_xent_pack<__nv_bfloat16, 1>, grid, dim3(256), 0, sm,
+                          static_cast<const __nv_bfloat16*>(weight), ldw, d, p.V, wp, p.v_pad, ldd)
+             : launch_pdl(k_xent_pack<float, 3>, grid, dim3(256), 0, sm, static_cast<const float*>(weight), ldw, d,
+                          p.V, wp, p.v_pad, ldd);
+}
+
+// The label's logits and, with pack, the packed rows.
+int xent_rows_pass(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, const void* weight,
+                   int64_t ldw, int dtype, bool pack, cudaStream_t sm, const DeviceInfo& dev) {
+  int64_t blocks = ((pack ? p.t_pad : p.T) + 7) / 8;
+  if (blocks > 8ll * dev.sm_count) blocks = 8ll * dev.sm_count;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  __nv_bfloat16* dst = pack ? sv.hp : nullptr;
+  const int d = static_cast<int>(p.d), ldd = static_cast<int>(p.ldd);
+  return dtype == ETHOS_BF16
+             ? launch_pdl(k_xent_rows<__nv_bfloat16, 1>, grid, dim3(256), 0, sm,
+                          static_cast<const __nv_bfloat16*>(hidden), ldh, static_cast<const __nv_bfloat16*>(weight),
+                          ldw, d, sv.rw, dst, p.t_pad, ldd)
+             : launch_pdl(k_xent_rows<float, 3>, grid, dim3(256), 0, sm, static_cast<const float*>(hidden), ldh,
+                          static_cast<const float*>(weight), ldw, d, sv.rw, dst, p.t_pad, ldd);
+}
+
+int xent_index(const XentPlan& p, const XentSave& sv, const void* labels, int labels_i64, int64_t ignore_index,
+               float* loss_rows, int* redo_tile, int* err, cudaStream_t sm) {
+  const bool compact = p.T > XE_ROWS_DIRECT;
+  const int T = static_cast<int>(p.T);
+  return labels_i64 ? launch_pdl(k_xent_index<int64_t>, dim3(1), dim3(1024), 0, sm,
+                                 static_cast<const int64_t*>(labels), T, p.V, ignore_index, compact, sv.rw, loss_rows,
+                                 redo_tile, err)
+                    : launch_pdl(k_xent_index<int32_t>, dim3(1), dim3(1024), 0, sm,
+                                 static_cast<const int32_t*>(labels), T, p.V, ignore_index, compact, sv.rw, loss_rows,
+                                 redo_tile, err);
 }
 
 template <int MODE, int PLANES>
 int launch_xent(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1, const CUtensorMap& b1,
                 const XeArgs& args, int64_t units, int* err, cudaStream_t sm, const DeviceInfo& dev) {
   auto kern = k_xent_gemm<MODE, PLANES>;
-  int st = smem_attr_once(reinterpret_cast<const void*>(kern), XE_SMEM);
+  int st = smem_attr_once(reinterpret_cast<const void*>(kern), xe_smem<PLANES>());
   if (st != ETHOS_OK) return st;
-  int64_t pairs = max_pair_clusters(reinterpret_cast<const void*>(kern), XE_THREADS, XE_SMEM, dev);
+  int64_t pairs = max_pair_clusters(reinterpret_cast<const void*>(kern), XE_THREADS, xe_smem<PLANES>(), dev);
   if (pairs <= 0) return ETHOS_ERR_CUDA;
   if (pairs > units) pairs = units;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(static_cast<unsigned>(XE_THREADS));
-  cfg.dynamicSmemBytes = static_cast<size_t>(XE_SMEM);
+  cfg.dynamicSmemBytes = static_cast<size_t>(xe_smem<PLANES>());
   cfg.stream = sm;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -288,10 +359,59 @@ struct XentRowsOperand {
   int64_t rows, cols, ld, plane_rows;
   bool direct;
 };
-XentRowsOperand xent_rows(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, int dtype) {
-  const bool direct = dtype == ETHOS_BF16 && p.T <= XE_ROWS_DIRECT && p.d % 8 == 0 && ldh % 8 == 0 && aligned16(hidden);
+XentRowsOperand xent_rows(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, int dtype,
+                          bool packed = false) {
+  const bool direct = !packed && dtype == ETHOS_BF16 && p.T <= XE_ROWS_DIRECT && p.d % 8 == 0 && ldh % 8 == 0 && aligned16(hidden);
   if (direct) return XentRowsOperand{hidden, p.T, p.d, ldh, 0, true};
   return XentRowsOperand{sv.hp, p.planes * p.t_pad, p.ldd, p.ldd, p.t_pad, false};
+}
+
+// The logits' GEMM over the whole vocabulary: row statistics, and E (KEEP).
+template <int MODE>
+int xent_logits(const XentPlan& p, const XentSave& sv, const XentRowsOperand& h, const void* weight, int64_t ldw,
+                const XentFwd& ws, __nv_bfloat16* e, int64_t lde, const int* redo_tile, int* err, cudaStream_t sm,
+                const DeviceInfo& dev) {
+  CUtensorMap ta, tb;
+  int st;
+  if ((st = make_tmap_bf16(&ta, h.ptr, h.rows, h.cols, G2_BM, h.ld)) != ETHOS_OK) return st;
+  st = p.pack_w ? make_tmap_bf16(&tb, ws.wp, p.planes * p.v_pad, p.ldd, G2_BM, p.ldd)
+                : make_tmap_bf16(&tb, weight, p.V, p.d, G2_BM, ldw);
+  if (st != ETHOS_OK) return st;
+  XeArgs a = {};
+  a.rw = sv.rw;
+  a.p[0] = XeProduct{static_cast<int>(h.plane_rows), static_cast<int>(p.v_pad), static_cast<int>(p.T),
+                     static_cast<int>(p.V), static_cast<int>(p.d)};
+  a.run = p.run;
+  a.part = ws.part;
+  a.part_ld = p.t_pad;
+  a.redo_tile = redo_tile;
+  a.dl = e;
+  a.ldl = lde;
+  const int64_t units = p.t_pad / XE_TILE * p.runs;
+  if constexpr (MODE == XE_KEEP) return launch_xent<MODE, 1>(ta, tb, ta, tb, a, units, err, sm, dev);
+  else return launch_xent_planes<MODE>(p.planes, ta, tb, ta, tb, a, units, err, sm, dev);
+}
+
+int xent_loss(const XentPlan& p, const XentSave& sv, const XentFwd& ws, bool keep, int reduction, float* loss,
+              cudaStream_t sm) {
+  return launch_pdl(k_xent_loss, dim3(static_cast<unsigned>((p.T + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS)), dim3(256), 0,
+                    sm, sv.rw, static_cast<const float2*>(ws.part), 2 * p.runs, p.t_pad, keep, reduction, loss,
+                    ws.block_sum);
+}
+
+int64_t xent_grad_units(const XentPlan& p, int64_t n, int slots, const XeArgs& g) {
+  const int64_t nt = (p.d + p.tile_n - 1) / p.tile_n;
+  return (g.do_dh ? p.t_pad / XE_TILE * nt * slots : 0) + (g.do_dw ? (n + XE_TILE - 1) / XE_TILE * nt : 0);
+}
+
+template <class D>
+int xent_dhidden(const XentPlan& p, const XentSave& sv, const float* acc, int slots, const float* grad, int reduction,
+                 const void* label_rows, int64_t ldw, void* out, cudaStream_t sm, const DeviceInfo& dev) {
+  int64_t blocks = (p.T * ((p.d + 7) / 8) + 255) / 256;
+  if (blocks > 16ll * dev.sm_count) blocks = 16ll * dev.sm_count;
+  return launch_pdl(k_xent_dhidden<D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm, acc, slots,
+                    p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad, reduction, static_cast<const D*>(label_rows), ldw, p.T,
+                    static_cast<int>(p.d), static_cast<D*>(out));
 }
 
 int xent_check(int64_t tokens, int64_t vocab, int64_t dim, int64_t ldh, int64_t ldw, int dtype, int reduction) {
@@ -349,16 +469,13 @@ int ethos_embedding_backward(const void* ids, int ids_i64, const void* dy, int d
   DeviceInfo* dev = nullptr;
   int st = base_device_info(&dev);
   if (st != ETHOS_OK) return st;
-  st = ids_i64 ? embed_sort<int64_t>(s, ids, tokens, vocab, padding, dev_err, sm, *dev)
-               : embed_sort<int32_t>(s, ids, tokens, vocab, padding, dev_err, sm, *dev);
+  if (padding < 0) padding = EMB_NO_PADDING;
+  st = ids_i64 ? embed_sort<int64_t>(s, ids, tokens, nullptr, vocab, padding, dev_err, sm, *dev)
+               : embed_sort<int32_t>(s, ids, tokens, nullptr, vocab, padding, dev_err, sm, *dev);
   if (st != ETHOS_OK) return st;
   const int d = static_cast<int>(dim);
-  const bool al = aligned16(dy) && aligned16(d_weight);
-  if (dtype == ETHOS_BF16)
-    return al && d % 8 == 0 ? embed_rows<__nv_bfloat16, true>(s, dy, tokens, vocab, d, scale, d_weight, sm, *dev)
-                            : embed_rows<__nv_bfloat16, false>(s, dy, tokens, vocab, d, scale, d_weight, sm, *dev);
-  return al && d % 4 == 0 ? embed_rows<float, true>(s, dy, tokens, vocab, d, scale, d_weight, sm, *dev)
-                          : embed_rows<float, false>(s, dy, tokens, vocab, d, scale, d_weight, sm, *dev);
+  return dtype == ETHOS_BF16 ? embed_table_grad<__nv_bfloat16>(s, dy, tokens, vocab, d, scale, d_weight, sm, *dev)
+                             : embed_table_grad<float>(s, dy, tokens, vocab, d, scale, d_weight, sm, *dev);
 }
 
 size_t ethos_balance_scratch_size(void) { return sizeof(BalScratch); }
@@ -458,40 +575,127 @@ int ethos_xent_forward(const void* hidden, int64_t ldh, const void* weight, int6
   DeviceInfo* dev = nullptr;
   if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
-  const bool compact = tokens > XE_ROWS_DIRECT;
-  float* loss_rows = reduction == XE_NONE ? loss : nullptr;
-  const int T = static_cast<int>(tokens);
-  st = labels_i64 ? launch_pdl(k_xent_index<int64_t>, dim3(1), dim3(1024), 0, sm, static_cast<const int64_t*>(labels),
-                               T, vocab, ignore_index, compact, sv.rw, loss_rows, dev_err)
-                  : launch_pdl(k_xent_index<int32_t>, dim3(1), dim3(1024), 0, sm, static_cast<const int32_t*>(labels),
-                               T, vocab, ignore_index, compact, sv.rw, loss_rows, dev_err);
-  if (st != ETHOS_OK) return st;
+  if ((st = xent_index(p, sv, labels, labels_i64, ignore_index, reduction == XE_NONE ? loss : nullptr, nullptr,
+                       dev_err, sm)) != ETHOS_OK)
+    return st;
   const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype);
-  if (!h.direct &&
-      (st = xent_pack_any(dtype, hidden, ldh, dim, sv.rw.idx, &sv.rw.meta->rows, 0, sv.hp, p.t_pad, p.ldd, sm,
-                          *dev)) != ETHOS_OK)
+  if ((st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, !h.direct, sm, *dev)) != ETHOS_OK) return st;
+  if (p.pack_w && (st = xent_pack_w(p, dtype, weight, ldw, ws.wp, sm, *dev)) != ETHOS_OK) return st;
+  if ((st = xent_logits<XE_STATS>(p, sv, h, weight, ldw, ws, nullptr, 0, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
     return st;
-  if (p.pack_w && (st = xent_pack_any(dtype, weight, ldw, dim, nullptr, nullptr, vocab, ws.wp, p.v_pad, p.ldd, sm,
-                                      *dev)) != ETHOS_OK)
-    return st;
-  CUtensorMap ta, tb;
-  if ((st = make_tmap_bf16(&ta, h.ptr, h.rows, h.cols, G2_BM, h.ld)) != ETHOS_OK) return st;
-  st = p.pack_w ? make_tmap_bf16(&tb, ws.wp, p.planes * p.v_pad, p.ldd, G2_BM, p.ldd)
-                : make_tmap_bf16(&tb, weight, vocab, dim, G2_BM, ldw);
+  return xent_loss(p, sv, ws, false, reduction, loss, sm);
+}
+
+size_t ethos_xent_forward_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype) {
+  if (xent_check(tokens, vocab, dim, dim, dim, dtype, 0) != ETHOS_OK) return 0;
+  const XentPlan p = xent_plan(tokens, vocab, dim, dtype);
+  if (!p.keep) return 0;
+  Carve c{nullptr, 0, 0};
+  XentKeep s;
+  carve_xent_keep(c, p, &s);
+  return c.off + 256;
+}
+
+int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype,
+                                const void* labels, int labels_i64, int64_t ignore_index, int reduction,
+                                int64_t tokens, int64_t vocab, int64_t dim, float* loss, void* save,
+                                size_t save_bytes, void* d_hidden, void* d_weight, void* workspace,
+                                size_t workspace_bytes, int* dev_err, void* stream) {
+  int st = xent_check(tokens, vocab, dim, ldh, ldw, dtype, reduction);
   if (st != ETHOS_OK) return st;
-  XeArgs a = {};
-  a.rw = sv.rw;
-  a.p[0] = XeProduct{static_cast<int>(h.plane_rows), static_cast<int>(p.v_pad), T, static_cast<int>(vocab),
-                     static_cast<int>(dim)};
-  a.run = p.run;
-  a.part = ws.part;
-  a.part_ld = p.t_pad;
-  if ((st = launch_xent_planes<XE_STATS>(p.planes, ta, tb, ta, tb, a, p.t_pad / XE_TILE * p.runs, dev_err, sm,
-                                         *dev)) != ETHOS_OK)
+  if (!hidden || !weight || !labels || !loss || !dev_err || reduction == XE_NONE) return ETHOS_ERR_INVALID_ARG;
+  const XentPlan p = xent_plan(tokens, vocab, dim, dtype);
+  if (!p.keep) return ETHOS_ERR_UNSUPPORTED_SHAPE;
+  Carve cs{static_cast<char*>(save), 0, save_bytes}, cw{static_cast<char*>(workspace), 0, workspace_bytes};
+  XentSave sv;
+  XentKeep ws;
+  carve_save(cs, p, &sv);
+  carve_xent_keep(cw, p, &ws);
+  if (!save || !workspace || cs.off > save_bytes || cw.off > workspace_bytes) return ETHOS_ERR_WORKSPACE;
+  if (!aligned16(save) || !aligned16(workspace)) return ETHOS_ERR_ALIGNMENT;
+  if (!p.pack_w && (ldw % 8 != 0 || !aligned16(weight))) return ETHOS_ERR_ALIGNMENT;
+  DeviceInfo* dev = nullptr;
+  if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
+  cudaStream_t sm = static_cast<cudaStream_t>(stream);
+  const int D = static_cast<int>(dim);
+  if ((st = xent_index(p, sv, labels, labels_i64, ignore_index, nullptr, ws.redo_tile, dev_err, sm)) != ETHOS_OK)
     return st;
-  return launch_pdl(k_xent_loss, dim3(static_cast<unsigned>((tokens + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS)), dim3(256), 0,
-                    sm, sv.rw, static_cast<const float2*>(ws.part), 2 * p.runs, p.t_pad, reduction, loss,
-                    ws.block_sum);
+  if ((st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, true, sm, *dev)) != ETHOS_OK) return st;
+  if (p.pack_w && (st = xent_pack_w(p, dtype, weight, ldw, ws.f.wp, sm, *dev)) != ETHOS_OK) return st;
+  const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype, true);
+  // E and the sums; rows whose shift was too low once more with their maximum
+  if ((st = xent_logits<XE_KEEP>(p, sv, h, weight, ldw, ws.f, ws.e, ws.lde, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
+    return st;
+  const dim3 row_blocks(static_cast<unsigned>((tokens + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS));
+  if ((st = launch_pdl(k_xent_check, row_blocks, dim3(256), 0, sm, sv.rw, static_cast<const float2*>(ws.f.part),
+                       2 * p.runs, p.t_pad, ws.redo_tile)) != ETHOS_OK)
+    return st;
+  if ((st = xent_logits<XE_KEEP>(p, sv, h, weight, ldw, ws.f, ws.e, ws.lde, ws.redo_tile, dev_err, sm, *dev)) !=
+      ETHOS_OK)
+    return st;
+  if ((st = xent_loss(p, sv, ws.f, true, reduction, loss, sm)) != ETHOS_OK) return st;
+  if (!d_hidden && !d_weight) return ETHOS_OK;
+  if (d_weight) {
+    int64_t blocks = (p.t_pad * (p.ldd / 8) + 255) / 256;
+    if (blocks > 8ll * dev->sm_count) blocks = 8ll * dev->sm_count;
+    if ((st = launch_pdl(k_xent_scaled_rows, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
+                         static_cast<const __nv_bfloat16*>(sv.hp), sv.rw, static_cast<int>(p.ldd), ws.hr)) != ETHOS_OK)
+      return st;
+    // label rows of dW: (p[y] - 1) h[t] summed by label
+    if ((st = embed_sort<int32_t>(ws.sort, sv.rw.yc, p.t_pad, &sv.rw.meta->rows, vocab, -1, dev_err, sm, *dev)) !=
+        ETHOS_OK)
+      return st;
+    st = D % 8 == 0 ? embed_rows<__nv_bfloat16, true, float, true>(ws.sort, sv.hp, p.ldd, sv.rw.q, p.t_pad, vocab, D,
+                                                                   1.0f, ws.label_rows, sm, *dev)
+                    : embed_rows<__nv_bfloat16, false, float, true>(ws.sort, sv.hp, p.ldd, sv.rw.q, p.t_pad, vocab, D,
+                                                                    1.0f, ws.label_rows, sm, *dev);
+    if (st != ETHOS_OK) return st;
+  }
+  const void* wptr = p.pack_w ? static_cast<const void*>(ws.f.wp) : weight;
+  const int64_t wld = p.pack_w ? p.ldd : ldw;
+  CUtensorMap ek, em, wk, hb;
+  if ((st = make_tmap_bf16(&ek, ws.e, p.t_pad, ws.lde, G2_BM, ws.lde)) != ETHOS_OK) return st;
+  if ((st = make_tmap_bf16(&em, ws.e, p.t_pad, ws.lde, G2_BK, ws.lde)) != ETHOS_OK) return st;
+  if ((st = make_tmap_bf16(&wk, wptr, p.pack_w ? p.v_pad : vocab, p.pack_w ? p.ldd : dim, G2_BK, wld)) != ETHOS_OK)
+    return st;
+  if ((st = make_tmap_bf16(&hb, ws.hr, p.t_pad, p.ldd, G2_BK, p.ldd)) != ETHOS_OK) return st;
+  const int T = static_cast<int>(tokens), V = static_cast<int>(vocab);
+  XeArgs g = {};
+  g.rw = sv.rw;
+  g.reduction = reduction;
+  g.p[0] = XeProduct{0, 0, T, D, V};
+  g.p[1] = XeProduct{0, 0, V, D, T};
+  g.dh_slots = p.slots;
+  g.dh_acc = ws.dh;
+  g.dh_slot_size = p.t_pad * p.dh_ld;
+  g.dh_ld = p.dh_ld;
+  g.dw = d_weight;
+  g.dw_bf16 = 1;
+  g.label_rows = ws.label_rows;
+  g.label_offs = ws.sort.offs;
+  g.do_dh = d_hidden != nullptr;
+  g.do_dw = d_weight != nullptr;
+  if ((st = launch_xent<XE_GRADS, 1>(ek, wk, em, hb, g, xent_grad_units(p, vocab, p.slots, g), dev_err, sm, *dev)) !=
+      ETHOS_OK)
+    return st;
+  if (!d_hidden) return ETHOS_OK;
+  return xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots, nullptr, reduction, weight, ldw, d_hidden, sm, *dev);
+}
+
+int ethos_xent_scale(const float* factor, void* x, int dtype, int64_t n, void* stream) {
+  if (n < 0 || !known_dtype(dtype)) return ETHOS_ERR_INVALID_ARG;
+  if (n == 0) return ETHOS_OK;
+  if (!factor || !x) return ETHOS_ERR_INVALID_ARG;
+  DeviceInfo* dev = nullptr;
+  const int st = base_device_info(&dev);
+  if (st != ETHOS_OK) return st;
+  int64_t blocks = (n / 8 + 256) / 256;
+  if (blocks > 8ll * dev->sm_count) blocks = 8ll * dev->sm_count;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  cudaStream_t sm = static_cast<cudaStream_t>(stream);
+  return dtype == ETHOS_BF16
+             ? launch_pdl(k_xent_scale<__nv_bfloat16>, grid, dim3(256), 0, sm, factor, static_cast<__nv_bfloat16*>(x), n)
+             : launch_pdl(k_xent_scale<float>, grid, dim3(256), 0, sm, factor, static_cast<float*>(x), n);
 }
 
 int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype, int reduction,
@@ -516,11 +720,9 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
   if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
   const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype);
-  if (p.pack_w && (st = xent_pack_any(dtype, weight, ldw, dim, nullptr, nullptr, vocab, ws.wp, p.v_pad, p.ldd, sm,
-                                      *dev)) != ETHOS_OK)
-    return st;
+  if (p.pack_w && (st = xent_pack_w(p, dtype, weight, ldw, ws.wp, sm, *dev)) != ETHOS_OK) return st;
   const int T = static_cast<int>(tokens), D = static_cast<int>(dim);
-  const int64_t num_m = p.t_pad / XE_TILE, nt = (dim + XE_TILE - 1) / XE_TILE;
+  const int64_t num_m = p.t_pad / XE_TILE;
   const int esz = dtype == ETHOS_BF16 ? 2 : 4;
   CUtensorMap ha, hb;  // rows of hidden, K-major (A of the logits) and MN-major (B of dW)
   if ((st = make_tmap_bf16(&ha, h.ptr, h.rows, h.cols, G2_BM, h.ld)) != ETHOS_OK) return st;
@@ -545,7 +747,7 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     a.dl = ws.dl;
     a.dl_plane_rows = p.t_pad;
     a.ldl = p.piece;
-    if ((st = launch_xent_planes<XE_DLOGITS>(p.planes, ha, wb, ha, wb, a, num_m * ((n + XE_TILE - 1) / XE_TILE),
+    if ((st = launch_xent_planes<XE_DLOGITS>(p.planes, ha, wb, ha, wb, a, num_m * ((n + p.tile_n - 1) / p.tile_n),
                                              dev_err, sm, *dev)) != ETHOS_OK)
       return st;
     XeArgs g = {};
@@ -554,7 +756,7 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     g.reduction = reduction;
     g.p[0] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(p.v_pad), T, D, static_cast<int>(n)};
     g.p[1] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(h.plane_rows), static_cast<int>(n), D, T};
-    g.dh_slots = p.slots;
+    g.dh_slots = p.slots_piece;
     g.dh_accumulate = v0 > 0;
     g.dh_acc = ws.dh;
     g.dh_slot_size = p.t_pad * p.dh_ld;
@@ -563,20 +765,15 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     g.dw_bf16 = dtype == ETHOS_BF16;
     g.do_dh = d_hidden != nullptr;
     g.do_dw = d_weight != nullptr;
-    const int64_t units = (g.do_dh ? num_m * nt * p.slots : 0) + (g.do_dw ? (n + XE_TILE - 1) / XE_TILE * nt : 0);
+    const int64_t units = xent_grad_units(p, n, p.slots_piece, g);
     if ((st = launch_xent_planes<XE_GRADS>(p.planes, dk, wk, dm, hb, g, units, dev_err, sm, *dev)) != ETHOS_OK)
       return st;
   }
   if (!d_hidden) return ETHOS_OK;
-  int64_t blocks = (tokens * ((dim + 3) / 4) + 255) / 256;
-  if (blocks > 16ll * dev->sm_count) blocks = 16ll * dev->sm_count;
-  return dtype == ETHOS_BF16
-             ? launch_pdl(k_xent_dhidden<__nv_bfloat16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
-                          static_cast<const float*>(ws.dh), p.slots, p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad,
-                          reduction, tokens, D, static_cast<__nv_bfloat16*>(d_hidden))
-             : launch_pdl(k_xent_dhidden<float>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
-                          static_cast<const float*>(ws.dh), p.slots, p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad,
-                          reduction, tokens, D, static_cast<float*>(d_hidden));
+  return dtype == ETHOS_BF16 ? xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots_piece, grad, reduction, nullptr, 0,
+                                                           d_hidden, sm, *dev)
+                             : xent_dhidden<float>(p, sv, ws.dh, p.slots_piece, grad, reduction, nullptr, 0, d_hidden,
+                                                   sm, *dev);
 }
 
 }  // extern "C"

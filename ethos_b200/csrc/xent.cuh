@@ -6,50 +6,71 @@
 //   dl[t, v] = g[t] (exp(l[t, v] - lse[t]) - [v = y[t]])
 //   dh = dl W,   dW = dl^T h
 //
-// forward: one GEMM whose epilogue keeps, for each row, the running maximum and
-// the sum of exponentials over the tiles it sees, and picks the label's logit;
-// a second kernel joins the pieces of each row.  backward: for one piece of
-// the vocabulary after another, the logits are formed again, their gradient
-// goes to a [tokens, piece] bf16 buffer straight from the accumulators, and
-// one launch computes both products with it.  Four products of 2 T V d FLOPs,
-// bounded by the tensor cores; memory beyond inputs and outputs is one piece.
+// The label's column stays out of the exponentials: c = l[t, y] is a dot
+// product in fp32, and with S = sum_{v != y} exp(l[t, v] - c)
+//   loss = log(1 + S),  1 - p[y] = S / (1 + S),
+// so that a confident token's loss and gradient are not differences of nearly
+// equal numbers.
+//
+// Two ways, by what the caller needs:
+//
+//  keep    (bf16; loss and gradients in one call, for a gradient of the loss
+//          that is one number).  The GEMM's epilogue writes E = exp(l - c) of
+//          every other column as bf16 while it adds up S.  With r = 1/(1 + S)
+//          a row of p is r E, and the two products read E as it is:
+//            dh = r (E W) + (p[y] - 1) W[y],   dW = E^T (r h) + label rows,
+//          where row v of the label rows is the sum of (p[y] - 1) h[t] over the
+//          tokens with label v, in fp32, by the sort of embed.cuh.  Three
+//          products of 2 T V d FLOPs.  A row whose logits pass c by more than
+//          XE_KEEP_RANGE is done again with its largest logit for c.
+//  piece   (everything else).  The forward keeps, for each row, the running
+//          maximum and sum over the tiles it sees.  The backward forms the
+//          logits again, one piece of the vocabulary after another; their
+//          gradient goes to a [tokens, piece] bf16 buffer straight from the
+//          accumulators, and one launch computes both products with it.  Four
+//          products.
+//
+// Both are bounded by the tensor cores.
 //
 // Rows.  With more than XE_ROWS_DIRECT tokens the tokens that are not ignored
 // are packed first (their number stays on the device), so ignored tokens cost
 // nothing after that; fewer fit one row tile and keep their places.
 //
-// Types.  bf16: operands as they are; dl is rounded to bf16 (the operand type
-// of the two products), sums are fp32.  fp32: operands, and dl, are carried
-// as three bf16 planes whose sum is the fp32 value, and each product is six
-// plane products, the smallest first, with a fresh accumulator every
-// XE_FLUSH_KB blocks of 64 (the accumulator of the matrix unit loses about
-// half an ulp of the running sum per step), added up in fp32.
+// Types.  bf16: operands as they are; E (or dl) and r h are rounded to bf16,
+// the operand type of the products; sums are fp32.  fp32: operands, and dl, are
+// carried as three bf16 planes whose sum is the fp32 value, and each product is
+// six plane products, the smallest first, with a fresh accumulator every
+// XE_STEP_KB blocks of 64 (the accumulator of the matrix unit loses about half
+// an ulp of the running sum per step), added up in fp32.
 //
-// GEMM: k_xent_gemm runs on SM pairs as k_gemm2sm does (256 x 256 tile, each
-// CTA staging 128 rows of A and of B, cta_group::2 MMA, two accumulators in
-// TMEM, no multicast loads), with row counts read from the device, ragged M,
-// N and K, and units grouped so that the operand shared by concurrent pairs
-// stays in L2.
+// GEMM: k_xent_gemm runs on SM pairs as k_gemm2sm does (each CTA staging 128
+// rows of A and of each 256 of B, cta_group::2 MMA, no multicast loads), with
+// row counts read from the device, ragged M, N and K, and units grouped so that
+// the operand shared by concurrent pairs stays in L2.  bf16 tiles are 256 x
+// 512: both accumulators of the pair read one A tile, a quarter fewer operand
+// bytes per product than 256 x 256, whose feed from L2 bounded it.
 #pragma once
 
+#include "embed.cuh"
 #include "gemm2sm.cuh"
 
 namespace ethos {
 
 constexpr int XE_ROWS_DIRECT = 256;  // tokens that keep their places (one row tile)
-constexpr int XE_TILE = 256;         // tile rows and columns of an SM pair
+constexpr int XE_TILE = 256;         // rows of a pair's tile; columns of one accumulator
 constexpr int XE_GROUP_M = 64;       // row tiles walked before the next column tile
-constexpr int XE_FLUSH_KB = 8;       // fp32: K blocks of 64 per accumulator in the gradient products
-constexpr int XE_STG_WARP_BYTES = 32 * 64;
+constexpr int XE_STEP_KB = 8;        // fp32: K blocks of 64 per accumulation
 constexpr float XE_LOG2E = 1.4426950408889634f;
+constexpr float XE_KEEP_RANGE = 60.0f;  // e^60 times any sum over a vocabulary is finite in fp32 and bf16
 
-enum XeMode { XE_STATS, XE_DLOGITS, XE_GRADS };
+enum XeMode { XE_STATS, XE_KEEP, XE_DLOGITS, XE_GRADS };
 
 // What the forward leaves for the backward, at the start of the save buffer.
 struct XeMeta {
   int rows;       // rows of the packed problem
   int valid;      // tokens that are not ignored
   unsigned done;  // blocks of k_xent_loss that have added their part
+  int redo;       // KEEP: some row's shift was too low
 };
 
 // Row index, compacted: pos[t] = row of token t or -1, idx[r] = token of row
@@ -59,17 +80,23 @@ struct XeRows {
   int* pos;
   int* idx;
   int* yc;
-  float* lse;
   float* lab;  // the label's logit
+  float* c;    // KEEP: shift of the row's exponents
+  float* lse;
+  float* q;    // p[y] - 1
+  float* r;    // KEEP: 1 / sum of exp(l - c)
 };
 
 template <class I>
 __global__ void __launch_bounds__(1024) k_xent_index(const I* __restrict__ labels, int tokens, int64_t vocab,
                                                      int64_t ignore, bool compact, XeRows rw,
-                                                     float* __restrict__ loss_rows, int* err) {
+                                                     float* __restrict__ loss_rows, int* __restrict__ redo_tile,
+                                                     int* err) {
   __shared__ int warp_sum[32];
   pdl_launch_dependents();
   pdl_wait();
+  if (redo_tile != nullptr)
+    for (int i = threadIdx.x; i < (tokens + XE_TILE - 1) / XE_TILE; i += 1024) redo_tile[i] = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int base = 0;
   for (int t0 = 0; t0 < tokens; t0 += 1024) {
@@ -109,67 +136,114 @@ __global__ void __launch_bounds__(1024) k_xent_index(const I* __restrict__ label
     rw.meta->rows = compact ? base : tokens;
     rw.meta->valid = base;
     rw.meta->done = 0;
+    rw.meta->redo = 0;
   }
 }
 
 // ------------------------------------------------------------------- pack --
-// dst [PLANES][plane_rows][ldd] bf16 <- rows of src: plane 0 = bf16(v), plane
-// 1 = bf16(v - plane 0), plane 2 the rest.  With idx, row r is src[idx[r]] for
-// r < *rows, and rows up to the next multiple of XE_TILE are zero; without,
-// rows 0..count-1 and zeros up to plane_rows.  Columns d..ldd are zero.
+// 8 consecutive elements of a row as fp32 (columns from d on are zero)
+template <class S>
+__device__ __forceinline__ void load8(const S* s, int c, int d, bool vec, float (&v)[8]) {
+  if (vec && c + 8 <= d) {
+    if constexpr (sizeof(S) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(s + c), b = *reinterpret_cast<const float4*>(s + c + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(s + c);
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = __bfloat1622float2(h[j]);
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < d ? static_cast<float>(s[c + j]) : 0.0f;
+  }
+}
+// the leading bf16 part of 8 values, which is taken off them
+__device__ __forceinline__ uint4 take_plane(float (&v)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    const float2 f = __bfloat1622float2(h);
+    v[2 * j] -= f.x;
+    v[2 * j + 1] -= f.y;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <class S>
+__device__ __forceinline__ bool rows_vec(const S* p, int64_t ld) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % static_cast<int64_t>(16 / sizeof(S)) == 0;
+}
+
+// dst [PLANES][plane_rows][ldd] bf16 <- rows of src (the vocabulary): plane 0 =
+// bf16(v), plane 1 = bf16(v - plane 0), plane 2 the rest; columns d..ldd and
+// rows count..plane_rows are zero.
 template <class S, int PLANES>
-__global__ void __launch_bounds__(256) k_xent_pack(const S* __restrict__ src, int64_t lds, int d,
-                                                   const int* __restrict__ idx, const int* __restrict__ rows,
-                                                   int64_t count, __nv_bfloat16* __restrict__ dst, int64_t plane_rows,
-                                                   int ldd) {
+__global__ void __launch_bounds__(256) k_xent_pack(const S* __restrict__ src, int64_t lds, int d, int64_t count,
+                                                   __nv_bfloat16* __restrict__ dst, int64_t plane_rows, int ldd) {
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t n = rows != nullptr ? *rows : count;
-  const int64_t n_pad = rows != nullptr ? (n + XE_TILE - 1) / XE_TILE * XE_TILE : plane_rows;
   const int pieces = ldd / 8;
-  const int64_t total = n_pad * pieces;
-  const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0 && lds % (16 / sizeof(S)) == 0;
+  const int64_t total = plane_rows * pieces;
+  const bool vec = rows_vec(src, lds);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t r = i / pieces;
     const int c = static_cast<int>(i - r * pieces) * 8;
-    float v[8];
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r < count) load8(src + r * lds, c, d, vec, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    if (r < n) {
-      const S* s = src + (idx != nullptr ? static_cast<int64_t>(idx[r]) : r) * lds + c;
-      if (vec && c + 8 <= d) {
-        if constexpr (sizeof(S) == 4) {
-          const float4 a = reinterpret_cast<const float4*>(s)[0], b = reinterpret_cast<const float4*>(s)[1];
-          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4*>(s);
-          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    for (int p = 0; p < PLANES; ++p)
+      *reinterpret_cast<uint4*>(dst + (p * plane_rows + r) * ldd + c) = take_plane(v);
+  }
+}
+
+// One warp per row of the packed problem: the label's logit in fp32, and (dst
+// not null) the row's planes; rows up to the next multiple of XE_TILE are
+// zero.
+template <class S, int PLANES>
+__global__ void __launch_bounds__(256) k_xent_rows(const S* __restrict__ hidden, int64_t ldh,
+                                                   const S* __restrict__ weight, int64_t ldw, int d, XeRows rw,
+                                                   __nv_bfloat16* __restrict__ dst, int64_t plane_rows, int ldd) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int rows = rw.meta->rows;
+  const int upto = dst != nullptr ? (rows + XE_TILE - 1) / XE_TILE * XE_TILE : rows;
+  const bool hvec = rows_vec(hidden, ldh), wvec = rows_vec(weight, ldw);
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < upto; r += gridDim.x * 8) {
+    const bool in = r < rows;
+    const S* h = hidden + (in ? static_cast<int64_t>(rw.idx[r]) : 0) * ldh;
+    const int y = in ? rw.yc[r] : -1;
+    const S* w = weight + static_cast<int64_t>(y < 0 ? 0 : y) * ldw;
+    float dot = 0.0f;
+#pragma unroll 2
+    for (int c = lane * 8; c < ldd; c += 256) {
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (in) load8(h, c, d, hvec, v);
+      if (y >= 0) {
+        float x[8];
+        load8(w, c, d, wvec, x);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = __bfloat1622float2(h[j]);
-            v[2 * j] = f.x;
-            v[2 * j + 1] = f.y;
-          }
-        }
-      } else {
+        for (int j = 0; j < 8; ++j) dot = fmaf(v[j], x[j], dot);
+      }
+      if (dst != nullptr) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c + j < d) v[j] = static_cast<float>(s[j]);
+        for (int p = 0; p < PLANES; ++p)
+          *reinterpret_cast<uint4*>(dst + (p * plane_rows + r) * ldd + c) = take_plane(v);
       }
     }
 #pragma unroll
-    for (int p = 0; p < PLANES; ++p) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        const float2 f = __bfloat1622float2(h);
-        v[2 * j] -= f.x;
-        v[2 * j + 1] -= f.y;
-      }
-      *reinterpret_cast<uint4*>(dst + (p * plane_rows + r) * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (in && lane == 0) {
+      rw.lab[r] = dot;
+      rw.c[r] = dot;
     }
   }
 }
@@ -191,42 +265,87 @@ __device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2)
   m = hi;
 }
 
-__global__ void __launch_bounds__(256) k_xent_loss(XeRows rw, const float2* __restrict__ part, int parts,
-                                                   int64_t part_ld, int reduction, float* __restrict__ loss,
-                                                   double* __restrict__ block_sum) {
-  __shared__ double red[256];
-  __shared__ bool last;
-  pdl_launch_dependents();
-  pdl_wait();
+// (maximum, sum) of one row over all its pieces (without the label's column):
+// valid in threads 0..7, which hold rows blockIdx.x * 8 + threadIdx.x
+template <class Join>
+__device__ __forceinline__ void join_parts(const float2* __restrict__ part, int parts, int64_t part_ld, int rows,
+                                           float& m, float& s, Join join) {
+  __shared__ float2 wp[8][XE_LOSS_ROWS];
   const int row = blockIdx.x * XE_LOSS_ROWS + (threadIdx.x & (XE_LOSS_ROWS - 1));
-  const int py = threadIdx.x / XE_LOSS_ROWS;  // 0..31
-  const int rows = rw.meta->rows;
-  float m = -INFINITY, s = 0.0f;
+  m = -INFINITY;
+  s = 0.0f;
   if (row < rows) {
 #pragma unroll 4
-    for (int p = py; p < parts; p += 32) {
+    for (int p = threadIdx.x / XE_LOSS_ROWS; p < parts; p += 32) {
       const float2 v = part[p * part_ld + row];
-      lse_join(m, s, v.x, v.y);
+      join(m, s, v.x, v.y);
     }
   }
   // lanes of a warp hold 4 pieces of each of 8 rows; then over the 8 warps
 #pragma unroll
   for (int o = 16; o >= XE_LOSS_ROWS; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    lse_join(m, s, m2, s2);
+    join(m, s, m2, s2);
   }
-  __shared__ float2 wp[8][XE_LOSS_ROWS];
   if ((threadIdx.x & 31) < XE_LOSS_ROWS) wp[threadIdx.x >> 5][threadIdx.x & 31] = make_float2(m, s);
   __syncthreads();
+  if (threadIdx.x < XE_LOSS_ROWS)
+    for (int w = 1; w < 8; ++w) join(m, s, wp[w][threadIdx.x].x, wp[w][threadIdx.x].y);
+}
+struct JoinMax {  // KEEP: sums share the row's shift
+  __device__ __forceinline__ void operator()(float& m, float& s, float m2, float s2) const {
+    m = fmaxf(m, m2);
+    s += s2;
+  }
+};
+struct JoinLse {
+  __device__ __forceinline__ void operator()(float& m, float& s, float m2, float s2) const { lse_join(m, s, m2, s2); }
+};
+
+// KEEP: rows whose logits pass the shift by more than XE_KEEP_RANGE take their
+// maximum for it; redo_tile marks their row tiles, which k_xent_gemm then does
+// again.
+__global__ void __launch_bounds__(256) k_xent_check(XeRows rw, const float2* __restrict__ part, int parts,
+                                                    int64_t part_ld, int* __restrict__ redo_tile) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rows = rw.meta->rows;
+  float m, s;
+  join_parts(part, parts, part_ld, rows, m, s, JoinMax());
+  const int row = blockIdx.x * XE_LOSS_ROWS + threadIdx.x;
+  if (threadIdx.x < XE_LOSS_ROWS && row < rows && rw.yc[row] >= 0 && m - rw.c[row] > XE_KEEP_RANGE) {
+    rw.c[row] = m;
+    redo_tile[row / XE_TILE] = 1;  // any writer writes the same
+    rw.meta->redo = 1;
+  }
+}
+
+__global__ void __launch_bounds__(256) k_xent_loss(XeRows rw, const float2* __restrict__ part, int parts,
+                                                   int64_t part_ld, bool keep, int reduction,
+                                                   float* __restrict__ loss, double* __restrict__ block_sum) {
+  __shared__ double red[256];
+  __shared__ bool last;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rows = rw.meta->rows;
+  float m, s;
+  if (keep) join_parts(part, parts, part_ld, rows, m, s, JoinMax());
+  else join_parts(part, parts, part_ld, rows, m, s, JoinLse());
+  const int row = blockIdx.x * XE_LOSS_ROWS + threadIdx.x;
   double mine = 0.0;
   if (threadIdx.x < XE_LOSS_ROWS && row < rows) {
-    for (int w = 1; w < 8; ++w) lse_join(m, s, wp[w][threadIdx.x].x, wp[w][threadIdx.x].y);
-    const float lse = m + logf(s);
-    rw.lse[row] = lse;
+    const float l = rw.lab[row];
+    const float c = keep ? rw.c[row] : fmaxf(m, l);
+    // s: sum of exp(l[v] - c) over the other columns; b: the label's own
+    if (!keep && m != c) s *= expf(m - c);  // m < c = l (m is -inf when there is no other column)
+    const float b = c == l ? 1.0f : expf(l - c);
+    const float v = c == l ? log1pf(s) : (c - l) + logf(s + b);
+    rw.lse[row] = l + v;
+    rw.q[row] = -s / (s + b);
+    rw.r[row] = 1.0f / (s + b);
     if (rw.yc[row] >= 0) {
-      const float l = lse - rw.lab[row];
-      if (reduction == XE_NONE) loss[rw.idx[row]] = l;
-      mine = static_cast<double>(l);
+      if (reduction == XE_NONE) loss[rw.idx[row]] = v;
+      mine = static_cast<double>(v);
     }
   }
   if (reduction == XE_NONE) return;
@@ -255,50 +374,112 @@ __global__ void __launch_bounds__(256) k_xent_loss(XeRows rw, const float2* __re
   if (threadIdx.x == 0) *loss = static_cast<float>(reduction == XE_MEAN ? red[0] / rw.meta->valid : red[0]);
 }
 
+// KEEP: rows r h of the packed rows hp, rounded to bf16 (the second operand
+// of dW); zero rows stay zero.
+__global__ void __launch_bounds__(256) k_xent_scaled_rows(const __nv_bfloat16* __restrict__ hp, XeRows rw, int ldd,
+                                                          __nv_bfloat16* __restrict__ out) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rows = rw.meta->rows;
+  const int64_t upto = (rows + XE_TILE - 1) / XE_TILE * XE_TILE;
+  const int pieces = ldd / 8;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < upto * pieces;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = i / pieces;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row < rows && rw.yc[row] >= 0) {
+      Vec16<__nv_bfloat16>::load(hp + i * 8, v);
+      const float f = rw.r[row];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= f;
+    }
+    Vec16<__nv_bfloat16>::store(out + i * 8, v);
+  }
+}
+
 // -------------------------------------------------------------- dh output --
-// d_hidden[t] = scale * (sum over slots of acc[slot][pos[t]]), zero for an
-// ignored token.
+// The loss's gradient as a factor of the rows' gradients (NONE: in dl already)
+__device__ __forceinline__ float xe_scale(const XeRows& rw, const float* grad, int reduction) {
+  if (reduction == XE_NONE) return 1.0f;
+  const float g = grad != nullptr ? *grad : 1.0f;
+  const int valid = rw.meta->valid;
+  return reduction == XE_SUM ? g : (valid > 0 ? g / valid : 0.0f);
+}
+
+// d_hidden[t] = scale * (f sum over slots of acc[slot][pos[t]] + e W[y]), zero
+// for an ignored token; KEEP: f = r, e = p[y] - 1, else f = 1, e = 0.
 template <class D>
 __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ acc, int slots, int64_t slot_size,
                                                       int64_t lda, XeRows rw, const float* __restrict__ grad,
-                                                      int reduction, int64_t tokens, int d, D* __restrict__ out) {
+                                                      int reduction, const D* __restrict__ label_rows, int64_t ldw,
+                                                      int64_t tokens, int d, D* __restrict__ out) {
   pdl_launch_dependents();
   pdl_wait();
-  const float scale = reduction == XE_NONE ? 1.0f : (reduction == XE_SUM ? *grad : *grad / rw.meta->valid);
-  const int pieces = (d + 3) / 4;
+  const float scale = xe_scale(rw, grad, reduction);
+  const int pieces = (d + 7) / 8;
   const int64_t total = tokens * pieces;
-  const bool vec = d % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  const bool vec = d % 8 == 0 && rows_vec(out, d);
+  const bool wvec = label_rows != nullptr && rows_vec(label_rows, ldw);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t t = i / pieces;
-    const int c = static_cast<int>(i - t * pieces) * 4;
+    const int c = static_cast<int>(i - t * pieces) * 8;
     const int r = rw.pos[t];
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (r >= 0) {
       const float* a = acc + static_cast<int64_t>(r) * lda + c;
-#pragma unroll 4
+#pragma unroll 2
       for (int s = 0; s < slots; ++s) {
         const float4 x = *reinterpret_cast<const float4*>(a + s * slot_size);
-        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+        const float4 y = *reinterpret_cast<const float4*>(a + s * slot_size + 4);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
       }
-      v.x *= scale; v.y *= scale; v.z *= scale; v.w *= scale;
+      if (label_rows != nullptr) {
+        const float f = rw.r[r], e = rw.q[r];
+        float w[8];
+        load8(label_rows + static_cast<int64_t>(rw.yc[r]) * ldw, c, d, wvec, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = fmaf(v[j], f, e * w[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= scale;
     }
     D* o = out + t * d + c;
     if (vec) {
-      if constexpr (sizeof(D) == 4) {
-        *reinterpret_cast<float4*>(o) = v;
-      } else {
-        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-      }
+      store_row<D, true>(o, v);
     } else {
-      const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c + j < d) {
-          if constexpr (sizeof(D) == 4) o[j] = e[j];
-          else o[j] = __float2bfloat16_rn(e[j]);
-        }
+      for (int j = 0; j < 8; ++j) {
+        const float e[1] = {v[j]};
+        if (c + j < d) RowAccess<D, false>::store(o + j, e);
+      }
     }
+  }
+}
+
+// x *= *factor, unless it is 1 (the gradients of the KEEP way are those of a
+// loss whose own gradient is 1)
+template <class D>
+__global__ void __launch_bounds__(256) k_xent_scale(const float* __restrict__ factor, D* __restrict__ x, int64_t n) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const float f = *factor;
+  if (f == 1.0f) return;
+  constexpr int N = Vec16<D>::N;
+  const int64_t nv = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 ? n / N : 0;
+  const int64_t tid = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t nt = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = tid; i < nv; i += nt) {
+    float v[N];
+    Vec16<D>::load(x + i * N, v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] *= f;
+    Vec16<D>::store(x + i * N, v);
+  }
+  for (int64_t i = nv * N + tid; i < n; i += nt) {
+    const float v[1] = {static_cast<float>(x[i]) * f};
+    RowAccess<D, false>::store(x + i, v);
   }
 }
 
@@ -312,13 +493,14 @@ struct XeProduct {
 
 struct XeArgs {
   XeRows rw;
-  XeProduct p[2];  // STATS, DLOGITS: p[0]; GRADS: p[0] = dh, p[1] = dW
-  // STATS
+  XeProduct p[2];  // STATS, KEEP, DLOGITS: p[0]; GRADS: p[0] = dh, p[1] = dW
+  // STATS, KEEP: (maximum, sum) of each row over a unit's columns
   int run;  // column tiles per unit
   float2* part;
   int64_t part_ld;
-  // DLOGITS: gradient of the logits of columns [v0, v0 + N) into
-  // dl [PLANES][dl_plane_rows][ldl]
+  const int* redo_tile;  // KEEP, second launch: only the row tiles marked here
+  // KEEP: E; DLOGITS: gradient of the logits of columns [v0, v0 + N);
+  // [PLANES][dl_plane_rows][ldl], columns up to a multiple of 64 written
   int v0;
   const float* grad;
   int reduction;
@@ -333,12 +515,27 @@ struct XeArgs {
   int64_t dh_ld;
   void* dw;            // rows of this piece, [N rows][d] with pitch d
   int dw_bf16;
+  const float* label_rows;  // added to dW before scaling: row v's is label_rows[label_offs[v]]
+  const int* label_offs;    // where label_offs[v] < label_offs[v + 1]
   int do_dh, do_dw;
 };
 
+template <int PLANES>
+struct XeCfg {
+  // bf16: two accumulators side by side read one A tile; fp32: one, so that
+  // the epilogue can add up accumulations in registers
+  static constexpr int kHalves = PLANES == 1 ? 2 : 1;
+  static constexpr int kTileN = XE_TILE * kHalves;
+  static constexpr int kStageBytes = G2_A_BYTES + kHalves * G2_B_BYTES;
+  static constexpr int kStages = PLANES == 1 ? 4 : 6;
+  // blocks by which the second accumulator's MMAs follow the first's: while
+  // it finishes a tile the epilogue empties the first accumulator
+  static constexpr int kLag = 2;
+  static constexpr int kSegs = PLANES == 1 ? 1 : 6;
+};
 struct XeCtl {
-  uint64_t full[G2_STAGES];
-  uint64_t empty[G2_STAGES];
+  uint64_t full[6];
+  uint64_t empty[6];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t drain;
@@ -347,15 +544,19 @@ struct XeCtl {
 };
 constexpr int XE_EPI_WARPS = 8;
 constexpr int XE_THREADS = 64 + 32 * XE_EPI_WARPS;
-constexpr int XE_SMEM = G2_STAGES * G2_STAGE_BYTES + XE_EPI_WARPS * XE_STG_WARP_BYTES + 1024 +
-                        static_cast<int>(sizeof(XeCtl));
-static_assert(XE_SMEM <= 227 * 1024, "shared memory");
+template <int PLANES>
+constexpr int xe_smem() {
+  return XeCfg<PLANES>::kStages * XeCfg<PLANES>::kStageBytes + 1024 + static_cast<int>(sizeof(XeCtl));
+}
+static_assert(xe_smem<1>() <= 227 * 1024 && xe_smem<3>() <= 227 * 1024, "shared memory");
 
 // One accumulation: tile at (m0, n0) of product `prod`, K blocks [kb0, kb1)
 // over all plane products.
 struct XeStep {
   int prod, m0, n0, kb0, kb1;
-  bool first, last;  // of its unit
+  bool first, last;      // of its unit
+  bool kfirst, klast;    // of its tile
+  bool second;           // the tile has columns in the second accumulator
   int slot;
 };
 
@@ -363,87 +564,121 @@ struct XeStep {
 // CTAs walks the same sequence.
 template <int MODE, int PLANES>
 struct XeWalk {
+  static constexpr int TN = XeCfg<PLANES>::kTileN;
   const XeArgs& a;
-  int rows, num_m, num_n, nkb, units0, units, u, stride;
-  int j;           // accumulation within the unit
-  int mt_w, kb_w;  // GRADS: row tiles and K blocks of dW
+  int num_m, num_n, nkb, pair, pairs;
+  int u;           // unit (its number among the pair's units in GRADS)
+  int units;       // units of the launch (of the pair in GRADS)
+  int c, j;        // column tile and accumulation within the unit
+  int cols;        // STATS, KEEP: units along the columns; DLOGITS: column tiles
+  int kb_w;        // GRADS: K blocks of dW
   int kb_slot;     // GRADS: K blocks of dh per slot
-  __device__ XeWalk(const XeArgs& args, int rows_, int pair, int pairs)
-      : a(args), rows(rows_), u(pair), stride(pairs), j(0) {
+  int long_units, my_long, short0, short_step;
+  __device__ XeWalk(const XeArgs& args, int rows, int pair_, int pairs_) : a(args), pair(pair_), pairs(pairs_) {
     num_m = (rows + XE_TILE - 1) / XE_TILE;
-    num_n = (a.p[0].N + XE_TILE - 1) / XE_TILE;
+    num_n = (a.p[0].N + TN - 1) / TN;
     nkb = (a.p[0].K + G2_BK - 1) / G2_BK;
-    mt_w = kb_w = kb_slot = 0;
-    if (MODE == XE_STATS) {
-      units0 = units = num_m * ((num_n + a.run - 1) / a.run);
-    } else if (MODE == XE_DLOGITS) {
-      units0 = units = num_m * num_n;
-    } else {
-      kb_slot = (nkb + a.dh_slots - 1) / a.dh_slots;
-      units0 = a.do_dh ? num_m * num_n * a.dh_slots : 0;
-      mt_w = (a.p[1].M + XE_TILE - 1) / XE_TILE;
-      kb_w = (rows + G2_BK - 1) / G2_BK;
-      units = units0 + (a.do_dw ? mt_w * num_n : 0);
+    c = j = 0;
+    if (MODE != XE_GRADS) {
+      cols = MODE == XE_DLOGITS ? num_n : (num_n + a.run - 1) / a.run;
+      u = pair;
+      units = num_m * cols;
+      return;
     }
+    // dh tiles (long_units of them, kb_slot blocks each) in turn; then dW
+    // tiles (kb_w blocks each), fewer to the pairs that had one dh tile more
+    kb_slot = (nkb + a.dh_slots - 1) / a.dh_slots;
+    long_units = a.do_dh ? num_m * num_n * a.dh_slots : 0;
+    kb_w = (rows + G2_BK - 1) / G2_BK;
+    const int n2 = a.do_dw ? (a.p[1].M + XE_TILE - 1) / XE_TILE * num_n : 0;
+    const int extra = long_units % pairs;
+    my_long = long_units / pairs + (pair < extra ? 1 : 0);
+    const int diff = kb_w > 0 ? kb_slot / kb_w : 0;  // dW tiles that one dh tile is worth
+    int na = (n2 - diff * (pairs - extra) + pairs - 1) / pairs;
+    if (extra == 0 || na < 0) na = 0;
+    if (na * extra > n2) na = n2 / extra;
+    // pairs [0, extra) take na each, the others share the rest
+    const int rest = n2 - na * extra;
+    int mine;
+    if (pair < extra) {
+      mine = na;
+      short0 = pair;
+      short_step = extra;
+    } else {
+      const int others = pairs - extra;
+      mine = (rest - (pair - extra) + others - 1) / others;
+      short0 = na * extra + (pair - extra);
+      short_step = others;
+    }
+    u = 0;
+    units = my_long + (mine > 0 ? mine : 0);
   }
   // the next accumulation; false when the pair's units are done
   __device__ bool next(XeStep& s) {
-    if (u >= units) return false;
-    int steps;
-    s.slot = 0;
-    if (MODE == XE_STATS || MODE == XE_DLOGITS) {
-      // row tiles in groups of XE_GROUP_M, all columns of a group before the
-      // next: A's group and one column tile of B (or a run of them) in L2
-      const int cols = MODE == XE_STATS ? (num_n + a.run - 1) / a.run : num_n;
-      const int per_group = XE_GROUP_M * cols;
-      const int g = u / per_group;
-      const int gm = min(XE_GROUP_M, num_m - g * XE_GROUP_M);
-      const int v = u - g * per_group;
-      const int c = v / gm;
+    while (true) {
+      if (u >= units) return false;
+      int steps = 1, ntiles = 1;
+      s.slot = 0;
       s.prod = 0;
-      s.m0 = (g * XE_GROUP_M + v % gm) * XE_TILE;
-      s.kb0 = 0;
-      s.kb1 = nkb;
-      if (MODE == XE_STATS) {
-        steps = min(a.run, num_n - c * a.run);
-        s.n0 = (c * a.run + j) * XE_TILE;
-        s.slot = c;
-      } else {
-        steps = 1;
-        s.n0 = c * XE_TILE;
-      }
-    } else {
-      int kb0, kb1;
-      if (u < units0) {
-        const int t = u % (num_m * num_n);
-        s.slot = u / (num_m * num_n);
-        s.prod = 0;
+      int kb0 = 0, kb1 = nkb;
+      if (MODE != XE_GRADS) {
+        // row tiles in groups of XE_GROUP_M, all columns of a group before the
+        // next: A's group and one column tile of B (or a run of them) in L2
+        const int per_group = XE_GROUP_M * cols;
+        const int g = u / per_group;
+        const int gm = min(XE_GROUP_M, num_m - g * XE_GROUP_M);
+        const int v = u - g * per_group;
+        const int cu = v / gm;
+        const int mt = g * XE_GROUP_M + v % gm;
+        if (MODE == XE_KEEP && a.redo_tile != nullptr && !a.redo_tile[mt]) {
+          u += pairs;
+          continue;
+        }
+        s.m0 = mt * XE_TILE;
+        if (MODE == XE_DLOGITS) {
+          s.n0 = cu * TN;
+        } else {
+          ntiles = min(a.run, num_n - cu * a.run);
+          s.n0 = (cu * a.run + c) * TN;
+          s.slot = cu;
+        }
+      } else if (u < my_long) {
+        const int l = pair + u * pairs;
+        const int t = l % (num_m * num_n);
+        s.slot = l / (num_m * num_n);
         s.m0 = (t / num_n) * XE_TILE;
-        s.n0 = (t % num_n) * XE_TILE;
+        s.n0 = (t % num_n) * TN;
         kb0 = s.slot * kb_slot;
         kb1 = min(nkb, kb0 + kb_slot);
       } else {
-        const int t = u - units0;
+        const int t = short0 + (u - my_long) * short_step;
         s.prod = 1;
         s.m0 = (t / num_n) * XE_TILE;
-        s.n0 = (t % num_n) * XE_TILE;
-        kb0 = 0;
+        s.n0 = (t % num_n) * TN;
         kb1 = kb_w;
       }
-      const int fl = PLANES == 1 ? (1 << 28) : XE_FLUSH_KB;
+      const int fl = PLANES == 1 ? (1 << 28) : XE_STEP_KB;
       steps = max(1, (kb1 - kb0 + fl - 1) / fl);
       s.kb0 = kb0 + j * fl;
       s.kb1 = min(kb1, s.kb0 + fl);
+      s.kfirst = j == 0;
+      s.klast = j + 1 >= steps;
+      s.first = j == 0 && c == 0;
+      s.last = s.klast && c + 1 >= ntiles;
+      s.second = PLANES == 1 && s.n0 + XE_TILE < a.p[s.prod].N;
+      if (!s.klast) {
+        ++j;
+      } else {
+        j = 0;
+        if (!s.last) {
+          ++c;
+        } else {
+          c = 0;
+          u += MODE == XE_GRADS ? 1 : pairs;
+        }
+      }
+      return true;
     }
-    s.first = j == 0;
-    s.last = j + 1 >= steps;
-    if (s.last) {
-      j = 0;
-      u += stride;
-    } else {
-      ++j;
-    }
-    return true;
   }
 };
 
@@ -452,74 +687,66 @@ struct XeWalk {
 __device__ __forceinline__ int xe_plane_a(int seg) { return (0x058 >> (2 * seg)) & 3; }
 __device__ __forceinline__ int xe_plane_b(int seg) { return (0x112 >> (2 * seg)) & 3; }
 
-// 32 rows x 32 columns of fp32 accumulators to a row-major matrix of `cols`
-// columns, coalesced through the warp's staging block (two halves of 16
-// columns); `acc` adds to what is there.  Rows >= nrows are skipped.
-__device__ __forceinline__ void xe_store_f32(uint8_t* stg, int lane, int nrows, const float (&v)[32], float* dst,
-                                             int64_t ld, int col, int cols, bool vec, bool acc) {
-  const int sw = (lane >> 1) & 3;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<float4*>(stg + lane * 64 + ((j ^ sw) << 4)) =
-          make_float4(v[16 * h + 4 * j], v[16 * h + 4 * j + 1], v[16 * h + 4 * j + 2], v[16 * h + 4 * j + 3]);
-    __syncwarp();
-    if (vec) {
-      const int piece = lane & 3;
-      const int c = col + 16 * h + 4 * piece;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = 8 * k + (lane >> 2);
-        float4 u = *reinterpret_cast<const float4*>(stg + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-        if (r < nrows && c < cols) {
-          float4* o = reinterpret_cast<float4*>(dst + r * ld + c);
-          if (acc) {
-            const float4 p = *o;
-            u.x += p.x; u.y += p.y; u.z += p.z; u.w += p.w;
-          }
-          *o = u;
-        }
-      }
-    } else {
-      const int e = lane & 15;
-      const int c = col + 16 * h + e;
-      for (int r = lane >> 4; r < nrows; r += 2) {
-        const float u = *reinterpret_cast<const float*>(stg + r * 64 + (((e >> 2) ^ ((r >> 1) & 3)) << 4) + (e & 3) * 4);
-        if (c < cols) dst[r * ld + c] = acc ? dst[r * ld + c] + u : u;
-      }
-    }
-    __syncwarp();
-  }
+__device__ __forceinline__ void st_v8(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
+                                      uint32_t g, uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e),
+               "r"(f), "r"(g), "r"(h)
+               : "memory");
 }
-// the same, rounded to bf16 (no accumulation)
-__device__ __forceinline__ void xe_store_bf16(uint8_t* stg, int lane, int nrows, const float (&v)[32],
-                                              __nv_bfloat16* dst, int64_t ld, int col, int cols, bool vec) {
-  const int sw = (lane >> 1) & 3;
+
+// 32 columns of this lane's row from `col` on, of a matrix with `cols`
+// columns (32-byte stores, whole sectors; `align`: the byte alignment that
+// every row start shares, 32, 16 or less)
+__device__ __forceinline__ void row_store_bf16(__nv_bfloat16* row, int col, int cols, int align, const float (&v)[32]) {
+  if (align >= 16 && col + 32 <= cols) {
+    uint32_t w[16];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    *reinterpret_cast<uint4*>(stg + lane * 64 + ((j ^ sw) << 4)) =
-        make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                   pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-  __syncwarp();
-  if (vec) {
-    const int piece = lane & 3;
-    const int c = col + 8 * piece;
+    for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+    __nv_bfloat16* p = row + col;
+    if (align >= 32) {
+      st_v8(p, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+      st_v8(p + 16, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r = 8 * k + (lane >> 2);
-      const uint4 u = *reinterpret_cast<const uint4*>(stg + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
-      if (r < nrows && c < cols) *reinterpret_cast<uint4*>(dst + r * ld + c) = u;
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4*>(p + 8 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     }
   } else {
-    const int c = col + lane;
-    for (int r = 0; r < nrows; ++r) {
-      const __nv_bfloat16 u =
-          *reinterpret_cast<const __nv_bfloat16*>(stg + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
-      if (c < cols) dst[r * ld + c] = u;
-    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col + j < cols) row[col + j] = __float2bfloat16_rn(v[j]);
   }
-  __syncwarp();
+}
+__device__ __forceinline__ void row_store_f32(float* row, int col, int cols, int align, float (&v)[32], bool acc) {
+  if (align >= 16 && col + 32 <= cols) {
+    float* p = row + col;
+    if (acc) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 o = *reinterpret_cast<const float4*>(p + 4 * j);
+        v[4 * j] += o.x; v[4 * j + 1] += o.y; v[4 * j + 2] += o.z; v[4 * j + 3] += o.w;
+      }
+    }
+    if (align >= 32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        st_v8(p + 8 * j, __float_as_uint(v[8 * j]), __float_as_uint(v[8 * j + 1]), __float_as_uint(v[8 * j + 2]),
+              __float_as_uint(v[8 * j + 3]), __float_as_uint(v[8 * j + 4]), __float_as_uint(v[8 * j + 5]),
+              __float_as_uint(v[8 * j + 6]), __float_as_uint(v[8 * j + 7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<float4*>(p + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col + j < cols) row[col + j] = acc ? row[col + j] + v[j] : v[j];
+  }
+}
+__device__ __forceinline__ int byte_align(const void* p, int64_t pitch_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(pitch_bytes);
+  return (x & 31u) == 0 ? 32 : ((x & 15u) == 0 ? 16 : 1);
 }
 
 template <int MODE, int PLANES>
@@ -527,12 +754,14 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     k_xent_gemm(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0,
                 const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB1,
                 const __grid_constant__ XeArgs args, int* err) {
-  constexpr int SEGS = PLANES == 1 ? 1 : 6;
+  using Cfg = XeCfg<PLANES>;
+  constexpr int HALVES = Cfg::kHalves;
+  constexpr int STAGES = Cfg::kStages;
+  constexpr int STAGE_BYTES = Cfg::kStageBytes;
   constexpr int CHUNKS = (XE_TILE / 32) / (XE_EPI_WARPS / 4);  // 32-column chunks per epilogue warp
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
-  uint8_t* stg_s = smem + G2_STAGES * G2_STAGE_BYTES;
-  XeCtl* ctl = reinterpret_cast<XeCtl*>(stg_s + XE_EPI_WARPS * XE_STG_WARP_BYTES);
+  XeCtl* ctl = reinterpret_cast<XeCtl*>(smem + STAGES * STAGE_BYTES);
   const int warp = warp_id();
   const int lane = lane_id();
   const uint32_t rank = cluster_ctarank();
@@ -541,7 +770,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
   const int pairs = static_cast<int>(gridDim.x) >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < G2_STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(&ctl->full[s], 1);
       mbar_init(&ctl->empty[s], 1);
     }
@@ -563,32 +792,34 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
   const uint32_t tmem = ctl->tmem_base;
   pdl_launch_dependents();
   pdl_wait();  // set-up above touched only shared memory, TMEM and parameters
-  const int rows = *static_cast<const volatile int*>(&args.rw.meta->rows);
+  int rows = *static_cast<const volatile int*>(&args.rw.meta->rows);
+  if (MODE == XE_KEEP && args.redo_tile != nullptr && *static_cast<const volatile int*>(&args.rw.meta->redo) == 0)
+    rows = 0;  // no row to do again
   volatile int* abort = &ctl->abort;
-  XeWalk<MODE, PLANES> walk(args, rows, pair, pairs);
-  XeStep st;
 
   if (warp == 0) {
     if (lane == 0) {
+      XeWalk<MODE, PLANES> walk(args, rows, pair, pairs);
+      XeStep st;
       RingPos rp;
       bool ok = true;
       while (ok && walk.next(st)) {
         const int m0 = st.m0 + static_cast<int>(rank) * G2_BM;
         const int n0 = st.n0 + static_cast<int>(rank) * (XE_TILE / 2);
+        const int halves = st.second ? 2 : 1;
         const CUtensorMap* ta = st.prod == 0 ? &tmA0 : &tmA1;
         const CUtensorMap* tb = st.prod == 0 ? &tmB0 : &tmB1;
         const XeProduct& p = args.p[st.prod];
-        for (int seg = 0; ok && seg < SEGS; ++seg) {
-          const int ya = SEGS == 1 ? 0 : xe_plane_a(seg) * p.a_plane_rows;
-          const int yb = SEGS == 1 ? 0 : xe_plane_b(seg) * p.b_plane_rows;
+        for (int seg = 0; ok && seg < Cfg::kSegs; ++seg) {
+          const int ya = PLANES == 1 ? 0 : xe_plane_a(seg) * p.a_plane_rows;
+          const int yb = PLANES == 1 ? 0 : xe_plane_b(seg) * p.b_plane_rows;
           for (int kb = st.kb0; kb < st.kb1; ++kb) {
             if (!mbar_wait(&ctl->empty[rp.stage], rp.phase ^ 1u, abort, err, 1)) {
               ok = false;
               break;
             }
-            uint8_t* sa = smem + rp.stage * G2_STAGE_BYTES;
-            uint8_t* sb = sa + G2_A_BYTES;
-            if (leader) mbar_arrive_expect_tx(&ctl->full[rp.stage], 2 * G2_STAGE_BYTES);
+            uint8_t* sa = smem + rp.stage * STAGE_BYTES;
+            if (leader) mbar_arrive_expect_tx(&ctl->full[rp.stage], 2 * (G2_A_BYTES + halves * G2_B_BYTES));
             const uint32_t fb = cluster_map(smem_u32(&ctl->full[rp.stage]), 0);
             if (MODE == XE_GRADS && st.prod == 1) {
               tma_load_2d_pair(sa, ta, fb, m0, ya + kb * G2_BK);
@@ -596,13 +827,17 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
             } else {
               tma_load_2d_pair(sa, ta, fb, kb * G2_BK, ya + m0);
             }
-            if (MODE == XE_GRADS) {
-              tma_load_2d_pair(sb, tb, fb, n0, yb + kb * G2_BK);
-              tma_load_2d_pair(sb + 8192, tb, fb, n0 + 64, yb + kb * G2_BK);
-            } else {
-              tma_load_2d_pair(sb, tb, fb, kb * G2_BK, yb + n0);
+            for (int h = 0; h < halves; ++h) {
+              uint8_t* sb = sa + G2_A_BYTES + h * G2_B_BYTES;
+              const int nh = n0 + h * XE_TILE;
+              if (MODE == XE_GRADS) {
+                tma_load_2d_pair(sb, tb, fb, nh, yb + kb * G2_BK);
+                tma_load_2d_pair(sb + 8192, tb, fb, nh + 64, yb + kb * G2_BK);
+              } else {
+                tma_load_2d_pair(sb, tb, fb, kb * G2_BK, yb + nh);
+              }
             }
-            rp.advance(G2_STAGES);
+            rp.advance(STAGES);
           }
         }
       }
@@ -610,7 +845,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         // as in k_gemm2sm: both CTAs' copies complete on the leader's
         // barriers; the peer waits a bounded 100 us for its own to land
         if (leader) {
-          rp.drain(ctl->full, G2_STAGES, err, 5);
+          rp.drain(ctl->full, STAGES, err, 5);
         } else {
           const uint64_t t0 = global_timer_ns();
           while (global_timer_ns() - t0 < 100000ull) {
@@ -620,47 +855,97 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     }
   } else if (warp == 1) {
     if (lane == 0 && leader) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int it = 0;
+      // One stream of K blocks per accumulator.  With two, the second follows
+      // kLag blocks behind the first and releases the ring's stages.
+      XeWalk<MODE, PLANES> w0(args, rows, pair, pairs), w1(args, rows, pair, pairs);
+      XeStep s0, s1;
+      int stage0 = 0, stage1 = 0;
+      uint32_t phase0 = 0;
+      int it0 = 0, it1 = 0;          // accumulations begun, per accumulator stream
+      int b0 = 0, n0 = 0;            // block of stream 0's step, and their number
+      int b1 = 0, n1 = 0;
+      int ahead = 0;                 // blocks of stream 0 that stream 1 has yet to do
+      int begun0 = 0, done1 = 0;     // tiles begun by stream 0, finished by stream 1
+      bool more0 = true, more1 = HALVES == 2;
       bool ok = true;
-      while (ok && walk.next(st)) {
-        if (st.kb0 >= st.kb1) continue;  // nothing to add up (no rows)
+      auto mma_block = [&](const XeStep& st, int stage, int half, uint32_t d, bool first) {
         const bool a_mn = MODE == XE_GRADS && st.prod == 1;
         const uint32_t idesc = umma_idesc_bf16_f32_major(2 * G2_BM, XE_TILE, a_mn, MODE == XE_GRADS);
-        const int buf = it & 1;
-        const uint32_t acc_phase = static_cast<uint32_t>(it >> 1) & 1u;
-        ++it;
-        if (!mbar_wait(&ctl->acc_empty[buf], acc_phase ^ 1u, abort, err, 2)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem + static_cast<uint32_t>(buf * XE_TILE);
-        const int blocks = SEGS * (st.kb1 - st.kb0);
-        for (int b = 0; b < blocks; ++b) {
-          if (!mbar_wait(&ctl->full[stage], phase, abort, err, 3)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a_base = smem_u32(smem + stage * G2_STAGE_BYTES);
-          const uint32_t b_base = a_base + G2_A_BYTES;
+        const uint32_t a_base = smem_u32(smem + stage * STAGE_BYTES);
+        const uint32_t b_base = a_base + G2_A_BYTES + half * G2_B_BYTES;
 #pragma unroll
-          for (int k = 0; k < G2_BK / 16; ++k) {
-            const uint64_t ad = a_mn ? umma_desc_sw128_mn(a_base + k * 2048, 8192) : umma_desc_sw128(a_base + k * 32);
-            const uint64_t bd =
-                MODE == XE_GRADS ? umma_desc_sw128_mn(b_base + k * 2048, 8192) : umma_desc_sw128(b_base + k * 32);
-            umma_bf16_pair(d, ad, bd, idesc, (b > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < G2_BK / 16; ++k) {
+          const uint64_t ad = a_mn ? umma_desc_sw128_mn(a_base + k * 2048, 8192) : umma_desc_sw128(a_base + k * 32);
+          const uint64_t bd =
+              MODE == XE_GRADS ? umma_desc_sw128_mn(b_base + k * 2048, 8192) : umma_desc_sw128(b_base + k * 32);
+          umma_bf16_pair(d, ad, bd, idesc, (!first || k > 0) ? 1u : 0u);
+        }
+      };
+      while (ok && (more0 || more1)) {
+        // stream 0 may begin tile j once stream 1 is through tile j - 2: the
+        // epilogue takes the accumulators in the order of the tiles
+        const bool go0 = more0 && (HALVES == 1 || b0 != n0 || begun0 <= done1 + 1);
+        if (go0) {
+          if (b0 == n0) {  // next step with blocks
+            b0 = n0 = 0;
+            while (n0 == 0 && (more0 = w0.next(s0))) n0 = Cfg::kSegs * max(0, s0.kb1 - s0.kb0);
           }
-          umma_commit_pair_mc(&ctl->empty[stage], 0x3);
-          if (++stage == G2_STAGES) {
-            stage = 0;
-            phase ^= 1u;
+          if (more0) {
+            const int buf = HALVES == 2 ? 0 : it0 & 1;
+            const uint32_t par = static_cast<uint32_t>(HALVES == 2 ? it0 : it0 >> 1) & 1u;
+            if (b0 == 0) {
+              ++begun0;
+              if (!mbar_wait(&ctl->acc_empty[buf], par ^ 1u, abort, err, 2)) {
+                ok = false;
+                break;
+              }
+            }
+            if (!mbar_wait(&ctl->full[stage0], phase0, abort, err, 3)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            mma_block(s0, stage0, 0, tmem + static_cast<uint32_t>(buf * XE_TILE), b0 == 0);
+            if (HALVES == 1) umma_commit_pair_mc(&ctl->empty[stage0], 0x3);
+            if (++b0 == n0) {
+              umma_commit_pair_mc(&ctl->acc_full[buf], 0x3);
+              ++it0;
+            }
+            if (++stage0 == STAGES) {
+              stage0 = 0;
+              phase0 ^= 1u;
+            }
+            ++ahead;
           }
         }
-        if (!ok) break;
-        umma_commit_pair_mc(&ctl->acc_full[buf], 0x3);
+        if (HALVES == 2 && more1 && (ahead > Cfg::kLag || !more0 || !go0)) {
+          if (b1 == n1) {
+            b1 = n1 = 0;
+            while (n1 == 0 && (more1 = w1.next(s1))) n1 = Cfg::kSegs * max(0, s1.kb1 - s1.kb0);
+          }
+          if (more1) {
+            if (s1.second) {
+              if (b1 == 0) {
+                if (!mbar_wait(&ctl->acc_empty[1], (static_cast<uint32_t>(it1) & 1u) ^ 1u, abort, err, 2)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+              }
+              mma_block(s1, stage1, 1, tmem + static_cast<uint32_t>(XE_TILE), b1 == 0);
+            }
+            umma_commit_pair_mc(&ctl->empty[stage1], 0x3);
+            if (++b1 == n1) {
+              ++done1;
+              if (s1.second) {
+                umma_commit_pair_mc(&ctl->acc_full[1], 0x3);
+                ++it1;
+              }
+            }
+            if (++stage1 == STAGES) stage1 = 0;
+            --ahead;
+          }
+        }
       }
       if (!ok || *abort) {
         umma_commit_pair(&ctl->drain);
@@ -669,163 +954,204 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     }
   } else {
     // Epilogue warps never leave the walk early: after an abort they skip the
-    // work but still arrive on every acc_empty phase.
+    // work but still arrive on every acc_empty phase.  A warp takes its 128
+    // columns of an accumulator into registers and releases it before it
+    // works on them.
+    XeWalk<MODE, PLANES> walk(args, rows, pair, pairs);
+    XeStep st;
     const int q = warp & 3;
-    const int ch = (warp - 2) >> 2;  // column half of the tile
-    uint8_t* stg = stg_s + (warp - 2) * XE_STG_WARP_BYTES;
+    const int ch = (warp - 2) >> 2;  // column half of an accumulator
     const uint32_t acc_empty0 = cluster_map(smem_u32(&ctl->acc_empty[0]), 0);
     const uint32_t acc_empty1 = cluster_map(smem_u32(&ctl->acc_empty[1]), 0);
-    int it = 0;
+    int it[2] = {0, 0};  // accumulations taken (HALVES 1: all in it[0])
     bool ok = true;
     // per-row state (this lane's row of the tile)
     int y = -1;
-    float run_m = -INFINITY, run_s = 0.0f;       // STATS
-    float lse2 = 0.0f, lse = 0.0f, g = 0.0f;      // DLOGITS
-    float scale = 1.0f;                           // GRADS: dW
-    if (MODE == XE_GRADS && args.reduction != XE_NONE) {
-      scale = *args.grad;
-      if (args.reduction == XE_MEAN) {
-        const int valid = args.rw.meta->valid;
-        scale = valid > 0 ? scale / valid : 0.0f;
-      }
-    }
+    bool live = false;
+    float run_m = -INFINITY, run_s = 0.0f;  // STATS, KEEP
+    float c2 = 0.0f;                        // KEEP: shift, DLOGITS: logsumexp, in units of log 2
+    float g = 1.0f, at_label = 0.0f;        // DLOGITS
+    const float scale = MODE == XE_GRADS ? xe_scale(args.rw, args.grad, args.reduction) : 1.0f;
+    float v[CHUNKS][32];
     while (walk.next(st)) {
       const bool any = st.kb0 < st.kb1;
-      const int row0 = st.m0 + static_cast<int>(rank) * G2_BM + q * 32;
-      const int row = row0 + lane;
-      if (MODE == XE_STATS && st.first) {
-        y = row < rows ? args.rw.yc[row] : -1;
+      const int row = st.m0 + static_cast<int>(rank) * G2_BM + q * 32 + lane;
+      if ((MODE == XE_STATS || MODE == XE_KEEP) && st.first) {
+        live = row < rows;
+        y = live ? args.rw.yc[row] : -1;
+        if (MODE == XE_KEEP) {
+          live = y >= 0;
+          c2 = live ? args.rw.c[row] * XE_LOG2E : 0.0f;
+        }
         run_m = -INFINITY;
         run_s = 0.0f;
       }
-      if (MODE == XE_DLOGITS) {
+      if (MODE == XE_DLOGITS && st.kfirst) {
         y = row < rows ? args.rw.yc[row] : -1;
-        lse = row < rows ? args.rw.lse[row] : 0.0f;
-        lse2 = lse * XE_LOG2E;
-        g = 1.0f;
-        if (args.reduction == XE_NONE && y >= 0) g = args.grad[args.rw.idx[row]];
+        live = y >= 0;
+        c2 = live ? args.rw.lse[row] * XE_LOG2E : 0.0f;
+        at_label = live ? args.rw.q[row] : 0.0f;
+        g = args.reduction == XE_NONE && live ? args.grad[args.rw.idx[row]] : 1.0f;
       }
-      const int buf = it & 1;
-      const uint32_t acc_phase = static_cast<uint32_t>(it >> 1) & 1u;
-      if (any) {
-        ++it;
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->acc_full[buf], acc_phase, abort, err, 4));
-        tc_fence_after();
-      }
-      if (ok) {
 #pragma unroll 1
-        for (int c = ch * CHUNKS; c < (ch + 1) * CHUNKS; ++c) {
-          float v[32];
-          if (any) {
-            tmem_ld32(tmem_addr(tmem, q * 32, buf * XE_TILE + c * 32), v);
-          } else {
+      for (int half = 0; half < (st.second ? 2 : 1); ++half) {
+        const int buf = HALVES == 2 ? half : it[0] & 1;
+        if (any) {
+          const int n = HALVES == 2 ? it[half] : it[0] >> 1;
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->acc_full[buf], static_cast<uint32_t>(n) & 1u, abort, err, 4));
+          ++it[HALVES == 2 ? half : 0];
+          tc_fence_after();
+          if (ok) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+            for (int k = 0; k < CHUNKS; ++k) {
+              const uint32_t ta = tmem_addr(tmem, q * 32, buf * XE_TILE + (ch * CHUNKS + k) * 32);
+              if (HALVES == 1 && !st.kfirst) {
+                float x[32];
+                tmem_ld32(ta, x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[k][i] += x[i];
+              } else {
+                tmem_ld32(ta, v[k]);
+              }
+            }
           }
-          const int col = st.n0 + c * 32;
-          if (MODE == XE_STATS) {
-            const int N = args.p[0].N;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(buf ? acc_empty1 : acc_empty0);
+        } else {
+#pragma unroll
+          for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[k][i] = 0.0f;
+        }
+        if (!ok || !st.klast) continue;
+        const int col0 = st.n0 + half * XE_TILE + ch * CHUNKS * 32;
+        if (MODE == XE_STATS || MODE == XE_KEEP) {
+          const int N = args.p[0].N;
+#pragma unroll
+          for (int k = 0; k < CHUNKS; ++k) {
+            const int col = col0 + k * 32;
             if (col + 32 > N) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (col + i >= N) v[i] = -INFINITY;
+                if (col + i >= N) v[k][i] = -INFINITY;
             }
+            // the label's column is not among the others
             if (__any_sync(0xffffffffu, y >= col && y < col + 32)) {
-              float l = 0.0f;
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (y == col + i) l = v[i];
-              if (y >= col && y < col + 32) args.rw.lab[row] = l;
+                if (y == col + i) v[k][i] = -INFINITY;
             }
-            float m = run_m;
+          }
+          float m = run_m;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
-            if (m > -INFINITY) {
-              const float m2 = m * XE_LOG2E;
-              float s0 = 0.0f, s1 = 0.0f;
+          for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) m = fmaxf(m, v[k][i]);
+          float s0 = 0.0f, s1 = 0.0f;
+          if (MODE == XE_KEEP) {
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k) {
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
-                s0 += ex2_approx(fmaf(v[i], XE_LOG2E, -m2));
-                s1 += ex2_approx(fmaf(v[i + 1], XE_LOG2E, -m2));
+                v[k][i] = live ? ex2_approx(fmaf(v[k][i], XE_LOG2E, -c2)) : 0.0f;
+                v[k][i + 1] = live ? ex2_approx(fmaf(v[k][i + 1], XE_LOG2E, -c2)) : 0.0f;
+                s0 += v[k][i];
+                s1 += v[k][i + 1];
               }
-              run_s = fmaf(run_s, ex2_approx(fmaf(run_m, XE_LOG2E, -m2)), s0 + s1);
-              run_m = m;
-            } else {  // -inf or NaN only: NaN is carried into the sum
+              row_store_bf16(args.dl + row * args.ldl, col0 + k * 32, static_cast<int>(args.ldl), 32, v[k]);
+            }
+            run_s += s0 + s1;
+          } else if (m > -INFINITY) {
+            const float m2 = m * XE_LOG2E;
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                s0 += ex2_approx(fmaf(v[k][i], XE_LOG2E, -m2));
+                s1 += ex2_approx(fmaf(v[k][i + 1], XE_LOG2E, -m2));
+              }
+            run_s = fmaf(run_s, ex2_approx(fmaf(run_m, XE_LOG2E, -m2)), s0 + s1);
+          } else {  // -inf or NaN only: NaN is carried into the sum
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (isnan(v[i])) run_s = v[i];
-            }
-          } else if (MODE == XE_DLOGITS) {
-            const bool live = y >= 0;
+                if (isnan(v[k][i])) run_s = v[k][i];
+          }
+          run_m = m;
+        } else if (MODE == XE_DLOGITS) {
+          const int N = args.p[0].N;
+#pragma unroll
+          for (int k = 0; k < CHUNKS; ++k) {
+            const int col = col0 + k * 32;
             const int gc = args.v0 + col;  // column in the vocabulary
-            const int N = args.p[0].N;
-            // p - 1 at the label, without the cancellation
-            const bool label = live && y >= gc && y < gc + 32;
-            const bool any_label = __any_sync(0xffffffffu, label);
-            float at_label = 0.0f;
-            if (any_label) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[k][i] = ex2_approx(fmaf(v[k][i], XE_LOG2E, -c2));
+            if (__any_sync(0xffffffffu, y >= gc && y < gc + 32)) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (y == gc + i) at_label = v[i];
-              at_label = expm1f(at_label - lse);
+                if (y == gc + i) v[k][i] = at_label;
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = ex2_approx(fmaf(v[i], XE_LOG2E, -lse2));
-            if (any_label) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (y == gc + i) v[i] = at_label;
-            }
-            if (args.reduction == XE_NONE) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] *= g;
-            }
-            if (!live) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-            }
+            for (int i = 0; i < 32; ++i) v[k][i] = live ? v[k][i] * g : 0.0f;
             if (col + 32 > N) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (col + i >= N) v[i] = 0.0f;
+                if (col + i >= N) v[k][i] = 0.0f;
             }
 #pragma unroll
             for (int pl = 0; pl < PLANES; ++pl) {
-              xe_store_bf16(stg, lane, 32, v,
-                            args.dl + (pl * args.dl_plane_rows + row0) * args.ldl, args.ldl, col,
-                            static_cast<int>(args.ldl), true);
+              row_store_bf16(args.dl + (pl * args.dl_plane_rows + row) * args.ldl, col, static_cast<int>(args.ldl), 32,
+                             v[k]);
               if (pl + 1 < PLANES) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
+                for (int i = 0; i < 32; ++i) v[k][i] -= __bfloat162float(__float2bfloat16_rn(v[k][i]));
               }
             }
-          } else if (st.prod == 0) {
-            xe_store_f32(stg, lane, min(32, rows - row0), v,
-                         args.dh_acc + st.slot * args.dh_slot_size + row0 * args.dh_ld, args.dh_ld, col,
-                         static_cast<int>(args.dh_ld), true, args.dh_accumulate != 0 || !st.first);
-          } else {
+          }
+        } else if (st.prod == 0) {
+          if (row < rows) {
+            float* o = args.dh_acc + st.slot * args.dh_slot_size + row * args.dh_ld;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= scale;
-            const int d = args.p[1].N;
-            const int nr = min(32, args.p[1].M - row0);
-            if (args.dw_bf16) {
-              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(args.dw) + static_cast<int64_t>(row0) * d;
-              xe_store_bf16(stg, lane, nr, v, o, d, col, d,
-                            d % 8 == 0 && (reinterpret_cast<uintptr_t>(args.dw) & 15u) == 0);
-            } else {
-              float* o = static_cast<float*>(args.dw) + static_cast<int64_t>(row0) * d;
-              xe_store_f32(stg, lane, nr, v, o, d, col, d,
-                           d % 4 == 0 && (reinterpret_cast<uintptr_t>(args.dw) & 15u) == 0, !st.first);
+            for (int k = 0; k < CHUNKS; ++k)
+              row_store_f32(o, col0 + k * 32, static_cast<int>(args.dh_ld), 32, v[k], args.dh_accumulate != 0);
+          }
+        } else if (row < args.p[1].M) {
+          const int d = args.p[1].N;
+          const float* extra = nullptr;
+          if (args.label_rows != nullptr) {
+            const int at = args.label_offs[row];
+            if (at < args.label_offs[row + 1]) extra = args.label_rows + static_cast<int64_t>(at) * d;
+          }
+          const int esz = args.dw_bf16 ? 2 : 4;
+          const int align = byte_align(args.dw, static_cast<int64_t>(d) * esz);
+#pragma unroll
+          for (int k = 0; k < CHUNKS; ++k) {
+            const int col = col0 + k * 32;
+            if (extra != nullptr) {
+              if (d % 4 == 0 && col + 32 <= d) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                  const float4 e = *reinterpret_cast<const float4*>(extra + col + i);
+                  v[k][i] += e.x; v[k][i + 1] += e.y; v[k][i + 2] += e.z; v[k][i + 3] += e.w;
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (col + i < d) v[k][i] += extra[col + i];
+              }
             }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[k][i] *= scale;
+            if (args.dw_bf16)
+              row_store_bf16(static_cast<__nv_bfloat16*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k]);
+            else
+              row_store_f32(static_cast<float*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k], false);
           }
         }
       }
-      if (any) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_remote(buf ? acc_empty1 : acc_empty0);
-      }
-      if (MODE == XE_STATS && st.last && ok && row < rows)
+      if ((MODE == XE_STATS || MODE == XE_KEEP) && st.last && ok && row < rows)
         args.part[(st.slot * 2 + ch) * args.part_ld + row] = make_float2(run_m, run_s);
     }
   }

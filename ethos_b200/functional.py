@@ -80,18 +80,33 @@ def balance_loss(weights, ids, num_experts, mask=None):
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, labels, ignore_index, reduction):
+    def forward(ctx, hidden, weight, labels, ignore_index, reduction, need_hidden, need_weight):
+        ctx.grads = None
+        ctx.reduction = reduction
+        if reduction != "none" and (need_hidden or need_weight):
+            both = ops.linear_cross_entropy_forward_backward(hidden, weight, labels, ignore_index, reduction,
+                                                             need_hidden, need_weight)
+            if both is not None:
+                loss, save, dh, dw = both
+                ctx.grads = (dh, dw)
+                ctx.save_for_backward(hidden, weight, save)
+                return loss
         loss, save = ops.linear_cross_entropy_forward(hidden, weight, labels, ignore_index, reduction)
         ctx.save_for_backward(hidden, weight, save)
-        ctx.reduction = reduction
         return loss
 
     @staticmethod
     def backward(ctx, grad):
         hidden, weight, save = ctx.saved_tensors
-        dh, dw = ops.linear_cross_entropy_backward(grad, hidden, weight, save, ctx.reduction,
-                                                   ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return dh, dw, None, None, None
+        need = ctx.needs_input_grad
+        grads, ctx.grads = ctx.grads, None
+        if grads is not None:
+            # the loss's own gradients, scaled where they are
+            grad = grad.to(torch.float32)
+            dh, dw = (ops.scale_(g, grad) if g is not None and n else None for g, n in zip(grads, need))
+        else:  # also a second pass through the graph: the first one's results belong to its caller
+            dh, dw = ops.linear_cross_entropy_backward(grad, hidden, weight, save, ctx.reduction, need[0], need[1])
+        return dh, dw, None, None, None, None, None
 
 
 def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="mean"):
@@ -101,11 +116,19 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
 
     The loss is fp32: per token, or summed or averaged over the tokens whose
     label is not ``ignore_index`` (the mean over none is NaN, as torch has
-    it).  Ignored tokens take no part in the products.  The backward forms the
-    logits again, a piece of the vocabulary at a time, so memory does not grow
-    with ``T * V``; gradients have the operands' dtype."""
+    it).  Ignored tokens take no part in the products; gradients have the
+    operands' dtype.
+
+    Where gradients are needed and the loss is one number, bf16 operands get
+    them in the forward call, which keeps the logits' exponentials (bf16, up
+    to 4 GiB of workspace) for its own length; the backward multiplies them by
+    the loss's gradient.  Otherwise the backward forms the logits again, a
+    piece of the vocabulary at a time.  Neither way keeps anything of size
+    ``T * V`` between the calls."""
     if labels.shape != hidden.shape[:-1]:
         raise ValueError(f"labels {tuple(labels.shape)} do not belong to hidden {tuple(hidden.shape)}")
     flat = hidden.reshape(-1, hidden.shape[-1]) if hidden.dim() != 2 else hidden
-    loss = _LinearCrossEntropy.apply(flat, weight, labels.reshape(-1), ignore_index, reduction)
+    grad = torch.is_grad_enabled()
+    loss = _LinearCrossEntropy.apply(flat, weight, labels.reshape(-1), ignore_index, reduction,
+                                     grad and flat.requires_grad, grad and weight.requires_grad)
     return loss.view(labels.shape) if reduction == "none" else loss

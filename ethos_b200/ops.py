@@ -17,6 +17,7 @@ __all__ = [
     "device_error_word", "check_device_error", "PackedWeights", "layer_backward", "layer_forward_f32",
     "router_forward_f32", "layer_backward_f32", "embedding_forward", "embedding_backward", "balance_forward",
     "balance_backward", "linear_cross_entropy_forward", "linear_cross_entropy_backward",
+    "linear_cross_entropy_forward_backward", "scale_",
 ]
 
 _ERR_WORDS = {}
@@ -687,11 +688,9 @@ def _xent_weight(w):
     return w
 
 
-def linear_cross_entropy_forward(hidden, weight, labels, ignore_index=-100, reduction="mean"):
-    """Cross entropy of the logits ``hidden @ weight.T`` without keeping them
-    (ethos_xent_forward): ``hidden [T, d]``, ``weight [V, d]`` of one dtype
-    (fp32 or bf16), ``labels [T]`` int32 or int64.  Returns ``(loss fp32 [T]
-    or scalar, save)``; ``save`` goes to ``linear_cross_entropy_backward``."""
+def _xent_args(hidden, weight, labels, reduction):
+    """Checks shared by the forward calls; the operands as the library reads
+    them."""
     _require_cuda(hidden, "hidden")
     dev = hidden.device
     _on(dev, weight, "weight")
@@ -704,13 +703,21 @@ def linear_cross_entropy_forward(hidden, weight, labels, ignore_index=-100, redu
         raise ValueError(f"hidden [T, d] and weight [V, d]: got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if weight.dtype != hidden.dtype:
         raise ValueError(f"hidden is {hidden.dtype}, weight {weight.dtype}")
-    (T, d), V = hidden.shape, weight.shape[0]
-    if tuple(labels.shape) != (T,):
-        raise ValueError(f"labels: [{T}], got {tuple(labels.shape)}")
+    if tuple(labels.shape) != (hidden.shape[0],):
+        raise ValueError(f"labels: [{hidden.shape[0]}], got {tuple(labels.shape)}")
+    return _xent_rows(hidden), _xent_weight(weight), labels.contiguous(), code, i64, red
+
+
+def linear_cross_entropy_forward(hidden, weight, labels, ignore_index=-100, reduction="mean"):
+    """Cross entropy of the logits ``hidden @ weight.T`` without keeping them
+    (ethos_xent_forward): ``hidden [T, d]``, ``weight [V, d]`` of one dtype
+    (fp32 or bf16), ``labels [T]`` int32 or int64.  Returns ``(loss fp32 [T]
+    or scalar, save)``; ``save`` goes to ``linear_cross_entropy_backward``."""
+    hidden, weight, labels, code, i64, red = _xent_args(hidden, weight, labels, reduction)
+    (T, d), V, dev = hidden.shape, weight.shape[0], hidden.device
     loss = torch.empty((T,) if red == 0 else (), dtype=torch.float32, device=dev)
     if T == 0:  # as torch: nothing, 0, and the mean of nothing
         return (loss if red == 0 else loss.fill_(0.0 if red == 1 else float("nan"))), None
-    hidden, weight, labels = _xent_rows(hidden), _xent_weight(weight), labels.contiguous()
     save = _bytes(_size("ethos_xent_save_size", T, V, d, code), dev)
     ws = _bytes(_size("ethos_xent_forward_workspace_size", T, V, d, code), dev)
     check(lib().ethos_xent_forward(hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), code,
@@ -718,6 +725,42 @@ def linear_cross_entropy_forward(hidden, weight, labels, ignore_index=-100, redu
                                    save.data_ptr(), save.numel(), ws.data_ptr(), ws.numel(),
                                    device_error_word(dev).data_ptr(), _raw_stream(dev.index)), "ethos_xent_forward")
     return loss, save
+
+
+def linear_cross_entropy_forward_backward(hidden, weight, labels, ignore_index=-100, reduction="mean",
+                                          need_hidden=True, need_weight=True):
+    """``(loss, save, d_hidden, d_weight)`` in one call, the gradients those of
+    the loss itself, "sum" or "mean" (ethos_xent_forward_backward: three
+    products instead of four).  None where that way is not open (fp32, or
+    over 4 GiB of exponentials): ``linear_cross_entropy_forward`` and
+    ``_backward`` serve those."""
+    hidden, weight, labels, code, i64, red = _xent_args(hidden, weight, labels, reduction)
+    (T, d), V, dev = hidden.shape, weight.shape[0], hidden.device
+    ws_bytes = _size("ethos_xent_forward_backward_workspace_size", T, V, d, code)
+    if ws_bytes == 0 or red == 0:
+        return None
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    dh = hidden.new_empty((T, d)) if need_hidden else None
+    dw = weight.new_empty((V, d)) if need_weight else None
+    save = _bytes(_size("ethos_xent_save_size", T, V, d, code), dev)
+    ws = _bytes(ws_bytes, dev)
+    check(lib().ethos_xent_forward_backward(
+        hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), code, labels.data_ptr(), i64,
+        ignore_index, red, T, V, d, loss.data_ptr(), save.data_ptr(), save.numel(),
+        dh.data_ptr() if need_hidden else 0, dw.data_ptr() if need_weight else 0, ws.data_ptr(), ws.numel(),
+        device_error_word(dev).data_ptr(), _raw_stream(dev.index)), "ethos_xent_forward_backward")
+    return loss, save, dh, dw
+
+
+def scale_(x, factor):
+    """``x *= factor`` in place (``factor`` a fp32 device scalar); nothing is
+    read or written when it is 1 (ethos_xent_scale)."""
+    _require_cuda(x, "x")
+    if not x.is_contiguous():
+        raise ValueError("x: contiguous")
+    check(lib().ethos_xent_scale(factor.data_ptr(), x.data_ptr(), _dtype_code(x, "x"), x.numel(),
+                                 _raw_stream(x.device.index)), "ethos_xent_scale")
+    return x
 
 
 def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", need_hidden=True, need_weight=True):

@@ -525,6 +525,23 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
                         size_t save_bytes, void* d_hidden, void* d_weight, void* workspace, size_t workspace_bytes,
                         int* dev_err, void* stream);
 
+/* Loss (SUM or MEAN) and, in the same call, the gradients for a loss whose own
+ * gradient is 1 (either may be NULL): the exponentials of the logits are kept
+ * as bf16 in the workspace between the products instead of being formed twice
+ * (three products, not four).  bf16 operands, and at most 4 GiB of
+ * exponentials (tokens * vocab * 2 bytes); the workspace size is 0 where that
+ * does not hold.  `save` is as ethos_xent_forward leaves it. */
+size_t ethos_xent_forward_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype);
+int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype,
+                                const void* labels, int labels_i64, int64_t ignore_index, int reduction,
+                                int64_t tokens, int64_t vocab, int64_t dim, float* loss, void* save,
+                                size_t save_bytes, void* d_hidden, void* d_weight, void* workspace,
+                                size_t workspace_bytes, int* dev_err, void* stream);
+
+/* x[0..n) *= factor[0] (device fp32), nothing written when it is 1: applies
+ * the loss's own gradient to the gradients above. */
+int ethos_xent_scale(const float* factor, void* x, int dtype, int64_t n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

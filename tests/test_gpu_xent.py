@@ -189,6 +189,57 @@ def test_extreme_logits(T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [6, 300, 900])
+def test_hopeless_labels_with_gradients(T):
+    """bf16, gradients in the forward call: rows whose largest logit passes
+    the label's by hundreds (the exponentials are then taken relative to the
+    largest), next to rows that need no such thing, in one row tile and in
+    several.  Operand values are exact in bf16, logits whole numbers."""
+    V, d = 1100, 16
+    W = torch.zeros(V, d)
+    W[:, 0] = (torch.arange(V) % 17).float()
+    W[:, 1] = (torch.arange(V) % 5).float()
+    g = torch.Generator().manual_seed(12)
+    h = torch.zeros(T, d)
+    h[:, 1] = torch.randint(0, 3, (T,), generator=g).float()
+    y = torch.randint(0, V, (T,), generator=g)
+    h[1::7, 0] = 40.0      # gaps of up to 640 between logits
+    h[3, 0] = 4.0          # 64: just over the range
+    y[3] = 17              # logit 0 in column 0 (17 % 17)
+    h, W = h.bfloat16(), W.bfloat16()
+    for reduction in ("sum", "mean"):
+        want, dh_w, dw_w, q = _exact(h, W, y, reduction)
+        hg, wg = h.cuda().requires_grad_(True), W.cuda().requires_grad_(True)
+        loss = EF.linear_cross_entropy(hg, wg, y.cuda(), reduction=reduction)
+        scale = T if reduction == "sum" else 1
+        assert abs(loss.item() - want) <= scale * _loss_bound(q) + 2.0 ** -23 * abs(want)
+        dh, dw = torch.autograd.grad(loss, (hg, wg))
+        assert _rel(dh, dh_w) <= _grad_bound(q, "ch", V / 16, torch.bfloat16)
+        assert _rel(dw, dw_w) <= _grad_bound(q, "cw", T / 16, torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_gradient_of_the_loss_scales_and_second_pass():
+    """The loss inside a larger expression, and two passes through its graph
+    (the second finds the first's gradients untouched)."""
+    h, W, y = _inputs(400, 900, 64, torch.bfloat16, seed=13, ignored=0.3)
+    hg, wg = h.cuda().requires_grad_(True), W.cuda().requires_grad_(True)
+    _, dh_w, dw_w, q = _exact(h, W, y, "mean")
+    loss = EF.linear_cross_entropy(hg, wg, y.cuda())
+    a = torch.autograd.grad(0.3 * loss, (hg, wg), retain_graph=True)
+    keep = [t.clone() for t in a]
+    b = torch.autograd.grad(loss, (hg, wg))
+    for got, want, key, steps, f in ((a[0], dh_w, "ch", 900 / 16, 0.3), (a[1], dw_w, "cw", 400 / 16, 0.3),
+                                     (b[0], dh_w, "ch", 900 / 16, 1.0), (b[1], dw_w, "cw", 400 / 16, 1.0)):
+        # 0.3 is one more rounding to bf16
+        assert _rel(got, f * want) <= _grad_bound(q, key, steps, torch.bfloat16) + 2.0 ** -9
+    assert all(torch.equal(x, z) for x, z in zip(a, keep))
+    with torch.no_grad():
+        assert torch.equal(EF.linear_cross_entropy(hg, wg, y.cuda(), reduction="none").sum() > 0,
+                           torch.tensor(True, device="cuda"))
+
+
+@pytest.mark.gpu
 def test_nan_and_infinity_stay_in_their_rows():
     h, W, y = _inputs(300, 600, 32, torch.float32, seed=4)
     h[7, 3], h[9, 0] = float("nan"), float("inf")
@@ -374,5 +425,20 @@ def test_entry_point_argument_checks():
         a.update(o)
         return L.ethos_xent_backward(*a.values())
 
+    both = L.ethos_xent_forward_backward_workspace_size(T, V, d, 1)
+    assert both >= 512 * 1024 * 2
+    assert L.ethos_xent_forward_backward_workspace_size(T, V, d, 0) == 0            # fp32
+    assert L.ethos_xent_forward_backward_workspace_size(16384, 100277, 1024, 1) < 4.5 * 2 ** 30
+    assert L.ethos_xent_forward_backward_workspace_size(1 << 20, 100277, 1024, 1) == 0
+
+    def fb(**o):
+        a = dict(h=v, ldh=d, w=v, ldw=d, dt=1, y=v, i64=1, ig=-100, red=2, T=T, V=V, d=d, loss=v, save=v, sb=save,
+                 dh=v, dw=v, ws=v, wb=both, err=v, st=None)
+        a.update(o)
+        return L.ethos_xent_forward_backward(*a.values())
+
+    assert fb(red=0) == 1 and fb(y=None) == 1 and fb(dt=0) == 2 and fb(wb=64) == 4 and fb(sb=0) == 4
+    assert fb(ldw=d + 4) == 3
+    assert L.ethos_xent_scale(None, v, 1, 4, None) == 1 and L.ethos_xent_scale(v, v, 1, 0, None) == 0
     assert backward(g=None) == 1 and backward(save=None) == 4 and backward(wb=64) == 4
     assert backward(dh=None, dw=None) == 0
