@@ -323,6 +323,13 @@ int launch_xent(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap&
   auto kern = k_xent_gemm<MODE, PLANES>;
   int st = smem_attr_once(reinterpret_cast<const void*>(kern), xe_smem<PLANES>());
   if (st != ETHOS_OK) return st;
+  // the kernel divides its registers anew and would wait for ever for more
+  // than the launch has
+  static const bool regs_ok = [] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, k_xent_gemm<MODE, PLANES>) == cudaSuccess && fa.numRegs == XE_LAUNCH_REGS;
+  }();
+  if (!regs_ok) return ETHOS_ERR_CUDA;
   int64_t pairs = max_pair_clusters(reinterpret_cast<const void*>(kern), XE_THREADS, xe_smem<PLANES>(), dev);
   if (pairs <= 0) return ETHOS_ERR_CUDA;
   if (pairs > units) pairs = units;

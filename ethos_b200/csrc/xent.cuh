@@ -528,8 +528,10 @@ struct XeCfg {
   static constexpr int kTileN = XE_TILE * kHalves;
   static constexpr int kStageBytes = G2_A_BYTES + kHalves * G2_B_BYTES;
   static constexpr int kStages = PLANES == 1 ? 4 : 6;
-  // blocks by which the second accumulator's MMAs follow the first's: while
-  // it finishes a tile the epilogue empties the first accumulator
+  // blocks by which the second accumulator's MMAs follow the first's at the
+  // end of a tile and the start of the next: while one accumulator works the
+  // epilogue empties the other.  In between they go together, so that the
+  // ring's stages are free for the copies.
   static constexpr int kLag = 2;
   static constexpr int kSegs = PLANES == 1 ? 1 : 6;
 };
@@ -542,8 +544,38 @@ struct XeCtl {
   uint32_t tmem_base;
   int abort;
 };
+// Warps 0 (copies), 1 (MMA), 2 and 3 (idle), 4.. (epilogue).  The epilogue
+// holds 128 accumulator columns per lane, more than an even split of the
+// registers allows, so the first four warps give registers up: the launch's
+// 384 x 168 are divided 128 x 88 + 256 x 208, the same sum (the host checks that
+// the kernel was compiled for XE_LAUNCH_REGS before it launches it).
 constexpr int XE_EPI_WARPS = 8;
-constexpr int XE_THREADS = 64 + 32 * XE_EPI_WARPS;
+constexpr int XE_EPI_WARP0 = 4;
+constexpr int XE_THREADS = 32 * (XE_EPI_WARP0 + XE_EPI_WARPS);
+constexpr int XE_LAUNCH_REGS = 168, XE_LEAN_REGS = 88, XE_EPI_REGS = 208;
+static_assert(XE_EPI_WARP0 * XE_LEAN_REGS + XE_EPI_WARPS * XE_EPI_REGS <=
+                  (XE_EPI_WARP0 + XE_EPI_WARPS) * XE_LAUNCH_REGS,
+              "register split");
+
+// mbar_wait, expanded in place (a kernel that moves registers between its
+// warps makes no calls)
+__device__ __forceinline__ bool xe_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int site) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  const uint64_t limit = *static_cast<volatile unsigned long long*>(&g_wait_limit_ns);
+#pragma unroll 1
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 0u) {
+      if (abort != nullptr && *abort) return false;
+      if (global_timer_ns() - t0 > limit) {
+        if (abort != nullptr) *abort = 1;
+        record_error(err, ETHOS_ERR_TIMEOUT_BASE + site);
+        return false;
+      }
+    }
+  }
+}
 template <int PLANES>
 constexpr int xe_smem() {
   return XeCfg<PLANES>::kStages * XeCfg<PLANES>::kStageBytes + 1024 + static_cast<int>(sizeof(XeCtl));
@@ -744,9 +776,46 @@ __device__ __forceinline__ void row_store_f32(float* row, int col, int cols, int
       if (col + j < cols) row[col + j] = acc ? row[col + j] + v[j] : v[j];
   }
 }
+// a when kFirst, else b (arrays of which the other one has no elements to speak of)
+template <bool kFirst, class A, class B>
+__device__ __forceinline__ auto& pick(A& a, B& b) {
+  if constexpr (kFirst) return a;
+  else return b;
+}
 __device__ __forceinline__ int byte_align(const void* p, int64_t pitch_bytes) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(pitch_bytes);
   return (x & 31u) == 0 ? 32 : ((x & 15u) == 0 ? 16 : 1);
+}
+
+// One lane of a converged warp.  The copy and MMA warps run their loops whole
+// and only issue from one lane, so that addresses and descriptors stay in
+// uniform registers: with the loops on a single lane, issue bound the MMA warp
+// (about 1750 cycles for the eight MMAs of a block that take 1024, with or
+// without copies).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// The 128-byte-swizzle descriptors of umma_desc_sw128 (K-major) and
+// umma_desc_sw128_mn (LBO 8192): constant high word, low word of the address.
+constexpr uint32_t XE_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t xe_desc_lo(uint32_t smem_addr, bool mn) {
+  return ((smem_addr & 0x3FFFFu) >> 4) | (mn ? (8192u >> 4) << 16 : 1u << 16);
+}
+__device__ __forceinline__ void xe_mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %4};\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(XE_DESC_HI), "r"(accumulate)
+      : "memory");
 }
 
 template <int MODE, int PLANES>
@@ -797,8 +866,9 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     rows = 0;  // no row to do again
   volatile int* abort = &ctl->abort;
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < XE_EPI_WARP0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(XE_LEAN_REGS));
+    if (warp == 0) {
       XeWalk<MODE, PLANES> walk(args, rows, pair, pairs);
       XeStep st;
       RingPos rp;
@@ -806,7 +876,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
       while (ok && walk.next(st)) {
         const int m0 = st.m0 + static_cast<int>(rank) * G2_BM;
         const int n0 = st.n0 + static_cast<int>(rank) * (XE_TILE / 2);
-        const int halves = st.second ? 2 : 1;
+        const uint32_t bytes = 2u * (G2_A_BYTES + (st.second ? 2 : 1) * G2_B_BYTES);
         const CUtensorMap* ta = st.prod == 0 ? &tmA0 : &tmA1;
         const CUtensorMap* tb = st.prod == 0 ? &tmB0 : &tmB1;
         const XeProduct& p = args.p[st.prod];
@@ -814,29 +884,32 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
           const int ya = PLANES == 1 ? 0 : xe_plane_a(seg) * p.a_plane_rows;
           const int yb = PLANES == 1 ? 0 : xe_plane_b(seg) * p.b_plane_rows;
           for (int kb = st.kb0; kb < st.kb1; ++kb) {
-            if (!mbar_wait(&ctl->empty[rp.stage], rp.phase ^ 1u, abort, err, 1)) {
-              ok = false;
-              break;
-            }
+            ok = __all_sync(0xffffffffu, xe_wait(&ctl->empty[rp.stage], rp.phase ^ 1u, abort, err, 1));
+            if (!ok) break;
             uint8_t* sa = smem + rp.stage * STAGE_BYTES;
-            if (leader) mbar_arrive_expect_tx(&ctl->full[rp.stage], 2 * (G2_A_BYTES + halves * G2_B_BYTES));
+            uint8_t* sb = sa + G2_A_BYTES;
             const uint32_t fb = cluster_map(smem_u32(&ctl->full[rp.stage]), 0);
-            if (MODE == XE_GRADS && st.prod == 1) {
-              tma_load_2d_pair(sa, ta, fb, m0, ya + kb * G2_BK);
-              tma_load_2d_pair(sa + 8192, ta, fb, m0 + 64, ya + kb * G2_BK);
-            } else {
-              tma_load_2d_pair(sa, ta, fb, kb * G2_BK, ya + m0);
-            }
-            for (int h = 0; h < halves; ++h) {
-              uint8_t* sb = sa + G2_A_BYTES + h * G2_B_BYTES;
-              const int nh = n0 + h * XE_TILE;
-              if (MODE == XE_GRADS) {
-                tma_load_2d_pair(sb, tb, fb, nh, yb + kb * G2_BK);
-                tma_load_2d_pair(sb + 8192, tb, fb, nh + 64, yb + kb * G2_BK);
+            if (elect_one()) {
+              if (leader) mbar_arrive_expect_tx(&ctl->full[rp.stage], bytes);
+              if (MODE == XE_GRADS && st.prod == 1) {
+                tma_load_2d_pair(sa, ta, fb, m0, ya + kb * G2_BK);
+                tma_load_2d_pair(sa + 8192, ta, fb, m0 + 64, ya + kb * G2_BK);
               } else {
-                tma_load_2d_pair(sb, tb, fb, kb * G2_BK, yb + nh);
+                tma_load_2d_pair(sa, ta, fb, kb * G2_BK, ya + m0);
+              }
+              if (MODE == XE_GRADS) {
+                tma_load_2d_pair(sb, tb, fb, n0, yb + kb * G2_BK);
+                tma_load_2d_pair(sb + 8192, tb, fb, n0 + 64, yb + kb * G2_BK);
+                if (st.second) {
+                  tma_load_2d_pair(sb + G2_B_BYTES, tb, fb, n0 + XE_TILE, yb + kb * G2_BK);
+                  tma_load_2d_pair(sb + G2_B_BYTES + 8192, tb, fb, n0 + XE_TILE + 64, yb + kb * G2_BK);
+                }
+              } else {
+                tma_load_2d_pair(sb, tb, fb, kb * G2_BK, yb + n0);
+                if (st.second) tma_load_2d_pair(sb + G2_B_BYTES, tb, fb, kb * G2_BK, yb + n0 + XE_TILE);
               }
             }
+            __syncwarp();
             rp.advance(STAGES);
           }
         }
@@ -845,16 +918,25 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         // as in k_gemm2sm: both CTAs' copies complete on the leader's
         // barriers; the peer waits a bounded 100 us for its own to land
         if (leader) {
-          rp.drain(ctl->full, STAGES, err, 5);
+          int sg = rp.stage;
+          uint32_t ph = rp.phase;
+          for (int i = 0; i < STAGES && i < rp.issued; ++i) {
+            if (sg == 0) {
+              sg = STAGES - 1;
+              ph ^= 1u;
+            } else {
+              --sg;
+            }
+            xe_wait(&ctl->full[sg], ph, nullptr, err, 5);
+          }
         } else {
           const uint64_t t0 = global_timer_ns();
           while (global_timer_ns() - t0 < 100000ull) {
           }
         }
       }
-    }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
       // One stream of K blocks per accumulator.  With two, the second follows
       // kLag blocks behind the first and releases the ring's stages.
       XeWalk<MODE, PLANES> w0(args, rows, pair, pairs), w1(args, rows, pair, pairs);
@@ -868,18 +950,26 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
       int begun0 = 0, done1 = 0;     // tiles begun by stream 0, finished by stream 1
       bool more0 = true, more1 = HALVES == 2;
       bool ok = true;
+      const uint32_t smem0 = smem_u32(smem);
       auto mma_block = [&](const XeStep& st, int stage, int half, uint32_t d, bool first) {
         const bool a_mn = MODE == XE_GRADS && st.prod == 1;
-        const uint32_t idesc = umma_idesc_bf16_f32_major(2 * G2_BM, XE_TILE, a_mn, MODE == XE_GRADS);
-        const uint32_t a_base = smem_u32(smem + stage * STAGE_BYTES);
-        const uint32_t b_base = a_base + G2_A_BYTES + half * G2_B_BYTES;
+        constexpr bool b_mn = MODE == XE_GRADS;
+        const uint32_t idesc = umma_idesc_bf16_f32_major(2 * G2_BM, XE_TILE, a_mn, b_mn);
+        const uint32_t a_base = smem0 + static_cast<uint32_t>(stage * STAGE_BYTES);
+        const uint32_t a_lo = xe_desc_lo(a_base, a_mn);
+        const uint32_t b_lo = xe_desc_lo(a_base + static_cast<uint32_t>(G2_A_BYTES + half * G2_B_BYTES), b_mn);
+        const uint32_t a_step = a_mn ? 2048u >> 4 : 32u >> 4;
+        constexpr uint32_t b_step = b_mn ? 2048u >> 4 : 32u >> 4;
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < G2_BK / 16; ++k) {
-          const uint64_t ad = a_mn ? umma_desc_sw128_mn(a_base + k * 2048, 8192) : umma_desc_sw128(a_base + k * 32);
-          const uint64_t bd =
-              MODE == XE_GRADS ? umma_desc_sw128_mn(b_base + k * 2048, 8192) : umma_desc_sw128(b_base + k * 32);
-          umma_bf16_pair(d, ad, bd, idesc, (!first || k > 0) ? 1u : 0u);
+          for (int k = 0; k < G2_BK / 16; ++k)
+            xe_mma(d, a_lo + k * a_step, b_lo + k * b_step, idesc, (!first || k > 0) ? 1u : 0u);
         }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma_commit_pair_mc(bar, 0x3);
+        __syncwarp();
       };
       while (ok && (more0 || more1)) {
         // stream 0 may begin tile j once stream 1 is through tile j - 2: the
@@ -895,20 +985,16 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
             const uint32_t par = static_cast<uint32_t>(HALVES == 2 ? it0 : it0 >> 1) & 1u;
             if (b0 == 0) {
               ++begun0;
-              if (!mbar_wait(&ctl->acc_empty[buf], par ^ 1u, abort, err, 2)) {
-                ok = false;
-                break;
-              }
+              ok = __all_sync(0xffffffffu, xe_wait(&ctl->acc_empty[buf], par ^ 1u, abort, err, 2));
+              if (!ok) break;
             }
-            if (!mbar_wait(&ctl->full[stage0], phase0, abort, err, 3)) {
-              ok = false;
-              break;
-            }
+            ok = __all_sync(0xffffffffu, xe_wait(&ctl->full[stage0], phase0, abort, err, 3));
+            if (!ok) break;
             tc_fence_after();
             mma_block(s0, stage0, 0, tmem + static_cast<uint32_t>(buf * XE_TILE), b0 == 0);
-            if (HALVES == 1) umma_commit_pair_mc(&ctl->empty[stage0], 0x3);
+            if (HALVES == 1) commit(&ctl->empty[stage0]);
             if (++b0 == n0) {
-              umma_commit_pair_mc(&ctl->acc_full[buf], 0x3);
+              commit(&ctl->acc_full[buf]);
               ++it0;
             }
             if (++stage0 == STAGES) {
@@ -918,7 +1004,9 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
             ++ahead;
           }
         }
-        if (HALVES == 2 && more1 && (ahead > Cfg::kLag || !more0 || !go0)) {
+        // b0: blocks of the current tile that stream 0 has done (n0 at its end)
+        const int lag = more0 && go0 && (b0 <= Cfg::kLag || n0 - b0 <= Cfg::kLag) ? Cfg::kLag : 0;
+        while (HALVES == 2 && more1 && (ahead > lag || !more0 || !go0)) {
           if (b1 == n1) {
             b1 = n1 = 0;
             while (n1 == 0 && (more1 = w1.next(s1))) n1 = Cfg::kSegs * max(0, s1.kb1 - s1.kb0);
@@ -926,33 +1014,38 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
           if (more1) {
             if (s1.second) {
               if (b1 == 0) {
-                if (!mbar_wait(&ctl->acc_empty[1], (static_cast<uint32_t>(it1) & 1u) ^ 1u, abort, err, 2)) {
-                  ok = false;
-                  break;
-                }
+                ok = __all_sync(0xffffffffu, xe_wait(&ctl->acc_empty[1], (static_cast<uint32_t>(it1) & 1u) ^ 1u, abort,
+                                                     err, 2));
+                if (!ok) break;
                 tc_fence_after();
               }
               mma_block(s1, stage1, 1, tmem + static_cast<uint32_t>(XE_TILE), b1 == 0);
             }
-            umma_commit_pair_mc(&ctl->empty[stage1], 0x3);
+            commit(&ctl->empty[stage1]);
             if (++b1 == n1) {
               ++done1;
               if (s1.second) {
-                umma_commit_pair_mc(&ctl->acc_full[1], 0x3);
+                commit(&ctl->acc_full[1]);
                 ++it1;
               }
             }
             if (++stage1 == STAGES) stage1 = 0;
             --ahead;
+            if (!go0 && begun0 <= done1 + 1) break;  // stream 0 may go on
           }
         }
       }
-      if (!ok || *abort) {
-        umma_commit_pair(&ctl->drain);
-        mbar_wait(&ctl->drain, 0, nullptr, err, 6);
+      if (!__all_sync(0xffffffffu, ok && !*abort)) {
+        // drain: every MMA of the pair done before the memory goes away (the
+        // same lane issued them all)
+        if (elect_one()) umma_commit_pair(&ctl->drain);
+        __syncwarp();
+        xe_wait(&ctl->drain, 0, nullptr, err, 6);
       }
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(XE_EPI_REGS));
     // Epilogue warps never leave the walk early: after an abort they skip the
     // work but still arrive on every acc_empty phase.  A warp takes its 128
     // columns of an accumulator into registers and releases it before it
@@ -960,10 +1053,10 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     XeWalk<MODE, PLANES> walk(args, rows, pair, pairs);
     XeStep st;
     const int q = warp & 3;
-    const int ch = (warp - 2) >> 2;  // column half of an accumulator
+    const int ch = (warp - XE_EPI_WARP0) >> 2;  // column half of an accumulator
     const uint32_t acc_empty0 = cluster_map(smem_u32(&ctl->acc_empty[0]), 0);
     const uint32_t acc_empty1 = cluster_map(smem_u32(&ctl->acc_empty[1]), 0);
-    int it[2] = {0, 0};  // accumulations taken (HALVES 1: all in it[0])
+    int it0 = 0, it1 = 0;  // accumulations taken (HALVES 1: all in it0)
     bool ok = true;
     // per-row state (this lane's row of the tile)
     int y = -1;
@@ -972,7 +1065,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     float c2 = 0.0f;                        // KEEP: shift, DLOGITS: logsumexp, in units of log 2
     float g = 1.0f, at_label = 0.0f;        // DLOGITS
     const float scale = MODE == XE_GRADS ? xe_scale(args.rw, args.grad, args.reduction) : 1.0f;
-    float v[CHUNKS][32];
+    float sum[HALVES == 1 ? CHUNKS : 1][32];  // fp32: accumulations added up
     while (walk.next(st)) {
       const bool any = st.kb0 < st.kb1;
       const int row = st.m0 + static_cast<int>(rank) * G2_BM + q * 32 + lane;
@@ -995,37 +1088,58 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
       }
 #pragma unroll 1
       for (int half = 0; half < (st.second ? 2 : 1); ++half) {
-        const int buf = HALVES == 2 ? half : it[0] & 1;
-        if (any) {
-          const int n = HALVES == 2 ? it[half] : it[0] >> 1;
-          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->acc_full[buf], static_cast<uint32_t>(n) & 1u, abort, err, 4));
-          ++it[HALVES == 2 ? half : 0];
-          tc_fence_after();
-          if (ok) {
-#pragma unroll
-            for (int k = 0; k < CHUNKS; ++k) {
-              const uint32_t ta = tmem_addr(tmem, q * 32, buf * XE_TILE + (ch * CHUNKS + k) * 32);
-              if (HALVES == 1 && !st.kfirst) {
-                float x[32];
-                tmem_ld32(ta, x);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[k][i] += x[i];
-              } else {
-                tmem_ld32(ta, v[k]);
-              }
+        const int col0 = st.n0 + half * XE_TILE + ch * CHUNKS * 32;
+        if (!any) {  // no rows to add up: zeros
+          if (MODE == XE_GRADS && st.prod == 1 && row < args.p[1].M) {
+            const int d = args.p[1].N;
+            for (int c = col0; c < min(d, col0 + CHUNKS * 32); ++c) {
+              if (args.dw_bf16) static_cast<__nv_bfloat16*>(args.dw)[static_cast<int64_t>(row) * d + c] = __float2bfloat16_rn(0.0f);
+              else static_cast<float*>(args.dw)[static_cast<int64_t>(row) * d + c] = 0.0f;
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_remote(buf ? acc_empty1 : acc_empty0);
-        } else {
-#pragma unroll
-          for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[k][i] = 0.0f;
+          continue;
         }
+        const int buf = HALVES == 2 ? half : it0 & 1;
+        const int n = HALVES == 2 ? (half ? it1 : it0) : it0 >> 1;
+        if (ok) ok = __all_sync(0xffffffffu, xe_wait(&ctl->acc_full[buf], static_cast<uint32_t>(n) & 1u, abort, err, 4));
+        if (half) ++it1;
+        else ++it0;
+        tc_fence_after();
+        float fresh[HALVES == 2 ? CHUNKS : 1][32];
+        float(&v)[CHUNKS][32] = pick<HALVES == 1>(sum, fresh);
+        if (ok) {
+          const uint32_t ta = tmem_addr(tmem, q * 32, buf * XE_TILE + ch * CHUNKS * 32);
+          if constexpr (HALVES == 2) {
+#pragma unroll
+            for (int k = 0; k < CHUNKS; k += 2) {
+              float x[64];
+              tmem_ld64(ta + 32 * k, x);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                v[k][i] = x[i];
+                v[k + 1][i] = x[32 + i];
+              }
+            }
+          } else {
+            if (st.kfirst) {
+#pragma unroll
+              for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[k][i] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k) {
+              float x[32];
+              tmem_ld32(ta + 32 * k, x);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[k][i] += x[i];
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(buf ? acc_empty1 : acc_empty0);
         if (!ok || !st.klast) continue;
-        const int col0 = st.n0 + half * XE_TILE + ch * CHUNKS * 32;
         if (MODE == XE_STATS || MODE == XE_KEEP) {
           const int N = args.p[0].N;
 #pragma unroll
