@@ -100,12 +100,12 @@ EXPORTS = {
     # ids, ids_i64, dy, dtype, tokens, vocab, dim, padding, scale, d_weight, workspace,
     # workspace_bytes, dev_err, stream
     "ethos_embedding_backward": (_I, [_P, _I, _P, _I, _I64, _I64, _I64, _I64, _F, _P, _P, _SZ, _P, _P]),
-    "ethos_balance_scratch_size": (_SZ, []),
-    # ids, ids_i64, weights, dtype, mask, tokens, heads, k, experts, counts, loss, scratch, dev_err,
-    # stream
-    "ethos_balance_forward": (_I, [_P, _I, _P, _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
-    # ids, ids_i64, dtype, mask, tokens, heads, k, experts, counts, scratch, grad, d_weights, stream
-    "ethos_balance_backward": (_I, [_P, _I, _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
+    "ethos_balance_scratch_size": (_SZ, [_I64, _I64, _I64]),
+    # ids, ids_i64, weights, dtype, mask, tokens, heads, k, experts, counts, loss, scratch,
+    # scratch_bytes, dev_err, stream
+    "ethos_balance_forward": (_I, [_P, _I, _P, _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _SZ, _P, _P]),
+    # dtype, tokens, heads, k, experts, scratch, scratch_bytes, grad, d_weights, stream
+    "ethos_balance_backward": (_I, [_I, _I64, _I64, _I64, _I64, _P, _SZ, _P, _P, _P]),
     "ethos_xent_save_size": (_SZ, [_I64, _I64, _I64, _I]),
     "ethos_xent_forward_workspace_size": (_SZ, [_I64, _I64, _I64, _I]),
     # hidden, ldh, weight, ldw, dtype, labels, labels_i64, ignore_index, reduction, tokens, vocab, dim,
@@ -117,7 +117,7 @@ EXPORTS = {
     # loss, save, save_bytes, d_hidden, d_weight, workspace, workspace_bytes, dev_err, stream
     "ethos_xent_forward_backward": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _I64, _I, _I64, _I64, _I64, _P, _P, _SZ, _P,
                                          _P, _P, _SZ, _P, _P]),
-    "ethos_xent_scale": (_I, [_P, _P, _I, _I64, _P]),
+    "ethos_xent_scale": (_I, [_P, _P, _I64, _P, _I64, _I, _P]),
     "ethos_xent_backward_workspace_size": (_SZ, [_I64, _I64, _I64, _I]),
     # hidden, ldh, weight, ldw, dtype, reduction, tokens, vocab, dim, grad, save, save_bytes, d_hidden,
     # d_weight, workspace, workspace_bytes, dev_err, stream

@@ -11,6 +11,12 @@
 // loss needs no per-expert sums of weights: the counts are integers, whose
 // atomics give the same result in any order, and the weighted sum has a fixed
 // order.
+//
+// Counting.  Popular experts make atomics on one address queue up in L2: 2.1 M
+// selections that crowd (density ~ id^-1/2 of 262 144 experts) took 41 us.  So
+// with many selections each block counts one range of experts in shared memory
+// over its part of the selections, and adds its non-zero counts to the global
+// ones; the ids are read once per range (6 times at 262 144 experts).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -20,40 +26,129 @@
 namespace ethos {
 
 constexpr int BAL_THREADS = 256;
-constexpr int BAL_MAX_BLOCKS = 1184;  // 8 per SM of a B200
+constexpr int BAL_MAX_BLOCKS = 1184;   // 8 per SM of a B200
+constexpr int BAL_COUNT_THREADS = 1024;
+constexpr int BAL_RANGE = 51200;       // experts counted by one block (200 KB of shared memory)
 
-// scratch of one call, after the counts
+// Scratch of one call: the header, then sel [tokens * H * k] fp32, the count of
+// each selection's expert (0 for a selection left out), for the backward.
 struct BalScratch {
   int tokens;     // unmasked tokens
   unsigned done;  // blocks of k_balance_loss that have added their part
+  int live[BAL_MAX_BLOCKS];
   double part[BAL_MAX_BLOCKS];
 };
 
+// 4 consecutive ids (16-byte loads)
+__device__ __forceinline__ void load_ids4(const int32_t* p, int (&e)[4]) {
+  const int4 v = *reinterpret_cast<const int4*>(p);
+  e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w;
+}
+__device__ __forceinline__ int narrow_id(int64_t x) {  // out of int32: out of any range
+  return x < 0 || x > INT32_MAX ? -1 : static_cast<int>(x);
+}
+__device__ __forceinline__ void load_ids4(const int64_t* p, int (&e)[4]) {
+  const longlong2 a = reinterpret_cast<const longlong2*>(p)[0], b = reinterpret_cast<const longlong2*>(p)[1];
+  e[0] = narrow_id(a.x); e[1] = narrow_id(a.y); e[2] = narrow_id(b.x); e[3] = narrow_id(b.y);
+}
+__device__ __forceinline__ int load_id(const int32_t* p) { return *p; }
+__device__ __forceinline__ int load_id(const int64_t* p) { return narrow_id(*p); }
+
+// Calls f(i, id) for the selections i in [i0, i1) of unmasked tokens, threads
+// of the block in turn, four at a time where addresses allow.
+template <class I, class F>
+__device__ __forceinline__ void each_selection(const I* __restrict__ ids, const uint8_t* __restrict__ mask,
+                                               int per_token, bool quads, int i0, int i1, F f) {
+  if (quads) {  // per_token % 4 == 0, ids 16-byte aligned: a quad is of one token
+#pragma unroll 2
+    for (int i = i0 + 4 * static_cast<int>(threadIdx.x); i < i1; i += 4 * static_cast<int>(blockDim.x)) {
+      if (mask != nullptr && !mask[i / per_token]) continue;
+      int e[4];
+      load_ids4(ids + i, e);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(i + j, e[j]);
+    }
+  } else {
+    for (int i = i0 + static_cast<int>(threadIdx.x); i < i1; i += static_cast<int>(blockDim.x)) {
+      if (mask != nullptr && !mask[i / per_token]) continue;
+      f(i, load_id(ids + i));
+    }
+  }
+}
+
+// Unmasked tokens of part b of `parts`, into live[b] (thread 0 of the block).
+__device__ __forceinline__ void count_live(const uint8_t* __restrict__ mask, int tokens, int b, int parts,
+                                           BalScratch* __restrict__ s) {
+  __shared__ int sum;
+  const int per = (tokens + parts - 1) / parts;
+  const int t0 = min(tokens, b * per), t1 = min(tokens, t0 + per);
+  if (threadIdx.x == 0) {
+    sum = 0;
+    if (b == 0) s->done = 0;
+  }
+  __syncthreads();
+  int n = mask == nullptr && threadIdx.x == 0 ? t1 - t0 : 0;
+  if (mask != nullptr)
+    for (int t = t0 + static_cast<int>(threadIdx.x); t < t1; t += static_cast<int>(blockDim.x)) n += mask[t] ? 1 : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  if ((threadIdx.x & 31) == 0 && n) atomicAdd(&sum, n);
+  __syncthreads();
+  if (threadIdx.x == 0) s->live[b] = sum;
+}
+
+// Few selections: atomics on the global counts.
 template <class I>
 __global__ void __launch_bounds__(BAL_THREADS) k_balance_count(const I* __restrict__ ids,
-                                                               const uint8_t* __restrict__ mask, int64_t tokens,
-                                                               int per_token, int64_t experts,
+                                                               const uint8_t* __restrict__ mask, int tokens,
+                                                               int per_token, int experts, bool quads,
                                                                int* __restrict__ counts, BalScratch* __restrict__ s,
                                                                int* err) {
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t n = tokens * per_token;
-  const int64_t nt = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t tid = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  for (int64_t i = tid; i < n; i += nt) {
-    if (mask != nullptr && !mask[i / per_token]) continue;
-    const int64_t e = static_cast<int64_t>(__ldg(ids + i));
-    if (e < 0 || e >= experts) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
-    else atomicAdd(counts + e, 1);
-  }
-  if (mask != nullptr) {
-    int live = 0;
-    for (int64_t t = tid; t < tokens; t += nt) live += mask[t] ? 1 : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) live += __shfl_xor_sync(0xffffffffu, live, o);
-    if ((threadIdx.x & 31) == 0 && live) atomicAdd(&s->tokens, live);
-  } else if (tid == 0) {
-    s->tokens = static_cast<int>(tokens);
+  const int n = tokens * per_token, b = blockIdx.x, parts = gridDim.x;
+  const int per = ((n + parts - 1) / parts + 3) / 4 * 4;
+  const int64_t i0 = static_cast<int64_t>(b) * per;
+  if (i0 < n)
+    each_selection(ids, mask, per_token, quads, static_cast<int>(i0), static_cast<int>(i0 + per < n ? i0 + per : n),
+                   [&](int, int e) {
+                     if (e < 0 || e >= experts) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
+                     else atomicAdd(counts + e, 1);
+                   });
+  count_live(mask, tokens, b, parts, s);
+}
+
+// Many: block b counts the experts [r range, (r + 1) range), r = b % ranges,
+// over part b / ranges of the selections.
+template <class I>
+__global__ void __launch_bounds__(BAL_COUNT_THREADS) k_balance_count_ranges(const I* __restrict__ ids,
+                                                                            const uint8_t* __restrict__ mask,
+                                                                            int tokens, int per_token, int experts,
+                                                                            bool quads, int ranges, int range,
+                                                                            int* __restrict__ counts,
+                                                                            BalScratch* __restrict__ s, int* err) {
+  extern __shared__ int mine[];
+  pdl_launch_dependents();
+  const int r = blockIdx.x % ranges, b = blockIdx.x / ranges, parts = gridDim.x / ranges;
+  const int lo = r * range, width = min(range, experts - lo);
+  for (int i = threadIdx.x; i < width; i += BAL_COUNT_THREADS) mine[i] = 0;
+  __syncthreads();
+  pdl_wait();
+  const int n = tokens * per_token;
+  const int per = ((n + parts - 1) / parts + 3) / 4 * 4;
+  const int64_t i0 = static_cast<int64_t>(b) * per;
+  if (i0 < n)
+    each_selection(ids, mask, per_token, quads, static_cast<int>(i0), static_cast<int>(i0 + per < n ? i0 + per : n),
+                   [&](int, int e) {
+                     if (r == 0 && (e < 0 || e >= experts)) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
+                     const unsigned at = static_cast<unsigned>(e - lo);
+                     if (at < static_cast<unsigned>(width)) atomicAdd(mine + at, 1);
+                   });
+  if (r == 0) count_live(mask, tokens, b, parts, s);
+  __syncthreads();
+  for (int i = threadIdx.x; i < width; i += BAL_COUNT_THREADS) {
+    const int c = mine[i];
+    if (c) atomicAdd(counts + lo + i, c);
   }
 }
 
@@ -64,24 +159,64 @@ __device__ __forceinline__ double balance_coef(int live, int64_t experts, int he
   return static_cast<double>(experts) / (nh * nh * k);
 }
 
+__device__ __forceinline__ void load_w4(const float* p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void load_w4(const __nv_bfloat16* p, float (&v)[4]) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ void store_w4(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store_w4(__nv_bfloat16* p, const float (&v)[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// Sums w c[id] and leaves c[id] in sel.  Thread by thread the terms are fixed,
+// blocks add in fp64, and the last block adds the blocks in order.
 template <class I, class W>
 __global__ void __launch_bounds__(BAL_THREADS) k_balance_loss(const I* __restrict__ ids, const W* __restrict__ w,
-                                                              const uint8_t* __restrict__ mask, int64_t tokens,
-                                                              int heads, int k, int64_t experts,
+                                                              const uint8_t* __restrict__ mask, int tokens, int heads,
+                                                              int k, int experts, bool quads, int live_parts,
                                                               const int* __restrict__ counts,
-                                                              BalScratch* __restrict__ s, float* __restrict__ loss) {
+                                                              BalScratch* __restrict__ s, float* __restrict__ sel,
+                                                              float* __restrict__ loss) {
   __shared__ double red[BAL_THREADS];
   __shared__ bool last;
   pdl_launch_dependents();
   pdl_wait();
   const int per_token = heads * k;
-  const int64_t n = tokens * per_token;
-  const int64_t nt = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int n = tokens * per_token;
+  const int nt = gridDim.x * BAL_THREADS, tid = blockIdx.x * BAL_THREADS + threadIdx.x;
   double acc = 0.0;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += nt) {
-    if (mask != nullptr && !mask[i / per_token]) continue;
-    const int64_t e = static_cast<int64_t>(__ldg(ids + i));
-    if (e >= 0 && e < experts) acc += static_cast<double>(static_cast<float>(w[i]) * static_cast<float>(counts[e]));
+  if (quads) {
+#pragma unroll 2
+    for (int64_t i = 4ll * tid; i < n; i += 4ll * nt) {
+      int e[4];
+      float x[4], c[4];
+      load_ids4(ids + i, e);
+      load_w4(w + i, x);
+      const bool in = mask == nullptr || mask[static_cast<int>(i) / per_token];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = in && e[j] >= 0 && e[j] < experts ? static_cast<float>(__ldg(counts + e[j])) : 0.0f;
+      store_w4(sel + i, c);
+      // a weight left out is not read into the sum (it may be NaN)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc += static_cast<double>(c[j] != 0.0f ? x[j] * c[j] : 0.0f);
+    }
+  } else {
+    for (int64_t i = tid; i < n; i += nt) {
+      const int e = load_id(ids + i);
+      const bool in = mask == nullptr || mask[static_cast<int>(i) / per_token];
+      const float c = in && e >= 0 && e < experts ? static_cast<float>(__ldg(counts + e)) : 0.0f;
+      sel[i] = c;
+      acc += static_cast<double>(c != 0.0f ? static_cast<float>(w[i]) * c : 0.0f);
+    }
   }
   red[threadIdx.x] = acc;
   __syncthreads();
@@ -96,40 +231,48 @@ __global__ void __launch_bounds__(BAL_THREADS) k_balance_loss(const I* __restric
   }
   __syncthreads();
   if (!last) return;
-  // the last block adds the parts in block order
   __threadfence();
+  __shared__ int live;
+  if (threadIdx.x == 0) live = 0;
   acc = 0.0;
   for (int b = threadIdx.x; b < static_cast<int>(gridDim.x); b += BAL_THREADS)
     acc += *static_cast<volatile double*>(&s->part[b]);
+  int l = 0;
+  for (int b = threadIdx.x; b < live_parts; b += BAL_THREADS) l += s->live[b];
   red[threadIdx.x] = acc;
   __syncthreads();
+  if (l) atomicAdd(&live, l);
   for (int o = BAL_THREADS / 2; o > 0; o >>= 1) {
     if (static_cast<int>(threadIdx.x) < o) red[threadIdx.x] += red[threadIdx.x + o];
     __syncthreads();
   }
-  if (threadIdx.x == 0) *loss = static_cast<float>(red[0] * balance_coef(s->tokens, experts, heads, k));
+  if (threadIdx.x == 0) {
+    s->tokens = live;
+    *loss = static_cast<float>(red[0] * balance_coef(live, experts, heads, k));
+  }
 }
 
-template <class I, class W>
-__global__ void __launch_bounds__(BAL_THREADS) k_balance_bwd(const I* __restrict__ ids,
-                                                             const uint8_t* __restrict__ mask, int64_t tokens,
-                                                             int heads, int k, int64_t experts,
-                                                             const int* __restrict__ counts,
+// dw = grad C sel
+template <class W>
+__global__ void __launch_bounds__(BAL_THREADS) k_balance_bwd(int n, int heads, int k, int experts, bool quads,
                                                              const BalScratch* __restrict__ s,
+                                                             const float* __restrict__ sel,
                                                              const float* __restrict__ grad, W* __restrict__ dw) {
   pdl_launch_dependents();
   pdl_wait();
   const float c = static_cast<float>(balance_coef(s->tokens, experts, heads, k) * static_cast<double>(*grad));
-  const int per_token = heads * k;
-  const int64_t n = tokens * per_token;
-  const int64_t nt = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += nt) {
-    float v = 0.0f;
-    if (mask == nullptr || mask[i / per_token]) {
-      const int64_t e = static_cast<int64_t>(__ldg(ids + i));
-      if (e >= 0 && e < experts) v = c * static_cast<float>(counts[e]);
+  const int nt = gridDim.x * BAL_THREADS, tid = blockIdx.x * BAL_THREADS + threadIdx.x;
+  if (quads) {
+#pragma unroll 4
+    for (int64_t i = 4ll * tid; i < n; i += 4ll * nt) {
+      float x[4];
+      load_w4(sel + i, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] *= c;
+      store_w4(dw + i, x);
     }
-    dw[i] = static_cast<W>(v);
+  } else {
+    for (int64_t i = tid; i < n; i += nt) dw[i] = static_cast<W>(sel[i] * c);
   }
 }
 

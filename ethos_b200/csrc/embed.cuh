@@ -20,19 +20,32 @@
 
 namespace ethos {
 
-constexpr int EMB_SORT_THREADS = 512;
+constexpr int EMB_SORT_THREADS = 1024;
 constexpr int EMB_SORT_WARPS = EMB_SORT_THREADS / 32;
 constexpr int EMB_MAX_RANGE = 1024;  // ids owned by one block of the sort
 constexpr int EMB_CHUNK = 32;        // sorted tokens summed by one unit
 constexpr int64_t EMB_NO_PADDING = INT64_MIN;
 
-template <class T>
-struct Vec16;  // 16-byte vector of T as fp32 values
+// N consecutive elements of a row as fp32 values: one 16-byte access, or
+// (kVec false, a row pitch or base that is not 16-byte aligned) one element.
+// Raw is what a load leaves in registers until it is used.
+template <class T, bool kVec>
+struct RowAccess {  // one element
+  static constexpr int N = 1;
+  using Raw = T;
+  static __device__ __forceinline__ Raw load_raw(const T* p) { return *p; }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&v)[1]) { v[0] = static_cast<float>(r); }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[1]) {
+    if constexpr (std::is_same<T, float>::value) *p = v[0];
+    else *p = __float2bfloat16_rn(v[0]);
+  }
+};
 template <>
-struct Vec16<float> {
+struct RowAccess<float, true> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
+  using Raw = float4;
+  static __device__ __forceinline__ Raw load_raw(const float* p) { return *reinterpret_cast<const float4*>(p); }
+  static __device__ __forceinline__ void unpack(const Raw& a, float (&v)[4]) {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   }
   static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
@@ -40,10 +53,11 @@ struct Vec16<float> {
   }
 };
 template <>
-struct Vec16<__nv_bfloat16> {
+struct RowAccess<__nv_bfloat16, true> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+  using Raw = uint4;
+  static __device__ __forceinline__ Raw load_raw(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
+  static __device__ __forceinline__ void unpack(const Raw& u, float (&v)[8]) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -60,27 +74,10 @@ struct Vec16<__nv_bfloat16> {
     *reinterpret_cast<uint4*>(p) = u;
   }
 };
-// N consecutive elements of a row: one 16-byte access, or (kVec false, a row
-// pitch or base that is not 16-byte aligned) one element
-template <class T, bool kVec>
-struct RowAccess {
-  static constexpr int N = kVec ? Vec16<T>::N : 1;
-  static __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
-    if constexpr (kVec) {
-      Vec16<T>::load(p, v);
-    } else {
-      v[0] = static_cast<float>(*p);
-    }
-  }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[N]) {
-    if constexpr (kVec) {
-      Vec16<T>::store(p, v);
-    } else if constexpr (std::is_same<T, float>::value) {
-      *p = v[0];
-    } else {
-      *p = __float2bfloat16_rn(v[0]);
-    }
-  }
+template <class T>
+struct Vec16 : RowAccess<T, true> {
+  using A = RowAccess<T, true>;
+  static __device__ __forceinline__ void load(const T* p, float (&v)[A::N]) { A::unpack(A::load_raw(p), v); }
 };
 
 // ---------------------------------------------------------------- forward --
@@ -106,7 +103,7 @@ __global__ void __launch_bounds__(256) k_embed_fwd(const I* __restrict__ ids, co
 #pragma unroll
       for (int j = 0; j < A::N; ++j) v[j] = 0.0f;
     } else {
-      A::load(w + id * ldw + c, v);
+      A::unpack(A::load_raw(w + id * ldw + c), v);
 #pragma unroll
       for (int j = 0; j < A::N; ++j) v[j] *= scale;
     }
@@ -147,7 +144,7 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __rest
   const int64_t t0 = static_cast<int64_t>(warp) * part;
   const int64_t t1 = t0 + part < tokens ? t0 + part : tokens;
   int below = 0;
-#pragma unroll 4
+#pragma unroll 8
   for (int64_t t = t0 + lane; t < t1; t += 32) {
     const int64_t id = static_cast<int64_t>(__ldg(ids + t));
     if (id == padding) continue;
@@ -166,16 +163,13 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __rest
   int base = 0;
 #pragma unroll
   for (int w = 0; w < EMB_SORT_WARPS; ++w) base += below_sum[w];
-  // exclusive scan over the ids (two per thread), then over the warps of each id
-  static_assert(EMB_MAX_RANGE <= 2 * EMB_SORT_THREADS, "two ids per thread");
-  int tot[2] = {0, 0};
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = 2 * static_cast<int>(threadIdx.x) + j;
-    if (r < n)
-      for (int w = 0; w < EMB_SORT_WARPS; ++w) tot[j] += cnt[w * range + r];
-  }
-  int incl = tot[0] + tot[1];
+  // exclusive scan over the ids (one per thread), then over the warps of each id
+  static_assert(EMB_MAX_RANGE <= EMB_SORT_THREADS, "one id per thread");
+  const int r = threadIdx.x;
+  int tot = 0;
+  if (r < n)
+    for (int w = 0; w < EMB_SORT_WARPS; ++w) tot += cnt[w * range + r];
+  int incl = tot;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, incl, o);
@@ -183,44 +177,49 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __rest
   }
   if (lane == 31) warp_sum[warp] = incl;
   __syncthreads();
-  int run = base + incl - (tot[0] + tot[1]);
-  for (int w = 0; w < warp; ++w) run += warp_sum[w];
+  int at0 = base + incl - tot;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = 2 * static_cast<int>(threadIdx.x) + j;
-    if (r < n) {
-      offs[lo + r] = run;
-      int at = run;
-      for (int w = 0; w < EMB_SORT_WARPS; ++w) {
-        const int c = cnt[w * range + r];
-        cnt[w * range + r] = at;
-        at += c;
-      }
-      run = at;
-      if (lo + r == vocab - 1) offs[vocab] = at;
+  for (int w = 0; w < EMB_SORT_WARPS; ++w)
+    if (w < warp) at0 += warp_sum[w];
+  if (r < n) {
+    offs[lo + r] = at0;
+    for (int w = 0; w < EMB_SORT_WARPS; ++w) {
+      const int c = cnt[w * range + r];
+      cnt[w * range + r] = at0;
+      at0 += c;
     }
+    if (lo + r == vocab - 1) offs[vocab] = at0;
   }
   __syncthreads();
-  // placement in token order: lanes of one id rank by lane number
-  for (int64_t tb = t0; tb < t1; tb += 32) {
-    const int64_t t = tb + lane;
-    int r = -1;
-    if (t < t1) {
-      const int64_t id = static_cast<int64_t>(__ldg(ids + t));
-      if (id != padding && id >= lo && id < lo + n) r = static_cast<int>(id - lo);
+  // placement in token order: lanes of one id rank by lane number; ids of
+  // several rounds are loaded ahead
+  constexpr int AHEAD = 4;
+  for (int64_t tb = t0; tb < t1; tb += 32 * AHEAD) {
+    int own[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int64_t t = tb + 32 * a + lane;
+      own[a] = -1;
+      if (t < t1) {
+        const int64_t id = static_cast<int64_t>(__ldg(ids + t));
+        if (id != padding && id >= lo && id < lo + n) own[a] = static_cast<int>(id - lo);
+      }
     }
-    const unsigned in = __ballot_sync(0xffffffffu, r >= 0);
-    if (in == 0) continue;
-    if (r >= 0) {
-      const unsigned same = __match_any_sync(in, r);
-      const int rank = __popc(same & ((1u << lane) - 1u));
-      const int at = mine[r] + rank;
-      __syncwarp(in);
-      if (rank == 0) mine[r] = at + __popc(same);
-      perm[at] = static_cast<int>(t);
-      sid[at] = static_cast<int>(lo + r);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const unsigned in = __ballot_sync(0xffffffffu, own[a] >= 0);
+      if (in == 0) continue;
+      if (own[a] >= 0) {
+        const unsigned same = __match_any_sync(in, own[a]);
+        const int rank = __popc(same & ((1u << lane) - 1u));
+        const int at = mine[own[a]] + rank;
+        __syncwarp(in);
+        if (rank == 0) mine[own[a]] = at + __popc(same);
+        perm[at] = static_cast<int>(tb + 32 * a + lane);
+        sid[at] = static_cast<int>(lo + own[a]);
+      }
+      __syncwarp();
     }
-    __syncwarp();
   }
 }
 
@@ -234,7 +233,7 @@ __device__ __forceinline__ void store_row(O* p, const float (&v)[N]) {
 #pragma unroll
     for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
   } else {
-    Vec16<O>::store(p, v);
+    RowAccess<O, true>::store(p, v);
   }
 }
 
@@ -255,117 +254,149 @@ __global__ void __launch_bounds__(256) k_embed_rows(const T* __restrict__ dy, in
                                                     O* __restrict__ dw) {
   using A = RowAccess<T, kVec>;
   constexpr int N = A::N;
-  constexpr int U = 4;  // rows in flight per thread
+  constexpr int U = 8;  // rows in flight per thread
+  static_assert(EMB_CHUNK % U == 0, "whole batches");
+  __shared__ int s_sid[32][EMB_CHUNK + 2];  // with the neighbours' ids at both ends
+  __shared__ int s_tok[32][EMB_CHUNK];
+  __shared__ float s_f[32][EMB_CHUNK];
   pdl_launch_dependents();
   pdl_wait();
   const int places = offs[vocab];
   const int sum_blocks = chunk_blocks * col_blocks;
   if (static_cast<int>(blockIdx.x) < sum_blocks) {
-    const int cb = blockIdx.x % col_blocks;
-    const int64_t chunk = static_cast<int64_t>(blockIdx.x / col_blocks) * blockDim.y + threadIdx.y;
-    const int c = (cb * blockDim.x + threadIdx.x) * N;
+    const int cb = blockIdx.x % col_blocks, ty = threadIdx.y;
+    const int64_t chunk = static_cast<int64_t>(blockIdx.x / col_blocks) * blockDim.y + ty;
     const int64_t p0 = chunk * EMB_CHUNK;
+    for (int i = threadIdx.x; i < EMB_CHUNK + 2; i += blockDim.x) {
+      const int64_t p = p0 - 1 + i;
+      s_sid[ty][i] = p >= 0 && p < places ? sid[p] : -1;
+    }
+    for (int i = threadIdx.x; i < EMB_CHUNK; i += blockDim.x) {
+      const int t = p0 + i < places ? perm[p0 + i] : 0;
+      s_tok[ty][i] = t;
+      if (row_scale != nullptr) s_f[ty][i] = p0 + i < places ? row_scale[t] : 0.0f;
+    }
+    __syncthreads();
+    const int c = (cb * blockDim.x + threadIdx.x) * N;
     if (c >= d || p0 >= places) return;
-    const int64_t p1 = p0 + EMB_CHUNK < places ? p0 + EMB_CHUNK : places;
-    const bool from_prev = p0 > 0 && sid[p0 - 1] == sid[p0];
-    const bool into_next = p1 < places && sid[p1] == sid[p1 - 1];
+    const int cnt = static_cast<int>(places - p0 < EMB_CHUNK ? places - p0 : EMB_CHUNK);
+    const int* id = s_sid[ty] + 1;
+    const bool from_prev = id[-1] == id[0];
+    const bool into_next = cnt == EMB_CHUNK && id[cnt] == id[cnt - 1];
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.0f;
-    int cur = sid[p0];
-    bool first = true;
-    for (int64_t p = p0; p < p1; p += U) {
-      float v[U][N];
-      int id[U];
+    int cur = id[0], begin = 0;  // the row being summed, its first place in the chunk
+    auto flush = [&](bool open_end) {
+      const bool head = begin == 0 && from_prev;
+      if (head || open_end) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        id[u] = -1;
-        if (p + u < p1) {
-          const int t = perm[p + u];
-          id[u] = sid[p + u];
-          A::load(dy + t * ldy + c, v[u]);
-          if (row_scale != nullptr) {
-            const float f = row_scale[t];
+        for (int j = 0; j < N; ++j) part[(chunk * 2 + (head ? 0 : 1)) * d + c + j] = acc[j];
+      } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[u][j] *= f;
-          }
-        }
+        for (int j = 0; j < N; ++j) acc[j] *= scale;
+        store_row<O, kVec>(dw + (kByPlace ? p0 + begin : static_cast<int64_t>(cur)) * d + c, acc);
       }
+    };
+    for (int i0 = 0; i0 < cnt; i0 += U) {
+      typename A::Raw raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u < cnt) raw[u] = A::load_raw(dy + s_tok[ty][i0 + u] * ldy + c);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (id[u] < 0) continue;
-        if (id[u] != cur) {  // the row `cur` ends here
-          if (first && from_prev) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) part[(chunk * 2) * d + c + j] = acc[j];
-          } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] *= scale;
-            store_row<O, kVec>(dw + static_cast<int64_t>(kByPlace ? offs[cur] : cur) * d + c, acc);
-          }
-          first = false;
-          cur = id[u];
+        const int i = i0 + u;
+        if (i >= cnt) continue;
+        if (id[i] != cur) {  // the row `cur` ends here
+          flush(false);
+          cur = id[i];
+          begin = i;
 #pragma unroll
           for (int j = 0; j < N; ++j) acc[j] = 0.0f;
         }
+        float v[N];
+        A::unpack(raw[u], v);
+        if (row_scale != nullptr) {
+          const float f = s_f[ty][i];
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += v[u][j];
+          for (int j = 0; j < N; ++j) acc[j] = fmaf(v[j], f, acc[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[j] += v[j];
+        }
       }
     }
-    const bool head = first && from_prev;
-    if (head || into_next) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) part[(chunk * 2 + (head ? 0 : 1)) * d + c + j] = acc[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] *= scale;
-      store_row<O, kVec>(dw + static_cast<int64_t>(kByPlace ? offs[cur] : cur) * d + c, acc);
-    }
+    flush(into_next);
     return;
   }
-  // rows without a token
+  // rows without a token, 32 ids of a warp at a time
   const int tid = threadIdx.y * blockDim.x + threadIdx.x;
   const int lane = tid & 31;
   const int64_t nw = static_cast<int64_t>(gridDim.x - sum_blocks) * 8;
   float z[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) z[j] = 0.0f;
-  for (int64_t v = static_cast<int64_t>(blockIdx.x - sum_blocks) * 8 + (tid >> 5); v < vocab; v += nw) {
-    if (offs[v] != offs[v + 1]) continue;
-    for (int c = lane * N; c < d; c += 32 * N) store_row<O, kVec>(dw + v * d + c, z);
+  for (int64_t v0 = (static_cast<int64_t>(blockIdx.x - sum_blocks) * 8 + (tid >> 5)) * 32; v0 < vocab; v0 += nw * 32) {
+    const int64_t v = v0 + lane;
+    unsigned empty = __ballot_sync(0xffffffffu, v < vocab && offs[v < vocab ? v : 0] == offs[v < vocab ? v + 1 : 0]);
+    while (empty) {
+      const int64_t row = v0 + __ffs(empty) - 1;
+      empty &= empty - 1;
+      for (int c = lane * N; c < d; c += 32 * N) store_row<O, kVec>(dw + row * d + c, z);
+    }
   }
 }
 
-// Rows that cross chunks: the chunk in which such a row begins adds its own
-// piece and the pieces of the following chunks, in order, and writes the row.
+// Rows that cross chunks: block of the chunk in which such a row begins; its
+// ty threads per column take contiguous parts of the following chunks' pieces,
+// and their sums are added in order.
+constexpr int EMB_JOIN_THREADS = 512;
 template <class T, bool kVec, class O, bool kByPlace>
-__global__ void __launch_bounds__(256) k_embed_join(int d, int64_t vocab, float scale, const int* __restrict__ offs,
-                                                    const int* __restrict__ sid, int col_blocks,
-                                                    const float* __restrict__ part, O* __restrict__ dw) {
+__global__ void __launch_bounds__(EMB_JOIN_THREADS) k_embed_join(int d, int64_t vocab, float scale,
+                                                                 const int* __restrict__ offs,
+                                                                 const int* __restrict__ sid, int col_blocks,
+                                                                 const float* __restrict__ part, O* __restrict__ dw) {
   constexpr int N = RowAccess<T, kVec>::N;
+  __shared__ float sums[EMB_JOIN_THREADS * N];
   pdl_launch_dependents();
   pdl_wait();
   const int places = offs[vocab];
-  const int cb = blockIdx.x % col_blocks;
-  const int64_t chunk = static_cast<int64_t>(blockIdx.x / col_blocks) * blockDim.y + threadIdx.y;
-  const int c = (cb * blockDim.x + threadIdx.x) * N;
+  const int cb = blockIdx.x % col_blocks, tx = threadIdx.x, ty = threadIdx.y;
+  const int64_t chunk = blockIdx.x / col_blocks;
   const int64_t p0 = chunk * EMB_CHUNK, p1 = p0 + EMB_CHUNK;
-  if (c >= d || p1 >= places) return;
+  if (p1 >= places) return;
   const int cur = sid[p1 - 1];
   if (sid[p1] != cur) return;                                     // does not continue
-  if (p0 > 0 && sid[p0] == cur && sid[p0 - 1] == cur) return;     // began in an earlier chunk
+  const int64_t start = offs[cur];
+  if (start < p0) return;                                         // began in an earlier chunk
   const int64_t last = (static_cast<int64_t>(offs[cur + 1]) - 1) / EMB_CHUNK;
+  const int c = (cb * blockDim.x + tx) * N;
+  const int64_t per = (last - chunk + blockDim.y - 1) / blockDim.y;
+  const int64_t k0 = chunk + 1 + ty * per, k1 = k0 + per - 1 < last ? k0 + per - 1 : last;
   float acc[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) acc[j] = part[(chunk * 2 + 1) * d + c + j];
-#pragma unroll 4
-  for (int64_t k = chunk + 1; k <= last; ++k) {
+  for (int j = 0; j < N; ++j) acc[j] = 0.0f;
+  if (c < d) {
+    if (ty == 0) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] += part[(k * 2) * d + c + j];
+      for (int j = 0; j < N; ++j) acc[j] = part[(chunk * 2 + 1) * d + c + j];
+    }
+#pragma unroll 4
+    for (int64_t k = k0; k <= k1; ++k) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] += part[(k * 2) * d + c + j];
+    }
   }
 #pragma unroll
+  for (int j = 0; j < N; ++j) sums[(ty * blockDim.x + tx) * N + j] = acc[j];
+  __syncthreads();
+  if (ty != 0 || c >= d) return;
+  for (int y = 1; y < static_cast<int>(blockDim.y); ++y)
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] += sums[(y * blockDim.x + tx) * N + j];
+#pragma unroll
   for (int j = 0; j < N; ++j) acc[j] *= scale;
-  store_row<O, kVec>(dw + static_cast<int64_t>(kByPlace ? offs[cur] : cur) * d + c, acc);
+  store_row<O, kVec>(dw + (kByPlace ? start : static_cast<int64_t>(cur)) * d + c, acc);
 }
 
 }  // namespace ethos

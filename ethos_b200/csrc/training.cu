@@ -71,7 +71,7 @@ int embed_rows(const EmbedScratch& s, const void* dy, int64_t ldy, const float* 
   const int col_blocks = (pieces + tx - 1) / tx;
   const int chunks = static_cast<int>((tokens + EMB_CHUNK - 1) / EMB_CHUNK);
   const int chunk_blocks = (chunks + ty - 1) / ty;
-  const int64_t fill_most = kByPlace ? 0 : (vocab + 7) / 8;
+  const int64_t fill_most = kByPlace ? 0 : (vocab + 255) / 256;
   const int fill = static_cast<int>(fill_most < 4 * dev.sm_count ? fill_most : 4 * dev.sm_count);
   const int64_t grid = static_cast<int64_t>(chunk_blocks) * col_blocks;
   if (grid + fill > (int64_t(1) << 31) - 1) return ETHOS_ERR_UNSUPPORTED_SHAPE;
@@ -80,7 +80,8 @@ int embed_rows(const EmbedScratch& s, const void* dy, int64_t ldy, const float* 
                       static_cast<const int*>(s.perm), static_cast<const int*>(s.sid), chunk_blocks, col_blocks,
                       s.part, dw);
   if (st != ETHOS_OK || chunks < 2) return st;
-  return launch_pdl(k_embed_join<T, kVec, O, kByPlace>, dim3(static_cast<unsigned>(grid)), dim3(tx, ty), 0, sm, d,
+  return launch_pdl(k_embed_join<T, kVec, O, kByPlace>, dim3(static_cast<unsigned>(chunks) * col_blocks),
+                    dim3(tx, EMB_JOIN_THREADS / tx), 0, sm, d,
                     vocab, scale, static_cast<const int*>(s.offs), static_cast<const int*>(s.sid), col_blocks,
                     static_cast<const float*>(s.part), dw);
 }
@@ -113,39 +114,71 @@ int embed_table_grad(const EmbedScratch& s, const void* dy, int64_t tokens, int6
 }
 
 // ---------------------------------------------------------------- balance --
+// Selections from which counting by ranges in shared memory is faster than
+// global atomics: the ranges cost about 10 us whatever the ids (reading them
+// once per range, emptying the counters), the atomics 1 us per 50 000
+// selections that crowd on few experts.
+constexpr int64_t kBalanceRanges = 400000;
+
+struct BalScratchAll {
+  BalScratch* head;
+  float* sel;
+};
+void carve_balance(Carve& c, int64_t n, BalScratchAll* s) {
+  s->head = c.take<BalScratch>(1);
+  s->sel = c.take<float>(static_cast<size_t>(n));
+}
+
 int balance_blocks(int64_t n, const DeviceInfo& dev) {
-  int64_t b = (n + BAL_THREADS - 1) / BAL_THREADS;
+  int64_t b = (n / 4 + BAL_THREADS) / BAL_THREADS;
   const int64_t most = 8ll * dev.sm_count < BAL_MAX_BLOCKS ? 8ll * dev.sm_count : BAL_MAX_BLOCKS;
-  return static_cast<int>(b < 1 ? 1 : (b < most ? b : most));
+  return static_cast<int>(b < most ? b : most);
 }
 
 template <class I, class W>
-int balance_forward(const void* ids, const void* weights, const uint8_t* mask, int64_t tokens, int heads, int k,
-                    int64_t experts, int32_t* counts, float* loss, BalScratch* s, int* err, cudaStream_t sm,
+int balance_forward(const void* ids_, const void* weights, const uint8_t* mask, int64_t tokens, int heads, int k,
+                    int experts, int32_t* counts, float* loss, const BalScratchAll& s, int* err, cudaStream_t sm,
                     const DeviceInfo& dev) {
-  const int blocks = balance_blocks(tokens * heads * k, dev);
-  int st = launch_pdl(k_balance_count<I>, dim3(blocks), dim3(BAL_THREADS), 0, sm, static_cast<const I*>(ids), mask,
-                      tokens, heads * k, experts, counts, s, err);
+  const I* ids = static_cast<const I*>(ids_);
+  const int T = static_cast<int>(tokens), per = heads * k;
+  const int64_t n = tokens * per;
+  const bool quads = per % 4 == 0 && aligned16(ids) && aligned16(weights);
+  const int blocks = balance_blocks(n, dev);
+  const int ranges = (experts + BAL_RANGE - 1) / BAL_RANGE;
+  int st, live_parts;
+  if (n >= kBalanceRanges && ranges <= dev.sm_count) {
+    auto kern = k_balance_count_ranges<I>;
+    if ((st = smem_attr_once(reinterpret_cast<const void*>(kern), BAL_RANGE * static_cast<int>(sizeof(int)))) !=
+        ETHOS_OK)
+      return st;
+    const int range = (experts + ranges - 1) / ranges;
+    live_parts = dev.sm_count / ranges;
+    st = launch_pdl(kern, dim3(static_cast<unsigned>(live_parts * ranges)), dim3(BAL_COUNT_THREADS),
+                    static_cast<size_t>(range) * sizeof(int), sm, ids, mask, T, per, experts, quads, ranges, range,
+                    counts, s.head, err);
+  } else {
+    live_parts = blocks;
+    st = launch_pdl(k_balance_count<I>, dim3(blocks), dim3(BAL_THREADS), 0, sm, ids, mask, T, per, experts, quads,
+                    counts, s.head, err);
+  }
   if (st != ETHOS_OK) return st;
-  return launch_pdl(k_balance_loss<I, W>, dim3(blocks), dim3(BAL_THREADS), 0, sm, static_cast<const I*>(ids),
-                    static_cast<const W*>(weights), mask, tokens, heads, k, experts,
-                    static_cast<const int*>(counts), s, loss);
+  return launch_pdl(k_balance_loss<I, W>, dim3(blocks), dim3(BAL_THREADS), 0, sm, ids,
+                    static_cast<const W*>(weights), mask, T, heads, k, experts, quads, live_parts,
+                    static_cast<const int*>(counts), s.head, s.sel, loss);
 }
 
-template <class I, class W>
-int balance_backward(const void* ids, const uint8_t* mask, int64_t tokens, int heads, int k, int64_t experts,
-                     const int32_t* counts, const BalScratch* s, const float* grad, void* dw, cudaStream_t sm,
-                     const DeviceInfo& dev) {
-  const int blocks = balance_blocks(tokens * heads * k, dev);
-  return launch_pdl(k_balance_bwd<I, W>, dim3(blocks), dim3(BAL_THREADS), 0, sm, static_cast<const I*>(ids), mask,
-                    tokens, heads, k, experts, static_cast<const int*>(counts), s, grad, static_cast<W*>(dw));
+template <class W>
+int balance_backward(int64_t n, int heads, int k, int experts, const BalScratchAll& s, const float* grad, void* dw,
+                     cudaStream_t sm, const DeviceInfo& dev) {
+  return launch_pdl(k_balance_bwd<W>, dim3(balance_blocks(n, dev)), dim3(BAL_THREADS), 0, sm, static_cast<int>(n),
+                    heads, k, experts, n % 4 == 0 && aligned16(dw), static_cast<const BalScratch*>(s.head),
+                    static_cast<const float*>(s.sel), grad, static_cast<W*>(dw));
 }
 
-int balance_check(const void* ids, int dtype, int64_t tokens, int64_t heads, int64_t k, int64_t experts) {
-  if ((!ids && tokens > 0) || tokens < 0 || heads < 1 || k < 1 || experts < 1) return ETHOS_ERR_INVALID_ARG;
-  if (!known_dtype(dtype)) return ETHOS_ERR_INVALID_ARG;
-  // counts are int32
-  if (heads > (1 << 20) || k > (1 << 20) || tokens > ((int64_t(1) << 31) - 1) / (heads * k))
+int balance_check(int dtype, int64_t tokens, int64_t heads, int64_t k, int64_t experts) {
+  if (tokens < 0 || heads < 1 || k < 1 || experts < 1 || !known_dtype(dtype)) return ETHOS_ERR_INVALID_ARG;
+  // selections are numbered, and counted, in int32
+  if (experts >= (1 << 30) || heads > (1 << 20) || k > (1 << 20) || tokens > (int64_t(1) << 30) / (heads * k))
     return ETHOS_ERR_UNSUPPORTED_SHAPE;
   return ETHOS_OK;
 }
@@ -190,11 +223,14 @@ XentPlan xent_plan(int64_t T, int64_t V, int64_t d, int dtype) {
   p.v_pad = up(V, XE_TILE);
   p.keep = p.planes == 1 && p.t_pad * up(V, 64) * 2 <= kKeepBytes;
   const int64_t num_m = p.t_pad / XE_TILE, num_n = (V + p.tile_n - 1) / p.tile_n;
-  // a unit's columns: long enough to make few pieces of each row, short enough
-  // for six units a pair
-  int64_t run = num_m * num_n / (kPairs * 6);
-  const int64_t most_run = 4096 / p.tile_n;
-  p.run = static_cast<int>(run < 1 ? 1 : (run > most_run ? most_run : run));
+  // a unit's columns: the most (up to 4096) that leave the last round of units
+  // as full as any choice does, within a percent
+  auto rounds = [&](int64_t run) { return (num_m * ((num_n + run - 1) / run) + kPairs - 1) / kPairs * run; };
+  int64_t best = rounds(1);
+  for (int64_t run = 2; run <= 4096 / p.tile_n; ++run) best = rounds(run) < best ? rounds(run) : best;
+  p.run = 1;
+  for (int64_t run = 2; run <= 4096 / p.tile_n; ++run)
+    if (100 * rounds(run) <= 101 * best) p.run = static_cast<int>(run);
   p.runs = static_cast<int>((num_n + p.run - 1) / p.run);
   int64_t most = kPieceBytes / (p.t_pad * 2 * p.planes) / XE_TILE * XE_TILE;
   if (most < kMinPiece) most = kMinPiece;
@@ -208,7 +244,8 @@ XentPlan xent_plan(int64_t T, int64_t V, int64_t d, int dtype) {
     // is at most about a third of a pair's share of the whole work
     const int64_t nt = (d + p.tile_n - 1) / p.tile_n;
     const int64_t kb_h = (V + G2_BK - 1) / G2_BK, kb_w = (T + G2_BK - 1) / G2_BK;
-    const int64_t share = (num_m * nt * kb_h + p.v_pad / XE_TILE * nt * kb_w) / (kPairs * 3);
+    const int64_t cost_w = kb_w > XE_STORE_KB ? kb_w : XE_STORE_KB;
+    const int64_t share = (num_m * nt * kb_h + p.v_pad / XE_TILE * nt * cost_w) / (kPairs * 3);
     const int64_t target = share > 8 ? share : 8;
     int64_t s = (kb_h + target - 1) / target;
     if (s > 64) s = 64;
@@ -243,7 +280,7 @@ struct XentFwd {
 void carve_xent_fwd(Carve& c, const XentPlan& p, XentFwd* s) {
   s->wp = p.pack_w ? c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.v_pad * p.ldd)) : nullptr;
   s->part = c.take<float2>(static_cast<size_t>(2 * p.runs * p.t_pad));
-  s->block_sum = c.take<double>(static_cast<size_t>((p.T + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS));
+  s->block_sum = c.take<double>(static_cast<size_t>(p.t_pad / XE_LOSS_ROWS));
 }
 struct XentBwd {
   __nv_bfloat16* wp;
@@ -399,11 +436,13 @@ int xent_logits(const XentPlan& p, const XentSave& sv, const XentRowsOperand& h,
   else return launch_xent_planes<MODE>(p.planes, ta, tb, ta, tb, a, units, err, sm, dev);
 }
 
-int xent_loss(const XentPlan& p, const XentSave& sv, const XentFwd& ws, bool keep, int reduction, float* loss,
-              cudaStream_t sm) {
-  return launch_pdl(k_xent_loss, dim3(static_cast<unsigned>((p.T + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS)), dim3(256), 0,
-                    sm, sv.rw, static_cast<const float2*>(ws.part), 2 * p.runs, p.t_pad, keep, reduction, loss,
-                    ws.block_sum);
+int xent_loss(const XentPlan& p, const XentSave& sv, const XentFwd& ws, int reduction, float* loss, cudaStream_t sm,
+              bool keep = false, bool again = false, int* redo_tile = nullptr, __nv_bfloat16* hr = nullptr) {
+  const int64_t rows = hr ? p.t_pad : p.T;
+  return launch_pdl(k_xent_loss, dim3(static_cast<unsigned>((rows + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS)), dim3(256), 0,
+                    sm, sv.rw, static_cast<const float2*>(ws.part), 2 * p.runs, p.t_pad, keep, again, redo_tile,
+                    reduction, loss, ws.block_sum, static_cast<const __nv_bfloat16*>(sv.hp), hr,
+                    static_cast<int>(p.ldd));
 }
 
 int64_t xent_grad_units(const XentPlan& p, int64_t n, int slots, const XeArgs& g) {
@@ -485,58 +524,61 @@ int ethos_embedding_backward(const void* ids, int ids_i64, const void* dy, int d
                              : embed_table_grad<float>(s, dy, tokens, vocab, d, scale, d_weight, sm, *dev);
 }
 
-size_t ethos_balance_scratch_size(void) { return sizeof(BalScratch); }
+size_t ethos_balance_scratch_size(int64_t tokens, int64_t heads, int64_t k) {
+  if (balance_check(ETHOS_F32, tokens, heads, k, 1) != ETHOS_OK) return 0;
+  Carve c{nullptr, 0, 0};
+  BalScratchAll s;
+  carve_balance(c, tokens * heads * k, &s);
+  return c.off + 256;
+}
 
 int ethos_balance_forward(const void* ids, int ids_i64, const void* weights, int dtype, const uint8_t* mask,
                           int64_t tokens, int64_t heads, int64_t k, int64_t experts, int32_t* counts, float* loss,
-                          void* scratch, int* dev_err, void* stream) {
-  int st = balance_check(ids, dtype, tokens, heads, k, experts);
+                          void* scratch, size_t scratch_bytes, int* dev_err, void* stream) {
+  int st = balance_check(dtype, tokens, heads, k, experts);
   if (st != ETHOS_OK) return st;
-  if ((!weights && tokens > 0) || !counts || !loss || !scratch || !dev_err) return ETHOS_ERR_INVALID_ARG;
-  if ((reinterpret_cast<uintptr_t>(scratch) & 15u) != 0) return ETHOS_ERR_ALIGNMENT;
+  if ((tokens > 0 && (!ids || !weights)) || !counts || !loss || !dev_err) return ETHOS_ERR_INVALID_ARG;
+  Carve c{static_cast<char*>(scratch), 0, scratch_bytes};
+  BalScratchAll s;
+  carve_balance(c, tokens * heads * k, &s);
+  if (!scratch || c.off > scratch_bytes) return ETHOS_ERR_WORKSPACE;
+  if (!aligned16(scratch)) return ETHOS_ERR_ALIGNMENT;
   DeviceInfo* dev = nullptr;
   if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
-  BalScratch* s = static_cast<BalScratch*>(scratch);
   if (cudaMemsetAsync(counts, 0, sizeof(int32_t) * static_cast<size_t>(experts), sm) != cudaSuccess)
     return ETHOS_ERR_CUDA;
-  if (cudaMemsetAsync(s, 0, offsetof(BalScratch, part), sm) != cudaSuccess) return ETHOS_ERR_CUDA;
-  const int H = static_cast<int>(heads), K = static_cast<int>(k);
+  const int H = static_cast<int>(heads), K = static_cast<int>(k), N = static_cast<int>(experts);
   if (ids_i64)
-    return dtype == ETHOS_BF16
-               ? balance_forward<int64_t, __nv_bfloat16>(ids, weights, mask, tokens, H, K, experts, counts, loss, s,
-                                                         dev_err, sm, *dev)
-               : balance_forward<int64_t, float>(ids, weights, mask, tokens, H, K, experts, counts, loss, s, dev_err,
-                                                 sm, *dev);
-  return dtype == ETHOS_BF16
-             ? balance_forward<int32_t, __nv_bfloat16>(ids, weights, mask, tokens, H, K, experts, counts, loss, s,
-                                                       dev_err, sm, *dev)
-             : balance_forward<int32_t, float>(ids, weights, mask, tokens, H, K, experts, counts, loss, s, dev_err,
-                                               sm, *dev);
+    return dtype == ETHOS_BF16 ? balance_forward<int64_t, __nv_bfloat16>(ids, weights, mask, tokens, H, K, N, counts,
+                                                                         loss, s, dev_err, sm, *dev)
+                               : balance_forward<int64_t, float>(ids, weights, mask, tokens, H, K, N, counts, loss, s,
+                                                                 dev_err, sm, *dev);
+  return dtype == ETHOS_BF16 ? balance_forward<int32_t, __nv_bfloat16>(ids, weights, mask, tokens, H, K, N, counts,
+                                                                       loss, s, dev_err, sm, *dev)
+                             : balance_forward<int32_t, float>(ids, weights, mask, tokens, H, K, N, counts, loss, s,
+                                                               dev_err, sm, *dev);
 }
 
-int ethos_balance_backward(const void* ids, int ids_i64, int dtype, const uint8_t* mask, int64_t tokens,
-                           int64_t heads, int64_t k, int64_t experts, const int32_t* counts, const void* scratch,
-                           const float* grad, void* d_weights, void* stream) {
-  int st = balance_check(ids, dtype, tokens, heads, k, experts);
+int ethos_balance_backward(int dtype, int64_t tokens, int64_t heads, int64_t k, int64_t experts,
+                           const void* scratch, size_t scratch_bytes, const float* grad, void* d_weights,
+                           void* stream) {
+  int st = balance_check(dtype, tokens, heads, k, experts);
   if (st != ETHOS_OK) return st;
   if (tokens == 0) return ETHOS_OK;
-  if (!counts || !scratch || !grad || !d_weights) return ETHOS_ERR_INVALID_ARG;
+  if (!grad || !d_weights) return ETHOS_ERR_INVALID_ARG;
+  Carve c{static_cast<char*>(const_cast<void*>(scratch)), 0, scratch_bytes};
+  BalScratchAll s;
+  carve_balance(c, tokens * heads * k, &s);
+  if (!scratch || c.off > scratch_bytes) return ETHOS_ERR_WORKSPACE;
+  if (!aligned16(scratch)) return ETHOS_ERR_ALIGNMENT;
   DeviceInfo* dev = nullptr;
   if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
-  const BalScratch* s = static_cast<const BalScratch*>(scratch);
-  const int H = static_cast<int>(heads), K = static_cast<int>(k);
-  if (ids_i64)
-    return dtype == ETHOS_BF16
-               ? balance_backward<int64_t, __nv_bfloat16>(ids, mask, tokens, H, K, experts, counts, s, grad,
-                                                          d_weights, sm, *dev)
-               : balance_backward<int64_t, float>(ids, mask, tokens, H, K, experts, counts, s, grad, d_weights, sm,
-                                                  *dev);
-  return dtype == ETHOS_BF16 ? balance_backward<int32_t, __nv_bfloat16>(ids, mask, tokens, H, K, experts, counts, s,
-                                                                        grad, d_weights, sm, *dev)
-                             : balance_backward<int32_t, float>(ids, mask, tokens, H, K, experts, counts, s, grad,
-                                                                d_weights, sm, *dev);
+  const int H = static_cast<int>(heads), K = static_cast<int>(k), N = static_cast<int>(experts);
+  return dtype == ETHOS_BF16
+             ? balance_backward<__nv_bfloat16>(tokens * heads * k, H, K, N, s, grad, d_weights, sm, *dev)
+             : balance_backward<float>(tokens * heads * k, H, K, N, s, grad, d_weights, sm, *dev);
 }
 
 size_t ethos_xent_save_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype) {
@@ -590,7 +632,7 @@ int ethos_xent_forward(const void* hidden, int64_t ldh, const void* weight, int6
   if (p.pack_w && (st = xent_pack_w(p, dtype, weight, ldw, ws.wp, sm, *dev)) != ETHOS_OK) return st;
   if ((st = xent_logits<XE_STATS>(p, sv, h, weight, ldw, ws, nullptr, 0, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
     return st;
-  return xent_loss(p, sv, ws, false, reduction, loss, sm);
+  return xent_loss(p, sv, ws, reduction, loss, sm);
 }
 
 size_t ethos_xent_forward_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype) {
@@ -633,21 +675,14 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   // E and the sums; rows whose shift was too low once more with their maximum
   if ((st = xent_logits<XE_KEEP>(p, sv, h, weight, ldw, ws.f, ws.e, ws.lde, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
     return st;
-  const dim3 row_blocks(static_cast<unsigned>((tokens + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS));
-  if ((st = launch_pdl(k_xent_check, row_blocks, dim3(256), 0, sm, sv.rw, static_cast<const float2*>(ws.f.part),
-                       2 * p.runs, p.t_pad, ws.redo_tile)) != ETHOS_OK)
-    return st;
+  __nv_bfloat16* hr = d_weight ? ws.hr : nullptr;
+  if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, true, false, ws.redo_tile, hr)) != ETHOS_OK) return st;
   if ((st = xent_logits<XE_KEEP>(p, sv, h, weight, ldw, ws.f, ws.e, ws.lde, ws.redo_tile, dev_err, sm, *dev)) !=
       ETHOS_OK)
     return st;
-  if ((st = xent_loss(p, sv, ws.f, true, reduction, loss, sm)) != ETHOS_OK) return st;
+  if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, true, true, ws.redo_tile, hr)) != ETHOS_OK) return st;
   if (!d_hidden && !d_weight) return ETHOS_OK;
   if (d_weight) {
-    int64_t blocks = (p.t_pad * (p.ldd / 8) + 255) / 256;
-    if (blocks > 8ll * dev->sm_count) blocks = 8ll * dev->sm_count;
-    if ((st = launch_pdl(k_xent_scaled_rows, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
-                         static_cast<const __nv_bfloat16*>(sv.hp), sv.rw, static_cast<int>(p.ldd), ws.hr)) != ETHOS_OK)
-      return st;
     // label rows of dW: (p[y] - 1) h[t] summed by label
     if ((st = embed_sort<int32_t>(ws.sort, sv.rw.yc, p.t_pad, &sv.rw.meta->rows, vocab, -1, dev_err, sm, *dev)) !=
         ETHOS_OK)
@@ -689,20 +724,21 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   return xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots, nullptr, reduction, weight, ldw, d_hidden, sm, *dev);
 }
 
-int ethos_xent_scale(const float* factor, void* x, int dtype, int64_t n, void* stream) {
-  if (n < 0 || !known_dtype(dtype)) return ETHOS_ERR_INVALID_ARG;
-  if (n == 0) return ETHOS_OK;
-  if (!factor || !x) return ETHOS_ERR_INVALID_ARG;
+int ethos_xent_scale(const float* factor, void* x, int64_t nx, void* y, int64_t ny, int dtype, void* stream) {
+  if (nx < 0 || ny < 0 || !known_dtype(dtype)) return ETHOS_ERR_INVALID_ARG;
+  if (nx + ny == 0) return ETHOS_OK;
+  if (!factor || (nx > 0 && !x) || (ny > 0 && !y)) return ETHOS_ERR_INVALID_ARG;
   DeviceInfo* dev = nullptr;
   const int st = base_device_info(&dev);
   if (st != ETHOS_OK) return st;
-  int64_t blocks = (n / 8 + 256) / 256;
+  int64_t blocks = ((nx + ny) / 8 + 256) / 256;
   if (blocks > 8ll * dev->sm_count) blocks = 8ll * dev->sm_count;
   const dim3 grid(static_cast<unsigned>(blocks));
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
-  return dtype == ETHOS_BF16
-             ? launch_pdl(k_xent_scale<__nv_bfloat16>, grid, dim3(256), 0, sm, factor, static_cast<__nv_bfloat16*>(x), n)
-             : launch_pdl(k_xent_scale<float>, grid, dim3(256), 0, sm, factor, static_cast<float*>(x), n);
+  return dtype == ETHOS_BF16 ? launch_pdl(k_xent_scale<__nv_bfloat16>, grid, dim3(256), 0, sm, factor,
+                                          static_cast<__nv_bfloat16*>(x), nx, static_cast<__nv_bfloat16*>(y), ny)
+                             : launch_pdl(k_xent_scale<float>, grid, dim3(256), 0, sm, factor,
+                                          static_cast<float*>(x), nx, static_cast<float*>(y), ny);
 }
 
 int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype, int reduction,

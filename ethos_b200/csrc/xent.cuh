@@ -60,6 +60,7 @@ constexpr int XE_ROWS_DIRECT = 256;  // tokens that keep their places (one row t
 constexpr int XE_TILE = 256;         // rows of a pair's tile; columns of one accumulator
 constexpr int XE_GROUP_M = 64;       // row tiles walked before the next column tile
 constexpr int XE_STEP_KB = 8;        // fp32: K blocks of 64 per accumulation
+constexpr int XE_STORE_KB = 6;       // K blocks that take as long as writing a tile of dW (3 us)
 constexpr float XE_LOG2E = 1.4426950408889634f;
 constexpr float XE_KEEP_RANGE = 60.0f;  // e^60 times any sum over a vocabulary is finite in fp32 and bf16
 
@@ -275,7 +276,7 @@ __device__ __forceinline__ void join_parts(const float2* __restrict__ part, int 
   m = -INFINITY;
   s = 0.0f;
   if (row < rows) {
-#pragma unroll 4
+#pragma unroll 8
     for (int p = threadIdx.x / XE_LOSS_ROWS; p < parts; p += 32) {
       const float2 v = part[p * part_ld + row];
       join(m, s, v.x, v.y);
@@ -302,55 +303,77 @@ struct JoinLse {
   __device__ __forceinline__ void operator()(float& m, float& s, float m2, float s2) const { lse_join(m, s, m2, s2); }
 };
 
+// Losses, and what the gradients need of each row.
 // KEEP: rows whose logits pass the shift by more than XE_KEEP_RANGE take their
 // maximum for it; redo_tile marks their row tiles, which k_xent_gemm then does
-// again.
-__global__ void __launch_bounds__(256) k_xent_check(XeRows rw, const float2* __restrict__ part, int parts,
-                                                    int64_t part_ld, int* __restrict__ redo_tile) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int rows = rw.meta->rows;
-  float m, s;
-  join_parts(part, parts, part_ld, rows, m, s, JoinMax());
-  const int row = blockIdx.x * XE_LOSS_ROWS + threadIdx.x;
-  if (threadIdx.x < XE_LOSS_ROWS && row < rows && rw.yc[row] >= 0 && m - rw.c[row] > XE_KEEP_RANGE) {
-    rw.c[row] = m;
-    redo_tile[row / XE_TILE] = 1;  // any writer writes the same
-    rw.meta->redo = 1;
-  }
-}
-
+// again, and a second launch of this kernel (again = true) with it; both end at
+// once when no row is marked.  hr receives the rows r h of the packed rows hp,
+// rounded to bf16 (the second operand of dW).
 __global__ void __launch_bounds__(256) k_xent_loss(XeRows rw, const float2* __restrict__ part, int parts,
-                                                   int64_t part_ld, bool keep, int reduction,
-                                                   float* __restrict__ loss, double* __restrict__ block_sum) {
+                                                   int64_t part_ld, bool keep, bool again,
+                                                   int* __restrict__ redo_tile, int reduction,
+                                                   float* __restrict__ loss, double* __restrict__ block_sum,
+                                                   const __nv_bfloat16* __restrict__ hp,
+                                                   __nv_bfloat16* __restrict__ hr, int ldd) {
   __shared__ double red[256];
+  __shared__ float row_r[XE_LOSS_ROWS];
   __shared__ bool last;
   pdl_launch_dependents();
   pdl_wait();
+  if (again && rw.meta->redo == 0) return;
   const int rows = rw.meta->rows;
   float m, s;
   if (keep) join_parts(part, parts, part_ld, rows, m, s, JoinMax());
   else join_parts(part, parts, part_ld, rows, m, s, JoinLse());
-  const int row = blockIdx.x * XE_LOSS_ROWS + threadIdx.x;
+  const int row0 = blockIdx.x * XE_LOSS_ROWS;
+  const int row = row0 + threadIdx.x;
   double mine = 0.0;
-  if (threadIdx.x < XE_LOSS_ROWS && row < rows) {
-    const float l = rw.lab[row];
-    const float c = keep ? rw.c[row] : fmaxf(m, l);
-    // s: sum of exp(l[v] - c) over the other columns; b: the label's own
-    if (!keep && m != c) s *= expf(m - c);  // m < c = l (m is -inf when there is no other column)
-    const float b = c == l ? 1.0f : expf(l - c);
-    const float v = c == l ? log1pf(s) : (c - l) + logf(s + b);
-    rw.lse[row] = l + v;
-    rw.q[row] = -s / (s + b);
-    rw.r[row] = 1.0f / (s + b);
-    if (rw.yc[row] >= 0) {
-      if (reduction == XE_NONE) loss[rw.idx[row]] = v;
-      mine = static_cast<double>(v);
+  if (threadIdx.x < XE_LOSS_ROWS) {
+    float r = 0.0f;
+    if (row < rows) {
+      const float l = rw.lab[row];
+      const bool live = rw.yc[row] >= 0;
+      float c = keep ? rw.c[row] : fmaxf(m, l);
+      if (keep && live && m - c > XE_KEEP_RANGE) {
+        rw.c[row] = m;
+        redo_tile[row / XE_TILE] = 1;  // any writer writes the same
+        rw.meta->redo = 1;
+      }
+      // s: sum of exp(l[v] - c) over the other columns; b: the label's own
+      if (!keep && m != c) s *= expf(m - c);  // m < c = l (m is -inf when there is no other column)
+      const float b = c == l ? 1.0f : expf(l - c);
+      const float v = c == l ? log1pf(s) : (c - l) + logf(s + b);
+      r = live ? 1.0f / (s + b) : 0.0f;
+      rw.lse[row] = l + v;
+      rw.q[row] = -s / (s + b);
+      rw.r[row] = r;
+      if (live) {
+        if (reduction == XE_NONE) loss[rw.idx[row]] = v;
+        mine = static_cast<double>(v);
+      }
+    }
+    row_r[threadIdx.x] = r;
+  }
+  red[threadIdx.x] = mine;
+  __syncthreads();
+  if (hr != nullptr) {
+    const int upto = (rows + XE_TILE - 1) / XE_TILE * XE_TILE;
+    const int pieces = ldd / 8;
+    for (int i = threadIdx.x; i < XE_LOSS_ROWS * pieces; i += 256) {
+      const int k = i / pieces;
+      if (row0 + k >= upto) break;
+      const int64_t at = static_cast<int64_t>(row0 + k) * ldd + static_cast<int64_t>(i - k * pieces) * 8;
+      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      const float f = row_r[k];
+      if (f != 0.0f) {  // ignored and padding rows stay zero whatever they hold
+        Vec16<__nv_bfloat16>::load(hp + at, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= f;
+      }
+      Vec16<__nv_bfloat16>::store(hr + at, x);
     }
   }
   if (reduction == XE_NONE) return;
-  red[threadIdx.x] = mine;
-  __syncthreads();
   if (threadIdx.x == 0) {
     double b = 0.0;
     for (int i = 0; i < XE_LOSS_ROWS; ++i) b += red[i];
@@ -370,30 +393,10 @@ __global__ void __launch_bounds__(256) k_xent_loss(XeRows rw, const float2* __re
     if (static_cast<int>(threadIdx.x) < o) red[threadIdx.x] += red[threadIdx.x + o];
     __syncthreads();
   }
-  // no token left: 0 for the sum, NaN for the mean
-  if (threadIdx.x == 0) *loss = static_cast<float>(reduction == XE_MEAN ? red[0] / rw.meta->valid : red[0]);
-}
-
-// KEEP: rows r h of the packed rows hp, rounded to bf16 (the second operand
-// of dW); zero rows stay zero.
-__global__ void __launch_bounds__(256) k_xent_scaled_rows(const __nv_bfloat16* __restrict__ hp, XeRows rw, int ldd,
-                                                          __nv_bfloat16* __restrict__ out) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int rows = rw.meta->rows;
-  const int64_t upto = (rows + XE_TILE - 1) / XE_TILE * XE_TILE;
-  const int pieces = ldd / 8;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < upto * pieces;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = i / pieces;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (row < rows && rw.yc[row] >= 0) {
-      Vec16<__nv_bfloat16>::load(hp + i * 8, v);
-      const float f = rw.r[row];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= f;
-    }
-    Vec16<__nv_bfloat16>::store(out + i * 8, v);
+  if (threadIdx.x == 0) {
+    rw.meta->done = 0;
+    // no token left: 0 for the sum, NaN for the mean
+    *loss = static_cast<float>(reduction == XE_MEAN ? red[0] / rw.meta->valid : red[0]);
   }
 }
 
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ 
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (r >= 0) {
       const float* a = acc + static_cast<int64_t>(r) * lda + c;
-#pragma unroll 2
+#pragma unroll 8
       for (int s = 0; s < slots; ++s) {
         const float4 x = *reinterpret_cast<const float4*>(a + s * slot_size);
         const float4 y = *reinterpret_cast<const float4*>(a + s * slot_size + 4);
@@ -458,28 +461,33 @@ __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ 
   }
 }
 
-// x *= *factor, unless it is 1 (the gradients of the KEEP way are those of a
+// x *= *factor and y *= *factor, unless it is 1 (the gradients of the KEEP way are those of a
 // loss whose own gradient is 1)
 template <class D>
-__global__ void __launch_bounds__(256) k_xent_scale(const float* __restrict__ factor, D* __restrict__ x, int64_t n) {
+__global__ void __launch_bounds__(256) k_xent_scale(const float* __restrict__ factor, D* __restrict__ x, int64_t nx,
+                                                    D* __restrict__ y, int64_t ny) {
   pdl_launch_dependents();
   pdl_wait();
   const float f = *factor;
   if (f == 1.0f) return;
   constexpr int N = Vec16<D>::N;
-  const int64_t nv = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 ? n / N : 0;
   const int64_t tid = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const int64_t nt = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = tid; i < nv; i += nt) {
-    float v[N];
-    Vec16<D>::load(x + i * N, v);
+  for (int t = 0; t < 2; ++t) {
+    D* p = t == 0 ? x : y;
+    const int64_t n = t == 0 ? nx : ny;
+    const int64_t nv = (reinterpret_cast<uintptr_t>(p) & 15u) == 0 ? n / N : 0;
+    for (int64_t i = tid; i < nv; i += nt) {
+      float v[N];
+      Vec16<D>::load(p + i * N, v);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] *= f;
-    Vec16<D>::store(x + i * N, v);
-  }
-  for (int64_t i = nv * N + tid; i < n; i += nt) {
-    const float v[1] = {static_cast<float>(x[i]) * f};
-    RowAccess<D, false>::store(x + i, v);
+      for (int j = 0; j < N; ++j) v[j] *= f;
+      Vec16<D>::store(p + i * N, v);
+    }
+    for (int64_t i = nv * N + tid; i < n; i += nt) {
+      const float v[1] = {static_cast<float>(p[i]) * f};
+      RowAccess<D, false>::store(p + i, v);
+    }
   }
 }
 
@@ -625,7 +633,9 @@ struct XeWalk {
     const int n2 = a.do_dw ? (a.p[1].M + XE_TILE - 1) / XE_TILE * num_n : 0;
     const int extra = long_units % pairs;
     my_long = long_units / pairs + (pair < extra ? 1 : 0);
-    const int diff = kb_w > 0 ? kb_slot / kb_w : 0;  // dW tiles that one dh tile is worth
+    // dW tiles that one dh tile is worth; writing a tile takes about as long as
+    // XE_STORE_KB blocks, so shorter contractions do not make it cheaper
+    const int diff = (max(kb_slot, XE_STORE_KB) + max(kb_w, XE_STORE_KB) / 2) / max(kb_w, XE_STORE_KB);
     int na = (n2 - diff * (pairs - extra) + pairs - 1) / pairs;
     if (extra == 0 || na < 0) na = 0;
     if (na * extra > n2) na = n2 / extra;

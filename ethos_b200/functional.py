@@ -48,8 +48,8 @@ class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weights, ids, num_experts, mask):
         loss, counts, scratch = ops.balance_forward(weights, ids, num_experts, mask)
-        ctx.save_for_backward(ids, mask, counts, scratch)
-        ctx.dtype = weights.dtype
+        ctx.save_for_backward(scratch)
+        ctx.shape, ctx.num_experts, ctx.dtype = weights.shape, num_experts, weights.dtype
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)  # no zeros for the counts
         return loss, counts
@@ -58,8 +58,8 @@ class _BalanceLoss(torch.autograd.Function):
     def backward(ctx, grad, _):
         if grad is None:
             return None, None, None, None
-        ids, mask, counts, scratch = ctx.saved_tensors
-        return ops.balance_backward(grad, ids, counts, scratch, ctx.dtype, mask), None, None, None
+        scratch, = ctx.saved_tensors
+        return ops.balance_backward(grad, scratch, ctx.shape, ctx.num_experts, ctx.dtype), None, None, None
 
 
 def balance_loss(weights, ids, num_experts, mask=None):
@@ -102,8 +102,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         grads, ctx.grads = ctx.grads, None
         if grads is not None:
             # the loss's own gradients, scaled where they are
-            grad = grad.to(torch.float32)
-            dh, dw = (ops.scale_(g, grad) if g is not None and n else None for g, n in zip(grads, need))
+            dh, dw = (g if n else None for g, n in zip(grads, need))
+            ops.scale_(grad.to(torch.float32), dh, dw)
         else:  # also a second pass through the graph: the first one's results belong to its caller
             dh, dw = ops.linear_cross_entropy_backward(grad, hidden, weight, save, ctx.reduction, need[0], need[1])
         return dh, dw, None, None, None, None, None

@@ -641,28 +641,25 @@ def balance_forward(weights, ids, num_experts, mask=None):
     weights, ids = weights.contiguous(), ids.contiguous()
     counts = torch.empty((num_experts,), dtype=torch.int32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    scratch = _bytes(_size("ethos_balance_scratch_size"), dev)
+    scratch = _bytes(_size("ethos_balance_scratch_size", T, H, k), dev)
     check(lib().ethos_balance_forward(ids.data_ptr(), i64, weights.data_ptr(), code, mptr, T, H, k, num_experts,
-                                      counts.data_ptr(), loss.data_ptr(), scratch.data_ptr(),
+                                      counts.data_ptr(), loss.data_ptr(), scratch.data_ptr(), scratch.numel(),
                                       device_error_word(dev).data_ptr(), _raw_stream(dev.index)),
           "ethos_balance_forward")
     return loss, counts, scratch
 
 
-def balance_backward(grad, ids, counts, scratch, dtype, mask=None):
-    """``grad * dloss/dweights`` of ``balance_forward`` in ``dtype``; ``grad`` is
-    a fp32 device scalar, ``counts`` and ``scratch`` the forward's."""
-    _require_cuda(ids, "ids")
-    T, H, k = ids.shape
-    dev = ids.device
+def balance_backward(grad, scratch, shape, num_experts, dtype):
+    """``grad * dloss/dweights`` of ``balance_forward``, ``shape`` = (T, H, k),
+    in ``dtype``; ``grad`` is a fp32 device scalar, ``scratch`` the forward's."""
+    _require_cuda(grad, "grad")
+    T, H, k = shape
+    dev = scratch.device
     dw = torch.empty((T, H, k), dtype=dtype, device=dev)
-    ids = ids.contiguous()
-    mask = mask.contiguous() if mask is not None else None
     grad = grad.to(torch.float32)
-    check(lib().ethos_balance_backward(ids.data_ptr(), _ids_i64(ids, "ids"), _dtype_code(dw, "weights"),
-                                       0 if mask is None else mask.data_ptr(), T, H, k, counts.numel(),
-                                       counts.data_ptr(), scratch.data_ptr(), grad.data_ptr(), dw.data_ptr(),
-                                       _raw_stream(dev.index)), "ethos_balance_backward")
+    check(lib().ethos_balance_backward(_dtype_code(dw, "weights"), T, H, k, num_experts, scratch.data_ptr(),
+                                       scratch.numel(), grad.data_ptr(), dw.data_ptr(), _raw_stream(dev.index)),
+          "ethos_balance_backward")
     return dw
 
 
@@ -752,15 +749,19 @@ def linear_cross_entropy_forward_backward(hidden, weight, labels, ignore_index=-
     return loss, save, dh, dw
 
 
-def scale_(x, factor):
-    """``x *= factor`` in place (``factor`` a fp32 device scalar); nothing is
-    read or written when it is 1 (ethos_xent_scale)."""
-    _require_cuda(x, "x")
-    if not x.is_contiguous():
-        raise ValueError("x: contiguous")
-    check(lib().ethos_xent_scale(factor.data_ptr(), x.data_ptr(), _dtype_code(x, "x"), x.numel(),
-                                 _raw_stream(x.device.index)), "ethos_xent_scale")
-    return x
+def scale_(factor, x=None, y=None):
+    """``x *= factor`` and ``y *= factor`` in place (contiguous, of one dtype;
+    None: none; ``factor`` a fp32 device scalar); nothing is read or written
+    when it is 1 (ethos_xent_scale)."""
+    _require_cuda(factor, "factor")
+    some = [t for t in (x, y) if t is not None]
+    if not some:
+        return
+    if any(not t.is_contiguous() or t.dtype != some[0].dtype for t in some):
+        raise ValueError("x and y: contiguous, of one dtype")
+    check(lib().ethos_xent_scale(factor.data_ptr(), 0 if x is None else x.data_ptr(), 0 if x is None else x.numel(),
+                                 0 if y is None else y.data_ptr(), 0 if y is None else y.numel(),
+                                 _dtype_code(some[0], "x"), _raw_stream(factor.device.index)), "ethos_xent_scale")
 
 
 def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", need_hidden=True, need_weight=True):

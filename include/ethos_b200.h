@@ -479,17 +479,18 @@ int ethos_embedding_backward(const void* ids, int ids_i64, const void* dy, int d
  * 0 = leave the token out.  With c[e] the selections of expert e and n tokens
  * left: loss = experts * sum_e (c[e] / (n heads k)) * (weights of e / (n
  * heads)), 1 for an even choice, 0 without tokens.  counts int32 [experts];
- * scratch (ethos_balance_scratch_size bytes) is kept for the backward. */
-size_t ethos_balance_scratch_size(void);
+ * scratch (ethos_balance_scratch_size bytes) is kept for the backward.
+ * tokens * heads * k <= 2^30, experts < 2^30. */
+size_t ethos_balance_scratch_size(int64_t tokens, int64_t heads, int64_t k);
 int ethos_balance_forward(const void* ids, int ids_i64, const void* weights, int dtype, const uint8_t* mask,
                           int64_t tokens, int64_t heads, int64_t k, int64_t experts, int32_t* counts, float* loss,
-                          void* scratch, int* dev_err, void* stream);
+                          void* scratch, size_t scratch_bytes, int* dev_err, void* stream);
 
 /* d_weights = grad * dloss/dweights (counts constant), in dtype; grad is a
- * device fp32 scalar, counts and scratch are the forward's. */
-int ethos_balance_backward(const void* ids, int ids_i64, int dtype, const uint8_t* mask, int64_t tokens,
-                           int64_t heads, int64_t k, int64_t experts, const int32_t* counts, const void* scratch,
-                           const float* grad, void* d_weights, void* stream);
+ * device fp32 scalar, scratch the forward's. */
+int ethos_balance_backward(int dtype, int64_t tokens, int64_t heads, int64_t k, int64_t experts,
+                           const void* scratch, size_t scratch_bytes, const float* grad, void* d_weights,
+                           void* stream);
 
 /* Cross entropy of the output head without its logits in memory:
  *   l = hidden weight^T,  loss[t] = logsumexp(l[t]) - l[t, labels[t]],
@@ -538,9 +539,9 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
                                 size_t save_bytes, void* d_hidden, void* d_weight, void* workspace,
                                 size_t workspace_bytes, int* dev_err, void* stream);
 
-/* x[0..n) *= factor[0] (device fp32), nothing written when it is 1: applies
- * the loss's own gradient to the gradients above. */
-int ethos_xent_scale(const float* factor, void* x, int dtype, int64_t n, void* stream);
+/* x[0..nx) and y[0..ny) *= factor[0] (device fp32), nothing written when it is
+ * 1: applies the loss's own gradient to the gradients above. */
+int ethos_xent_scale(const float* factor, void* x, int64_t nx, void* y, int64_t ny, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

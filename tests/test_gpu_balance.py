@@ -37,7 +37,8 @@ def _reference(w, ids, N, mask):
 
 
 CASES = [(1, 1, 1, 1), (1, 8, 16, 262144), (257, 3, 5, 1001), (2048, 8, 16, 4096), (4097, 8, 16, 262144),
-         (33, 1, 4, 7)]
+         (33, 1, 4, 7),
+         (6001, 8, 16, 120001), (150001, 1, 3, 777)]
 
 
 @pytest.mark.gpu
@@ -81,6 +82,23 @@ def test_no_tokens_and_views():
     want, counts, _ = _reference(w, ids, 99, None)
     loss, c = EF.balance_loss(wv, iv, 99)
     assert abs(loss.item() - want) <= 2.0 ** -22 * want and torch.equal(c.cpu().long(), counts)
+
+
+@pytest.mark.gpu
+def test_weights_of_masked_tokens_do_not_matter():
+    for T in (40, 5000):
+        w, ids = _inputs(T, 8, 16, 500, seed=9)
+        mask = torch.arange(T) % 3 != 0
+        bad_w, bad_ids = w.clone(), ids.clone()
+        bad_w[~mask] = float("nan")
+        bad_ids[~mask] = 1 << 40    # not looked at either
+        a = EF.balance_loss(w.cuda(), ids.cuda(), 500, mask=mask.cuda())
+        wg = bad_w.cuda().requires_grad_(True)
+        b = EF.balance_loss(wg, bad_ids.cuda(), 500, mask=mask.cuda())
+        ops.check_device_error("cuda")
+        assert torch.equal(a[0], b[0].detach()) and torch.equal(a[1], b[1])
+        dw, = torch.autograd.grad(b[0], wg)
+        assert torch.isfinite(dw).all() and not dw[~mask.cuda()].any()
 
 
 @pytest.mark.gpu
@@ -140,13 +158,16 @@ def test_refusals():
 def test_entry_point_argument_checks():
     L = _lib.lib()
     v = ctypes.c_void_p(256)
-    assert L.ethos_balance_scratch_size() > 8
+    need = L.ethos_balance_scratch_size(4, 2, 4)
+    assert need >= 4 * 32 and L.ethos_balance_scratch_size(-1, 2, 4) == 0
     fwd = lambda **o: L.ethos_balance_forward(*[o.get(n, x) for n, x in (  # noqa: E731
         ("ids", v), ("i64", 1), ("w", v), ("dtype", 0), ("mask", None), ("T", 4), ("H", 2), ("k", 4), ("N", 30),
-        ("counts", v), ("loss", v), ("scratch", v), ("err", v), ("stream", None))])
-    assert fwd(ids=None) == 1 and fwd(w=None) == 1 and fwd(counts=None) == 1 and fwd(scratch=None) == 1
-    assert fwd(dtype=7) == 1 and fwd(N=0) == 1 and fwd(T=-1) == 1
-    assert fwd(T=1 << 29) == 2                                    # counts would pass int32
+        ("counts", v), ("loss", v), ("scratch", v), ("bytes", need), ("err", v), ("stream", None))])
+    assert fwd(ids=None) == 1 and fwd(w=None) == 1 and fwd(counts=None) == 1 and fwd(scratch=None) == 4
+    assert fwd(dtype=7) == 1 and fwd(N=0) == 1 and fwd(T=-1) == 1 and fwd(bytes=64) == 4
+    assert fwd(T=1 << 29) == 2                                    # selections would pass int32
     assert fwd(scratch=ctypes.c_void_p(260)) == 3
-    assert L.ethos_balance_backward(None, 1, 0, None, 0, 2, 4, 30, None, None, None, None, None) == 0
-    assert L.ethos_balance_backward(v, 1, 0, None, 4, 2, 4, 30, None, v, v, v, None) == 1
+    bwd = lambda **o: L.ethos_balance_backward(*[o.get(n, x) for n, x in (  # noqa: E731
+        ("dtype", 0), ("T", 4), ("H", 2), ("k", 4), ("N", 30), ("scratch", v), ("bytes", need), ("grad", v),
+        ("dw", v), ("stream", None))])
+    assert bwd(T=0) == 0 and bwd(grad=None) == 1 and bwd(dw=None) == 1 and bwd(scratch=None) == 4 and bwd(bytes=8) == 4

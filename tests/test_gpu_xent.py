@@ -439,6 +439,7 @@ def test_entry_point_argument_checks():
 
     assert fb(red=0) == 1 and fb(y=None) == 1 and fb(dt=0) == 2 and fb(wb=64) == 4 and fb(sb=0) == 4
     assert fb(ldw=d + 4) == 3
-    assert L.ethos_xent_scale(None, v, 1, 4, None) == 1 and L.ethos_xent_scale(v, v, 1, 0, None) == 0
+    assert L.ethos_xent_scale(None, v, 4, None, 0, 1, None) == 1 and L.ethos_xent_scale(v, None, 4, None, 0, 1, None) == 1
+    assert L.ethos_xent_scale(v, v, 0, None, 0, 1, None) == 0
     assert backward(g=None) == 1 and backward(save=None) == 4 and backward(wb=64) == 4
     assert backward(dh=None, dw=None) == 0
