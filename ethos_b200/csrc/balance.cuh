@@ -14,9 +14,10 @@
 //
 // Counting.  Popular experts make atomics on one address queue up in L2: 2.1 M
 // selections that crowd (density ~ id^-1/2 of 262 144 experts) took 41 us.  So
-// with many selections each block counts one range of experts in shared memory
-// over its part of the selections, and adds its non-zero counts to the global
-// ones; the ids are read once per range (6 times at 262 144 experts).
+// with many selections each block counts the experts of one residue modulo a
+// power of two (so that crowded neighbours are spread) in shared memory over
+// its part of the selections, and adds its non-zero counts to the global ones;
+// the ids are read once per residue (8 times at 262 144 experts).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -28,7 +29,7 @@ namespace ethos {
 constexpr int BAL_THREADS = 256;
 constexpr int BAL_MAX_BLOCKS = 1184;   // 8 per SM of a B200
 constexpr int BAL_COUNT_THREADS = 1024;
-constexpr int BAL_RANGE = 51200;       // experts counted by one block (200 KB of shared memory)
+constexpr int BAL_RANGE = 51200;       // most experts counted by one block (200 KB of shared memory)
 
 // Scratch of one call: the header, then sel [tokens * H * k] fp32, the count of
 // each selection's expert (0 for a selection left out), for the backward.
@@ -60,13 +61,23 @@ template <class I, class F>
 __device__ __forceinline__ void each_selection(const I* __restrict__ ids, const uint8_t* __restrict__ mask,
                                                int per_token, bool quads, int i0, int i1, F f) {
   if (quads) {  // per_token % 4 == 0, ids 16-byte aligned: a quad is of one token
-#pragma unroll 2
-    for (int i = i0 + 4 * static_cast<int>(threadIdx.x); i < i1; i += 4 * static_cast<int>(blockDim.x)) {
-      if (mask != nullptr && !mask[i / per_token]) continue;
-      int e[4];
-      load_ids4(ids + i, e);
+    constexpr int U = 4;  // quads in flight
+    const int step = 4 * static_cast<int>(blockDim.x);
+    for (int64_t i = i0 + 4 * static_cast<int>(threadIdx.x); i < i1; i += U * step) {
+      int e[U][4];
+      bool in[U];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f(i + j, e[j]);
+      for (int u = 0; u < U; ++u) {
+        in[u] = i + u * step < i1;
+        if (in[u]) load_ids4(ids + i + u * step, e[u]);
+        if (in[u] && mask != nullptr) in[u] = mask[static_cast<unsigned>(i + u * step) / static_cast<unsigned>(per_token)];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!in[u]) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f(static_cast<int>(i) + u * step + j, e[u][j]);
+      }
     }
   } else {
     for (int i = i0 + static_cast<int>(threadIdx.x); i < i1; i += static_cast<int>(blockDim.x)) {
@@ -118,19 +129,20 @@ __global__ void __launch_bounds__(BAL_THREADS) k_balance_count(const I* __restri
   count_live(mask, tokens, b, parts, s);
 }
 
-// Many: block b counts the experts [r range, (r + 1) range), r = b % ranges,
-// over part b / ranges of the selections.
+// Many: block b counts the experts that are r = b % classes modulo classes (a
+// power of two, 2^shift) over part b / classes of the selections.
 template <class I>
 __global__ void __launch_bounds__(BAL_COUNT_THREADS) k_balance_count_ranges(const I* __restrict__ ids,
                                                                             const uint8_t* __restrict__ mask,
                                                                             int tokens, int per_token, int experts,
-                                                                            bool quads, int ranges, int range,
+                                                                            bool quads, int shift,
                                                                             int* __restrict__ counts,
                                                                             BalScratch* __restrict__ s, int* err) {
   extern __shared__ int mine[];
   pdl_launch_dependents();
-  const int r = blockIdx.x % ranges, b = blockIdx.x / ranges, parts = gridDim.x / ranges;
-  const int lo = r * range, width = min(range, experts - lo);
+  const int classes = 1 << shift;
+  const int r = blockIdx.x & (classes - 1), b = blockIdx.x >> shift, parts = gridDim.x >> shift;
+  const int width = (experts - r + classes - 1) >> shift;
   for (int i = threadIdx.x; i < width; i += BAL_COUNT_THREADS) mine[i] = 0;
   __syncthreads();
   pdl_wait();
@@ -140,15 +152,17 @@ __global__ void __launch_bounds__(BAL_COUNT_THREADS) k_balance_count_ranges(cons
   if (i0 < n)
     each_selection(ids, mask, per_token, quads, static_cast<int>(i0), static_cast<int>(i0 + per < n ? i0 + per : n),
                    [&](int, int e) {
-                     if (r == 0 && (e < 0 || e >= experts)) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
-                     const unsigned at = static_cast<unsigned>(e - lo);
-                     if (at < static_cast<unsigned>(width)) atomicAdd(mine + at, 1);
+                     if (static_cast<unsigned>(e) >= static_cast<unsigned>(experts)) {
+                       if (r == 0) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
+                     } else if ((e & (classes - 1)) == r) {
+                       atomicAdd(mine + (e >> shift), 1);
+                     }
                    });
   if (r == 0) count_live(mask, tokens, b, parts, s);
   __syncthreads();
   for (int i = threadIdx.x; i < width; i += BAL_COUNT_THREADS) {
     const int c = mine[i];
-    if (c) atomicAdd(counts + lo + i, c);
+    if (c) atomicAdd(counts + (i << shift) + r, c);
   }
 }
 

@@ -26,34 +26,37 @@ bool known_dtype(int dtype) { return dtype == ETHOS_F32 || dtype == ETHOS_BF16; 
 // -------------------------------------------------------------- embedding --
 template <class T, class I, bool kVec>
 int embed_fwd(const void* ids, const void* w, int64_t ldw, int64_t tokens, int64_t vocab, int d, float scale, void* out,
-              int* err, cudaStream_t sm, const DeviceInfo& dev) {
-  const int64_t pieces = tokens * (d / RowAccess<T, kVec>::N);
-  int64_t blocks = (pieces + 255) / 256;
-  const int64_t most = 16ll * dev.sm_count;
-  if (blocks > most) blocks = most;
-  return launch_pdl(k_embed_fwd<T, I, kVec>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm,
+              int* err, cudaStream_t sm) {
+  const int pieces = d / RowAccess<T, kVec>::N;
+  int tx = 8;
+  while (tx < pieces && tx < 256) tx *= 2;
+  const int ty = 256 / tx;
+  const int64_t blocks = (tokens + EMB_FWD_ROWS * ty - 1) / (EMB_FWD_ROWS * ty);
+  if (blocks > (int64_t(1) << 31) - 1) return ETHOS_ERR_UNSUPPORTED_SHAPE;
+  return launch_pdl(k_embed_fwd<T, I, kVec>, dim3(static_cast<unsigned>(blocks)), dim3(tx, ty), 0, sm,
                     static_cast<const I*>(ids), static_cast<const T*>(w), ldw, tokens, d, vocab, scale,
                     static_cast<T*>(out), err);
 }
 
 template <class T>
 int embed_fwd_ids(const void* ids, int ids_i64, const void* w, int64_t ldw, int64_t tokens, int64_t vocab, int d,
-                  float scale, void* out, int* err, cudaStream_t sm, const DeviceInfo& dev) {
+                  float scale, void* out, int* err, cudaStream_t sm) {
   constexpr int N = Vec16<T>::N;
   const bool vec = d % N == 0 && ldw % N == 0 && aligned16(w) && aligned16(out);
   if (ids_i64)
-    return vec ? embed_fwd<T, int64_t, true>(ids, w, ldw, tokens, vocab, d, scale, out, err, sm, dev)
-               : embed_fwd<T, int64_t, false>(ids, w, ldw, tokens, vocab, d, scale, out, err, sm, dev);
-  return vec ? embed_fwd<T, int32_t, true>(ids, w, ldw, tokens, vocab, d, scale, out, err, sm, dev)
-             : embed_fwd<T, int32_t, false>(ids, w, ldw, tokens, vocab, d, scale, out, err, sm, dev);
+    return vec ? embed_fwd<T, int64_t, true>(ids, w, ldw, tokens, vocab, d, scale, out, err, sm)
+               : embed_fwd<T, int64_t, false>(ids, w, ldw, tokens, vocab, d, scale, out, err, sm);
+  return vec ? embed_fwd<T, int32_t, true>(ids, w, ldw, tokens, vocab, d, scale, out, err, sm)
+             : embed_fwd<T, int32_t, false>(ids, w, ldw, tokens, vocab, d, scale, out, err, sm);
 }
 
 struct EmbedScratch {
-  int *offs, *perm, *sid;
+  int2* span;
+  int *perm, *sid;
   float* part;
 };
 void carve_embed(Carve& c, int64_t tokens, int64_t vocab, int64_t dim, EmbedScratch* s) {
-  s->offs = c.take<int>(static_cast<size_t>(vocab + 1));
+  s->span = c.take<int2>(static_cast<size_t>(vocab + 1));
   s->perm = c.take<int>(static_cast<size_t>(tokens));
   s->sid = c.take<int>(static_cast<size_t>(tokens));
   s->part = c.take<float>(static_cast<size_t>((tokens + EMB_CHUNK - 1) / EMB_CHUNK * 2 * dim));
@@ -71,18 +74,18 @@ int embed_rows(const EmbedScratch& s, const void* dy, int64_t ldy, const float* 
   const int col_blocks = (pieces + tx - 1) / tx;
   const int chunks = static_cast<int>((tokens + EMB_CHUNK - 1) / EMB_CHUNK);
   const int chunk_blocks = (chunks + ty - 1) / ty;
-  const int64_t fill_most = kByPlace ? 0 : (vocab + 255) / 256;
+  const int64_t fill_most = kByPlace ? 0 : (vocab + 8 * EMB_FILL - 1) / (8 * EMB_FILL);
   const int fill = static_cast<int>(fill_most < 4 * dev.sm_count ? fill_most : 4 * dev.sm_count);
   const int64_t grid = static_cast<int64_t>(chunk_blocks) * col_blocks;
   if (grid + fill > (int64_t(1) << 31) - 1) return ETHOS_ERR_UNSUPPORTED_SHAPE;
   int st = launch_pdl(k_embed_rows<T, kVec, O, kByPlace>, dim3(static_cast<unsigned>(grid + fill)), dim3(tx, ty), 0,
-                      sm, static_cast<const T*>(dy), ldy, row_scale, d, vocab, scale, static_cast<const int*>(s.offs),
+                      sm, static_cast<const T*>(dy), ldy, row_scale, d, vocab, scale, static_cast<const int2*>(s.span),
                       static_cast<const int*>(s.perm), static_cast<const int*>(s.sid), chunk_blocks, col_blocks,
                       s.part, dw);
   if (st != ETHOS_OK || chunks < 2) return st;
   return launch_pdl(k_embed_join<T, kVec, O, kByPlace>, dim3(static_cast<unsigned>(chunks) * col_blocks),
                     dim3(tx, EMB_JOIN_THREADS / tx), 0, sm, d,
-                    vocab, scale, static_cast<const int*>(s.offs), static_cast<const int*>(s.sid), col_blocks,
+                    vocab, scale, static_cast<const int2*>(s.span), static_cast<const int*>(s.sid), col_blocks,
                     static_cast<const float*>(s.part), dw);
 }
 
@@ -93,14 +96,14 @@ int embed_sort(const EmbedScratch& s, const void* ids, int64_t tokens, const int
   int64_t blocks = dev.sm_count;
   if (blocks * EMB_MAX_RANGE < vocab) blocks = (vocab + EMB_MAX_RANGE - 1) / EMB_MAX_RANGE;
   const int range = static_cast<int>((vocab + blocks - 1) / blocks);
-  blocks = (vocab + range - 1) / range;
+  if (blocks > vocab) blocks = vocab;
   const int smem = EMB_SORT_WARPS * range * static_cast<int>(sizeof(int));
   auto kern = k_embed_sort<I>;
   const int st = smem_attr_once(reinterpret_cast<const void*>(kern),
                                 EMB_SORT_WARPS * EMB_MAX_RANGE * static_cast<int>(sizeof(int)));
   if (st != ETHOS_OK) return st;
   return launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(EMB_SORT_THREADS), static_cast<size_t>(smem), sm,
-                    static_cast<const I*>(ids), static_cast<int>(tokens), count, vocab, padding, range, s.offs,
+                    static_cast<const I*>(ids), static_cast<int>(tokens), count, vocab, padding, range, s.span,
                     s.perm, s.sid, err);
 }
 
@@ -144,18 +147,18 @@ int balance_forward(const void* ids_, const void* weights, const uint8_t* mask, 
   const int64_t n = tokens * per;
   const bool quads = per % 4 == 0 && aligned16(ids) && aligned16(weights);
   const int blocks = balance_blocks(n, dev);
-  const int ranges = (experts + BAL_RANGE - 1) / BAL_RANGE;
+  int shift = 0;
+  while ((experts >> shift) >= BAL_RANGE) ++shift;
   int st, live_parts;
-  if (n >= kBalanceRanges && ranges <= dev.sm_count) {
+  if (n >= kBalanceRanges && (1 << shift) <= dev.sm_count) {
     auto kern = k_balance_count_ranges<I>;
     if ((st = smem_attr_once(reinterpret_cast<const void*>(kern), BAL_RANGE * static_cast<int>(sizeof(int)))) !=
         ETHOS_OK)
       return st;
-    const int range = (experts + ranges - 1) / ranges;
-    live_parts = dev.sm_count / ranges;
-    st = launch_pdl(kern, dim3(static_cast<unsigned>(live_parts * ranges)), dim3(BAL_COUNT_THREADS),
-                    static_cast<size_t>(range) * sizeof(int), sm, ids, mask, T, per, experts, quads, ranges, range,
-                    counts, s.head, err);
+    live_parts = dev.sm_count >> shift;
+    st = launch_pdl(kern, dim3(static_cast<unsigned>(live_parts << shift)), dim3(BAL_COUNT_THREADS),
+                    static_cast<size_t>((experts >> shift) + 1) * sizeof(int), sm, ids, mask, T, per, experts, quads,
+                    shift, counts, s.head, err);
   } else {
     live_parts = blocks;
     st = launch_pdl(k_balance_count<I>, dim3(blocks), dim3(BAL_THREADS), 0, sm, ids, mask, T, per, experts, quads,
@@ -224,13 +227,15 @@ XentPlan xent_plan(int64_t T, int64_t V, int64_t d, int dtype) {
   p.keep = p.planes == 1 && p.t_pad * up(V, 64) * 2 <= kKeepBytes;
   const int64_t num_m = p.t_pad / XE_TILE, num_n = (V + p.tile_n - 1) / p.tile_n;
   // a unit's columns: the most (up to 4096) that leave the last round of units
-  // as full as any choice does, within a percent
+  // as full as any choice does, within a percent; one tile where six rounds
+  // are not reached (how many rows there are is known on the device only)
   auto rounds = [&](int64_t run) { return (num_m * ((num_n + run - 1) / run) + kPairs - 1) / kPairs * run; };
   int64_t best = rounds(1);
   for (int64_t run = 2; run <= 4096 / p.tile_n; ++run) best = rounds(run) < best ? rounds(run) : best;
   p.run = 1;
   for (int64_t run = 2; run <= 4096 / p.tile_n; ++run)
-    if (100 * rounds(run) <= 101 * best) p.run = static_cast<int>(run);
+    if (num_m * ((num_n + run - 1) / run) >= 6 * kPairs && 100 * rounds(run) <= 101 * best)
+      p.run = static_cast<int>(run);
   p.runs = static_cast<int>((num_n + p.run - 1) / p.run);
   int64_t most = kPieceBytes / (p.t_pad * 2 * p.planes) / XE_TILE * XE_TILE;
   if (most < kMinPiece) most = kMinPiece;
@@ -483,8 +488,8 @@ int ethos_embedding_forward(const void* ids, int ids_i64, const void* weight, in
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
   const int d = static_cast<int>(dim);
   return dtype == ETHOS_BF16
-             ? embed_fwd_ids<__nv_bfloat16>(ids, ids_i64, weight, ldw, tokens, vocab, d, scale, out, dev_err, sm, *dev)
-             : embed_fwd_ids<float>(ids, ids_i64, weight, ldw, tokens, vocab, d, scale, out, dev_err, sm, *dev);
+             ? embed_fwd_ids<__nv_bfloat16>(ids, ids_i64, weight, ldw, tokens, vocab, d, scale, out, dev_err, sm)
+             : embed_fwd_ids<float>(ids, ids_i64, weight, ldw, tokens, vocab, d, scale, out, dev_err, sm);
 }
 
 size_t ethos_embedding_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim) {
@@ -714,7 +719,7 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   g.dw = d_weight;
   g.dw_bf16 = 1;
   g.label_rows = ws.label_rows;
-  g.label_offs = ws.sort.offs;
+  g.label_span = ws.sort.span;
   g.do_dh = d_hidden != nullptr;
   g.do_dw = d_weight != nullptr;
   if ((st = launch_xent<XE_GRADS, 1>(ek, wk, em, hb, g, xent_grad_units(p, vocab, p.slots, g), dev_err, sm, *dev)) !=

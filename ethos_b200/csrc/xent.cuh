@@ -523,8 +523,8 @@ struct XeArgs {
   int64_t dh_ld;
   void* dw;            // rows of this piece, [N rows][d] with pitch d
   int dw_bf16;
-  const float* label_rows;  // added to dW before scaling: row v's is label_rows[label_offs[v]]
-  const int* label_offs;    // where label_offs[v] < label_offs[v + 1]
+  const float* label_rows;  // added to dW before scaling: row v's is label_rows[label_span[v].x],
+  const int2* label_span;   // where that span is not empty
   int do_dh, do_dw;
 };
 
@@ -1245,8 +1245,8 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
           const int d = args.p[1].N;
           const float* extra = nullptr;
           if (args.label_rows != nullptr) {
-            const int at = args.label_offs[row];
-            if (at < args.label_offs[row + 1]) extra = args.label_rows + static_cast<int64_t>(at) * d;
+            const int2 sp = args.label_span[row];
+            if (sp.x < sp.y) extra = args.label_rows + static_cast<int64_t>(sp.x) * d;
           }
           const int esz = args.dw_bf16 ? 2 : 4;
           const int align = byte_align(args.dw, static_cast<int64_t>(d) * esz);
