@@ -14,10 +14,14 @@
 //
 // Counting.  Popular experts make atomics on one address queue up in L2: 2.1 M
 // selections that crowd (density ~ id^-1/2 of 262 144 experts) took 41 us.  So
-// with many selections each block counts the experts of one residue modulo a
-// power of two (so that crowded neighbours are spread) in shared memory over
-// its part of the selections, and adds its non-zero counts to the global ones;
-// the ids are read once per residue (8 times at 262 144 experts).
+// with many selections each block counts one class of experts in shared memory
+// over its part of the selections, and adds its non-zero counts to the global
+// ones.  Classes interleave groups of 8 experts: crowded neighbours are spread
+// over the blocks (shared-memory atomics go at about one a cycle; with whole
+// ranges the block of the popular one took 65 us at 8.4 M selections), and the
+// 8 counts of a group still go out together.  The ids are read once per class
+// (L2 to SM); 16-bit counters, emptied before one can pass 65 535, make that 4
+// classes for 262 144 experts.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -29,7 +33,8 @@ namespace ethos {
 constexpr int BAL_THREADS = 256;
 constexpr int BAL_MAX_BLOCKS = 1184;   // 8 per SM of a B200
 constexpr int BAL_COUNT_THREADS = 1024;
-constexpr int BAL_RANGE = 51200;       // most experts counted by one block (200 KB of shared memory)
+constexpr int BAL_CLASS = 102400;      // most experts counted by one block (200 KB of shared memory)
+constexpr int BAL_EMPTY = 65532;       // selections between two emptyings of the 16-bit counters
 
 // Scratch of one call: the header, then sel [tokens * H * k] fp32, the count of
 // each selection's expert (0 for a selection left out), for the backward.
@@ -40,51 +45,74 @@ struct BalScratch {
   double part[BAL_MAX_BLOCKS];
 };
 
-// 4 consecutive ids (16-byte loads)
-__device__ __forceinline__ void load_ids4(const int32_t* p, int (&e)[4]) {
-  const int4 v = *reinterpret_cast<const int4*>(p);
+// 16 bytes read once: not kept in L1, which is left to the counts
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+// 4 consecutive ids (16-byte loads) as unsigned 32-bit numbers; an id that does
+// not fit (negative, or 2^31 and more) becomes one that no table has
+__device__ __forceinline__ void load_ids4(const int32_t* p, unsigned (&e)[4]) {
+  const uint4 v = load_once(p);
   e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w;
 }
-__device__ __forceinline__ int narrow_id(int64_t x) {  // out of int32: out of any range
-  return x < 0 || x > INT32_MAX ? -1 : static_cast<int>(x);
+__device__ __forceinline__ void load_ids4(const int64_t* p, unsigned (&e)[4]) {
+  const uint4 a = load_once(p), b = load_once(p + 2);
+  e[0] = a.y ? ~0u : a.x; e[1] = a.w ? ~0u : a.z; e[2] = b.y ? ~0u : b.x; e[3] = b.w ? ~0u : b.z;
 }
-__device__ __forceinline__ void load_ids4(const int64_t* p, int (&e)[4]) {
-  const longlong2 a = reinterpret_cast<const longlong2*>(p)[0], b = reinterpret_cast<const longlong2*>(p)[1];
-  e[0] = narrow_id(a.x); e[1] = narrow_id(a.y); e[2] = narrow_id(b.x); e[3] = narrow_id(b.y);
+__device__ __forceinline__ unsigned load_id(const int32_t* p) { return static_cast<unsigned>(*p); }
+__device__ __forceinline__ unsigned load_id(const int64_t* p) {
+  const uint64_t x = static_cast<uint64_t>(*p);
+  return (x >> 32) ? ~0u : static_cast<unsigned>(x);
 }
-__device__ __forceinline__ int load_id(const int32_t* p) { return *p; }
-__device__ __forceinline__ int load_id(const int64_t* p) { return narrow_id(*p); }
 
-// Calls f(i, id) for the selections i in [i0, i1) of unmasked tokens, threads
-// of the block in turn, four at a time where addresses allow.
-template <class I, class F>
+// Calls f(id) for the selections [i0, i1) of unmasked tokens, threads of the
+// block in turn, four at a time where addresses allow.
+template <bool kMask, class I, class F>
 __device__ __forceinline__ void each_selection(const I* __restrict__ ids, const uint8_t* __restrict__ mask,
-                                               int per_token, bool quads, int i0, int i1, F f) {
+                                               unsigned per_token, bool quads, unsigned i0, unsigned i1, F f) {
   if (quads) {  // per_token % 4 == 0, ids 16-byte aligned: a quad is of one token
-    constexpr int U = 4;  // quads in flight
-    const int step = 4 * static_cast<int>(blockDim.x);
-    for (int64_t i = i0 + 4 * static_cast<int>(threadIdx.x); i < i1; i += U * step) {
-      int e[U][4];
-      bool in[U];
+    constexpr unsigned U = 4;  // quads in flight
+    const unsigned step = 4 * blockDim.x;
+    unsigned i = i0 + 4 * threadIdx.x;
+    for (; i + (U - 1) * step < i1; i += U * step) {
+      unsigned e[U][4];
+      uint8_t in[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        in[u] = i + u * step < i1;
-        if (in[u]) load_ids4(ids + i + u * step, e[u]);
-        if (in[u] && mask != nullptr) in[u] = mask[static_cast<unsigned>(i + u * step) / static_cast<unsigned>(per_token)];
+      for (unsigned u = 0; u < U; ++u) {
+        load_ids4(ids + i + u * step, e[u]);
+        if (kMask) in[u] = mask[(i + u * step) / per_token];
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!in[u]) continue;
+      for (unsigned u = 0; u < U; ++u) {
+        if (kMask && !in[u]) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f(static_cast<int>(i) + u * step + j, e[u][j]);
+        for (int j = 0; j < 4; ++j) f(e[u][j]);
       }
+    }
+    for (; i < i1; i += step) {
+      unsigned e[4];
+      load_ids4(ids + i, e);
+      if (kMask && !mask[i / per_token]) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(e[j]);
     }
   } else {
-    for (int i = i0 + static_cast<int>(threadIdx.x); i < i1; i += static_cast<int>(blockDim.x)) {
-      if (mask != nullptr && !mask[i / per_token]) continue;
-      f(i, load_id(ids + i));
+    for (unsigned i = i0 + threadIdx.x; i < i1; i += blockDim.x) {
+      if (kMask && !mask[i / per_token]) continue;
+      f(load_id(ids + i));
     }
   }
+}
+template <class I, class F>
+__device__ __forceinline__ void each_selection(const I* __restrict__ ids, const uint8_t* __restrict__ mask,
+                                               int per_token, bool quads, int64_t i0, int64_t i1, F f) {
+  if (i0 >= i1) return;
+  if (mask != nullptr)
+    each_selection<true>(ids, mask, per_token, quads, static_cast<unsigned>(i0), static_cast<unsigned>(i1), f);
+  else
+    each_selection<false>(ids, mask, per_token, quads, static_cast<unsigned>(i0), static_cast<unsigned>(i1), f);
 }
 
 // Unmasked tokens of part b of `parts`, into live[b] (thread 0 of the block).
@@ -113,57 +141,58 @@ template <class I>
 __global__ void __launch_bounds__(BAL_THREADS) k_balance_count(const I* __restrict__ ids,
                                                                const uint8_t* __restrict__ mask, int tokens,
                                                                int per_token, int experts, bool quads,
-                                                               int* __restrict__ counts, BalScratch* __restrict__ s,
-                                                               int* err) {
+                                                               int* __restrict__ counts,
+                                                               BalScratch* __restrict__ s) {
   pdl_launch_dependents();
   pdl_wait();
   const int n = tokens * per_token, b = blockIdx.x, parts = gridDim.x;
   const int per = ((n + parts - 1) / parts + 3) / 4 * 4;
   const int64_t i0 = static_cast<int64_t>(b) * per;
-  if (i0 < n)
-    each_selection(ids, mask, per_token, quads, static_cast<int>(i0), static_cast<int>(i0 + per < n ? i0 + per : n),
-                   [&](int, int e) {
-                     if (e < 0 || e >= experts) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
-                     else atomicAdd(counts + e, 1);
-                   });
+  each_selection(ids, mask, per_token, quads, i0, i0 + per < n ? i0 + per : n, [&](unsigned e) {
+    if (e < static_cast<unsigned>(experts)) atomicAdd(counts + e, 1);
+  });
   count_live(mask, tokens, b, parts, s);
 }
 
-// Many: block b counts the experts that are r = b % classes modulo classes (a
-// power of two, 2^shift) over part b / classes of the selections.
+// Many: block b counts class r = b mod 2^shift, the experts whose group of 8
+// is r modulo 2^shift, over part b / 2^shift of the selections.  Counter l of
+// the class is expert 8 ((l / 8) 2^shift + r) + l % 8; two counters a word,
+// `words` of them.
 template <class I>
-__global__ void __launch_bounds__(BAL_COUNT_THREADS) k_balance_count_ranges(const I* __restrict__ ids,
-                                                                            const uint8_t* __restrict__ mask,
-                                                                            int tokens, int per_token, int experts,
-                                                                            bool quads, int shift,
-                                                                            int* __restrict__ counts,
-                                                                            BalScratch* __restrict__ s, int* err) {
-  extern __shared__ int mine[];
+__global__ void __launch_bounds__(BAL_COUNT_THREADS) k_balance_count_classes(const I* __restrict__ ids,
+                                                                             const uint8_t* __restrict__ mask,
+                                                                             int tokens, int per_token, int experts,
+                                                                             bool quads, int shift, int words,
+                                                                             int* __restrict__ counts,
+                                                                             BalScratch* __restrict__ s) {
+  extern __shared__ unsigned mine[];
   pdl_launch_dependents();
-  const int classes = 1 << shift;
-  const int r = blockIdx.x & (classes - 1), b = blockIdx.x >> shift, parts = gridDim.x >> shift;
-  const int width = (experts - r + classes - 1) >> shift;
-  for (int i = threadIdx.x; i < width; i += BAL_COUNT_THREADS) mine[i] = 0;
+  const unsigned classes = 1u << shift, r = blockIdx.x & (classes - 1);
+  const int b = blockIdx.x >> shift, parts = gridDim.x >> shift;
+  for (int i = threadIdx.x; i < words; i += BAL_COUNT_THREADS) mine[i] = 0;
   __syncthreads();
   pdl_wait();
   const int n = tokens * per_token;
   const int per = ((n + parts - 1) / parts + 3) / 4 * 4;
-  const int64_t i0 = static_cast<int64_t>(b) * per;
-  if (i0 < n)
-    each_selection(ids, mask, per_token, quads, static_cast<int>(i0), static_cast<int>(i0 + per < n ? i0 + per : n),
-                   [&](int, int e) {
-                     if (static_cast<unsigned>(e) >= static_cast<unsigned>(experts)) {
-                       if (r == 0) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
-                     } else if ((e & (classes - 1)) == r) {
-                       atomicAdd(mine + (e >> shift), 1);
-                     }
-                   });
-  if (r == 0) count_live(mask, tokens, b, parts, s);
-  __syncthreads();
-  for (int i = threadIdx.x; i < width; i += BAL_COUNT_THREADS) {
-    const int c = mine[i];
-    if (c) atomicAdd(counts + (i << shift) + r, c);
+  const int64_t i0 = static_cast<int64_t>(b) * per, i1 = i0 + per < n ? i0 + per : n;
+  for (int64_t a = i0; a < i1; a += BAL_EMPTY) {
+    each_selection(ids, mask, per_token, quads, a, a + BAL_EMPTY < i1 ? a + BAL_EMPTY : i1, [&](unsigned e) {
+      if (((e >> 3) & (classes - 1)) == r && e < static_cast<unsigned>(experts))
+        atomicAdd(mine + ((e >> (3 + shift)) << 2) + ((e & 7) >> 1), 1u << (16 * (e & 1)));
+    });
+    __syncthreads();
+    for (int i = threadIdx.x; i < words; i += BAL_COUNT_THREADS) {
+      const unsigned c = mine[i];
+      if (c) {
+        mine[i] = 0;
+        int* at = counts + ((((static_cast<unsigned>(i) >> 2) << shift) + r) << 3) + 2 * (i & 3);
+        if (c & 0xffffu) atomicAdd(at, static_cast<int>(c & 0xffffu));
+        if (c >> 16) atomicAdd(at + 1, static_cast<int>(c >> 16));
+      }
+    }
+    __syncthreads();
   }
+  if (r == 0) count_live(mask, tokens, b, parts, s);
 }
 
 // C = N / (n^2 H^2 k), 0 without tokens
@@ -174,8 +203,8 @@ __device__ __forceinline__ double balance_coef(int live, int64_t experts, int he
 }
 
 __device__ __forceinline__ void load_w4(const float* p, float (&v)[4]) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  const uint4 a = load_once(p);
+  v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
 }
 __device__ __forceinline__ void load_w4(const __nv_bfloat16* p, float (&v)[4]) {
   const uint2 u = *reinterpret_cast<const uint2*>(p);
@@ -191,15 +220,16 @@ __device__ __forceinline__ void store_w4(__nv_bfloat16* p, const float (&v)[4]) 
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// Sums w c[id] and leaves c[id] in sel.  Thread by thread the terms are fixed,
-// blocks add in fp64, and the last block adds the blocks in order.
+// Sums w c[id] and leaves c[id] in sel; an id outside [0, experts) is recorded
+// and left out, as the count kernels leave it out.  Thread by thread the terms
+// are fixed, blocks add in fp64, and the last block adds the blocks in order.
 template <class I, class W>
 __global__ void __launch_bounds__(BAL_THREADS) k_balance_loss(const I* __restrict__ ids, const W* __restrict__ w,
                                                               const uint8_t* __restrict__ mask, int tokens, int heads,
                                                               int k, int experts, bool quads, int live_parts,
                                                               const int* __restrict__ counts,
                                                               BalScratch* __restrict__ s, float* __restrict__ sel,
-                                                              float* __restrict__ loss) {
+                                                              float* __restrict__ loss, int* err) {
   __shared__ double red[BAL_THREADS];
   __shared__ bool last;
   pdl_launch_dependents();
@@ -208,26 +238,48 @@ __global__ void __launch_bounds__(BAL_THREADS) k_balance_loss(const I* __restric
   const int n = tokens * per_token;
   const int nt = gridDim.x * BAL_THREADS, tid = blockIdx.x * BAL_THREADS + threadIdx.x;
   double acc = 0.0;
+  // c of one selection
+  auto count_of = [&](unsigned e, bool in) {
+    if (!in) return 0.0f;
+    if (e >= static_cast<unsigned>(experts)) {
+      record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
+      return 0.0f;
+    }
+    return static_cast<float>(__ldg(counts + e));
+  };
   if (quads) {
-#pragma unroll 2
-    for (int64_t i = 4ll * tid; i < n; i += 4ll * nt) {
-      int e[4];
-      float x[4], c[4];
-      load_ids4(ids + i, e);
-      load_w4(w + i, x);
-      const bool in = mask == nullptr || mask[static_cast<int>(i) / per_token];
+    constexpr int U = 1;
+    for (int64_t i = 4ll * tid; i < n; i += 4ll * U * nt) {
+      unsigned e[U][4];
+      float x[U][4], c[U][4];
+      bool in[U];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = in && e[j] >= 0 && e[j] < experts ? static_cast<float>(__ldg(counts + e[j])) : 0.0f;
-      store_w4(sel + i, c);
-      // a weight left out is not read into the sum (it may be NaN)
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = i + 4ll * u * nt;
+        in[u] = at < n;
+        if (in[u]) {
+          load_ids4(ids + at, e[u]);
+          load_w4(w + at, x[u]);
+          if (mask != nullptr) in[u] = mask[static_cast<unsigned>(at) / static_cast<unsigned>(per_token)] != 0;
+        }
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc += static_cast<double>(c[j] != 0.0f ? x[j] * c[j] : 0.0f);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[u][j] = count_of(e[u][j], in[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = i + 4ll * u * nt;
+        if (at < n) store_w4(sel + at, c[u]);
+        // a weight left out is not read into the sum (it may be NaN)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc += static_cast<double>(c[u][j] != 0.0f ? x[u][j] * c[u][j] : 0.0f);
+      }
     }
   } else {
     for (int64_t i = tid; i < n; i += nt) {
-      const int e = load_id(ids + i);
-      const bool in = mask == nullptr || mask[static_cast<int>(i) / per_token];
-      const float c = in && e >= 0 && e < experts ? static_cast<float>(__ldg(counts + e)) : 0.0f;
+      const bool in = mask == nullptr || mask[static_cast<unsigned>(i) / static_cast<unsigned>(per_token)];
+      const float c = count_of(load_id(ids + i), in);
       sel[i] = c;
       acc += static_cast<double>(c != 0.0f ? static_cast<float>(w[i]) * c : 0.0f);
     }

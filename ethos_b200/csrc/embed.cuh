@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(256) k_embed_fwd(const I* __restrict__ ids, co
 
 // ------------------------------------------------------------------- sort --
 // Groups the tokens by id, in token order within an id.  Block b owns the ids
-// that are b modulo the number of blocks: frequent ids are low ids in practice,
+// that are b modulo the number of blocks (2^shift): frequent ids are low ids in practice,
 // and blocks that owned ranges left one with most of the tokens (26 us against
 // MEASURED_SORT at 16 384 Zipf-distributed tokens of 100 277 ids).  Every block reads
 // all ids: it counts those of lower blocks, which is where its part of the
@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(256) k_embed_fwd(const I* __restrict__ ids, co
 template <class I>
 __global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __restrict__ ids, int tokens,
                                                                  const int* __restrict__ count, int64_t vocab,
-                                                                 int64_t padding, int range, int2* __restrict__ span,
+                                                                 int64_t padding, int range, int shift,
+                                                                 int2* __restrict__ span,
                                                                  int* __restrict__ perm, int* __restrict__ sid,
                                                                  int* err) {
   extern __shared__ int cnt[];  // [EMB_SORT_WARPS][range]
@@ -166,8 +167,8 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) k_embed_sort(const I* __rest
       if (report && owner == 0) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
       return -1;
     }
-    const unsigned u = static_cast<unsigned>(id), q = u / owners, o = u - q * owners;
-    return o == owner ? static_cast<int>(q) : (o < owner ? -2 : -1);
+    const unsigned u = static_cast<unsigned>(id), o = u & (owners - 1);
+    return o == owner ? static_cast<int>(u >> shift) : (o < owner ? -2 : -1);
   };
   int* mine = cnt + warp * range;
   const int part = ((tokens + EMB_SORT_WARPS * 32 - 1) / (EMB_SORT_WARPS * 32)) * 32;

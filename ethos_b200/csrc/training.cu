@@ -92,18 +92,19 @@ int embed_rows(const EmbedScratch& s, const void* dy, int64_t ldy, const float* 
 template <class I>
 int embed_sort(const EmbedScratch& s, const void* ids, int64_t tokens, const int* count, int64_t vocab,
                int64_t padding, int* err, cudaStream_t sm, const DeviceInfo& dev) {
-  // one block per SM, more when a block would own over EMB_MAX_RANGE ids
-  int64_t blocks = dev.sm_count;
-  if (blocks * EMB_MAX_RANGE < vocab) blocks = (vocab + EMB_MAX_RANGE - 1) / EMB_MAX_RANGE;
-  const int range = static_cast<int>((vocab + blocks - 1) / blocks);
-  if (blocks > vocab) blocks = vocab;
+  // a power of two of blocks, so that owner and local number are bits of the
+  // id: 128 (of 148 SMs), more when a block would own over EMB_MAX_RANGE ids
+  int shift = 7;
+  while ((vocab >> shift) >= EMB_MAX_RANGE) ++shift;
+  const int64_t blocks = int64_t(1) << shift;
+  const int range = static_cast<int>((vocab + blocks - 1) >> shift);
   const int smem = EMB_SORT_WARPS * range * static_cast<int>(sizeof(int));
   auto kern = k_embed_sort<I>;
   const int st = smem_attr_once(reinterpret_cast<const void*>(kern),
                                 EMB_SORT_WARPS * EMB_MAX_RANGE * static_cast<int>(sizeof(int)));
   if (st != ETHOS_OK) return st;
   return launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(EMB_SORT_THREADS), static_cast<size_t>(smem), sm,
-                    static_cast<const I*>(ids), static_cast<int>(tokens), count, vocab, padding, range, s.span,
+                    static_cast<const I*>(ids), static_cast<int>(tokens), count, vocab, padding, range, shift, s.span,
                     s.perm, s.sid, err);
 }
 
@@ -117,11 +118,11 @@ int embed_table_grad(const EmbedScratch& s, const void* dy, int64_t tokens, int6
 }
 
 // ---------------------------------------------------------------- balance --
-// Selections from which counting by ranges in shared memory is faster than
-// global atomics: the ranges cost about 10 us whatever the ids (reading them
-// once per range, emptying the counters), the atomics 1 us per 50 000
-// selections that crowd on few experts.
-constexpr int64_t kBalanceRanges = 400000;
+// Selections from which counting by classes in shared memory is taken over
+// global atomics.  With the loss pass, 262 144 selections took 20-26 us by
+// classes whatever the ids, and 18 (even) to 58 us (crowded on few experts) by
+// atomics; 131 072 took 21-27 against 18-35.
+constexpr int64_t kBalanceClasses = 200000;
 
 struct BalScratchAll {
   BalScratch* head;
@@ -147,27 +148,27 @@ int balance_forward(const void* ids_, const void* weights, const uint8_t* mask, 
   const int64_t n = tokens * per;
   const bool quads = per % 4 == 0 && aligned16(ids) && aligned16(weights);
   const int blocks = balance_blocks(n, dev);
-  int shift = 0;
-  while ((experts >> shift) >= BAL_RANGE) ++shift;
+  int shift = 0;  // log2 of the classes: groups of 8 experts, shared evenly
+  const int groups = (experts + 7) / 8;
+  while (((groups + (1 << shift) - 1) >> shift) * 8 > BAL_CLASS) ++shift;
   int st, live_parts;
-  if (n >= kBalanceRanges && (1 << shift) <= dev.sm_count) {
-    auto kern = k_balance_count_ranges<I>;
-    if ((st = smem_attr_once(reinterpret_cast<const void*>(kern), BAL_RANGE * static_cast<int>(sizeof(int)))) !=
-        ETHOS_OK)
-      return st;
+  if (n >= kBalanceClasses && (1 << shift) <= dev.sm_count) {
+    auto kern = k_balance_count_classes<I>;
+    if ((st = smem_attr_once(reinterpret_cast<const void*>(kern), BAL_CLASS * 2)) != ETHOS_OK) return st;
+    const int words = ((groups + (1 << shift) - 1) >> shift) * 4;
     live_parts = dev.sm_count >> shift;
     st = launch_pdl(kern, dim3(static_cast<unsigned>(live_parts << shift)), dim3(BAL_COUNT_THREADS),
-                    static_cast<size_t>((experts >> shift) + 1) * sizeof(int), sm, ids, mask, T, per, experts, quads,
-                    shift, counts, s.head, err);
+                    static_cast<size_t>(words) * 4, sm, ids, mask, T, per, experts, quads, shift, words, counts,
+                    s.head);
   } else {
     live_parts = blocks;
     st = launch_pdl(k_balance_count<I>, dim3(blocks), dim3(BAL_THREADS), 0, sm, ids, mask, T, per, experts, quads,
-                    counts, s.head, err);
+                    counts, s.head);
   }
   if (st != ETHOS_OK) return st;
   return launch_pdl(k_balance_loss<I, W>, dim3(blocks), dim3(BAL_THREADS), 0, sm, ids,
                     static_cast<const W*>(weights), mask, T, heads, k, experts, quads, live_parts,
-                    static_cast<const int*>(counts), s.head, s.sel, loss);
+                    static_cast<const int*>(counts), s.head, s.sel, loss, err);
 }
 
 template <class W>
