@@ -126,6 +126,10 @@ EXPORTS = {
     "ethos_test_gemm_withhold": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _P]),
 }
 
+# the same with the routing weights' gradient before the stream
+for _n in ("ethos_layer_backward", "ethos_layer_backward_f32"):
+    EXPORTS[_n.replace("backward", "backward_routed")] = (_I, EXPORTS[_n][1] + [_P])
+
 _lock = threading.Lock()
 _lib = None
 

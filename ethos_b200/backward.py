@@ -4,7 +4,7 @@ all-reduce overlapped with it).
 
 Maps the gradients computed by ``ethos_layer_backward`` (one C-ABI call, see
 include/ethos_b200.h) onto the inputs of ``_EthosLayerFunction``: x, the layer
-and the need-grad flag (no gradients), then the parameters in the order of ``EthosExpertLayer._grad_params`` --
+and two flags (no gradients), then the parameters in the order of ``EthosExpertLayer._grad_params`` --
 expert_latents, net.0, net.2, query_projs weights, query_projs biases,
 query_norms weights, query_norms biases, sub_keys_1, sub_keys_2.
 """
@@ -49,10 +49,14 @@ def _overlapped_allreduce(layer, g, events):
         comm["log"].append((events[0], events[1], marks[0], marks[1]))
 
 
-def layer_backward(ctx, gy):
+def layer_backward(ctx, gy, gw=None):
+    """``gw``: the gradient of the routing weights, where the forward returned
+    them (None: none)."""
     layer = ctx.layer
     sv = ctx.saved
     pw = sv["pw"]
+    if gy is None:  # only the routing weights were used
+        gy = torch.zeros_like(sv["xin"])
     H = layer.num_heads
     dq = layer.router.d_query
     eps, _ = layer.router._bn_eps_momentum()
@@ -63,12 +67,12 @@ def layer_backward(ctx, gy):
     events = [torch.cuda.Event(enable_timing=timing), torch.cuda.Event(enable_timing=timing)] if overlap else None
     if pw.fp32:
         g = ops.layer_backward_f32(gy.reshape(-1, gy.shape[-1]), sv["xin"], pw, sv, ctx.training_bn, eps,
-                                   stage_events=events)
+                                   stage_events=events, d_weights=gw)
     else:
         # a bf16 input gets its gradient from the dx GEMM directly in bf16
         dx_dtype = torch.bfloat16 if ctx.x_dtype == torch.bfloat16 else torch.float32
         g = ops.layer_backward(gy.reshape(-1, gy.shape[-1]), sv["xin"], pw, sv, ctx.training_bn, eps,
-                               stage_events=events, dx_dtype=dx_dtype)
+                               stage_events=events, dx_dtype=dx_dtype, d_weights=gw)
     if overlap:
         _overlapped_allreduce(layer, g, events)
     params = ctx.params
@@ -84,8 +88,8 @@ def layer_backward(ctx, gy):
     flat += [g["d_bn"][1, h * dq:(h + 1) * dq] for h in range(H)]
     flat += [g["d_bn"][2, h * dq:(h + 1) * dq] for h in range(H)]
     flat += [g["d_keys"][0], g["d_keys"][1]]
-    out = [grads[0], None, None]  # x, layer, need_grad (not tensors)
-    for p, gp, need in zip(params, flat, ctx.needs_input_grad[3:]):
+    out = [grads[0], None, None, None]  # x, layer, need_grad, routing (not tensors)
+    for p, gp, need in zip(params, flat, ctx.needs_input_grad[4:]):
         out.append(gp.to(p.dtype).view_as(p) if need else None)
     ctx.saved = None
     return tuple(out)

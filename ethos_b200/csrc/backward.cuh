@@ -664,4 +664,11 @@ __global__ void k_transpose_f32(const float* __restrict__ in, int rows, int cols
   }
 }
 
+// y += x
+__global__ void k_add_f32(float* __restrict__ y, const float* __restrict__ x, int64_t n) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x)
+    y[i] += x[i];
+}
+
 }  // namespace ethos

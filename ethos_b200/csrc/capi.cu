@@ -763,6 +763,14 @@ int router_bwd_core(const ethos_dims& d, const RouterBwdIO& io, const BwdScratch
   return launch_status();
 }
 
+// dw += add (nothing when add is null)
+int add_routing_grad(float* dw, const float* add, int64_t n, cudaStream_t sm, const DeviceInfo& dev) {
+  if (add == nullptr) return ETHOS_OK;
+  count_launch();
+  k_add_f32<<<static_cast<unsigned>(dev.sm_count * 8), 256, 0, sm>>>(dw, add, n);
+  return launch_status();
+}
+
 }  // namespace
 
 // =================================================================== ABI ==
@@ -1131,14 +1139,14 @@ size_t ethos_backward_workspace_size(const ethos_dims* dims) {
   return c.off + 256;
 }
 
-int ethos_layer_backward(const ethos_dims* dims, int bn_training, float bn_eps, const void* dy, int dy_fp32,
-                         const void* x, const void* w_cat, const float* bn, const void* key_cat, const void* latents,
-                         const void* w1, const void* wv, const int32_t* ids, const float* weights,
-                         const float* save_xp, const void* save_hacc, const float* save_dot, const float* save_qpre,
-                         const float* save_bn, const void* save_qs, const void* htab, const void* gtab,
-                         void* dx, int dx_bf16, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
-                         float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
-                         void* const* stage_events, void* stream) {
+static int layer_backward_bf16(const ethos_dims* dims, int bn_training, float bn_eps, const void* dy, int dy_fp32,
+                               const void* x, const void* w_cat, const float* bn, const void* key_cat, const void* latents,
+                               const void* w1, const void* wv, const int32_t* ids, const float* weights,
+                               const float* save_xp, const void* save_hacc, const float* save_dot, const float* save_qpre,
+                               const float* save_bn, const void* save_qs, const void* htab, const void* gtab,
+                               void* dx, int dx_bf16, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
+                               float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
+                               void* const* stage_events, const float* dw_add, void* stream) {
   int st = check_dims_impl(dims);
   if (st != ETHOS_OK) return st;
   if (!dy || !x || !w_cat || !bn || !key_cat || !latents || !w1 || !wv || !ids || !weights || !save_xp ||
@@ -1216,6 +1224,8 @@ int ethos_layer_backward(const ethos_dims* dims, int bn_training, float bn_eps, 
     if ((st = expert_bwd_core(d, io, s, dev_err, sm, *dev)) != ETHOS_OK) return st;
   }
   mark(stage_events, ETHOS_BWD_STAGE_EXPERTS, sm);  // d_latents, d_w1 final
+  // the routing weights' gradient from elsewhere (a loss on the weights)
+  if ((st = add_routing_grad(s.dw, dw_add, static_cast<int64_t>(T) * H * d.top_k, sm, *dev)) != ETHOS_OK) return st;
   // (9)-(11) router: dq (bf16 into du[:, :HQ]), d_keys, d_bn
   {
     RouterBwdIO io;
@@ -1283,6 +1293,35 @@ int ethos_layer_backward(const ethos_dims* dims, int bn_training, float bn_eps, 
   }
   mark(stage_events, ETHOS_BWD_STAGE_END, sm);
   return ETHOS_OK;
+}
+
+int ethos_layer_backward(const ethos_dims* dims, int bn_training, float bn_eps, const void* dy, int dy_fp32,
+                         const void* x, const void* w_cat, const float* bn, const void* key_cat, const void* latents,
+                         const void* w1, const void* wv, const int32_t* ids, const float* weights,
+                         const float* save_xp, const void* save_hacc, const float* save_dot, const float* save_qpre,
+                         const float* save_bn, const void* save_qs, const void* htab, const void* gtab,
+                         void* dx, int dx_bf16, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
+                         float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
+                         void* const* stage_events, void* stream) {
+  return layer_backward_bf16(dims, bn_training, bn_eps, dy, dy_fp32, x, w_cat, bn, key_cat, latents, w1, wv, ids,
+                             weights, save_xp, save_hacc, save_dot, save_qpre, save_bn, save_qs, htab, gtab, dx,
+                             dx_bf16, d_latents, d_w1, d_w2, d_wq, d_bn, d_keys, workspace, workspace_bytes, dev_err,
+                             stage_events, nullptr, stream);
+}
+
+int ethos_layer_backward_routed(const ethos_dims* dims, int bn_training, float bn_eps, const void* dy, int dy_fp32,
+                                const void* x, const void* w_cat, const float* bn, const void* key_cat, const void* latents,
+                                const void* w1, const void* wv, const int32_t* ids, const float* weights,
+                                const float* save_xp, const void* save_hacc, const float* save_dot, const float* save_qpre,
+                                const float* save_bn, const void* save_qs, const void* htab, const void* gtab,
+                                void* dx, int dx_bf16, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
+                                float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
+                                void* const* stage_events, const float* d_weights,
+                                void* stream) {
+  return layer_backward_bf16(dims, bn_training, bn_eps, dy, dy_fp32, x, w_cat, bn, key_cat, latents, w1, wv, ids,
+                             weights, save_xp, save_hacc, save_dot, save_qpre, save_bn, save_qs, htab, gtab, dx,
+                             dx_bf16, d_latents, d_w1, d_w2, d_wq, d_bn, d_keys, workspace, workspace_bytes, dev_err,
+                             stage_events, d_weights, stream);
 }
 
 size_t ethos_expert_backward_workspace_size(const ethos_dims* dims) {
@@ -1902,14 +1941,14 @@ size_t ethos_backward_workspace_size_f32(const ethos_dims* dims) {
   return c.off + 256;
 }
 
-int ethos_layer_backward_f32(const ethos_dims* dims, int bn_training, float bn_eps, const float* dy, const float* x,
-                             const float* w_cat, const float* bn, const float* keys, const float* latents,
-                             const float* w1, const float* wv, const int32_t* ids, const float* weights,
-                             const float* save_xp, const float* save_hacc, const float* save_dot,
-                             const float* save_qpre, const float* save_bn, const float* save_qhat, const float* htab,
-                             const float* gtab, float* dx, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
-                             float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
-                             void* const* stage_events, void* stream) {
+static int layer_backward_f32(const ethos_dims* dims, int bn_training, float bn_eps, const float* dy, const float* x,
+                              const float* w_cat, const float* bn, const float* keys, const float* latents,
+                              const float* w1, const float* wv, const int32_t* ids, const float* weights,
+                              const float* save_xp, const float* save_hacc, const float* save_dot,
+                              const float* save_qpre, const float* save_bn, const float* save_qhat, const float* htab,
+                              const float* gtab, float* dx, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
+                              float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
+                              void* const* stage_events, const float* dw_add, void* stream) {
   int st = check_dims_f32(dims);
   if (st != ETHOS_OK) return st;
   if (!dy || !x || !w_cat || !bn || !keys || !latents || !w1 || !wv || !ids || !weights || !save_xp ||
@@ -2007,6 +2046,8 @@ int ethos_layer_backward_f32(const ethos_dims* dims, int bn_training, float bn_e
                        true, dev_err, sm, *dev)) != ETHOS_OK)
     return st;
   mark(stage_events, ETHOS_BWD_STAGE_EXPERTS, sm);  // d_latents, d_w1 final
+  // the routing weights' gradient from elsewhere (a loss on the weights)
+  if ((st = add_routing_grad(s.dw, dw_add, static_cast<int64_t>(T) * R, sm, *dev)) != ETHOS_OK) return st;
   // (9) router: softmax backward, dq^ and the dense score gradient dS
   switch (d.top_k) {
     case 4: st = launch_router_bwd_f32<4>(d, ids, weights, s.dw, keys, s.dqhat, s.dS, sm, *dev); break;
@@ -2066,6 +2107,33 @@ int ethos_layer_backward_f32(const ethos_dims* dims, int bn_training, float bn_e
     return st;
   mark(stage_events, ETHOS_BWD_STAGE_END, sm);
   return ETHOS_OK;
+}
+
+int ethos_layer_backward_f32(const ethos_dims* dims, int bn_training, float bn_eps, const float* dy, const float* x,
+                             const float* w_cat, const float* bn, const float* keys, const float* latents,
+                             const float* w1, const float* wv, const int32_t* ids, const float* weights,
+                             const float* save_xp, const float* save_hacc, const float* save_dot,
+                             const float* save_qpre, const float* save_bn, const float* save_qhat, const float* htab,
+                             const float* gtab, float* dx, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
+                             float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
+                             void* const* stage_events, void* stream) {
+  return layer_backward_f32(dims, bn_training, bn_eps, dy, x, w_cat, bn, keys, latents, w1, wv, ids, weights, save_xp,
+                            save_hacc, save_dot, save_qpre, save_bn, save_qhat, htab, gtab, dx, d_latents, d_w1, d_w2,
+                            d_wq, d_bn, d_keys, workspace, workspace_bytes, dev_err, stage_events, nullptr, stream);
+}
+
+int ethos_layer_backward_routed_f32(const ethos_dims* dims, int bn_training, float bn_eps, const float* dy, const float* x,
+                                    const float* w_cat, const float* bn, const float* keys, const float* latents,
+                                    const float* w1, const float* wv, const int32_t* ids, const float* weights,
+                                    const float* save_xp, const float* save_hacc, const float* save_dot,
+                                    const float* save_qpre, const float* save_bn, const float* save_qhat, const float* htab,
+                                    const float* gtab, float* dx, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
+                                    float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
+                                    void* const* stage_events, const float* d_weights,
+                                    void* stream) {
+  return layer_backward_f32(dims, bn_training, bn_eps, dy, x, w_cat, bn, keys, latents, w1, wv, ids, weights, save_xp,
+                            save_hacc, save_dot, save_qpre, save_bn, save_qhat, htab, gtab, dx, d_latents, d_w1, d_w2,
+                            d_wq, d_bn, d_keys, workspace, workspace_bytes, dev_err, stage_events, d_weights, stream);
 }
 
 }  // extern "C"

@@ -28,12 +28,18 @@ the output head's GEMM runs with the vocabulary padded to a multiple of 8
 (an odd row length of the logits otherwise sends cuBLAS to an unaligned
 kernel: 30 ms instead of 2-3 ms at config 4); the logits returned are a view
 of the unpadded columns.
+
+``EthosDecoder.loss`` is the training path (train.py:188-203 computes logits and
+their cross entropy): token embedding, cross entropy of the head and, where
+asked for, the balance of the routing run on this repository's kernels
+(``ethos_b200.functional``), and the logits are never in memory.
 """
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import functional as EF
 from .layer import EthosExpertLayer
 
 __all__ = ["DecoderConfig", "RMSNorm", "LatentAttention", "SwiGLU", "DecoderBlock", "EthosDecoder"]
@@ -191,10 +197,17 @@ class DecoderBlock(nn.Module):
         h = x + self.self_attn(self.input_layernorm(x))
         return h + self.mlp(self.post_attention_layernorm(h))
 
+    def forward_routed(self, x):
+        """``(output, routing weights, expert ids)`` of an expert block."""
+        h = x + self.self_attn(self.input_layernorm(x))
+        y, weights, ids = self.mlp(self.post_attention_layernorm(h), return_routing=True)
+        return h + y, weights, ids
+
 
 class EthosDecoder(nn.Module):
     """``CompressedMoEModel`` with the B200 expert layers: ``forward(input_ids
-    [B, S]) -> logits [B, S, vocab]`` (causal, positions 0..S-1)."""
+    [B, S]) -> logits [B, S, vocab]`` (causal, positions 0..S-1), and ``loss``
+    for training, which needs no logits."""
 
     def __init__(self, config):
         super().__init__()
@@ -221,3 +234,32 @@ class EthosDecoder(nn.Module):
         # aligned rows for cuBLAS; the extra columns are dropped by the view
         return F.linear(h, F.pad(w, (0, 0, 0, pad)))[..., :w.shape[0]]
 
+    def loss(self, input_ids, labels, balance_coef=0.0, ignore_index=-100, mask=None):
+        """Training loss of one batch: the mean cross entropy of the tokens
+        whose label is not ``ignore_index`` (``labels[b, s]`` is the token that
+        should follow ``input_ids[b, :s + 1]``), plus ``balance_coef`` times
+        the mean over the expert layers of the balance loss of their routing
+        (``functional.balance_loss``; ``mask`` bool ``[B, S]``, False where a
+        token, such as padding, should not count in it).
+
+        Returns ``(loss, parts)``, ``parts`` a dict of detached tensors:
+        ``cross_entropy`` and, with a balance coefficient, ``balance`` ``[L]``
+        and ``expert_counts`` int32 ``[L, N]`` of the L expert layers."""
+        h = EF.embedding(input_ids, self.tok_embeddings.weight)
+        flat_mask = None if mask is None else mask.reshape(-1)
+        balance, counts = [], []
+        for blk in self.layers:
+            if balance_coef and isinstance(blk.mlp, EthosExpertLayer):
+                h, weights, ids = blk.forward_routed(h)
+                b, c = EF.balance_loss(weights, ids, blk.mlp.num_experts, mask=flat_mask)
+                balance.append(b)
+                counts.append(c)
+            else:
+                h = blk(h)
+        ce = EF.linear_cross_entropy(self.norm(h), self.output.weight, labels, ignore_index=ignore_index)
+        parts = {"cross_entropy": ce.detach()}
+        if not balance:
+            return ce, parts
+        balance = torch.stack(balance)
+        parts["balance"], parts["expert_counts"] = balance.detach(), torch.stack(counts)
+        return ce + balance_coef * balance.mean(), parts

@@ -177,7 +177,7 @@ class _EthosLayerFunction(torch.autograd.Function):
     """Autograd boundary around the fused forward (and backward) kernels."""
 
     @staticmethod
-    def forward(ctx, x2d, layer, need_grad, *params):
+    def forward(ctx, x2d, layer, need_grad, routing, *params):
         # need_grad is decided by the caller: inside Function.forward grad
         # mode is always off and needs_input_grad ignores torch.no_grad()
         pw = layer._packed(x2d.device, fresh=need_grad)
@@ -199,12 +199,19 @@ class _EthosLayerFunction(torch.autograd.Function):
         ctx.params = params
         if need_grad:
             ctx.saved = dict(out, xin=xin, pw=pw)
-        return out["y"].to(x2d.dtype)
+        if not routing:
+            return out["y"].to(x2d.dtype)
+        # the routing weights and ids themselves, as outputs of their own
+        # (aliases: ctx keeps the tensors, and would otherwise keep itself)
+        w, ids = out["weights"].detach(), out["ids"].detach()
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        return out["y"].to(x2d.dtype), w, ids
 
     @staticmethod
-    def backward(ctx, gy):
+    def backward(ctx, gy, gw=None, _=None):
         from . import backward as bwd  # noqa: WPS433 (kept local: built after the forward)
-        return bwd.layer_backward(ctx, gy)
+        return bwd.layer_backward(ctx, gy, gw)
 
 
 class EthosExpertLayer(nn.Module):
@@ -305,15 +312,22 @@ class EthosExpertLayer(nn.Module):
         ps += [r.sub_keys_1.weight, r.sub_keys_2.weight]
         return ps
 
-    def forward(self, x):
+    def forward(self, x, return_routing=False):
+        """``y [B, S, d_model]``; with ``return_routing`` also the routing
+        weights (fp32 ``[B * S, H, k]``, differentiable: a loss on them, such
+        as ``functional.balance_loss``, reaches the router) and the expert ids
+        (int32, the same shape)."""
         ops._require_cuda(x, "x")
         batch_size, seq_len, d_model = x.shape
         x2d = x.reshape(-1, d_model)
         _check_token_count(x2d.shape[0], self.router._bn_training(), self.router.d_query)
         params = self._grad_params()
         need_grad = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params))
-        y = _EthosLayerFunction.apply(x2d, self, need_grad, *params)
-        return y.view(batch_size, seq_len, d_model)
+        out = _EthosLayerFunction.apply(x2d, self, need_grad, return_routing, *params)
+        if not return_routing:
+            return out.view(batch_size, seq_len, d_model)
+        y, weights, ids = out
+        return y.view(batch_size, seq_len, d_model), weights, ids
 
 
 def swap_expert_layers(model, config=None):

@@ -310,7 +310,16 @@ def _numel(shape):
 BWD_STAGE_EXPERTS, BWD_STAGE_END = 0, 1  # ETHOS_BWD_STAGE_* (include/ethos_b200.h)
 
 
-def layer_backward(dy, x16, pw, saved, bn_training, eps, stage_events=None, dx_dtype=torch.float32):
+def _routing_grad(d_weights, T, d):
+    """The routing weights' gradient as the library reads it (None: none)."""
+    if d_weights is None:
+        return None
+    if tuple(d_weights.shape) != (T, d["num_heads"], d["top_k"]):
+        raise ValueError(f"d_weights: [T, H, k], got {tuple(d_weights.shape)}")
+    return d_weights.to(torch.float32).contiguous()
+
+
+def layer_backward(dy, x16, pw, saved, bn_training, eps, stage_events=None, dx_dtype=torch.float32, d_weights=None):
     """Gradients of the layer (see ethos_layer_backward).  ``dy`` [T, d] bf16
     or fp32; ``saved`` is the dict returned by ``layer_forward(save=True)``.
     Returns a dict of fp32 tensors (dx in ``dx_dtype``, fp32 or bf16): dx,
@@ -318,7 +327,9 @@ def layer_backward(dy, x16, pw, saved, bn_training, eps, stage_events=None, dx_d
     d_bn [3, H*dq] (bias, gamma, beta), d_keys [2, K, dq/2], and the flat fp32
     buffer holding all parameter gradients (``flat``, ``layout``).
     ``stage_events``: optional [experts_done, end] ``torch.cuda.Event`` (or
-    None entries), recorded as ETHOS_BWD_STAGE_* describe."""
+    None entries), recorded as ETHOS_BWD_STAGE_* describe.  ``d_weights``:
+    optional gradient of the routing weights [T, H, k] from elsewhere (a loss
+    on the weights), added before the router's backward."""
     if stage_events is not None and len(stage_events) != 2:
         raise ValueError("stage_events: one event (or None) per ETHOS_BWD_STAGE_*")
     _require_cuda(dy, "dy")
@@ -355,16 +366,19 @@ def layer_backward(dy, x16, pw, saved, bn_training, eps, stage_events=None, dx_d
     if dy.dtype not in (torch.bfloat16, torch.float32):
         dy = dy.float()
     err = device_error_word(dev)
-    check(L.ethos_layer_backward(ctypes.byref(dims), 1 if bn_training else 0, float(eps), _vp(dy),
-                                 1 if dy.dtype == torch.float32 else 0, _vp(x16), _vp(pw.w_cat), _vp(pw.bn),
-                                 _vp(pw.key_cat), _vp(pw.latents), _vp(pw.w1), _vp(pw.wv), _vp(saved["ids"]),
-                                 _vp(saved["weights"]), _vp(saved["xp"]), _vp(saved["hacc"]), _vp(saved["dot"]),
-                                 _vp(saved["qpre"]), _vp(saved.get("bn_stats")), _vp(saved["qs"]),
-                                 _vp(saved.get("htab")), _vp(saved.get("gtab")), _vp(g["dx"]),
-                                 1 if dx_dtype == torch.bfloat16 else 0,
-                                 _vp(g["d_latents"]), _vp(g["d_w1"]), _vp(g["d_w2"]), _vp(g["d_wq"]),
-                                 _vp(g["d_bn"]), _vp(g["d_keys"]), _vp(ws), ws_bytes, _vp(err),
-                                 _events(stage_events), _stream(dev)),
+    dwt = _routing_grad(d_weights, T, d)
+    call = L.ethos_layer_backward if dwt is None else L.ethos_layer_backward_routed
+    extra = () if dwt is None else (_vp(dwt),)
+    check(call(ctypes.byref(dims), 1 if bn_training else 0, float(eps), _vp(dy),
+               1 if dy.dtype == torch.float32 else 0, _vp(x16), _vp(pw.w_cat), _vp(pw.bn),
+               _vp(pw.key_cat), _vp(pw.latents), _vp(pw.w1), _vp(pw.wv), _vp(saved["ids"]),
+               _vp(saved["weights"]), _vp(saved["xp"]), _vp(saved["hacc"]), _vp(saved["dot"]),
+               _vp(saved["qpre"]), _vp(saved.get("bn_stats")), _vp(saved["qs"]),
+               _vp(saved.get("htab")), _vp(saved.get("gtab")), _vp(g["dx"]),
+               1 if dx_dtype == torch.bfloat16 else 0,
+               _vp(g["d_latents"]), _vp(g["d_w1"]), _vp(g["d_w2"]), _vp(g["d_wq"]),
+               _vp(g["d_bn"]), _vp(g["d_keys"]), _vp(ws), ws_bytes, _vp(err),
+               _events(stage_events), *extra, _stream(dev)),
           "ethos_layer_backward")
     return g
 
@@ -500,9 +514,9 @@ def router_forward_f32(x2d, pw, bn_training, eps, momentum):
     return out["weights"], out["ids"]
 
 
-def layer_backward_f32(dy, x32, pw, saved, bn_training, eps, stage_events=None):
+def layer_backward_f32(dy, x32, pw, saved, bn_training, eps, stage_events=None, d_weights=None):
     """Gradients of ``layer_forward_f32(save=True)`` (ethos_layer_backward_f32);
-    the same dict as ``layer_backward``."""
+    the same dict as ``layer_backward``, and the same ``d_weights``."""
     if stage_events is not None and len(stage_events) != 2:
         raise ValueError("stage_events: one event (or None) per ETHOS_BWD_STAGE_*")
     _require_cuda(dy, "dy")
@@ -523,14 +537,17 @@ def layer_backward_f32(dy, x32, pw, saved, bn_training, eps, stage_events=None):
     g["layout"] = layout
     dy = dy.contiguous().float()
     err = device_error_word(dev)
-    check(L.ethos_layer_backward_f32(ctypes.byref(dims), 1 if bn_training else 0, float(eps), _vp(dy), _vp(x32),
-                                     _vp(pw.w_cat), _vp(pw.bn), _vp(pw.key_cat), _vp(pw.latents), _vp(pw.w1),
-                                     _vp(pw.wv), _vp(saved["ids"]), _vp(saved["weights"]), _vp(saved["xp"]),
-                                     _vp(saved["hacc"]), _vp(saved["dot"]), _vp(saved["qpre"]),
-                                     _vp(saved.get("bn_stats")), _vp(saved["qhat"]), _vp(saved.get("htab")),
-                                     _vp(saved.get("gtab")), _vp(g["dx"]), _vp(g["d_latents"]), _vp(g["d_w1"]),
-                                     _vp(g["d_w2"]), _vp(g["d_wq"]), _vp(g["d_bn"]), _vp(g["d_keys"]), _vp(ws),
-                                     ws_bytes, _vp(err), _events(stage_events), _stream(dev)),
+    dwt = _routing_grad(d_weights, T, d)
+    call = L.ethos_layer_backward_f32 if dwt is None else L.ethos_layer_backward_routed_f32
+    extra = () if dwt is None else (_vp(dwt),)
+    check(call(ctypes.byref(dims), 1 if bn_training else 0, float(eps), _vp(dy), _vp(x32),
+               _vp(pw.w_cat), _vp(pw.bn), _vp(pw.key_cat), _vp(pw.latents), _vp(pw.w1),
+               _vp(pw.wv), _vp(saved["ids"]), _vp(saved["weights"]), _vp(saved["xp"]),
+               _vp(saved["hacc"]), _vp(saved["dot"]), _vp(saved["qpre"]),
+               _vp(saved.get("bn_stats")), _vp(saved["qhat"]), _vp(saved.get("htab")),
+               _vp(saved.get("gtab")), _vp(g["dx"]), _vp(g["d_latents"]), _vp(g["d_w1"]),
+               _vp(g["d_w2"]), _vp(g["d_wq"]), _vp(g["d_bn"]), _vp(g["d_keys"]), _vp(ws),
+               ws_bytes, _vp(err), _events(stage_events), *extra, _stream(dev)),
           "ethos_layer_backward_f32")
     return g
 

@@ -450,6 +450,29 @@ size_t ethos_grad_clip_workspace_size(void);
 int ethos_grad_clip_coef(const ethos_adam_tensor* tensors, int num_tensors, float max_norm, void* workspace,
                          size_t workspace_bytes, float* out, int* dev_err, void* stream);
 
+/* ethos_layer_backward and ethos_layer_backward_f32 with a gradient of the
+ * routing weights from elsewhere (d_weights fp32 [T, H, k], e.g. of a balance
+ * loss), added to the one that the layer's output gives before the router's
+ * backward; NULL: none. */
+int ethos_layer_backward_routed(const ethos_dims* dims, int bn_training, float bn_eps, const void* dy, int dy_fp32,
+                         const void* x, const void* w_cat, const float* bn, const void* key_cat, const void* latents,
+                         const void* w1, const void* wv, const int32_t* ids, const float* weights,
+                         const float* save_xp, const void* save_hacc, const float* save_dot, const float* save_qpre,
+                         const float* save_bn, const void* save_qs, const void* htab, const void* gtab,
+                         void* dx, int dx_bf16, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
+                         float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
+                         void* const* stage_events, const float* d_weights,
+                         void* stream);
+int ethos_layer_backward_routed_f32(const ethos_dims* dims, int bn_training, float bn_eps, const float* dy, const float* x,
+                             const float* w_cat, const float* bn, const float* keys, const float* latents,
+                             const float* w1, const float* wv, const int32_t* ids, const float* weights,
+                             const float* save_xp, const float* save_hacc, const float* save_dot,
+                             const float* save_qpre, const float* save_bn, const float* save_qhat, const float* htab,
+                             const float* gtab, float* dx, float* d_latents, float* d_w1, float* d_w2, float* d_wq,
+                             float* d_bn, float* d_keys, void* workspace, size_t workspace_bytes, int* dev_err,
+                             void* const* stage_events, const float* d_weights,
+                         void* stream);
+
 /* ------------------------------------------- training: the model's ends --
  * Operators of a training step around the expert layers: the token embedding
  * (model.py:374), the balance of the routing, and the cross entropy of the
