@@ -362,7 +362,7 @@ int xent_index(const XentPlan& p, const XentSave& sv, const void* labels, int la
 
 template <int MODE, int PLANES>
 int launch_xent(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1, const CUtensorMap& b1,
-                const XeArgs& args, int64_t units, int* err, cudaStream_t sm, const DeviceInfo& dev) {
+                const CUtensorMap& c, const XeArgs& args, int64_t units, int* err, cudaStream_t sm, const DeviceInfo& dev) {
   auto kern = k_xent_gemm<MODE, PLANES>;
   int st = smem_attr_once(reinterpret_cast<const void*>(kern), xe_smem<PLANES>());
   if (st != ETHOS_OK) return st;
@@ -391,15 +391,15 @@ int launch_xent(const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap&
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   count_launch();
-  if (cudaLaunchKernelEx(&cfg, kern, a0, b0, a1, b1, args, err) != cudaSuccess) return ETHOS_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, kern, a0, b0, a1, b1, c, args, err) != cudaSuccess) return ETHOS_ERR_CUDA;
   return launch_status();
 }
 template <int MODE>
 int launch_xent_planes(int planes, const CUtensorMap& a0, const CUtensorMap& b0, const CUtensorMap& a1,
-                       const CUtensorMap& b1, const XeArgs& args, int64_t units, int* err, cudaStream_t sm,
-                       const DeviceInfo& dev) {
-  return planes == 1 ? launch_xent<MODE, 1>(a0, b0, a1, b1, args, units, err, sm, dev)
-                     : launch_xent<MODE, 3>(a0, b0, a1, b1, args, units, err, sm, dev);
+                       const CUtensorMap& b1, const CUtensorMap& c, const XeArgs& args, int64_t units, int* err,
+                       cudaStream_t sm, const DeviceInfo& dev) {
+  return planes == 1 ? launch_xent<MODE, 1>(a0, b0, a1, b1, c, args, units, err, sm, dev)
+                     : launch_xent<MODE, 3>(a0, b0, a1, b1, c, args, units, err, sm, dev);
 }
 
 // The rows of hidden that the products read: hidden itself (bf16, aligned, no
@@ -438,8 +438,13 @@ int xent_logits(const XentPlan& p, const XentSave& sv, const XentRowsOperand& h,
   a.dl = e;
   a.ldl = lde;
   const int64_t units = p.t_pad / XE_TILE * p.runs;
-  if constexpr (MODE == XE_KEEP) return launch_xent<MODE, 1>(ta, tb, ta, tb, a, units, err, sm, dev);
-  else return launch_xent_planes<MODE>(p.planes, ta, tb, ta, tb, a, units, err, sm, dev);
+  if constexpr (MODE == XE_KEEP) {
+    CUtensorMap tc;
+    if ((st = make_tmap_bf16(&tc, e, p.t_pad, lde, 32, lde)) != ETHOS_OK) return st;
+    return launch_xent<MODE, 1>(ta, tb, ta, tb, tc, a, units, err, sm, dev);
+  } else {
+    return launch_xent_planes<MODE>(p.planes, ta, tb, ta, tb, ta, a, units, err, sm, dev);
+  }
 }
 
 int xent_loss(const XentPlan& p, const XentSave& sv, const XentFwd& ws, int reduction, float* loss, cudaStream_t sm,
@@ -449,6 +454,14 @@ int xent_loss(const XentPlan& p, const XentSave& sv, const XentFwd& ws, int redu
                     sm, sv.rw, static_cast<const float2*>(ws.part), 2 * p.runs, p.t_pad, keep, again, redo_tile,
                     reduction, loss, ws.block_sum, static_cast<const __nv_bfloat16*>(sv.hp), hr,
                     static_cast<int>(p.ldd));
+}
+
+// dW's tensor map (bf16 rows of 16-byte pieces), or any map where it has none.
+int xent_dw_tmap(CUtensorMap* m, const CUtensorMap& other, XeArgs* g, int64_t rows, int64_t d) {
+  g->dw_tma = g->dw != nullptr && g->dw_bf16 && d % 8 == 0 && aligned16(g->dw);
+  if (g->dw_tma) return make_tmap_bf16(m, g->dw, rows, d, 32, d);
+  *m = other;
+  return ETHOS_OK;
 }
 
 int64_t xent_grad_units(const XentPlan& p, int64_t n, int slots, const XeArgs& g) {
@@ -723,7 +736,9 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   g.label_span = ws.sort.span;
   g.do_dh = d_hidden != nullptr;
   g.do_dw = d_weight != nullptr;
-  if ((st = launch_xent<XE_GRADS, 1>(ek, wk, em, hb, g, xent_grad_units(p, vocab, p.slots, g), dev_err, sm, *dev)) !=
+  CUtensorMap wc;
+  if ((st = xent_dw_tmap(&wc, ek, &g, vocab, dim)) != ETHOS_OK) return st;
+  if ((st = launch_xent<XE_GRADS, 1>(ek, wk, em, hb, wc, g, xent_grad_units(p, vocab, p.slots, g), dev_err, sm, *dev)) !=
       ETHOS_OK)
     return st;
   if (!d_hidden) return ETHOS_OK;
@@ -796,7 +811,9 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     a.dl = ws.dl;
     a.dl_plane_rows = p.t_pad;
     a.ldl = p.piece;
-    if ((st = launch_xent_planes<XE_DLOGITS>(p.planes, ha, wb, ha, wb, a, num_m * ((n + p.tile_n - 1) / p.tile_n),
+    CUtensorMap dc;
+    if ((st = make_tmap_bf16(&dc, ws.dl, p.planes * p.t_pad, p.piece, 32, p.piece)) != ETHOS_OK) return st;
+    if ((st = launch_xent_planes<XE_DLOGITS>(p.planes, ha, wb, ha, wb, dc, a, num_m * ((n + p.tile_n - 1) / p.tile_n),
                                              dev_err, sm, *dev)) != ETHOS_OK)
       return st;
     XeArgs g = {};
@@ -815,7 +832,9 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     g.do_dh = d_hidden != nullptr;
     g.do_dw = d_weight != nullptr;
     const int64_t units = xent_grad_units(p, n, p.slots_piece, g);
-    if ((st = launch_xent_planes<XE_GRADS>(p.planes, dk, wk, dm, hb, g, units, dev_err, sm, *dev)) != ETHOS_OK)
+    CUtensorMap wc;
+    if ((st = xent_dw_tmap(&wc, dk, &g, n, dim)) != ETHOS_OK) return st;
+    if ((st = launch_xent_planes<XE_GRADS>(p.planes, dk, wk, dm, hb, wc, g, units, dev_err, sm, *dev)) != ETHOS_OK)
       return st;
   }
   if (!d_hidden) return ETHOS_OK;

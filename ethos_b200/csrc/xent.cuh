@@ -523,6 +523,7 @@ struct XeArgs {
   int64_t dh_ld;
   void* dw;            // rows of this piece, [N rows][d] with pitch d
   int dw_bf16;
+  int dw_tma;          // dW through the tensor map tmC (16-byte rows)
   const float* label_rows;  // added to dW before scaling: row v's is label_rows[label_span[v].x],
   const int2* label_span;   // where that span is not empty
   int do_dh, do_dw;
@@ -584,9 +585,14 @@ __device__ __forceinline__ bool xe_wait(uint64_t* bar, uint32_t parity, volatile
     }
   }
 }
+// bf16 outputs (E, dl, dW) leave through TMA stores of each warp's staged 32 x 64
+// block: written from the lanes, whose rows are far apart, E took KEEP from
+// MEASURED_STG
+constexpr int XE_STG_WARP_BYTES = 32 * 128;
 template <int PLANES>
 constexpr int xe_smem() {
-  return XeCfg<PLANES>::kStages * XeCfg<PLANES>::kStageBytes + 1024 + static_cast<int>(sizeof(XeCtl));
+  return XeCfg<PLANES>::kStages * XeCfg<PLANES>::kStageBytes + (PLANES == 1 ? XE_EPI_WARPS * XE_STG_WARP_BYTES : 0) +
+         1024 + static_cast<int>(sizeof(XeCtl));
 }
 static_assert(xe_smem<1>() <= 227 * 1024 && xe_smem<3>() <= 227 * 1024, "shared memory");
 
@@ -792,6 +798,30 @@ __device__ __forceinline__ auto& pick(A& a, B& b) {
   if constexpr (kFirst) return a;
   else return b;
 }
+// 64 bf16 columns of the warp's 32 rows (v0, v1: this lane's row) at (col, row0)
+// of the matrix behind tm, through the warp's staging block
+__device__ __forceinline__ void block_store_bf16(const CUtensorMap* tm, uint8_t* stg, int lane, const float (&v0)[32],
+                                                 const float (&v1)[32], int col, int row0) {
+  if (lane == 0) bulk_wait_read<0>();  // the block's last store has read it
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint4 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* x = (c == 0 ? v0 : v1) + 8 * j;
+      w[j] = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                        pack_bf16x2(x[6], x[7]));
+    }
+    stage_row_sw128(stg, lane, c, w);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(tm, stg, col, row0);
+    bulk_commit();
+  }
+}
 __device__ __forceinline__ int byte_align(const void* p, int64_t pitch_bytes) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(pitch_bytes);
   return (x & 31u) == 0 ? 32 : ((x & 15u) == 0 ? 16 : 1);
@@ -832,7 +862,7 @@ template <int MODE, int PLANES>
 __global__ void __launch_bounds__(XE_THREADS, 1)
     k_xent_gemm(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmB0,
                 const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB1,
-                const __grid_constant__ XeArgs args, int* err) {
+                const __grid_constant__ CUtensorMap tmC, const __grid_constant__ XeArgs args, int* err) {
   using Cfg = XeCfg<PLANES>;
   constexpr int HALVES = Cfg::kHalves;
   constexpr int STAGES = Cfg::kStages;
@@ -840,7 +870,8 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
   constexpr int CHUNKS = (XE_TILE / 32) / (XE_EPI_WARPS / 4);  // 32-column chunks per epilogue warp
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
-  XeCtl* ctl = reinterpret_cast<XeCtl*>(smem + STAGES * STAGE_BYTES);
+  uint8_t* stg_s = smem + STAGES * STAGE_BYTES;
+  XeCtl* ctl = reinterpret_cast<XeCtl*>(stg_s + (PLANES == 1 ? XE_EPI_WARPS * XE_STG_WARP_BYTES : 0));
   const int warp = warp_id();
   const int lane = lane_id();
   const uint32_t rank = cluster_ctarank();
@@ -1064,13 +1095,14 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     XeStep st;
     const int q = warp & 3;
     const int ch = (warp - XE_EPI_WARP0) >> 2;  // column half of an accumulator
+    uint8_t* stg = stg_s + (warp - XE_EPI_WARP0) * XE_STG_WARP_BYTES;  // PLANES 1
     const uint32_t acc_empty0 = cluster_map(smem_u32(&ctl->acc_empty[0]), 0);
     const uint32_t acc_empty1 = cluster_map(smem_u32(&ctl->acc_empty[1]), 0);
     int it0 = 0, it1 = 0;  // accumulations taken (HALVES 1: all in it0)
     bool ok = true;
     // per-row state (this lane's row of the tile)
     int y = -1;
-    bool live = false;
+    bool live = false, all_live = false;
     float run_m = -INFINITY, run_s = 0.0f;  // STATS, KEEP
     float c2 = 0.0f;                        // KEEP: shift, DLOGITS: logsumexp, in units of log 2
     float g = 1.0f, at_label = 0.0f;        // DLOGITS
@@ -1086,6 +1118,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
           live = y >= 0;
           c2 = live ? args.rw.c[row] * XE_LOG2E : 0.0f;
         }
+        all_live = __all_sync(0xffffffffu, live);
         run_m = -INFINITY;
         run_s = 0.0f;
       }
@@ -1171,30 +1204,45 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
 #pragma unroll
           for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) m = fmaxf(m, v[k][i]);
-          float s0 = 0.0f, s1 = 0.0f;
+            for (int i = 0; i < 32; i += 2) m = fmaxf(m, fmaxf(v[k][i], v[k][i + 1]));
+          // exponentials in pairs: one packed fma and one packed add for two
+          unsigned long long sum2 = pk2(0.0f, 0.0f);
+          const unsigned long long l2 = pk2(XE_LOG2E, XE_LOG2E);
+          float s0, s1;
           if (MODE == XE_KEEP) {
+            const unsigned long long mc = pk2(-c2, -c2);
 #pragma unroll
             for (int k = 0; k < CHUNKS; ++k) {
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
-                v[k][i] = live ? ex2_approx(fmaf(v[k][i], XE_LOG2E, -c2)) : 0.0f;
-                v[k][i + 1] = live ? ex2_approx(fmaf(v[k][i + 1], XE_LOG2E, -c2)) : 0.0f;
-                s0 += v[k][i];
-                s1 += v[k][i + 1];
+                float t0, t1;
+                upk2(ffma2(pk2(v[k][i], v[k][i + 1]), l2, mc), t0, t1);
+                v[k][i] = ex2_approx(t0);
+                v[k][i + 1] = ex2_approx(t1);
               }
-              row_store_bf16(args.dl + row * args.ldl, col0 + k * 32, static_cast<int>(args.ldl), 32, v[k]);
+              if (!all_live) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[k][i] = live ? v[k][i] : 0.0f;
+              }
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) sum2 = fadd2(sum2, pk2(v[k][i], v[k][i + 1]));
+              if (k % 2 == 1 && col0 + (k - 1) * 32 < args.ldl)
+                block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32, row - lane);
             }
+            upk2(sum2, s0, s1);
             run_s += s0 + s1;
           } else if (m > -INFINITY) {
             const float m2 = m * XE_LOG2E;
+            const unsigned long long mm = pk2(-m2, -m2);
 #pragma unroll
             for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
-                s0 += ex2_approx(fmaf(v[k][i], XE_LOG2E, -m2));
-                s1 += ex2_approx(fmaf(v[k][i + 1], XE_LOG2E, -m2));
+                float t0, t1;
+                upk2(ffma2(pk2(v[k][i], v[k][i + 1]), l2, mm), t0, t1);
+                sum2 = fadd2(sum2, pk2(ex2_approx(t0), ex2_approx(t1)));
               }
+            upk2(sum2, s0, s1);
             run_s = fmaf(run_s, ex2_approx(fmaf(run_m, XE_LOG2E, -m2)), s0 + s1);
           } else {  // -inf or NaN only: NaN is carried into the sum
 #pragma unroll
@@ -1224,13 +1272,18 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
               for (int i = 0; i < 32; ++i)
                 if (col + i >= N) v[k][i] = 0.0f;
             }
+            if constexpr (PLANES == 1) {
+              if (k % 2 == 1 && col0 + (k - 1) * 32 < args.ldl)
+                block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32, row - lane);
+            } else {
 #pragma unroll
-            for (int pl = 0; pl < PLANES; ++pl) {
-              row_store_bf16(args.dl + (pl * args.dl_plane_rows + row) * args.ldl, col, static_cast<int>(args.ldl), 32,
-                             v[k]);
-              if (pl + 1 < PLANES) {
+              for (int pl = 0; pl < PLANES; ++pl) {
+                row_store_bf16(args.dl + (pl * args.dl_plane_rows + row) * args.ldl, col, static_cast<int>(args.ldl),
+                               32, v[k]);
+                if (pl + 1 < PLANES) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[k][i] -= __bfloat162float(__float2bfloat16_rn(v[k][i]));
+                  for (int i = 0; i < 32; ++i) v[k][i] -= __bfloat162float(__float2bfloat16_rn(v[k][i]));
+                }
               }
             }
           }
@@ -1241,10 +1294,11 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
             for (int k = 0; k < CHUNKS; ++k)
               row_store_f32(o, col0 + k * 32, static_cast<int>(args.dh_ld), 32, v[k], args.dh_accumulate != 0);
           }
-        } else if (row < args.p[1].M) {
+        } else {
           const int d = args.p[1].N;
+          const bool in = row < args.p[1].M;
           const float* extra = nullptr;
-          if (args.label_rows != nullptr) {
+          if (args.label_rows != nullptr && in) {
             const int2 sp = args.label_span[row];
             if (sp.x < sp.y) extra = args.label_rows + static_cast<int64_t>(sp.x) * d;
           }
@@ -1268,16 +1322,22 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
             }
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[k][i] *= scale;
-            if (args.dw_bf16)
-              row_store_bf16(static_cast<__nv_bfloat16*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k]);
-            else
-              row_store_f32(static_cast<float*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k], false);
+            if (PLANES == 1 && args.dw_tma) {
+              if (k % 2 == 1 && col0 + (k - 1) * 32 < d)
+                block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32, row - lane);
+            } else if (in) {
+              if (args.dw_bf16)
+                row_store_bf16(static_cast<__nv_bfloat16*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k]);
+              else
+                row_store_f32(static_cast<float*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k], false);
+            }
           }
         }
       }
       if ((MODE == XE_STATS || MODE == XE_KEEP) && st.last && ok && row < rows)
         args.part[(st.slot * 2 + ch) * args.part_ld + row] = make_float2(run_m, run_s);
     }
+    if (PLANES == 1 && lane == 0) bulk_wait<0>();  // the stores have read their blocks and written
   }
 
   // Teardown as in k_gemm2sm: every accumulator was consumed (or the roles
