@@ -206,6 +206,7 @@ struct XentPlan {
   int tile_n;              // columns of a GEMM tile
   bool keep;               // the keep way is open
   bool pack_w;             // the table is read through bf16 planes
+  bool pad_dw;             // bf16 dW of an odd width goes through padded rows
   int64_t ldd;             // columns of a plane
   int64_t t_pad, v_pad;    // rows of a plane
   int run, runs;           // STATS: column tiles per unit, units along the vocabulary
@@ -222,6 +223,7 @@ XentPlan xent_plan(int64_t T, int64_t V, int64_t d, int dtype) {
   p.planes = dtype == ETHOS_F32 ? 3 : 1;
   p.tile_n = p.planes == 1 ? XeCfg<1>::kTileN : XeCfg<3>::kTileN;
   p.pack_w = dtype == ETHOS_F32 || d % 8 != 0;
+  p.pad_dw = dtype == ETHOS_BF16 && d % 8 != 0;
   p.ldd = up(d, 8);
   p.t_pad = up(T, XE_TILE);
   p.v_pad = up(V, XE_TILE);
@@ -285,18 +287,21 @@ struct XentFwd {
 };
 void carve_xent_fwd(Carve& c, const XentPlan& p, XentFwd* s) {
   s->wp = p.pack_w ? c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.v_pad * p.ldd)) : nullptr;
-  s->part = c.take<float2>(static_cast<size_t>(2 * p.runs * p.t_pad));
+  const int64_t parts = 2 * p.runs > XE_FEW_BLOCKS ? 2 * p.runs : XE_FEW_BLOCKS;
+  s->part = c.take<float2>(static_cast<size_t>(parts * p.t_pad));
   s->block_sum = c.take<double>(static_cast<size_t>(p.t_pad / XE_LOSS_ROWS));
 }
 struct XentBwd {
   __nv_bfloat16* wp;
   __nv_bfloat16* dl;
   float* dh;
+  __nv_bfloat16* dwp;  // rows of dW at a pitch of whole 16-byte pieces
 };
 void carve_xent_bwd(Carve& c, const XentPlan& p, XentBwd* s) {
   s->wp = p.pack_w ? c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.v_pad * p.ldd)) : nullptr;
   s->dl = c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.t_pad * p.piece));
   s->dh = c.take<float>(static_cast<size_t>(p.slots_piece * p.t_pad * p.dh_ld));
+  s->dwp = p.pad_dw ? c.take<__nv_bfloat16>(static_cast<size_t>(p.piece * p.ldd)) : nullptr;
 }
 struct XentKeep {
   XentFwd f;
@@ -307,6 +312,7 @@ struct XentKeep {
   float* dh;
   EmbedScratch sort;
   float* label_rows;
+  __nv_bfloat16* dwp;
 };
 void carve_xent_keep(Carve& c, const XentPlan& p, XentKeep* s) {
   carve_xent_fwd(c, p, &s->f);
@@ -317,6 +323,7 @@ void carve_xent_keep(Carve& c, const XentPlan& p, XentKeep* s) {
   s->dh = c.take<float>(static_cast<size_t>(p.slots * p.t_pad * p.dh_ld));
   carve_embed(c, p.t_pad, p.V, p.d, &s->sort);
   s->label_rows = c.take<float>(static_cast<size_t>(p.t_pad * p.d));
+  s->dwp = p.pad_dw ? c.take<__nv_bfloat16>(static_cast<size_t>(p.v_pad * p.ldd)) : nullptr;
 }
 
 int xent_pack_w(const XentPlan& p, int dtype, const void* weight, int64_t ldw, __nv_bfloat16* wp, cudaStream_t sm,
@@ -448,20 +455,69 @@ int xent_logits(const XentPlan& p, const XentSave& sv, const XentRowsOperand& h,
 }
 
 int xent_loss(const XentPlan& p, const XentSave& sv, const XentFwd& ws, int reduction, float* loss, cudaStream_t sm,
-              bool keep = false, bool again = false, int* redo_tile = nullptr, __nv_bfloat16* hr = nullptr) {
+              int parts, bool keep = false, bool again = false, int* redo_tile = nullptr, __nv_bfloat16* hr = nullptr) {
   const int64_t rows = hr ? p.t_pad : p.T;
   return launch_pdl(k_xent_loss, dim3(static_cast<unsigned>((rows + XE_LOSS_ROWS - 1) / XE_LOSS_ROWS)), dim3(256), 0,
-                    sm, sv.rw, static_cast<const float2*>(ws.part), 2 * p.runs, p.t_pad, keep, again, redo_tile,
+                    sm, sv.rw, static_cast<const float2*>(ws.part), parts, p.t_pad, keep, again, redo_tile,
                     reduction, loss, ws.block_sum, static_cast<const __nv_bfloat16*>(sv.hp), hr,
                     static_cast<int>(p.ldd));
 }
 
-// dW's tensor map (bf16 rows of 16-byte pieces), or any map where it has none.
-int xent_dw_tmap(CUtensorMap* m, const CUtensorMap& other, XeArgs* g, int64_t rows, int64_t d) {
-  g->dw_tma = g->dw != nullptr && g->dw_bf16 && d % 8 == 0 && aligned16(g->dw);
-  if (g->dw_tma) return make_tmap_bf16(m, g->dw, rows, d, 32, d);
+// dW's tensor map: its rows, or the padded rows dwp, as 16-byte pieces (bf16);
+// any map where it has neither.
+int xent_dw_tmap(CUtensorMap* m, const CUtensorMap& other, XeArgs* g, int64_t rows, int64_t d, __nv_bfloat16* dwp,
+                 int64_t ldd) {
+  g->dw_tma = g->dw != nullptr && g->dw_bf16 && (dwp != nullptr || aligned16(g->dw));
+  if (g->dw_tma)
+    return dwp != nullptr ? make_tmap_bf16(m, dwp, rows, ldd, 32, ldd) : make_tmap_bf16(m, g->dw, rows, d, 32, d);
   *m = other;
   return ETHOS_OK;
+}
+int xent_unpad(const __nv_bfloat16* dwp, int64_t ldd, int64_t rows, int64_t d, void* dw, cudaStream_t sm,
+               const DeviceInfo& dev) {
+  int64_t blocks = (rows * d / 8 + 256) / 256;
+  if (blocks > 16ll * dev.sm_count) blocks = 16ll * dev.sm_count;
+  return launch_pdl(k_xent_unpad, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm, dwp, ldd,
+                    static_cast<int>(d), rows * d, static_cast<__nv_bfloat16*>(dw));
+}
+
+// The forward of at most XE_FEW tokens.
+template <class S, bool kVec>
+int xent_few_t(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+               const void* labels, int labels_i64, int64_t ignore, float* loss_rows, const XentFwd& ws, int* err,
+               cudaStream_t sm) {
+  const S* h = static_cast<const S*>(hidden);
+  const S* w = static_cast<const S*>(weight);
+  const int tt = p.T <= 1 ? 1 : (p.T <= 2 ? 2 : (p.T <= 4 ? 4 : 8));
+  const int step = 32 * RowAccess<S, kVec>::N;
+  const size_t smem = static_cast<size_t>(tt) * up(p.d, step) * sizeof(float);
+  auto go = [&](auto kern) {
+    const int st = smem_attr_once(reinterpret_cast<const void*>(kern), XE_FEW_SMEM);
+    if (st != ETHOS_OK) return st;
+    return launch_pdl(kern, dim3(XE_FEW_BLOCKS), dim3(256), smem, sm, h, ldh, w, ldw, static_cast<int>(p.d),
+                      static_cast<int>(p.V), static_cast<int>(p.T), labels, labels_i64 != 0, ignore, sv.rw, loss_rows,
+                      ws.part, p.t_pad, err);
+  };
+  if (tt == 1) return go(k_xent_few<S, kVec, 1>);
+  if (tt == 2) return go(k_xent_few<S, kVec, 2>);
+  if (tt == 4) return go(k_xent_few<S, kVec, 4>);
+  return go(k_xent_few<S, kVec, 8>);
+}
+bool xent_is_few(const XentPlan& p) { return p.T <= XE_FEW && up(p.T, 8) * up(p.d, 256) * 4 <= XE_FEW_SMEM; }
+int xent_few(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+             int dtype, const void* labels, int labels_i64, int64_t ignore, float* loss_rows, const XentFwd& ws,
+             int* err, cudaStream_t sm) {
+  const int esz = dtype == ETHOS_BF16 ? 2 : 4;
+  const bool vec = p.d * esz % 16 == 0 && ldw * esz % 16 == 0 && aligned16(weight);
+  if (dtype == ETHOS_BF16)
+    return vec ? xent_few_t<__nv_bfloat16, true>(p, sv, hidden, ldh, weight, ldw, labels, labels_i64, ignore, loss_rows,
+                                                 ws, err, sm)
+               : xent_few_t<__nv_bfloat16, false>(p, sv, hidden, ldh, weight, ldw, labels, labels_i64, ignore,
+                                                  loss_rows, ws, err, sm);
+  return vec ? xent_few_t<float, true>(p, sv, hidden, ldh, weight, ldw, labels, labels_i64, ignore, loss_rows, ws, err,
+                                       sm)
+             : xent_few_t<float, false>(p, sv, hidden, ldh, weight, ldw, labels, labels_i64, ignore, loss_rows, ws,
+                                        err, sm);
 }
 
 int64_t xent_grad_units(const XentPlan& p, int64_t n, int slots, const XeArgs& g) {
@@ -643,15 +699,25 @@ int ethos_xent_forward(const void* hidden, int64_t ldh, const void* weight, int6
   DeviceInfo* dev = nullptr;
   if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
-  if ((st = xent_index(p, sv, labels, labels_i64, ignore_index, reduction == XE_NONE ? loss : nullptr, nullptr,
-                       dev_err, sm)) != ETHOS_OK)
-    return st;
   const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype);
+  float* loss_rows = reduction == XE_NONE ? loss : nullptr;
+  if (xent_is_few(p)) {
+    if ((st = xent_few(p, sv, hidden, ldh, weight, ldw, dtype, labels, labels_i64, ignore_index, loss_rows, ws,
+                       dev_err, sm)) != ETHOS_OK)
+      return st;
+    // the backward's packed rows
+    if (!h.direct &&
+        (st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, true, sm, *dev)) != ETHOS_OK)
+      return st;
+    return xent_loss(p, sv, ws, reduction, loss, sm, XE_FEW_BLOCKS);
+  }
+  if ((st = xent_index(p, sv, labels, labels_i64, ignore_index, loss_rows, nullptr, dev_err, sm)) != ETHOS_OK)
+    return st;
   if ((st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, !h.direct, sm, *dev)) != ETHOS_OK) return st;
   if (p.pack_w && (st = xent_pack_w(p, dtype, weight, ldw, ws.wp, sm, *dev)) != ETHOS_OK) return st;
   if ((st = xent_logits<XE_STATS>(p, sv, h, weight, ldw, ws, nullptr, 0, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
     return st;
-  return xent_loss(p, sv, ws, reduction, loss, sm);
+  return xent_loss(p, sv, ws, reduction, loss, sm, 2 * p.runs);
 }
 
 size_t ethos_xent_forward_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype) {
@@ -695,11 +761,11 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   if ((st = xent_logits<XE_KEEP>(p, sv, h, weight, ldw, ws.f, ws.e, ws.lde, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
     return st;
   __nv_bfloat16* hr = d_weight ? ws.hr : nullptr;
-  if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, true, false, ws.redo_tile, hr)) != ETHOS_OK) return st;
+  if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, 2 * p.runs, true, false, ws.redo_tile, hr)) != ETHOS_OK) return st;
   if ((st = xent_logits<XE_KEEP>(p, sv, h, weight, ldw, ws.f, ws.e, ws.lde, ws.redo_tile, dev_err, sm, *dev)) !=
       ETHOS_OK)
     return st;
-  if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, true, true, ws.redo_tile, hr)) != ETHOS_OK) return st;
+  if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, 2 * p.runs, true, true, ws.redo_tile, hr)) != ETHOS_OK) return st;
   if (!d_hidden && !d_weight) return ETHOS_OK;
   if (d_weight) {
     // label rows of dW: (p[y] - 1) h[t] summed by label
@@ -737,10 +803,11 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   g.do_dh = d_hidden != nullptr;
   g.do_dw = d_weight != nullptr;
   CUtensorMap wc;
-  if ((st = xent_dw_tmap(&wc, ek, &g, vocab, dim)) != ETHOS_OK) return st;
-  if ((st = launch_xent<XE_GRADS, 1>(ek, wk, em, hb, wc, g, xent_grad_units(p, vocab, p.slots, g), dev_err, sm, *dev)) !=
-      ETHOS_OK)
+  if ((st = xent_dw_tmap(&wc, ek, &g, vocab, dim, ws.dwp, p.ldd)) != ETHOS_OK) return st;
+  if ((st = launch_xent<XE_GRADS, 1>(ek, wk, em, hb, wc, g, xent_grad_units(p, vocab, p.slots, g), dev_err, sm,
+                                     *dev)) != ETHOS_OK)
     return st;
+  if (d_weight && p.pad_dw && (st = xent_unpad(ws.dwp, p.ldd, vocab, dim, d_weight, sm, *dev)) != ETHOS_OK) return st;
   if (!d_hidden) return ETHOS_OK;
   return xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots, nullptr, reduction, weight, ldw, d_hidden, sm, *dev);
 }
@@ -833,9 +900,10 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     g.do_dw = d_weight != nullptr;
     const int64_t units = xent_grad_units(p, n, p.slots_piece, g);
     CUtensorMap wc;
-    if ((st = xent_dw_tmap(&wc, dk, &g, n, dim)) != ETHOS_OK) return st;
+    if ((st = xent_dw_tmap(&wc, dk, &g, n, dim, ws.dwp, p.ldd)) != ETHOS_OK) return st;
     if ((st = launch_xent_planes<XE_GRADS>(p.planes, dk, wk, dm, hb, wc, g, units, dev_err, sm, *dev)) != ETHOS_OK)
       return st;
+    if (d_weight && p.pad_dw && (st = xent_unpad(ws.dwp, p.ldd, n, dim, g.dw, sm, *dev)) != ETHOS_OK) return st;
   }
   if (!d_hidden) return ETHOS_OK;
   return dtype == ETHOS_BF16 ? xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots_piece, grad, reduction, nullptr, 0,

@@ -249,13 +249,7 @@ __global__ void __launch_bounds__(256) k_xent_rows(const S* __restrict__ hidden,
   }
 }
 
-// ------------------------------------------------------------------- loss --
-// Joins the (maximum, sum) pieces of each row and writes its loss: 8 rows per
-// block, 32 threads along a row's pieces.  Sums over tokens have a fixed
-// order: block sums (fp64), added by the last block in block order.
-constexpr int XE_LOSS_ROWS = 8;
-enum XeReduction { XE_NONE, XE_SUM, XE_MEAN };
-
+// joins two (maximum, sum of exponentials relative to it) pairs
 __device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2) {
   const float hi = fmaxf(m, m2);
   if (hi == -INFINITY) {  // nothing seen yet, or logits of -inf (or NaN) only
@@ -265,6 +259,140 @@ __device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2)
   s = s * exp2f((m - hi) * XE_LOG2E) + s2 * exp2f((m2 - hi) * XE_LOG2E);
   m = hi;
 }
+
+// ------------------------------------------------------------- few tokens --
+// The forward for at most XE_FEW tokens: one pass over the vocabulary on the
+// fp32 units, bounded by its bytes (the tensor cores' 256-row tiles have
+// nothing to gain, and their copies stream rows of 128-byte pieces at 4.1 TB/s
+// against 5.7 TB/s of whole rows).  A warp takes 32 / TT rows of the vocabulary
+// at a time, lanes along the columns, TT >= tokens accumulators for each; the
+// 32 sums are transposed and reduced over the lanes so that lane l holds the
+// logit of row l / TT and token l % TT, and keeps a running (maximum, sum)
+// of its token.  The token's label is left out of the sum and its logit kept.
+// Block 0 also writes the row index that k_xent_index writes otherwise.
+constexpr int XE_FEW = 8;
+constexpr int XE_FEW_BLOCKS = 148;    // pieces of each row's sum
+constexpr int XE_FEW_SMEM = 128 * 1024;  // the tokens' states in fp32
+
+template <class S, bool kVec, int TT>
+__global__ void __launch_bounds__(256, 1) k_xent_few(const S* __restrict__ hidden, int64_t ldh,
+                                                     const S* __restrict__ weight, int64_t ldw, int d, int vocab,
+                                                     int tokens, const void* __restrict__ labels, bool labels_i64,
+                                                     int64_t ignore, XeRows rw, float* __restrict__ loss_rows,
+                                                     float2* __restrict__ part, int64_t part_ld, int* err) {
+  using A = RowAccess<S, kVec>;
+  constexpr int N = A::N, R = 32 / TT;
+  extern __shared__ float hs[];  // [TT][ld], zero beyond the tokens and columns
+  __shared__ float2 wp[8][TT];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int ld = (d + 32 * N - 1) / (32 * N) * (32 * N);
+  for (int i = threadIdx.x; i < TT * ld; i += 256) {
+    const int t = i / ld, c = i - t * ld;
+    hs[i] = t < tokens && c < d ? static_cast<float>(hidden[t * ldh + c]) : 0.0f;
+  }
+  // this lane's token and its label (-1: ignored, -2: no token)
+  const int t = lane % TT;
+  int64_t y = -2;
+  if (t < tokens) {
+    y = labels_i64 ? static_cast<const int64_t*>(labels)[t] : static_cast<const int32_t*>(labels)[t];
+    if (y == ignore) {
+      y = -1;
+    } else if (y < 0 || y >= vocab) {
+      if (blockIdx.x == 0) record_error(err, ETHOS_ERR_ID_OUT_OF_RANGE);
+      y = -1;
+    }
+  }
+  if (blockIdx.x == 0 && warp == 0) {
+    const unsigned valid = __ballot_sync(0xffffffffu, lane < TT && y >= 0);
+    if (lane < TT && lane < tokens) {
+      rw.idx[lane] = lane;
+      rw.yc[lane] = static_cast<int>(y);
+      rw.pos[lane] = y >= 0 ? lane : -1;
+      if (y < 0) {
+        rw.lab[lane] = 0.0f;
+        if (loss_rows != nullptr) loss_rows[lane] = 0.0f;
+      }
+    }
+    if (lane == 0) {
+      rw.meta->rows = tokens;
+      rw.meta->valid = __popc(valid);
+      rw.meta->done = 0;
+      rw.meta->redo = 0;
+    }
+  }
+  __syncthreads();
+  float m = -INFINITY, s = 0.0f;
+  // contiguous shares of the rows, the last group of each cut short
+  const int64_t me = blockIdx.x * 8 + warp, all = gridDim.x * 8;
+  const int begin = static_cast<int>(me * vocab / all), end = static_cast<int>((me + 1) * vocab / all);
+  for (int v0 = begin; v0 < end; v0 += R) {
+    float acc[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = 0.0f;
+    for (int c = lane * N; c < ld; c += 32 * N) {
+      typename A::Raw raw[R];
+      const S* w = weight + static_cast<int64_t>(v0) * ldw + c;
+      if (c < d) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (v0 + r < end) raw[r] = A::load_raw(w + r * ldw);
+      }
+      float h[TT][N];
+#pragma unroll
+      for (int k = 0; k < TT; ++k) {
+        if constexpr (N == 1) {
+          h[k][0] = hs[k * ld + c];
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; j += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(hs + k * ld + c + j);
+            h[k][j] = x.x; h[k][j + 1] = x.y; h[k][j + 2] = x.z; h[k][j + 3] = x.w;
+          }
+        }
+      }
+      if (c < d) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (v0 + r >= end) continue;
+          float x[N];
+          A::unpack(raw[r], x);
+#pragma unroll
+          for (int k = 0; k < TT; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j) acc[r * TT + k] = fmaf(x[j], h[k][j], acc[r * TT + k]);
+        }
+      }
+    }
+    const float l = warp_transpose_reduce32(acc, lane);
+    const int v = v0 + lane / TT;
+    if (v < end && t < tokens) {
+      if (v == y) rw.lab[t] = l;
+      else lse_join(m, s, l, l != l ? l : 1.0f);  // NaN stays in the sum
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= TT; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    lse_join(m, s, m2, s2);
+  }
+  if (lane < TT) wp[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x < tokens) {
+    m = wp[0][threadIdx.x].x;
+    s = wp[0][threadIdx.x].y;
+    for (int w = 1; w < 8; ++w) lse_join(m, s, wp[w][threadIdx.x].x, wp[w][threadIdx.x].y);
+    part[blockIdx.x * part_ld + threadIdx.x] = make_float2(m, s);
+  }
+}
+
+// ------------------------------------------------------------------- loss --
+// Joins the (maximum, sum) pieces of each row and writes its loss: 8 rows per
+// block, 32 threads along a row's pieces.  Sums over tokens have a fixed
+// order: block sums (fp64), added by the last block in block order.
+constexpr int XE_LOSS_ROWS = 8;
+enum XeReduction { XE_NONE, XE_SUM, XE_MEAN };
 
 // (maximum, sum) of one row over all its pieces (without the label's column):
 // valid in threads 0..7, which hold rows blockIdx.x * 8 + threadIdx.x
@@ -457,6 +585,36 @@ __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ 
         const float e[1] = {v[j]};
         if (c + j < d) RowAccess<D, false>::store(o + j, e);
       }
+    }
+  }
+}
+
+// dst [rows][d] <- src [rows][lds], bf16, eight consecutive elements of dst a
+// thread (dst rows of an odd width have no alignment of their own).
+__global__ void __launch_bounds__(256) k_xent_unpad(const __nv_bfloat16* __restrict__ src, int64_t lds, int d,
+                                                    int64_t total, __nv_bfloat16* __restrict__ dst) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15u) == 0;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x * 8) {
+    int64_t r = i / d;
+    int c = static_cast<int>(i - r * d);
+    __align__(16) __nv_bfloat16 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i + j < total) v[j] = src[r * lds + c];
+      if (++c == d) {
+        c = 0;
+        ++r;
+      }
+    }
+    if (vec && i + 8 <= total) {
+      *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j < total) dst[i + j] = v[j];
     }
   }
 }

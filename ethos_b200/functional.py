@@ -78,12 +78,21 @@ def balance_loss(weights, ids, num_experts, mask=None):
     return _BalanceLoss.apply(weights, ids, int(num_experts), mask)
 
 
+def _keeping_pays(T, V, d):
+    """Whether forming the logits a second time would take longer than the
+    five launches that keeping their exponentials takes on top (about 20 us):
+    its time is that of the products (1.2 PFLOP/s, rows in tiles of 256) or of
+    reading the table (4.5 TB/s)."""
+    rows = -(-T // 256) * 256
+    return max(2.0 * rows * V * d / 1.2e9, 2.0 * V * d / 4.5e6) > 20.0
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, reduction, need_hidden, need_weight):
         ctx.grads = None
         ctx.reduction = reduction
-        if reduction != "none" and (need_hidden or need_weight):
+        if reduction != "none" and (need_hidden or need_weight) and _keeping_pays(hidden.shape[0], *weight.shape):
             both = ops.linear_cross_entropy_forward_backward(hidden, weight, labels, ignore_index, reduction,
                                                              need_hidden, need_weight)
             if both is not None:
@@ -119,10 +128,10 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
     it).  Ignored tokens take no part in the products; gradients have the
     operands' dtype.
 
-    Where gradients are needed and the loss is one number, bf16 operands get
-    them in the forward call, which keeps the logits' exponentials (bf16, up
-    to 4 GiB of workspace) for its own length; the backward multiplies them by
-    the loss's gradient.  Otherwise the backward forms the logits again, a
+    Where gradients are needed, the loss is one number and the problem is not
+    a small one, bf16 operands get them in the forward call, which keeps the
+    logits' exponentials (bf16, up to 4 GiB of workspace) for its own length;
+    the backward multiplies them by the loss's gradient.  Otherwise the backward forms the logits again, a
     piece of the vocabulary at a time.  Neither way keeps anything of size
     ``T * V`` between the calls."""
     if labels.shape != hidden.shape[:-1]:

@@ -108,9 +108,35 @@ def test_loss_and_gradients(T, V, d, ignored, reduction, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("T,V,d,ignored", CASES)
+def test_loss_and_gradients_in_one_call(T, V, d, ignored, reduction):
+    """The keeping way at every size (functional.linear_cross_entropy takes it
+    for larger problems only), and each gradient alone."""
+    h, W, y = _inputs(T, V, d, torch.bfloat16, seed=T + V, ignored=ignored)
+    y[0] = V - 1
+    want, dh_w, dw_w, q = _exact(h, W, y, reduction)
+    args = (h.cuda(), W.cuda(), y.cuda(), -100, reduction)
+    loss, _, dh, dw = ops.linear_cross_entropy_forward_backward(*args)
+    ops.check_device_error("cuda")
+    scale = T if reduction == "sum" else 1
+    assert abs(loss.item() - want) <= scale * _loss_bound(q) + 2.0 ** -23 * abs(want)
+    assert torch.equal(ops.linear_cross_entropy_forward_backward(*args, need_weight=False)[2], dh)
+    assert torch.equal(ops.linear_cross_entropy_forward_backward(*args, need_hidden=False)[3], dw)
+    if V == 1:
+        assert not dh.any() and not dw.any()
+        return
+    assert _rel(dh, dh_w) <= _grad_bound(q, "ch", V / 16, torch.bfloat16)
+    assert _rel(dw, dw_w) <= _grad_bound(q, "cw", T / 16, torch.bfloat16)
+    assert not dh[(y == -100).cuda()].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep", [True, False])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("T", [5, 400])
-def test_every_token_ignored(T, dtype):
+@pytest.mark.parametrize("T", [5, 30, 400])
+def test_every_token_ignored(T, dtype, keep, monkeypatch):
+    monkeypatch.setattr(EF, "_keeping_pays", lambda *a: keep)
     h, W, y = _inputs(T, 90, 24, dtype, seed=2, ignored=2.0)
     for reduction in ("mean", "sum", "none"):
         hg, wg = h.cuda().requires_grad_(True), W.cuda().requires_grad_(True)
@@ -209,19 +235,19 @@ def test_hopeless_labels_with_gradients(T):
     h, W = h.bfloat16(), W.bfloat16()
     for reduction in ("sum", "mean"):
         want, dh_w, dw_w, q = _exact(h, W, y, reduction)
-        hg, wg = h.cuda().requires_grad_(True), W.cuda().requires_grad_(True)
-        loss = EF.linear_cross_entropy(hg, wg, y.cuda(), reduction=reduction)
+        loss, _, dh, dw = ops.linear_cross_entropy_forward_backward(h.cuda(), W.cuda(), y.cuda(), reduction=reduction)
         scale = T if reduction == "sum" else 1
         assert abs(loss.item() - want) <= scale * _loss_bound(q) + 2.0 ** -23 * abs(want)
-        dh, dw = torch.autograd.grad(loss, (hg, wg))
         assert _rel(dh, dh_w) <= _grad_bound(q, "ch", V / 16, torch.bfloat16)
         assert _rel(dw, dw_w) <= _grad_bound(q, "cw", T / 16, torch.bfloat16)
 
 
 @pytest.mark.gpu
-def test_gradient_of_the_loss_scales_and_second_pass():
+@pytest.mark.parametrize("keep", [True, False])
+def test_gradient_of_the_loss_scales_and_second_pass(keep, monkeypatch):
     """The loss inside a larger expression, and two passes through its graph
     (the second finds the first's gradients untouched)."""
+    monkeypatch.setattr(EF, "_keeping_pays", lambda *a: keep)
     h, W, y = _inputs(400, 900, 64, torch.bfloat16, seed=13, ignored=0.3)
     hg, wg = h.cuda().requires_grad_(True), W.cuda().requires_grad_(True)
     _, dh_w, dw_w, q = _exact(h, W, y, "mean")
@@ -252,6 +278,20 @@ def test_nan_and_infinity_stay_in_their_rows():
     assert torch.equal(torch.isnan(loss.detach()).cpu(), bad)
     dh, = torch.autograd.grad(loss.sum(), hg)
     assert torch.equal(torch.isnan(dh).any(1).cpu(), bad) and not dh[11].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [2, 9, 300])
+def test_nan_in_one_word_reaches_every_token(T, dtype):
+    for word in (0, 77, 499):
+        h, W, y = _inputs(T, 500, 64, dtype, seed=14)
+        y[:] = 5
+        W[word, 3] = float("nan")
+        assert torch.isnan(EF.linear_cross_entropy(h.cuda(), W.cuda(), y.cuda(), reduction="none")).all()
+        if dtype == torch.bfloat16:
+            loss, _, dh, _ = ops.linear_cross_entropy_forward_backward(h.cuda(), W.cuda(), y.cuda())
+            assert torch.isnan(loss) and torch.isnan(dh).any(1).all()
 
 
 @pytest.mark.gpu
@@ -373,6 +413,36 @@ def test_backward_in_a_thread_without_a_context():
     t.join()
     torch.cuda.synchronize()
     assert len(got) == 2 and all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 8])
+def test_few_tokens(T, dtype):
+    """The one-pass forward of up to eight tokens: vocabularies that leave
+    shares of one row or none, widths of whole and of partial lane steps, in
+    and out of alignment, ignored tokens, and its agreement with nine tokens
+    (which take the matrix units)."""
+    for V, d in ((1, 8), (31, 256), (3001, 264), (5000, 100), (9001, 515), (700, 1024)):
+        h, W, y = _inputs(9, V, d, dtype, seed=V + T, sharp=4.0)
+        y[1] = -100
+        want, _, _, q = _exact(h[:T], W, y[:T], "none", torch.ones(T))
+        got = EF.linear_cross_entropy(h[:T].cuda(), W.cuda(), y[:T].cuda(), reduction="none")
+        assert (got.double().cpu() - want).abs().max() <= _loss_bound(q), (V, d)
+        wide = torch.zeros(V, d + 5, dtype=dtype, device="cuda")
+        wide[:, 2:d + 2] = W.cuda()
+        again = EF.linear_cross_entropy(h[:T].cuda(), wide[:, 2:d + 2], y[:T].cuda(), reduction="none")
+        assert (again.double().cpu() - want).abs().max() <= _loss_bound(q), (V, d)
+        nine = EF.linear_cross_entropy(h.cuda(), W.cuda(), y.cuda(), reduction="none")[:T]
+        assert (nine.double().cpu() - want).abs().max() <= _loss_bound(q), (V, d)
+    h, W, y = _inputs(T, 400, 64, dtype, seed=T)
+    h[0, 0], W[7, 1] = float("inf"), 0.0
+    assert torch.isnan(EF.linear_cross_entropy(h.cuda(), W.cuda(), y.cuda(), reduction="none")[0])
+    ops.check_device_error("cuda")
+    y[0] = 400
+    EF.linear_cross_entropy(h.cuda(), W.cuda(), y.cuda())
+    with pytest.raises(_lib.EthosError):
+        ops.check_device_error("cuda")
 
 
 @pytest.mark.gpu
