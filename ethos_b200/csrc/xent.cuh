@@ -777,7 +777,8 @@ struct XeWalk {
   int cols;        // STATS, KEEP: units along the columns; DLOGITS: column tiles
   int kb_w;        // GRADS: K blocks of dW
   int kb_slot;     // GRADS: K blocks of dh per slot
-  int long_units, my_long, short0, short_step;
+  int long_units, my_long;     // GRADS: dh units of the launch, of this pair
+  int na, diff, extra;         // GRADS: see below
   __device__ XeWalk(const XeArgs& args, int rows, int pair_, int pairs_) : a(args), pair(pair_), pairs(pairs_) {
     num_m = (rows + XE_TILE - 1) / XE_TILE;
     num_n = (a.p[0].N + TN - 1) / TN;
@@ -789,35 +790,28 @@ struct XeWalk {
       units = num_m * cols;
       return;
     }
-    // dh tiles (long_units of them, kb_slot blocks each) in turn; then dW
-    // tiles (kb_w blocks each), fewer to the pairs that had one dh tile more
+    // dh units (long_units of them, kb_slot blocks each) in turn, so that the
+    // pairs below `extra` have one more than the others.  Then dW tiles (kb_w
+    // blocks each): na each, `diff` more to the others (the dW tiles that one
+    // dh unit is worth; writing a tile takes about as long as XE_STORE_KB
+    // blocks, so short contractions do not make it cheaper), and what is left
+    // one by one, the others first.
     kb_slot = (nkb + a.dh_slots - 1) / a.dh_slots;
     long_units = a.do_dh ? num_m * num_n * a.dh_slots : 0;
     kb_w = (rows + G2_BK - 1) / G2_BK;
     const int n2 = a.do_dw ? (a.p[1].M + XE_TILE - 1) / XE_TILE * num_n : 0;
-    const int extra = long_units % pairs;
+    extra = long_units % pairs;
+    const int others = pairs - extra;
     my_long = long_units / pairs + (pair < extra ? 1 : 0);
-    // dW tiles that one dh tile is worth; writing a tile takes about as long as
-    // XE_STORE_KB blocks, so shorter contractions do not make it cheaper
-    const int diff = (max(kb_slot, XE_STORE_KB) + max(kb_w, XE_STORE_KB) / 2) / max(kb_w, XE_STORE_KB);
-    int na = (n2 - diff * (pairs - extra) + pairs - 1) / pairs;
-    if (extra == 0 || na < 0) na = 0;
-    if (na * extra > n2) na = n2 / extra;
-    // pairs [0, extra) take na each, the others share the rest
-    const int rest = n2 - na * extra;
-    int mine;
-    if (pair < extra) {
-      mine = na;
-      short0 = pair;
-      short_step = extra;
-    } else {
-      const int others = pairs - extra;
-      mine = (rest - (pair - extra) + others - 1) / others;
-      short0 = na * extra + (pair - extra);
-      short_step = others;
+    diff = (max(kb_slot, XE_STORE_KB) + max(kb_w, XE_STORE_KB) / 2) / max(kb_w, XE_STORE_KB);
+    na = (n2 - diff * others) / pairs;
+    if (n2 < diff * others) {
+      na = 0;
+      diff = n2 / others;
     }
+    const int rem = n2 - na * pairs - diff * others;
     u = 0;
-    units = my_long + (mine > 0 ? mine : 0);
+    units = my_long + na + (pair >= extra ? diff : 0) + ((pair - extra + pairs) % pairs < rem ? 1 : 0);
   }
   // the next accumulation; false when the pair's units are done
   __device__ bool next(XeStep& s) {
@@ -857,7 +851,11 @@ struct XeWalk {
         kb0 = s.slot * kb_slot;
         kb1 = min(nkb, kb0 + kb_slot);
       } else {
-        const int t = short0 + (u - my_long) * short_step;
+        const int i = u - my_long, others = pairs - extra;
+        const int t = i < na ? i * pairs + pair
+                      : pair >= extra && i < na + diff
+                          ? na * pairs + (i - na) * others + pair - extra
+                          : na * pairs + diff * others + (pair - extra + pairs) % pairs;
         s.prod = 1;
         s.m0 = (t / num_n) * XE_TILE;
         s.n0 = (t % num_n) * TN;
@@ -1287,6 +1285,11 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         at_label = live ? args.rw.q[row] : 0.0f;
         g = args.reduction == XE_NONE && live ? args.grad[args.rw.idx[row]] : 1.0f;
       }
+      const float* extra = nullptr;  // GRADS: this row's label row (looked up before the wait)
+      if (MODE == XE_GRADS && st.prod == 1 && args.label_rows != nullptr && row < args.p[1].M) {
+        const int2 sp = args.label_span[row];
+        if (sp.x < sp.y) extra = args.label_rows + static_cast<int64_t>(sp.x) * args.p[1].N;
+      }
 #pragma unroll 1
       for (int half = 0; half < (st.second ? 2 : 1); ++half) {
         const int col0 = st.n0 + half * XE_TILE + ch * CHUNKS * 32;
@@ -1455,11 +1458,6 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         } else {
           const int d = args.p[1].N;
           const bool in = row < args.p[1].M;
-          const float* extra = nullptr;
-          if (args.label_rows != nullptr && in) {
-            const int2 sp = args.label_span[row];
-            if (sp.x < sp.y) extra = args.label_rows + static_cast<int64_t>(sp.x) * d;
-          }
           const int esz = args.dw_bf16 ? 2 : 4;
           const int align = byte_align(args.dw, static_cast<int64_t>(d) * esz);
 #pragma unroll
