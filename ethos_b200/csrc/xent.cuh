@@ -39,9 +39,12 @@
 // Types.  bf16: operands as they are; E (or dl) and r h are rounded to bf16,
 // the operand type of the products; sums are fp32.  fp32: operands, and dl, are
 // carried as three bf16 planes whose sum is the fp32 value, and each product is
-// six plane products, the smallest first, with a fresh accumulator every
-// XE_STEP_KB blocks of 64 (the accumulator of the matrix unit loses about half
-// an ulp of the running sum per step), added up in fp32.
+// six plane products.  The accumulator of the matrix unit loses about half an
+// ulp of the running sum per step of 16, so each K block of 64 (24 steps, the
+// smallest products first) has a fresh accumulator and the blocks are added up
+// in fp32 registers.  The six products read each plane from shared memory,
+// where it comes once: loaded for each product anew, the feed from L2 bound
+// the kernel (MEASURED_F32).
 //
 // GEMM: k_xent_gemm runs on SM pairs as k_gemm2sm does (each CTA staging 128
 // rows of A and of each 256 of B, cta_group::2 MMA, no multicast loads), with
@@ -59,7 +62,6 @@ namespace ethos {
 constexpr int XE_ROWS_DIRECT = 256;  // tokens that keep their places (one row tile)
 constexpr int XE_TILE = 256;         // rows of a pair's tile; columns of one accumulator
 constexpr int XE_GROUP_M = 64;       // row tiles walked before the next column tile
-constexpr int XE_STEP_KB = 8;        // fp32: K blocks of 64 per accumulation
 constexpr int XE_STORE_KB = 6;       // K blocks that take as long as writing a tile of dW (3 us)
 constexpr float XE_LOG2E = 1.4426950408889634f;
 constexpr float XE_KEEP_RANGE = 60.0f;  // e^60 times any sum over a vocabulary is finite in fp32 and bf16
@@ -693,14 +695,15 @@ struct XeCfg {
   // the epilogue can add up accumulations in registers
   static constexpr int kHalves = PLANES == 1 ? 2 : 1;
   static constexpr int kTileN = XE_TILE * kHalves;
-  static constexpr int kStageBytes = G2_A_BYTES + kHalves * G2_B_BYTES;
-  static constexpr int kStages = PLANES == 1 ? 4 : 6;
+  // fp32: all planes of a K block in one stage, for its six products
+  static constexpr int kStageBytes = PLANES * G2_A_BYTES + (PLANES == 1 ? kHalves : PLANES) * G2_B_BYTES;
+  static constexpr int kStages = PLANES == 1 ? 4 : 2;
   // blocks by which the second accumulator's MMAs follow the first's at the
   // end of a tile and the start of the next: while one accumulator works the
   // epilogue empties the other.  In between they go together, so that the
   // ring's stages are free for the copies.
   static constexpr int kLag = 2;
-  static constexpr int kSegs = PLANES == 1 ? 1 : 6;
+  static constexpr int kBOff = PLANES * G2_A_BYTES;  // B within a stage
 };
 struct XeCtl {
   uint64_t full[6];
@@ -861,7 +864,7 @@ struct XeWalk {
         s.n0 = (t % num_n) * TN;
         kb1 = kb_w;
       }
-      const int fl = PLANES == 1 ? (1 << 28) : XE_STEP_KB;
+      const int fl = PLANES == 1 ? (1 << 28) : 1;  // K blocks per accumulation
       steps = max(1, (kb1 - kb0 + fl - 1) / fl);
       s.kb0 = kb0 + j * fl;
       s.kb1 = min(kb1, s.kb0 + fl);
@@ -1073,42 +1076,47 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
       while (ok && walk.next(st)) {
         const int m0 = st.m0 + static_cast<int>(rank) * G2_BM;
         const int n0 = st.n0 + static_cast<int>(rank) * (XE_TILE / 2);
-        const uint32_t bytes = 2u * (G2_A_BYTES + (st.second ? 2 : 1) * G2_B_BYTES);
+        const uint32_t bytes = 2u * (PLANES * G2_A_BYTES + (PLANES == 1 ? (st.second ? 2 : 1) : PLANES) * G2_B_BYTES);
         const CUtensorMap* ta = st.prod == 0 ? &tmA0 : &tmA1;
         const CUtensorMap* tb = st.prod == 0 ? &tmB0 : &tmB1;
         const XeProduct& p = args.p[st.prod];
-        for (int seg = 0; ok && seg < Cfg::kSegs; ++seg) {
-          const int ya = PLANES == 1 ? 0 : xe_plane_a(seg) * p.a_plane_rows;
-          const int yb = PLANES == 1 ? 0 : xe_plane_b(seg) * p.b_plane_rows;
-          for (int kb = st.kb0; kb < st.kb1; ++kb) {
-            ok = __all_sync(0xffffffffu, xe_wait(&ctl->empty[rp.stage], rp.phase ^ 1u, abort, err, 1));
-            if (!ok) break;
-            uint8_t* sa = smem + rp.stage * STAGE_BYTES;
-            uint8_t* sb = sa + G2_A_BYTES;
-            const uint32_t fb = cluster_map(smem_u32(&ctl->full[rp.stage]), 0);
-            if (elect_one()) {
-              if (leader) mbar_arrive_expect_tx(&ctl->full[rp.stage], bytes);
+        for (int kb = st.kb0; kb < st.kb1; ++kb) {
+          ok = __all_sync(0xffffffffu, xe_wait(&ctl->empty[rp.stage], rp.phase ^ 1u, abort, err, 1));
+          if (!ok) break;
+          uint8_t* sa = smem + rp.stage * STAGE_BYTES;
+          uint8_t* sb = sa + Cfg::kBOff;
+          const uint32_t fb = cluster_map(smem_u32(&ctl->full[rp.stage]), 0);
+          if (elect_one()) {
+            if (leader) mbar_arrive_expect_tx(&ctl->full[rp.stage], bytes);
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl) {
+              const int ya = pl * p.a_plane_rows, yb = pl * p.b_plane_rows;
+              uint8_t* da = sa + pl * G2_A_BYTES;
+              uint8_t* db = sb + pl * G2_B_BYTES;
               if (MODE == XE_GRADS && st.prod == 1) {
-                tma_load_2d_pair(sa, ta, fb, m0, ya + kb * G2_BK);
-                tma_load_2d_pair(sa + 8192, ta, fb, m0 + 64, ya + kb * G2_BK);
+                tma_load_2d_pair(da, ta, fb, m0, ya + kb * G2_BK);
+                tma_load_2d_pair(da + 8192, ta, fb, m0 + 64, ya + kb * G2_BK);
               } else {
-                tma_load_2d_pair(sa, ta, fb, kb * G2_BK, ya + m0);
+                tma_load_2d_pair(da, ta, fb, kb * G2_BK, ya + m0);
               }
               if (MODE == XE_GRADS) {
-                tma_load_2d_pair(sb, tb, fb, n0, yb + kb * G2_BK);
-                tma_load_2d_pair(sb + 8192, tb, fb, n0 + 64, yb + kb * G2_BK);
-                if (st.second) {
-                  tma_load_2d_pair(sb + G2_B_BYTES, tb, fb, n0 + XE_TILE, yb + kb * G2_BK);
-                  tma_load_2d_pair(sb + G2_B_BYTES + 8192, tb, fb, n0 + XE_TILE + 64, yb + kb * G2_BK);
-                }
+                tma_load_2d_pair(db, tb, fb, n0, yb + kb * G2_BK);
+                tma_load_2d_pair(db + 8192, tb, fb, n0 + 64, yb + kb * G2_BK);
               } else {
-                tma_load_2d_pair(sb, tb, fb, kb * G2_BK, yb + n0);
-                if (st.second) tma_load_2d_pair(sb + G2_B_BYTES, tb, fb, kb * G2_BK, yb + n0 + XE_TILE);
+                tma_load_2d_pair(db, tb, fb, kb * G2_BK, yb + n0);
               }
             }
-            __syncwarp();
-            rp.advance(STAGES);
+            if (PLANES == 1 && st.second) {  // the second accumulator's columns
+              if (MODE == XE_GRADS) {
+                tma_load_2d_pair(sb + G2_B_BYTES, tb, fb, n0 + XE_TILE, kb * G2_BK);
+                tma_load_2d_pair(sb + G2_B_BYTES + 8192, tb, fb, n0 + XE_TILE + 64, kb * G2_BK);
+              } else {
+                tma_load_2d_pair(sb + G2_B_BYTES, tb, fb, kb * G2_BK, n0 + XE_TILE);
+              }
+            }
           }
+          __syncwarp();
+          rp.advance(STAGES);
         }
       }
       if (!ok) {
@@ -1154,13 +1162,19 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         const uint32_t idesc = umma_idesc_bf16_f32_major(2 * G2_BM, XE_TILE, a_mn, b_mn);
         const uint32_t a_base = smem0 + static_cast<uint32_t>(stage * STAGE_BYTES);
         const uint32_t a_lo = xe_desc_lo(a_base, a_mn);
-        const uint32_t b_lo = xe_desc_lo(a_base + static_cast<uint32_t>(G2_A_BYTES + half * G2_B_BYTES), b_mn);
+        const uint32_t b_lo = xe_desc_lo(a_base + static_cast<uint32_t>(Cfg::kBOff + half * G2_B_BYTES), b_mn);
         const uint32_t a_step = a_mn ? 2048u >> 4 : 32u >> 4;
         constexpr uint32_t b_step = b_mn ? 2048u >> 4 : 32u >> 4;
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < G2_BK / 16; ++k)
-            xe_mma(d, a_lo + k * a_step, b_lo + k * b_step, idesc, (!first || k > 0) ? 1u : 0u);
+          for (int seg = 0; seg < (PLANES == 1 ? 1 : 6); ++seg) {
+            const uint32_t ao = PLANES == 1 ? 0u : static_cast<uint32_t>(xe_plane_a(seg) * (G2_A_BYTES >> 4));
+            const uint32_t bo = PLANES == 1 ? 0u : static_cast<uint32_t>(xe_plane_b(seg) * (G2_B_BYTES >> 4));
+#pragma unroll
+            for (int k = 0; k < G2_BK / 16; ++k)
+              xe_mma(d, a_lo + ao + k * a_step, b_lo + bo + k * b_step, idesc,
+                     (!first || seg > 0 || k > 0) ? 1u : 0u);
+          }
         }
         __syncwarp();
       };
@@ -1175,7 +1189,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         if (go0) {
           if (b0 == n0) {  // next step with blocks
             b0 = n0 = 0;
-            while (n0 == 0 && (more0 = w0.next(s0))) n0 = Cfg::kSegs * max(0, s0.kb1 - s0.kb0);
+            while (n0 == 0 && (more0 = w0.next(s0))) n0 = max(0, s0.kb1 - s0.kb0);
           }
           if (more0) {
             const int buf = HALVES == 2 ? 0 : it0 & 1;
@@ -1206,7 +1220,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         while (HALVES == 2 && more1 && (ahead > lag || !more0 || !go0)) {
           if (b1 == n1) {
             b1 = n1 = 0;
-            while (n1 == 0 && (more1 = w1.next(s1))) n1 = Cfg::kSegs * max(0, s1.kb1 - s1.kb0);
+            while (n1 == 0 && (more1 = w1.next(s1))) n1 = max(0, s1.kb1 - s1.kb0);
           }
           if (more1) {
             if (s1.second) {
