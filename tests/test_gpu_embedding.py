@@ -122,6 +122,25 @@ def test_empty_batch_strides_and_views():
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A table of 2.3 G elements: rows at its far end are looked up and receive
+    their gradient, and nothing else does."""
+    V, d = 70000, 32776
+    W = torch.zeros(V, d, dtype=torch.bfloat16, device="cuda")
+    rows = torch.tensor([0, 65536, V - 1, 65537, V - 1], device="cuda")
+    W[rows] = torch.randn(5, d, device="cuda").bfloat16()
+    out = EF.embedding(rows, W)
+    assert torch.equal(out, W[rows])
+    dy = torch.randn(5, d, generator=torch.Generator().manual_seed(10)).bfloat16().cuda()
+    del W
+    dW = ops.embedding_backward(rows, dy, V)
+    assert torch.equal(dW[0], dy[0]) and torch.equal(dW[65536], dy[1]) and torch.equal(dW[65537], dy[3])
+    assert torch.equal(dW[V - 1], (dy[2].float() + dy[4].float()).bfloat16())
+    assert torch.count_nonzero(dW.view(torch.int16).any(1)).item() == 4
+    ops.check_device_error("cuda")
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """Central differences of a quadratic of the output, in one direction."""
     V, d, T = 9, 12, 40
