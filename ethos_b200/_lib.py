@@ -8,9 +8,9 @@ import ctypes
 import os
 import threading
 
-from .build import LIB_PATH
+from .build import BINDING_PATH, LIB_PATH
 
-__all__ = ["EthosDims", "EthosError", "EthosLibraryError", "lib", "check", "EXPORTS", "STATUS"]
+__all__ = ["EthosDims", "EthosError", "EthosLibraryError", "lib", "training", "check", "EXPORTS", "STATUS"]
 
 STATUS = {
     0: "ETHOS_OK", 1: "ETHOS_ERR_INVALID_ARG", 2: "ETHOS_ERR_UNSUPPORTED_SHAPE",
@@ -132,6 +132,7 @@ for _n in ("ethos_layer_backward", "ethos_layer_backward_f32"):
 
 _lock = threading.Lock()
 _lib = None
+_training = None
 
 
 def lib(path=None):
@@ -158,6 +159,22 @@ def lib(path=None):
         if path is None:
             _lib = handle
         return handle
+
+
+def training():
+    """Load (once) and return the autograd nodes of the training operators,
+    C++ over the same library; raises EthosLibraryError."""
+    global _training
+    if _training is None:
+        handle = lib()
+        try:
+            from . import _training as nodes
+            nodes.load(handle._name)
+        except (ImportError, RuntimeError) as e:
+            raise EthosLibraryError(f"cannot load {BINDING_PATH}: {e} (build it with "
+                                    "`python -m ethos_b200.build`)") from e
+        _training = nodes
+    return _training
 
 
 def check(status, what):

@@ -680,7 +680,7 @@ def balance_backward(grad, scratch, shape, num_experts, dtype):
     return dw
 
 
-_XENT_REDUCTION = {"none": 0, "sum": 1, "mean": 2}  # ETHOS_XENT_*
+XENT_REDUCTION = {"none": 0, "sum": 1, "mean": 2}  # ETHOS_XENT_*
 
 
 def _xent_rows(t):
@@ -710,7 +710,7 @@ def _xent_args(hidden, weight, labels, reduction):
     _on(dev, weight, "weight")
     _on(dev, labels, "labels")
     code, i64 = _dtype_code(hidden, "hidden"), _ids_i64(labels, "labels")
-    red = _XENT_REDUCTION.get(reduction)
+    red = XENT_REDUCTION.get(reduction)
     if red is None:
         raise ValueError(f"reduction: none, sum or mean, not {reduction!r}")
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
@@ -794,7 +794,7 @@ def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", 
     dw = weight.new_empty((V, d)) if need_weight else None
     if T == 0:
         return dh, dw.zero_() if dw is not None else None
-    code, red = _dtype_code(hidden, "hidden"), _XENT_REDUCTION[reduction]
+    code, red = _dtype_code(hidden, "hidden"), XENT_REDUCTION[reduction]
     hidden, weight = _xent_rows(hidden), _xent_weight(weight)
     grad = grad.to(torch.float32).contiguous()
     if grad.numel() != (T if red == 0 else 1):

@@ -10,7 +10,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from ethos_b200 import EthosConfig, EthosExpertLayer, functional as EF, ops
+from ethos_b200 import EthosConfig, EthosExpertLayer, _lib, functional as EF, ops
 from ethos_b200.init import seeded_input, seeded_state_dict, tensor_generator
 from helpers import dims_of, grad_names, load_golden, oracle_grads, rel_err
 from oracle import ethos_oracle as orc
@@ -212,3 +212,40 @@ def test_operators_in_a_cuda_graph():
         finally:
             EF._keeping_pays = old
     ops.check_device_error("cuda")
+
+
+@pytest.mark.gpu
+def test_a_gradient_cannot_be_differentiated():
+    ids = torch.tensor([1, 2, 2], device="cuda")
+    W = torch.randn(5, 8, device="cuda", requires_grad=True)
+    w3 = torch.rand(3, 1, 1, device="cuda", requires_grad=True)
+    h = torch.randn(3, 8, device="cuda", requires_grad=True)
+    for out, x in ((EF.embedding(ids, W).sum(), W), (EF.balance_loss(w3, ids.view(3, 1, 1), 5)[0], w3),
+                   (EF.linear_cross_entropy(h, W, ids), h)):
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(out, x, create_graph=True, retain_graph=True)
+        torch.autograd.grad(out, x)
+
+
+@pytest.mark.gpu
+def test_only_the_gradient_asked_for_is_formed():
+    """Both operands require a gradient, one is asked for; and a second pass
+    through the same graph gives the first one's values (up to the way)."""
+    g = torch.Generator().manual_seed(5)
+    h = torch.randn(300, 64, generator=g).cuda().requires_grad_()
+    W = torch.randn(1000, 64, generator=g).cuda().requires_grad_()
+    y = torch.randint(0, 1000, (300,), generator=g).cuda()
+    both = torch.autograd.grad(EF.linear_cross_entropy(h, W, y), (h, W))
+    loss = EF.linear_cross_entropy(h, W, y)
+    dh, = torch.autograd.grad(loss, h, retain_graph=True)
+    dw, = torch.autograd.grad(loss, W)
+    assert torch.equal(dh, both[0]) and torch.equal(dw, both[1])
+
+
+def test_binding_loads_and_reports():
+    """The C++ nodes load without a GPU, and their messages hold numbers."""
+    nodes = _lib.training()
+    with pytest.raises(RuntimeError, match="device 64"):
+        nodes.set_error_word(64, 0)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        EF.embedding(torch.zeros(3, dtype=torch.long), torch.zeros(5, 8))
