@@ -15,13 +15,14 @@
 // Counting.  Popular experts make atomics on one address queue up in L2: 2.1 M
 // selections that crowd (density ~ id^-1/2 of 262 144 experts) took 41 us.  So
 // with many selections each block counts one class of experts in shared memory
-// over its part of the selections, and adds its non-zero counts to the global
-// ones.  Classes interleave groups of 8 experts: crowded neighbours are spread
-// over the blocks (shared-memory atomics go at about one a cycle; with whole
-// ranges the block of the popular one took 65 us at 8.4 M selections), and the
-// 8 counts of a group still go out together.  The ids are read once per class
-// (L2 to SM); 16-bit counters, emptied before one can pass 65 535, make that 4
-// classes for 262 144 experts.
+// over its part of the selections, and adds its counters to the global counts,
+// or stores them for a pass that adds them up.  Classes interleave groups of 8
+// experts: crowded neighbours are spread over the blocks (with whole ranges the
+// block of the popular one took 65 us at 8.4 M selections), and the 8 counts of
+// a group still go out together.  The ids are read once per class (L2 to SM);
+// 16-bit counters make that 4 classes for 262 144 experts.  What bounds it is
+// shared-memory atomics, about one lane a cycle and SM: 30 of the count's 52 us
+// at 8.4 M selections of 262 144 experts.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -34,7 +35,10 @@ constexpr int BAL_THREADS = 256;
 constexpr int BAL_MAX_BLOCKS = 1184;   // 8 per SM of a B200
 constexpr int BAL_COUNT_THREADS = 1024;
 constexpr int BAL_CLASS = 102400;      // most experts counted by one block (200 KB of shared memory)
-constexpr int BAL_EMPTY = 65532;       // selections between two emptyings of the 16-bit counters
+// 16-bit counters: before each window of selections what a counter holds in
+// multiples of 4096 moves to the global count, so none can pass 65 535.
+constexpr unsigned BAL_MOVED = 0xf000f000u;
+constexpr int BAL_WINDOW = 65535 - 4095;
 
 // Scratch of one call: the header, then sel [tokens * H * k] fp32, the count of
 // each selection's expert (0 for a selection left out), for the backward.
@@ -158,41 +162,93 @@ __global__ void __launch_bounds__(BAL_THREADS) k_balance_count(const I* __restri
 // is r modulo 2^shift, over part b / 2^shift of the selections.  Counter l of
 // the class is expert 8 ((l / 8) 2^shift + r) + l % 8; two counters a word,
 // `words` of them.
+//
+// `part` null: the counters are added to the counts.  Else they go, as they
+// are, to part[blockIdx.x], and k_balance_join adds them up.
 template <class I>
 __global__ void __launch_bounds__(BAL_COUNT_THREADS) k_balance_count_classes(const I* __restrict__ ids,
                                                                              const uint8_t* __restrict__ mask,
                                                                              int tokens, int per_token, int experts,
                                                                              bool quads, int shift, int words,
                                                                              int* __restrict__ counts,
+                                                                             uint4* __restrict__ part,
                                                                              BalScratch* __restrict__ s) {
-  extern __shared__ unsigned mine[];
+  extern __shared__ uint4 mine4[];
+  unsigned* mine = reinterpret_cast<unsigned*>(mine4);
   pdl_launch_dependents();
   const unsigned classes = 1u << shift, r = blockIdx.x & (classes - 1);
   const int b = blockIdx.x >> shift, parts = gridDim.x >> shift;
-  for (int i = threadIdx.x; i < words; i += BAL_COUNT_THREADS) mine[i] = 0;
+  for (int i = threadIdx.x; i < words / 4; i += BAL_COUNT_THREADS) mine4[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   pdl_wait();
   const int n = tokens * per_token;
   const int per = ((n + parts - 1) / parts + 3) / 4 * 4;
   const int64_t i0 = static_cast<int64_t>(b) * per, i1 = i0 + per < n ? i0 + per : n;
-  for (int64_t a = i0; a < i1; a += BAL_EMPTY) {
-    each_selection(ids, mask, per_token, quads, a, a + BAL_EMPTY < i1 ? a + BAL_EMPTY : i1, [&](unsigned e) {
+  // adds what `bits` of word i holds to the counts
+  auto add = [&](int i, unsigned bits) {
+    int* at = counts + ((((static_cast<unsigned>(i) >> 2) << shift) + r) << 3) + 2 * (i & 3);
+    if (bits & 0xffffu) atomicAdd(at, static_cast<int>(bits & 0xffffu));
+    if (bits >> 16) atomicAdd(at + 1, static_cast<int>(bits >> 16));
+  };
+  for (int64_t a = i0; a < i1; a += BAL_WINDOW) {
+    if (a > i0) {
+      for (int i = threadIdx.x; i < words; i += BAL_COUNT_THREADS) {
+        const unsigned c = mine[i] & BAL_MOVED;
+        if (c) {
+          mine[i] -= c;
+          add(i, c);
+        }
+      }
+      __syncthreads();
+    }
+    each_selection(ids, mask, per_token, quads, a, a + BAL_WINDOW < i1 ? a + BAL_WINDOW : i1, [&](unsigned e) {
       if (((e >> 3) & (classes - 1)) == r && e < static_cast<unsigned>(experts))
         atomicAdd(mine + ((e >> (3 + shift)) << 2) + ((e & 7) >> 1), 1u << (16 * (e & 1)));
     });
     __syncthreads();
-    for (int i = threadIdx.x; i < words; i += BAL_COUNT_THREADS) {
-      const unsigned c = mine[i];
-      if (c) {
-        mine[i] = 0;
-        int* at = counts + ((((static_cast<unsigned>(i) >> 2) << shift) + r) << 3) + 2 * (i & 3);
-        if (c & 0xffffu) atomicAdd(at, static_cast<int>(c & 0xffffu));
-        if (c >> 16) atomicAdd(at + 1, static_cast<int>(c >> 16));
-      }
-    }
-    __syncthreads();
+  }
+  if (part != nullptr) {
+    uint4* out = part + static_cast<size_t>(blockIdx.x) * (words / 4);
+    for (int i = threadIdx.x; i < words / 4; i += BAL_COUNT_THREADS) out[i] = mine4[i];
+  } else {
+    for (int i = threadIdx.x; i < words; i += BAL_COUNT_THREADS)
+      if (mine[i]) add(i, mine[i]);
   }
   if (r == 0) count_live(mask, tokens, b, parts, s);
+}
+
+// Adds the blocks' counters to the counts: 32 groups of 8 experts (neighbours
+// within a class) a block, warp by warp over the parts.
+__global__ void __launch_bounds__(BAL_THREADS) k_balance_join(const uint4* __restrict__ part, int parts, int shift,
+                                                              int words, int experts, int* __restrict__ counts) {
+  __shared__ int sum[BAL_THREADS / 32][8][32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int quads = words / 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = blockIdx.x * 32 + lane;  // of quads << shift
+  const int r = g / quads, l = g - r * quads;
+  int c[8] = {};
+  if (g < quads << shift) {
+#pragma unroll 4
+    for (int p = warp; p < parts; p += BAL_THREADS / 32) {
+      const uint4 v = part[static_cast<size_t>((p << shift) + r) * quads + l];
+      const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        c[2 * j] += static_cast<int>(w[j] & 0xffffu);
+        c[2 * j + 1] += static_cast<int>(w[j] >> 16);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum[warp][j][lane] = c[j];
+  __syncthreads();
+  int t = 0;
+#pragma unroll
+  for (int v = 0; v < BAL_THREADS / 32; ++v) t += sum[v][warp][lane];
+  // expert `warp` of this lane's group
+  const int e = (((l << shift) + r) << 3) + warp;
+  if (g < quads << shift && e < experts && t) counts[e] += t;
 }
 
 // C = N / (n^2 H^2 k), 0 without tokens

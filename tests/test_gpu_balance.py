@@ -64,6 +64,30 @@ def test_loss_counts_and_gradient(T, H, k, N, masked, dtype, itype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("T,N,itype", [(65537, 262144, torch.int32), (65537, 262139, torch.int64),
+                                       (40009, 40001, torch.int32)])
+def test_many_selections_of_one_expert(T, N, itype, masked):
+    """Blocks that see one expert more often than a 16-bit counter holds, and
+    the pass that adds up the blocks' counters."""
+    g = torch.Generator().manual_seed(T)
+    ids = torch.randint(0, N, (T, 8, 16), generator=g)
+    ids[:, :5] = N - 2
+    ids, w = ids.to(itype).cuda(), torch.rand(T, 8, 16, generator=g).cuda().requires_grad_()
+    mask = (torch.rand(T, generator=g) >= 0.1).cuda() if masked else None
+    m = mask if masked else torch.ones(T, dtype=torch.bool, device="cuda")
+    n = int(m.sum())
+    want = torch.bincount(ids[m].flatten().long(), minlength=N)
+    loss, counts = EF.balance_loss(w, ids, N, mask=mask)
+    assert torch.equal(counts.long(), want)
+    sel = want.double()[ids.long()] * m[:, None, None] * (N / (n * 8) ** 2 / 16)
+    assert abs(loss.item() - float((sel * w.detach().double()).sum())) <= 2.0 ** -22 * loss.item()
+    dw, = torch.autograd.grad(loss, w)
+    assert ((dw.double() - sel).abs() <= 2.0 ** -22 * sel).all()
+    ops.check_device_error("cuda")
+
+
+@pytest.mark.gpu
 def test_even_choice_gives_one():
     N, H, k = 64, 2, 4
     ids = torch.arange(N * 8, device="cuda").remainder(N).view(-1, H, k)
