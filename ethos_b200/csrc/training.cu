@@ -353,25 +353,24 @@ int xent_pack_w(const XentPlan& p, int dtype, const void* weight, int64_t ldw, _
                           p.V, wp, p.v_pad, ldd);
 }
 
-// The label's logits and, with pack, the packed rows.
+// The packed rows and the labels' logits.
 int xent_rows_pass(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, const void* weight,
-                   int64_t ldw, int dtype, bool pack, cudaStream_t sm, const DeviceInfo& dev) {
-  int64_t blocks = ((pack ? p.t_pad : p.T) + 7) / 8;
+                   int64_t ldw, int dtype, cudaStream_t sm, const DeviceInfo& dev) {
+  int64_t blocks = (p.t_pad + 7) / 8;
   if (blocks > 8ll * dev.sm_count) blocks = 8ll * dev.sm_count;
   const dim3 grid(static_cast<unsigned>(blocks));
-  __nv_bfloat16* dst = pack ? sv.hp : nullptr;
   const int d = static_cast<int>(p.d), ldd = static_cast<int>(p.ldd);
   return dtype == ETHOS_BF16
              ? launch_pdl(k_xent_rows<__nv_bfloat16, 1>, grid, dim3(256), 0, sm,
                           static_cast<const __nv_bfloat16*>(hidden), ldh, static_cast<const __nv_bfloat16*>(weight),
-                          ldw, d, sv.rw, dst, p.t_pad, ldd)
+                          ldw, d, sv.rw, sv.hp, p.t_pad, ldd)
              : launch_pdl(k_xent_rows<float, 3>, grid, dim3(256), 0, sm, static_cast<const float*>(hidden), ldh,
-                          static_cast<const float*>(weight), ldw, d, sv.rw, dst, p.t_pad, ldd);
+                          static_cast<const float*>(weight), ldw, d, sv.rw, sv.hp, p.t_pad, ldd);
 }
 
 int xent_index(const XentPlan& p, const XentSave& sv, const void* labels, int labels_i64, int64_t ignore_index,
                float* loss_rows, int* redo_tile, int* err, cudaStream_t sm) {
-  const bool compact = p.T > XE_ROWS_DIRECT;
+  const bool compact = p.T > XE_ROWS_IN_PLACE;
   const int T = static_cast<int>(p.T);
   return labels_i64 ? launch_pdl(k_xent_index<int64_t>, dim3(1), dim3(1024), 0, sm,
                                  static_cast<const int64_t*>(labels), T, p.V, ignore_index, compact, sv.rw, loss_rows,
@@ -423,34 +422,20 @@ int launch_xent_planes(int planes, const CUtensorMap& a0, const CUtensorMap& b0,
                      : launch_xent<MODE, 3>(a0, b0, a1, b1, c, args, units, err, sm, dev);
 }
 
-// The rows of hidden that the products read: hidden itself (bf16, aligned, no
-// more than XE_ROWS_DIRECT tokens) or the packed rows in the save buffer.
-struct XentRowsOperand {
-  const void* ptr;
-  int64_t rows, cols, ld, plane_rows;
-  bool direct;
-};
-XentRowsOperand xent_rows(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, int dtype,
-                          bool packed = false) {
-  const bool direct = !packed && dtype == ETHOS_BF16 && p.T <= XE_ROWS_DIRECT && p.d % 8 == 0 && ldh % 8 == 0 && aligned16(hidden);
-  if (direct) return XentRowsOperand{hidden, p.T, p.d, ldh, 0, true};
-  return XentRowsOperand{sv.hp, p.planes * p.t_pad, p.ldd, p.ldd, p.t_pad, false};
-}
-
 // The logits' GEMM over the whole vocabulary: row statistics, and E (KEEP).
 template <int MODE>
-int xent_logits(const XentPlan& p, const XentSave& sv, const XentRowsOperand& h, const void* weight, int64_t ldw,
-                const XentFwd& ws, __nv_bfloat16* e, int64_t lde, const int* redo_tile, int* err, cudaStream_t sm,
+int xent_logits(const XentPlan& p, const XentSave& sv, const void* weight, int64_t ldw, const XentFwd& ws,
+                __nv_bfloat16* e, int64_t lde, const int* redo_tile, int* err, cudaStream_t sm,
                 const DeviceInfo& dev) {
   CUtensorMap ta, tb;
   int st;
-  if ((st = make_tmap_bf16(&ta, h.ptr, h.rows, h.cols, G2_BM, h.ld)) != ETHOS_OK) return st;
+  if ((st = make_tmap_bf16(&ta, sv.hp, p.planes * p.t_pad, p.ldd, G2_BM, p.ldd)) != ETHOS_OK) return st;
   st = p.pack_w ? make_tmap_bf16(&tb, ws.wp, p.planes * p.v_pad, p.ldd, G2_BM, p.ldd)
                 : make_tmap_bf16(&tb, weight, p.V, p.d, G2_BM, ldw);
   if (st != ETHOS_OK) return st;
   XeArgs a = {};
   a.rw = sv.rw;
-  a.p[0] = XeProduct{static_cast<int>(h.plane_rows), static_cast<int>(p.v_pad), static_cast<int>(p.T),
+  a.p[0] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(p.v_pad), static_cast<int>(p.T),
                      static_cast<int>(p.V), static_cast<int>(p.d)};
   a.run = p.run;
   a.part = ws.part;
@@ -713,23 +698,18 @@ int ethos_xent_forward(const void* hidden, int64_t ldh, const void* weight, int6
   DeviceInfo* dev = nullptr;
   if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
-  const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype);
   float* loss_rows = reduction == XE_NONE ? loss : nullptr;
   if (xent_is_few(p)) {
     if ((st = xent_few(p, sv, hidden, ldh, weight, ldw, dtype, labels, labels_i64, ignore_index, loss_rows, ws,
                        dev_err, sm)) != ETHOS_OK)
       return st;
-    // the backward's packed rows
-    if (!h.direct &&
-        (st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, true, sm, *dev)) != ETHOS_OK)
-      return st;
     return xent_loss(p, sv, ws, reduction, loss, sm, XE_FEW_BLOCKS);
   }
   if ((st = xent_index(p, sv, labels, labels_i64, ignore_index, loss_rows, nullptr, dev_err, sm)) != ETHOS_OK)
     return st;
-  if ((st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, !h.direct, sm, *dev)) != ETHOS_OK) return st;
+  if ((st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, sm, *dev)) != ETHOS_OK) return st;
   if (p.pack_w && (st = xent_pack_w(p, dtype, weight, ldw, ws.wp, sm, *dev)) != ETHOS_OK) return st;
-  if ((st = xent_logits<XE_STATS>(p, sv, h, weight, ldw, ws, nullptr, 0, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
+  if ((st = xent_logits<XE_STATS>(p, sv, weight, ldw, ws, nullptr, 0, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
     return st;
   return xent_loss(p, sv, ws, reduction, loss, sm, 2 * p.runs);
 }
@@ -768,15 +748,14 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   const int D = static_cast<int>(dim);
   if ((st = xent_index(p, sv, labels, labels_i64, ignore_index, nullptr, ws.redo_tile, dev_err, sm)) != ETHOS_OK)
     return st;
-  if ((st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, true, sm, *dev)) != ETHOS_OK) return st;
+  if ((st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, sm, *dev)) != ETHOS_OK) return st;
   if (p.pack_w && (st = xent_pack_w(p, dtype, weight, ldw, ws.f.wp, sm, *dev)) != ETHOS_OK) return st;
-  const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype, true);
   // E and the sums; rows whose shift was too low once more with their maximum
-  if ((st = xent_logits<XE_KEEP>(p, sv, h, weight, ldw, ws.f, ws.e, ws.lde, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
+  if ((st = xent_logits<XE_KEEP>(p, sv, weight, ldw, ws.f, ws.e, ws.lde, nullptr, dev_err, sm, *dev)) != ETHOS_OK)
     return st;
   __nv_bfloat16* hr = d_weight ? ws.hr : nullptr;
   if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, 2 * p.runs, true, false, ws.redo_tile, hr)) != ETHOS_OK) return st;
-  if ((st = xent_logits<XE_KEEP>(p, sv, h, weight, ldw, ws.f, ws.e, ws.lde, ws.redo_tile, dev_err, sm, *dev)) !=
+  if ((st = xent_logits<XE_KEEP>(p, sv, weight, ldw, ws.f, ws.e, ws.lde, ws.redo_tile, dev_err, sm, *dev)) !=
       ETHOS_OK)
     return st;
   if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, 2 * p.runs, true, true, ws.redo_tile, hr)) != ETHOS_OK) return st;
@@ -864,14 +843,15 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
   DeviceInfo* dev = nullptr;
   if ((st = base_device_info(&dev)) != ETHOS_OK) return st;
   cudaStream_t sm = static_cast<cudaStream_t>(stream);
-  const XentRowsOperand h = xent_rows(p, sv, hidden, ldh, dtype);
+  // the forward of few tokens has not packed them
+  if (xent_is_few(p) && (st = xent_rows_pass(p, sv, hidden, ldh, weight, ldw, dtype, sm, *dev)) != ETHOS_OK) return st;
   if (p.pack_w && (st = xent_pack_w(p, dtype, weight, ldw, ws.wp, sm, *dev)) != ETHOS_OK) return st;
   const int T = static_cast<int>(tokens), D = static_cast<int>(dim);
   const int64_t num_m = p.t_pad / XE_TILE;
   const int esz = dtype == ETHOS_BF16 ? 2 : 4;
   CUtensorMap ha, hb;  // rows of hidden, K-major (A of the logits) and MN-major (B of dW)
-  if ((st = make_tmap_bf16(&ha, h.ptr, h.rows, h.cols, G2_BM, h.ld)) != ETHOS_OK) return st;
-  if ((st = make_tmap_bf16(&hb, h.ptr, h.rows, h.cols, G2_BK, h.ld)) != ETHOS_OK) return st;
+  if ((st = make_tmap_bf16(&ha, sv.hp, p.planes * p.t_pad, p.ldd, G2_BM, p.ldd)) != ETHOS_OK) return st;
+  if ((st = make_tmap_bf16(&hb, sv.hp, p.planes * p.t_pad, p.ldd, G2_BK, p.ldd)) != ETHOS_OK) return st;
   for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
     const int64_t n = vocab - v0 < p.piece ? vocab - v0 : p.piece;
     const void* wptr = p.pack_w ? static_cast<const void*>(ws.wp + v0 * p.ldd)
@@ -885,7 +865,7 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     if ((st = make_tmap_bf16(&dm, ws.dl, p.planes * p.t_pad, p.piece, G2_BK, p.piece)) != ETHOS_OK) return st;
     XeArgs a = {};
     a.rw = sv.rw;
-    a.p[0] = XeProduct{static_cast<int>(h.plane_rows), static_cast<int>(p.v_pad), T, static_cast<int>(n), D};
+    a.p[0] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(p.v_pad), T, static_cast<int>(n), D};
     a.v0 = static_cast<int>(v0);
     a.grad = grad;
     a.reduction = reduction;
@@ -902,7 +882,7 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     g.grad = grad;
     g.reduction = reduction;
     g.p[0] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(p.v_pad), T, D, static_cast<int>(n)};
-    g.p[1] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(h.plane_rows), static_cast<int>(n), D, T};
+    g.p[1] = XeProduct{static_cast<int>(p.t_pad), static_cast<int>(p.t_pad), static_cast<int>(n), D, T};
     g.dh_slots = p.slots_piece;
     g.dh_accumulate = v0 > 0;
     g.dh_acc = ws.dh;

@@ -32,7 +32,7 @@
 //
 // Both are bounded by the tensor cores.
 //
-// Rows.  With more than XE_ROWS_DIRECT tokens the tokens that are not ignored
+// Rows.  With more than XE_ROWS_IN_PLACE tokens the tokens that are not ignored
 // are packed first (their number stays on the device), so ignored tokens cost
 // nothing after that; fewer fit one row tile and keep their places.
 //
@@ -60,7 +60,7 @@
 
 namespace ethos {
 
-constexpr int XE_ROWS_DIRECT = 256;  // tokens that keep their places (one row tile)
+constexpr int XE_ROWS_IN_PLACE = 256;  // tokens that keep their places (one row tile)
 constexpr int XE_TILE = 256;         // rows of a pair's tile; columns of one accumulator
 constexpr int XE_GROUP_M = 64;       // row tiles walked before the next column tile
 constexpr int XE_STORE_KB = 6;       // K blocks that take as long as writing a tile of dW (3 us)
@@ -208,8 +208,8 @@ __global__ void __launch_bounds__(256) k_xent_pack(const S* __restrict__ src, in
   }
 }
 
-// One warp per row of the packed problem: the label's logit in fp32, and (dst
-// not null) the row's planes; rows up to the next multiple of XE_TILE are
+// One warp per row of the packed problem: the label's logit in fp32, and the
+// row's planes; ignored rows, and rows up to the next multiple of XE_TILE, are
 // zero.
 template <class S, int PLANES>
 __global__ void __launch_bounds__(256) k_xent_rows(const S* __restrict__ hidden, int64_t ldh,
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(256) k_xent_rows(const S* __restrict__ hidden,
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int rows = rw.meta->rows;
-  const int upto = dst != nullptr ? (rows + XE_TILE - 1) / XE_TILE * XE_TILE : rows;
+  const int upto = (rows + XE_TILE - 1) / XE_TILE * XE_TILE;
   const bool hvec = rows_vec(hidden, ldh), wvec = rows_vec(weight, ldw);
   for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < upto; r += gridDim.x * 8) {
     const bool in = r < rows;
@@ -230,18 +230,16 @@ __global__ void __launch_bounds__(256) k_xent_rows(const S* __restrict__ hidden,
 #pragma unroll 2
     for (int c = lane * 8; c < ldd; c += 256) {
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (in) load8(h, c, d, hvec, v);
-      if (y >= 0) {
+      if (y >= 0) {  // rows of ignored tokens are zero whatever they hold
         float x[8];
+        load8(h, c, d, hvec, v);
         load8(w, c, d, wvec, x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) dot = fmaf(v[j], x[j], dot);
       }
-      if (dst != nullptr) {
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p)
-          *reinterpret_cast<uint4*>(dst + (p * plane_rows + r) * ldd + c) = take_plane(v);
-      }
+      for (int p = 0; p < PLANES; ++p)
+        *reinterpret_cast<uint4*>(dst + (p * plane_rows + r) * ldd + c) = take_plane(v);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);

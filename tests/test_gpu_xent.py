@@ -282,6 +282,30 @@ def test_nan_and_infinity_stay_in_their_rows():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [5, 200, 300])
+def test_what_an_ignored_token_holds_reaches_no_gradient(T, dtype):
+    """NaN, infinity or zeros in the states of ignored tokens: the same loss
+    and gradients, by every way."""
+    h, W, y = _inputs(T, 515, 72, dtype, seed=T)
+    y[1] = y[3] = -100
+    for reduction in ("none", "mean"):
+        got = []
+        for fill in (0.0, float("nan"), float("inf")):
+            h[1] = h[3] = fill
+            hg, wg = h.cuda().requires_grad_(), W.cuda().requires_grad_()
+            loss = EF.linear_cross_entropy(hg, wg, y.cuda(), reduction=reduction)
+            got.append((loss.detach(), *torch.autograd.grad(loss.sum(), (hg, wg))))
+            if reduction == "mean":
+                both = ops.linear_cross_entropy_forward_backward(h.cuda(), W.cuda(), y.cuda())
+                if both is not None:
+                    got[-1] += (both[0], both[2], both[3])
+        assert all(torch.isfinite(t.float()).all() for t in got[0])
+        for other in got[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T", [2, 9, 300])
 def test_nan_in_one_word_reaches_every_token(T, dtype):
     for word in (0, 77, 499):
