@@ -751,8 +751,8 @@ __device__ __forceinline__ bool xe_wait(uint64_t* bar, uint32_t parity, volatile
 constexpr int XE_STG_WARP_BYTES = 32 * 128;
 template <int PLANES>
 constexpr int xe_smem() {
-  return XeCfg<PLANES>::kStages * XeCfg<PLANES>::kStageBytes + (PLANES == 1 ? XE_EPI_WARPS * XE_STG_WARP_BYTES : 0) +
-         1024 + static_cast<int>(sizeof(XeCtl));
+  return XeCfg<PLANES>::kStages * XeCfg<PLANES>::kStageBytes + XE_EPI_WARPS * XE_STG_WARP_BYTES + 1024 +
+         static_cast<int>(sizeof(XeCtl));
 }
 static_assert(xe_smem<1>() <= 227 * 1024 && xe_smem<3>() <= 227 * 1024, "shared memory");
 
@@ -901,27 +901,13 @@ __device__ __forceinline__ void st_v8(void* p, uint32_t a, uint32_t b, uint32_t 
 }
 
 // 32 columns of this lane's row from `col` on, of a matrix with `cols`
-// columns (32-byte stores, whole sectors; `align`: the byte alignment that
-// every row start shares, 32, 16 or less)
-__device__ __forceinline__ void row_store_bf16(__nv_bfloat16* row, int col, int cols, int align, const float (&v)[32]) {
-  if (align >= 16 && col + 32 <= cols) {
-    uint32_t w[16];
+// columns: bf16 rows that TMA stores cannot take (dW at an odd address), and
+// fp32 ones (32-byte stores, whole sectors; `align`: the byte alignment that
+// every row start shares, 32, 16 or less; `acc`: added to what is there)
+__device__ __forceinline__ void row_store_bf16(__nv_bfloat16* row, int col, int cols, const float (&v)[32]) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-    __nv_bfloat16* p = row + col;
-    if (align >= 32) {
-      st_v8(p, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
-      st_v8(p + 16, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<uint4*>(p + 8 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col + j < cols) row[col + j] = __float2bfloat16_rn(v[j]);
-  }
+  for (int j = 0; j < 32; ++j)
+    if (col + j < cols) row[col + j] = __float2bfloat16_rn(v[j]);
 }
 __device__ __forceinline__ void row_store_f32(float* row, int col, int cols, int align, float (&v)[32], bool acc) {
   if (align >= 16 && col + 32 <= cols) {
@@ -1029,7 +1015,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   uint8_t* stg_s = smem + STAGES * STAGE_BYTES;
-  XeCtl* ctl = reinterpret_cast<XeCtl*>(stg_s + (PLANES == 1 ? XE_EPI_WARPS * XE_STG_WARP_BYTES : 0));
+  XeCtl* ctl = reinterpret_cast<XeCtl*>(stg_s + XE_EPI_WARPS * XE_STG_WARP_BYTES);
   const int warp = warp_id();
   const int lane = lane_id();
   const uint32_t rank = cluster_ctarank();
@@ -1264,7 +1250,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     XeStep st;
     const int q = warp & 3;
     const int ch = (warp - XE_EPI_WARP0) >> 2;  // column half of an accumulator
-    uint8_t* stg = stg_s + (warp - XE_EPI_WARP0) * XE_STG_WARP_BYTES;  // PLANES 1
+    uint8_t* stg = stg_s + (warp - XE_EPI_WARP0) * XE_STG_WARP_BYTES;
     const uint32_t acc_empty0 = cluster_map(smem_u32(&ctl->acc_empty[0]), 0);
     const uint32_t acc_empty1 = cluster_map(smem_u32(&ctl->acc_empty[1]), 0);
     int it0 = 0, it1 = 0;  // accumulations taken (HALVES 1: all in it0)
@@ -1446,17 +1432,17 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
               for (int i = 0; i < 32; ++i)
                 if (col + i >= N) v[k][i] = 0.0f;
             }
-            if constexpr (PLANES == 1) {
-              if (k % 2 == 1 && col0 + (k - 1) * 32 < args.ldl)
-                block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32, row - lane);
-            } else {
+            if (k % 2 == 1 && col0 + (k - 1) * 32 < args.ldl) {
 #pragma unroll
               for (int pl = 0; pl < PLANES; ++pl) {
-                row_store_bf16(args.dl + (pl * args.dl_plane_rows + row) * args.ldl, col, static_cast<int>(args.ldl),
-                               32, v[k]);
+                block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32,
+                                 pl * static_cast<int>(args.dl_plane_rows) + row - lane);
                 if (pl + 1 < PLANES) {
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) v[k][i] -= __bfloat162float(__float2bfloat16_rn(v[k][i]));
+                  for (int i = 0; i < 32; ++i) {
+                    v[k - 1][i] -= __bfloat162float(__float2bfloat16_rn(v[k - 1][i]));
+                    v[k][i] -= __bfloat162float(__float2bfloat16_rn(v[k][i]));
+                  }
                 }
               }
             }
@@ -1496,7 +1482,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
                 block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32, row - lane);
             } else if (in) {
               if (args.dw_bf16)
-                row_store_bf16(static_cast<__nv_bfloat16*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k]);
+                row_store_bf16(static_cast<__nv_bfloat16*>(args.dw) + static_cast<int64_t>(row) * d, col, d, v[k]);
               else
                 row_store_f32(static_cast<float*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k], false);
             }
@@ -1506,7 +1492,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
       if ((MODE == XE_STATS || MODE == XE_KEEP) && st.last && ok && row < rows)
         args.part[(st.slot * 2 + ch) * args.part_ld + row] = make_float2(run_m, run_s);
     }
-    if (PLANES == 1 && lane == 0) bulk_wait<0>();  // the stores have read their blocks and written
+    if (lane == 0) bulk_wait<0>();  // the stores have read their blocks and written
   }
 
   // Teardown as in k_gemm2sm: every accumulator was consumed (or the roles
