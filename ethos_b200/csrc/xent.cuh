@@ -63,6 +63,7 @@ namespace ethos {
 constexpr int XE_ROWS_IN_PLACE = 256;  // tokens that keep their places (one row tile)
 constexpr int XE_TILE = 256;         // rows of a pair's tile; columns of one accumulator
 constexpr int XE_GROUP_M = 64;       // row tiles walked before the next column tile
+constexpr int XE_NO_ROW = 1 << 29;   // beyond any operand's rows
 constexpr int XE_STORE_KB = 6;       // K blocks that take as long as writing a tile of dW (3 us)
 constexpr float XE_LOG2E = 1.4426950408889634f;
 constexpr float XE_KEEP_RANGE = 60.0f;  // e^60 times any sum over a vocabulary is finite in fp32 and bf16
@@ -1060,6 +1061,9 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
       bool ok = true;
       while (ok && walk.next(st)) {
         const int m0 = st.m0 + static_cast<int>(rank) * G2_BM;
+        // a half tile of rows past the last is filled with zeros (a coordinate
+        // out of range), which reads no memory
+        const int a_row = m0 < rows ? m0 : XE_NO_ROW;
         const int n0 = st.n0 + static_cast<int>(rank) * (XE_TILE / 2);
         const uint32_t bytes = 2u * (PLANES * G2_A_BYTES + (PLANES == 1 ? (st.second ? 2 : 1) : PLANES) * G2_B_BYTES);
         const CUtensorMap* ta = st.prod == 0 ? &tmA0 : &tmA1;
@@ -1082,7 +1086,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
                 tma_load_2d_pair(da, ta, fb, m0, ya + kb * G2_BK);
                 tma_load_2d_pair(da + 8192, ta, fb, m0 + 64, ya + kb * G2_BK);
               } else {
-                tma_load_2d_pair(da, ta, fb, kb * G2_BK, ya + m0);
+                tma_load_2d_pair(da, ta, fb, kb * G2_BK, ya + a_row);
               }
               if (MODE == XE_GRADS) {
                 tma_load_2d_pair(db, tb, fb, n0, yb + kb * G2_BK);
@@ -1266,6 +1270,9 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
     while (walk.next(st)) {
       const bool any = st.kb0 < st.kb1;
       const int row = st.m0 + static_cast<int>(rank) * G2_BM + q * 32 + lane;
+      // bf16 KEEP, DLOGITS: dW reads whole K blocks of rows, dh's rows past the
+      // last go nowhere (300 tokens of which 120 have labels: 298 -> 292 us)
+      const bool stored = PLANES != 1 || row - lane < (rows + G2_BK - 1) / G2_BK * G2_BK;
       if ((MODE == XE_STATS || MODE == XE_KEEP) && st.first) {
         live = row < rows;
         y = live ? args.rw.yc[row] : -1;
@@ -1386,7 +1393,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
               }
 #pragma unroll
               for (int i = 0; i < 32; i += 2) sum2 = fadd2(sum2, pk2(v[k][i], v[k][i + 1]));
-              if (k % 2 == 1 && col0 + (k - 1) * 32 < args.ldl)
+              if (k % 2 == 1 && stored && col0 + (k - 1) * 32 < args.ldl)
                 block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32, row - lane);
             }
             upk2(sum2, s0, s1);
@@ -1432,7 +1439,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
               for (int i = 0; i < 32; ++i)
                 if (col + i >= N) v[k][i] = 0.0f;
             }
-            if (k % 2 == 1 && col0 + (k - 1) * 32 < args.ldl) {
+            if (k % 2 == 1 && stored && col0 + (k - 1) * 32 < args.ldl) {
 #pragma unroll
               for (int pl = 0; pl < PLANES; ++pl) {
                 block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32,
