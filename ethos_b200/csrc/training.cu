@@ -266,7 +266,8 @@ XentPlan xent_plan(int64_t T, int64_t V, int64_t d, int dtype) {
     // is at most about a third of a pair's share of the whole work
     const int64_t nt = (d + p.tile_n - 1) / p.tile_n;
     const int64_t kb_h = (V + G2_BK - 1) / G2_BK, kb_w = (T + G2_BK - 1) / G2_BK;
-    const int64_t cost_w = kb_w > XE_STORE_KB ? kb_w : XE_STORE_KB;
+    const int64_t least = p.planes == 1 ? XeCfg<1>::kStoreKb : XeCfg<3>::kStoreKb;
+    const int64_t cost_w = kb_w > least ? kb_w : least;
     const int64_t share = (num_m * nt * kb_h + p.v_pad / XE_TILE * nt * cost_w) / (kPairs * 3);
     const int64_t target = share > 8 ? share : 8;
     int64_t s = (kb_h + target - 1) / target;

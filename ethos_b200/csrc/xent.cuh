@@ -64,7 +64,6 @@ constexpr int XE_ROWS_IN_PLACE = 256;  // tokens that keep their places (one row
 constexpr int XE_TILE = 256;         // rows of a pair's tile; columns of one accumulator
 constexpr int XE_GROUP_M = 64;       // row tiles walked before the next column tile
 constexpr int XE_NO_ROW = 1 << 29;   // beyond any operand's rows
-constexpr int XE_STORE_KB = 6;       // K blocks that take as long as writing a tile of dW (3 us)
 constexpr float XE_LOG2E = 1.4426950408889634f;
 constexpr float XE_KEEP_RANGE = 60.0f;  // e^60 times any sum over a vocabulary is finite in fp32 and bf16
 
@@ -706,6 +705,12 @@ struct XeCfg {
   // ring's stages are free for the copies.
   static constexpr int kLag = 2;
   static constexpr int kBOff = PLANES * G2_A_BYTES;  // B within a stage
+  // K blocks of dh that take as long as a tile of dW at the least (5 to 7 us,
+  // its loads, accumulator hand-over and stores).  Gradients of 120, 256 and 600
+  // tokens of 100 277 x 1024, in us: 282, 302, 450 with 6 (bf16), 257, 275, 429
+  // with 13, 259, 275, 422 with 16, 263, 280, 425 with 20; of 300 x 32 000 x
+  // 512: 170, 146, 137, 135.  An fp32 K block has six products.
+  static constexpr int kStoreKb = PLANES == 1 ? 16 : 6;
 };
 struct XeCtl {
   uint64_t full[6];
@@ -798,7 +803,7 @@ struct XeWalk {
     // dh units (long_units of them, kb_slot blocks each) in turn, so that the
     // pairs below `extra` have one more than the others.  Then dW tiles (kb_w
     // blocks each): na each, `diff` more to the others (the dW tiles that one
-    // dh unit is worth; writing a tile takes about as long as XE_STORE_KB
+    // dh unit is worth; writing a tile takes about as long as kStoreKb
     // blocks, so short contractions do not make it cheaper), and what is left
     // one by one, the others first.
     kb_slot = (nkb + a.dh_slots - 1) / a.dh_slots;
@@ -808,7 +813,8 @@ struct XeWalk {
     extra = long_units % pairs;
     const int others = pairs - extra;
     my_long = long_units / pairs + (pair < extra ? 1 : 0);
-    diff = (max(kb_slot, XE_STORE_KB) + max(kb_w, XE_STORE_KB) / 2) / max(kb_w, XE_STORE_KB);
+    constexpr int least = XeCfg<PLANES>::kStoreKb;
+    diff = (max(kb_slot, least) + max(kb_w, least) / 2) / max(kb_w, least);
     na = (n2 - diff * others) / pairs;
     if (n2 < diff * others) {
       na = 0;
