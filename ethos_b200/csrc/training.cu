@@ -263,12 +263,14 @@ XentPlan xent_plan(int64_t T, int64_t V, int64_t d, int dtype) {
     p.slots = 1;
   } else {
     // few row tiles and a long contraction: cut dh's K so that a tile's slice
-    // is at most about a third of a pair's share of the whole work
+    // is at most about half of a pair's share of the whole work (gradients of
+    // 120, 256 and 600 tokens of 100 277 x 1024, in us: 258, 275, 425 with a
+    // third, 250, 263, 414 with half, 268, 275, 400 with the whole of it)
     const int64_t nt = (d + p.tile_n - 1) / p.tile_n;
     const int64_t kb_h = (V + G2_BK - 1) / G2_BK, kb_w = (T + G2_BK - 1) / G2_BK;
     const int64_t least = p.planes == 1 ? XeCfg<1>::kStoreKb : XeCfg<3>::kStoreKb;
     const int64_t cost_w = kb_w > least ? kb_w : least;
-    const int64_t share = (num_m * nt * kb_h + p.v_pad / XE_TILE * nt * cost_w) / (kPairs * 3);
+    const int64_t share = (num_m * nt * kb_h + p.v_pad / XE_TILE * nt * cost_w) / (kPairs * 2);
     const int64_t target = share > 8 ? share : 8;
     int64_t s = (kb_h + target - 1) / target;
     if (s > 64) s = 64;
