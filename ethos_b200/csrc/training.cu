@@ -465,13 +465,15 @@ int xent_loss(const XentPlan& p, const XentSave& sv, const XentFwd& ws, int redu
                     static_cast<int>(p.ldd));
 }
 
-// dW's tensor map: its rows, or the padded rows dwp, as 16-byte pieces (bf16);
-// any map where it has neither.
-int xent_dw_tmap(CUtensorMap* m, const CUtensorMap& other, XeArgs* g, int64_t rows, int64_t d, __nv_bfloat16* dwp,
-                 int64_t ldd) {
-  g->dw_tma = g->dw != nullptr && g->dw_bf16 && (dwp != nullptr || aligned16(g->dw));
-  if (g->dw_tma)
-    return dwp != nullptr ? make_tmap_bf16(m, dwp, rows, ldd, 32, ldd) : make_tmap_bf16(m, g->dw, rows, d, 32, d);
+// Where the products leave dW, and its tensor map: its own rows [rows][d], or
+// the padded rows dwp, as 16-byte pieces (bf16); any map where it has neither.
+int xent_dw_out(CUtensorMap* m, const CUtensorMap& other, XeArgs* g, void* dw, int64_t rows, int64_t d,
+                __nv_bfloat16* dwp, int64_t ldd) {
+  g->do_dw = dw != nullptr;
+  g->dw = dw != nullptr && dwp != nullptr ? dwp : dw;
+  g->dw_ld = dwp != nullptr ? ldd : d;
+  g->dw_tma = g->do_dw && g->dw_bf16 && aligned16(g->dw);
+  if (g->dw_tma) return make_tmap_bf16(m, g->dw, rows, g->dw_ld, 32, g->dw_ld);
   *m = other;
   return ETHOS_OK;
 }
@@ -792,14 +794,12 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   g.dh_acc = ws.dh;
   g.dh_slot_size = p.t_pad * p.dh_ld;
   g.dh_ld = p.dh_ld;
-  g.dw = d_weight;
   g.dw_bf16 = 1;
   g.label_rows = ws.label_rows;
   g.label_span = ws.sort.span;
   g.do_dh = d_hidden != nullptr;
-  g.do_dw = d_weight != nullptr;
   CUtensorMap wc;
-  if ((st = xent_dw_tmap(&wc, ek, &g, vocab, dim, ws.dwp, p.ldd)) != ETHOS_OK) return st;
+  if ((st = xent_dw_out(&wc, ek, &g, d_weight, vocab, dim, ws.dwp, p.ldd)) != ETHOS_OK) return st;
   if ((st = launch_xent<XE_GRADS, 1>(ek, wk, em, hb, wc, g, xent_grad_units(p, vocab, p.slots, g), dev_err, sm,
                                      *dev)) != ETHOS_OK)
     return st;
@@ -891,16 +891,15 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     g.dh_acc = ws.dh;
     g.dh_slot_size = p.t_pad * p.dh_ld;
     g.dh_ld = p.dh_ld;
-    g.dw = d_weight ? static_cast<char*>(d_weight) + v0 * dim * esz : nullptr;
+    void* dw = d_weight ? static_cast<char*>(d_weight) + v0 * dim * esz : nullptr;
     g.dw_bf16 = dtype == ETHOS_BF16;
     g.do_dh = d_hidden != nullptr;
-    g.do_dw = d_weight != nullptr;
-    const int64_t units = xent_grad_units(p, n, p.slots_piece, g);
     CUtensorMap wc;
-    if ((st = xent_dw_tmap(&wc, dk, &g, n, dim, ws.dwp, p.ldd)) != ETHOS_OK) return st;
+    if ((st = xent_dw_out(&wc, dk, &g, dw, n, dim, ws.dwp, p.ldd)) != ETHOS_OK) return st;
+    const int64_t units = xent_grad_units(p, n, p.slots_piece, g);
     if ((st = launch_xent_planes<XE_GRADS>(p.planes, dk, wk, dm, hb, wc, g, units, dev_err, sm, *dev)) != ETHOS_OK)
       return st;
-    if (d_weight && p.pad_dw && (st = xent_unpad(ws.dwp, p.ldd, n, dim, g.dw, sm, *dev)) != ETHOS_OK) return st;
+    if (d_weight && p.pad_dw && (st = xent_unpad(ws.dwp, p.ldd, n, dim, dw, sm, *dev)) != ETHOS_OK) return st;
   }
   if (!d_hidden) return ETHOS_OK;
   return dtype == ETHOS_BF16 ? xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots_piece, grad, reduction, nullptr, 0,

@@ -682,7 +682,8 @@ struct XeArgs {
   float* dh_acc;       // [slots][rows][dh_ld]
   int64_t dh_slot_size;
   int64_t dh_ld;
-  void* dw;            // rows of this piece, [N rows][d] with pitch d
+  void* dw;            // rows of this piece, [N rows][d]; the padded rows where those are what is read
+  int64_t dw_ld;
   int dw_bf16;
   int dw_tma;          // dW through the tensor map tmC (16-byte rows)
   const float* label_rows;  // added to dW before scaling: row v's is label_rows[label_span[v].x],
@@ -1323,8 +1324,8 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
           if (MODE == XE_GRADS && st.prod == 1 && row < args.p[1].M) {
             const int d = args.p[1].N;
             for (int c = col0; c < min(d, col0 + CHUNKS * 32); ++c) {
-              if (args.dw_bf16) static_cast<__nv_bfloat16*>(args.dw)[static_cast<int64_t>(row) * d + c] = __float2bfloat16_rn(0.0f);
-              else static_cast<float*>(args.dw)[static_cast<int64_t>(row) * d + c] = 0.0f;
+              if (args.dw_bf16) static_cast<__nv_bfloat16*>(args.dw)[row * args.dw_ld + c] = __float2bfloat16_rn(0.0f);
+              else static_cast<float*>(args.dw)[row * args.dw_ld + c] = 0.0f;
             }
           }
           continue;
@@ -1485,7 +1486,7 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
           const int d = args.p[1].N;
           const bool in = row < args.p[1].M;
           const int esz = args.dw_bf16 ? 2 : 4;
-          const int align = byte_align(args.dw, static_cast<int64_t>(d) * esz);
+          const int align = byte_align(args.dw, args.dw_ld * esz);
 #pragma unroll
           for (int k = 0; k < CHUNKS; ++k) {
             const int col = col0 + k * 32;
@@ -1509,9 +1510,9 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
                 block_store_bf16(&tmC, stg, lane, v[k - 1], v[k], col0 + (k - 1) * 32, row - lane);
             } else if (in) {
               if (args.dw_bf16)
-                row_store_bf16(static_cast<__nv_bfloat16*>(args.dw) + static_cast<int64_t>(row) * d, col, d, v[k]);
+                row_store_bf16(static_cast<__nv_bfloat16*>(args.dw) + row * args.dw_ld, col, d, v[k]);
               else
-                row_store_f32(static_cast<float*>(args.dw) + static_cast<int64_t>(row) * d, col, d, align, v[k], false);
+                row_store_f32(static_cast<float*>(args.dw) + row * args.dw_ld, col, d, align, v[k], false);
             }
           }
         }

@@ -1,0 +1,56 @@
+"""Cross entropy of the output head where its buffers and its arithmetic can
+go wrong: workspaces that hold something else before the call, batches of which
+nothing is left, workspaces at every alignment the entry points accept."""
+
+import ctypes
+
+import pytest
+import torch
+
+from ethos_b200 import _lib, functional as EF, ops
+from test_gpu_xent import _exact, _grad_bound, _inputs, _loss_bound, _rel
+
+
+@pytest.fixture
+def dirty(monkeypatch):
+    """Workspaces and save buffers of ops.* calls arrive holding NaN (0xFF in
+    every byte, in bf16 and in fp32)."""
+    monkeypatch.setattr(ops, "_bytes", lambda n, dev: torch.full((n,), 255, dtype=torch.uint8, device=dev))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,d", [(30, 33), (400, 24), (400, 33), (300, 515), (700, 1031)])
+def test_no_token_left_gives_zero_gradients(T, d, dtype, dirty):
+    """Every label ignored, widths whose dW goes through padded rows among
+    them: zeros, whatever the workspace held."""
+    h, W, y = (t.cuda() for t in _inputs(T, 600, d, dtype, seed=2, ignored=2.0))
+    for reduction in ("none", "sum", "mean"):
+        loss, save = ops.linear_cross_entropy_forward(h, W, y, reduction=reduction)
+        grad = torch.ones_like(loss)
+        dh, dw = ops.linear_cross_entropy_backward(grad, h, W, save, reduction=reduction)
+        assert not dh.any() and not dw.any()
+        both = ops.linear_cross_entropy_forward_backward(h, W, y, reduction=reduction)
+        assert (both is None) == (dtype == torch.float32 or reduction == "none")
+        if both is not None:
+            assert not both[2].any() and not both[3].any()
+    ops.check_device_error("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,d,ignored", [(5, 70, 33, 0.2), (256, 511, 72, 0.5), (300, 777, 515, 0.97),
+                                           (700, 2049, 136, 0.6)])
+def test_what_the_workspace_held_does_not_matter(T, V, d, ignored, dirty):
+    """bf16, both ways: the same bits as with the allocator's memory."""
+    h, W, y = (t.cuda() for t in _inputs(T, V, d, torch.bfloat16, seed=T, ignored=ignored))
+    y[0] = V - 1
+    loss, save = ops.linear_cross_entropy_forward(h, W, y)
+    got = (loss, *ops.linear_cross_entropy_backward(torch.ones_like(loss), h, W, save))
+    both = ops.linear_cross_entropy_forward_backward(h, W, y)
+    for a in (got, (both[0], both[2], both[3])):
+        assert all(torch.isfinite(t.float()).all() for t in a)
+    want, dh_w, dw_w, q = _exact(h.cpu(), W.cpu(), y.cpu(), "mean")
+    for loss, dh, dw in (got, (both[0], both[2], both[3])):
+        assert abs(loss.item() - want) <= _loss_bound(q) + 2.0 ** -23 * abs(want)
+        assert _rel(dh, dh_w) <= _grad_bound(q, "ch", V / 16, torch.bfloat16)
+        assert _rel(dw, dw_w) <= _grad_bound(q, "cw", T / 16, torch.bfloat16)
