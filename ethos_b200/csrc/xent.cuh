@@ -1478,9 +1478,10 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         } else if (st.prod == 0) {
           if (row < rows) {
             float* o = args.dh_acc + st.slot * args.dh_slot_size + row * args.dh_ld;
+            const int align = byte_align(args.dh_acc, args.dh_ld * 4);  // a slot is whole rows
 #pragma unroll
             for (int k = 0; k < CHUNKS; ++k)
-              row_store_f32(o, col0 + k * 32, static_cast<int>(args.dh_ld), 32, v[k], args.dh_accumulate != 0);
+              row_store_f32(o, col0 + k * 32, static_cast<int>(args.dh_ld), align, v[k], args.dh_accumulate != 0);
           }
         } else {
           const int d = args.p[1].N;

@@ -54,3 +54,37 @@ def test_what_the_workspace_held_does_not_matter(T, V, d, ignored, dirty):
         assert abs(loss.item() - want) <= _loss_bound(q) + 2.0 ** -23 * abs(want)
         assert _rel(dh, dh_w) <= _grad_bound(q, "ch", V / 16, torch.bfloat16)
         assert _rel(dw, dw_w) <= _grad_bound(q, "cw", T / 16, torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,d", [(5, 300, 64), (300, 2049, 136), (40, 777, 33)])
+def test_workspaces_at_every_accepted_alignment(T, V, d, dtype, monkeypatch):
+    """The entry points take any 16-byte aligned workspace and save buffer (a
+    part of a caller's arena): the same bits at 16, 32 and 48 bytes past an
+    allocation's start."""
+    h, W, y = (t.cuda() for t in _inputs(T, V, d, dtype, seed=T, ignored=0.2))
+    y[0] = V - 1
+    want = None
+    for off in (0, 16, 32, 48):
+        def shifted(n, dev, off=off):
+            t = torch.empty(n + 64, dtype=torch.uint8, device=dev)[off:off + n]
+            assert t.data_ptr() % 64 == off
+            return t
+        monkeypatch.setattr(ops, "_bytes", shifted)
+        loss, save = ops.linear_cross_entropy_forward(h, W, y)
+        got = (loss, *ops.linear_cross_entropy_backward(torch.ones_like(loss), h, W, save))
+        both = ops.linear_cross_entropy_forward_backward(h, W, y)
+        if both is not None:
+            got += (both[0], both[2], both[3])
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    monkeypatch.undo()
+    # 8-byte alignment is refused
+    L, p = _lib.lib(), ctypes.c_void_p
+    save, ws = (ops._bytes(n + 64, h.device) for n in (L.ethos_xent_save_size(T, V, d, 1),
+                                                        L.ethos_xent_backward_workspace_size(T, V, d, 1)))
+    args = (h.data_ptr(), d, W.data_ptr(), d, 1, 2, T, V, d, loss.data_ptr())
+    for a, b in ((0, 8), (8, 0)):
+        assert L.ethos_xent_backward(*args, p(save.data_ptr() + a), save.numel() - a, h.data_ptr(), W.data_ptr(),
+                                     p(ws.data_ptr() + b), ws.numel() - b, loss.data_ptr(), None) == 3
