@@ -575,9 +575,16 @@ def _ids_i64(t, name):
 
 
 def _on(dev, t, name):
-    if t.device != dev:
+    if getattr(t, "device", None) != dev:
         _require_cuda(t, name)
         raise ValueError(f"{name} is on {t.device}, not on {dev}")
+
+
+def _scalar(t, name):
+    """One value, in fp32."""
+    if t.numel() != 1:
+        raise ValueError(f"{name}: one value, not {t.numel()}")
+    return t.to(torch.float32)
 
 
 @functools.lru_cache(maxsize=256)
@@ -668,14 +675,15 @@ def balance_forward(weights, ids, num_experts, mask=None):
 
 def balance_backward(grad, scratch, shape, num_experts, dtype):
     """``grad * dloss/dweights`` of ``balance_forward``, ``shape`` = (T, H, k),
-    in ``dtype``; ``grad`` is a fp32 device scalar, ``scratch`` the forward's."""
+    in ``dtype``; ``grad`` is a device scalar, ``scratch`` the forward's."""
     _require_cuda(grad, "grad")
     T, H, k = shape
-    dev = scratch.device
+    dev = grad.device
+    _on(dev, scratch, "scratch")
     dw = torch.empty((T, H, k), dtype=dtype, device=dev)
-    grad = grad.to(torch.float32)
+    grad = _scalar(grad, "grad")
     check(lib().ethos_balance_backward(_dtype_code(dw, "weights"), T, H, k, num_experts, scratch.data_ptr(),
-                                       scratch.numel(), grad.data_ptr(), dw.data_ptr(), _raw_stream(dev.index)),
+                                       scratch.nbytes, grad.data_ptr(), dw.data_ptr(), _raw_stream(dev.index)),
           "ethos_balance_backward")
     return dw
 
@@ -702,6 +710,19 @@ def _xent_weight(w):
     return w
 
 
+def _xent_operands(hidden, weight, reduction):
+    """Checks of every call: the operands belong together.  Returns the
+    reduction's code."""
+    red = XENT_REDUCTION.get(reduction)
+    if red is None:
+        raise ValueError(f"reduction: none, sum or mean, not {reduction!r}")
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"hidden [T, d] and weight [V, d]: got {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if weight.dtype != hidden.dtype:
+        raise ValueError(f"hidden is {hidden.dtype}, weight {weight.dtype}")
+    return red
+
+
 def _xent_args(hidden, weight, labels, reduction):
     """Checks shared by the forward calls; the operands as the library reads
     them."""
@@ -710,13 +731,7 @@ def _xent_args(hidden, weight, labels, reduction):
     _on(dev, weight, "weight")
     _on(dev, labels, "labels")
     code, i64 = _dtype_code(hidden, "hidden"), _ids_i64(labels, "labels")
-    red = XENT_REDUCTION.get(reduction)
-    if red is None:
-        raise ValueError(f"reduction: none, sum or mean, not {reduction!r}")
-    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
-        raise ValueError(f"hidden [T, d] and weight [V, d]: got {tuple(hidden.shape)} and {tuple(weight.shape)}")
-    if weight.dtype != hidden.dtype:
-        raise ValueError(f"hidden is {hidden.dtype}, weight {weight.dtype}")
+    red = _xent_operands(hidden, weight, reduction)
     if tuple(labels.shape) != (hidden.shape[0],):
         raise ValueError(f"labels: [{hidden.shape[0]}], got {tuple(labels.shape)}")
     return _xent_rows(hidden), _xent_weight(weight), labels.contiguous(), code, i64, red
@@ -768,17 +783,21 @@ def linear_cross_entropy_forward_backward(hidden, weight, labels, ignore_index=-
 
 def scale_(factor, x=None, y=None):
     """``x *= factor`` and ``y *= factor`` in place (contiguous, of one dtype;
-    None: none; ``factor`` a fp32 device scalar); nothing is read or written
+    None: none; ``factor`` a device scalar); nothing is read or written
     when it is 1 (ethos_xent_scale)."""
     _require_cuda(factor, "factor")
+    dev = factor.device
     some = [t for t in (x, y) if t is not None]
     if not some:
         return
+    for t in some:
+        _on(dev, t, "x and y")
     if any(not t.is_contiguous() or t.dtype != some[0].dtype for t in some):
         raise ValueError("x and y: contiguous, of one dtype")
+    code, factor = _dtype_code(some[0], "x"), _scalar(factor, "factor")
     check(lib().ethos_xent_scale(factor.data_ptr(), 0 if x is None else x.data_ptr(), 0 if x is None else x.numel(),
                                  0 if y is None else y.data_ptr(), 0 if y is None else y.numel(),
-                                 _dtype_code(some[0], "x"), _raw_stream(factor.device.index)), "ethos_xent_scale")
+                                 code, _raw_stream(dev.index)), "ethos_xent_scale")
 
 
 def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", need_hidden=True, need_weight=True):
@@ -789,19 +808,21 @@ def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", 
     dev = hidden.device
     _on(dev, weight, "weight")
     _on(dev, grad, "grad")
+    red = _xent_operands(hidden, weight, reduction)
     (T, d), V = hidden.shape, weight.shape[0]
+    if grad.numel() != (T if red == 0 else 1):
+        raise ValueError(f"grad of {grad.numel()} values for reduction {reduction!r}")
     dh = hidden.new_empty((T, d)) if need_hidden else None
     dw = weight.new_empty((V, d)) if need_weight else None
     if T == 0:
         return dh, dw.zero_() if dw is not None else None
-    code, red = _dtype_code(hidden, "hidden"), XENT_REDUCTION[reduction]
+    _on(dev, save, "save")
+    code = _dtype_code(hidden, "hidden")
     hidden, weight = _xent_rows(hidden), _xent_weight(weight)
     grad = grad.to(torch.float32).contiguous()
-    if grad.numel() != (T if red == 0 else 1):
-        raise ValueError(f"grad of {grad.numel()} values for reduction {reduction!r}")
     ws = _bytes(_size("ethos_xent_backward_workspace_size", T, V, d, code), dev)
     check(lib().ethos_xent_backward(hidden.data_ptr(), _pitch(hidden), weight.data_ptr(), _pitch(weight), code, red,
-                                    T, V, d, grad.data_ptr(), save.data_ptr(), save.numel(),
+                                    T, V, d, grad.data_ptr(), save.data_ptr(), save.nbytes,
                                     dh.data_ptr() if need_hidden else 0, dw.data_ptr() if need_weight else 0,
                                     ws.data_ptr(), ws.numel(), device_error_word(dev).data_ptr(),
                                     _raw_stream(dev.index)), "ethos_xent_backward")

@@ -1,0 +1,77 @@
+"""The training operators' calls without autograd (ethos_b200.ops) refuse what
+the library could only read out of bounds: host tensors, operands that do not
+belong together, gradients of another size."""
+
+import pytest
+import torch
+
+from ethos_b200 import _lib, ops
+
+
+@pytest.fixture
+def xent():
+    g = torch.Generator().manual_seed(1)
+    h, W = (torch.randn(n, 24, generator=g).bfloat16().cuda() for n in (10, 40))
+    y = torch.randint(0, 40, (10,), generator=g).cuda()
+    loss, save = ops.linear_cross_entropy_forward(h, W, y)
+    return h, W, torch.ones_like(loss), save
+
+
+@pytest.mark.gpu
+def test_cross_entropy_backward_refuses_operands_that_do_not_belong_together(xent):
+    h, W, one, save = xent
+    back = ops.linear_cross_entropy_backward
+    for wrong in (W.float(), W[:, :16], W[0]):
+        with pytest.raises(ValueError, match="weight"):
+            back(one, h, wrong, save)
+    with pytest.raises(ValueError, match="weight"):
+        back(one, h.float(), W, save)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        back(one, h, W, save.cpu())
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        back(one, h, W, None)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        back(one.cpu(), h, W, save)
+    with pytest.raises(ValueError, match="reduction"):
+        back(one, h, W, save, reduction="max")
+    for wrong, red in ((torch.ones(9, device="cuda"), "none"), (torch.ones(2, device="cuda"), "sum"),
+                       (torch.ones(0, device="cuda"), "mean")):
+        with pytest.raises(ValueError, match="grad of"):
+            back(wrong, h, W, save, reduction=red)
+    dh, dw = back(one, h, W, save)
+    assert dh.shape == h.shape and dw.shape == W.shape
+
+
+@pytest.mark.gpu
+def test_scale_refuses_and_takes_any_float_factor():
+    x = torch.arange(8, device="cuda", dtype=torch.float32)
+    two = torch.full((), 2.0, device="cuda")
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.scale_(two, x.cpu())
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.scale_(two, x, x.cpu())
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.scale_(two.cpu(), x)
+    with pytest.raises(ValueError, match="one value"):
+        ops.scale_(torch.ones(0, device="cuda"), x)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.scale_(two, x[::2])
+    with pytest.raises(ValueError, match="fp32 or bf16"):
+        ops.scale_(two, x.half())
+    ops.scale_(two.bfloat16(), x)    # read as what it is, not as fp32
+    assert torch.equal(x, 2.0 * torch.arange(8, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_balance_backward_refuses():
+    w = torch.rand(6, 2, 4, device="cuda")
+    ids = torch.zeros(6, 2, 4, dtype=torch.int32, device="cuda")
+    loss, _, scratch = ops.balance_forward(w, ids, 5)
+    one = torch.ones((), device="cuda")
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.balance_backward(one, scratch.cpu(), (6, 2, 4), 5, torch.float32)
+    with pytest.raises(ValueError, match="one value"):
+        ops.balance_backward(one[None][:0], scratch, (6, 2, 4), 5, torch.float32)
+    with pytest.raises(_lib.EthosError, match="WORKSPACE"):
+        ops.balance_backward(one, scratch, (6000, 2, 4), 5, torch.float32)
+    assert ops.balance_backward(one, scratch, (6, 2, 4), 5, torch.float32).shape == (6, 2, 4)
