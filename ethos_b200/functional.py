@@ -37,14 +37,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     every run) and rounded once; rows no token holds are zero.  The row of
     ``padding_idx`` (None: no such row) gets no gradient; a negative index
     counts from the end, as in ``torch.nn.Embedding``."""
-    if padding_idx is not None:
-        V = weight.shape[0]
-        if not -V <= padding_idx < V:
-            raise ValueError(f"padding_idx {padding_idx} is not in the table of {V} rows")
-        padding_idx = padding_idx % V
-    else:
-        padding_idx = -1
-    return _nodes(weight).embedding(ids, weight, scale, padding_idx)
+    row = -1 if padding_idx is None else ops.padding_row(padding_idx, weight.shape[0])
+    return _nodes(weight).embedding(ids, weight, scale, row)
 
 
 def balance_loss(weights, ids, num_experts, mask=None):

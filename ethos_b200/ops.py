@@ -620,12 +620,22 @@ def embedding_forward(ids, weight, scale=1.0):
     return out
 
 
+def padding_row(padding_idx, vocab):
+    """The table's row that gets no gradient, -1 for None."""
+    if padding_idx is None:
+        return -1
+    if not -vocab <= padding_idx < vocab:
+        raise ValueError(f"padding_idx {padding_idx} is not in the table of {vocab} rows")
+    return padding_idx % vocab
+
+
 def embedding_backward(ids, dy, vocab, scale=1.0, padding_idx=None):
     """Gradient of ``embedding_forward`` with respect to the table
     (ethos_embedding_backward): dense ``[vocab, d]`` in ``dy``'s dtype, summed
     in fp32 in token order, the same in every run.  Tokens equal to
-    ``padding_idx`` contribute nothing."""
+    ``padding_idx`` (negative: from the end) contribute nothing."""
     _require_cuda(dy, "dy")
+    padding = padding_row(padding_idx, vocab)
     dev = dy.device
     _on(dev, ids, "ids")
     code, i64 = _dtype_code(dy, "dy"), _ids_i64(ids, "ids")
@@ -637,9 +647,9 @@ def embedding_backward(ids, dy, vocab, scale=1.0, padding_idx=None):
     dw = dy.new_empty((vocab, d))
     ws = _bytes(_size("ethos_embedding_backward_workspace_size", T, vocab, d), dev)
     check(lib().ethos_embedding_backward(ids.data_ptr(), i64, dy.data_ptr(), code, T, vocab, d,
-                                         -1 if padding_idx is None else padding_idx, scale, dw.data_ptr(),
-                                         ws.data_ptr(), ws.numel(), device_error_word(dev).data_ptr(),
-                                         _raw_stream(dev.index)), "ethos_embedding_backward")
+                                         padding, scale, dw.data_ptr(), ws.data_ptr(), ws.numel(),
+                                         device_error_word(dev).data_ptr(), _raw_stream(dev.index)),
+          "ethos_embedding_backward")
     return dw
 
 

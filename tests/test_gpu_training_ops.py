@@ -5,7 +5,7 @@ belong together, gradients of another size."""
 import pytest
 import torch
 
-from ethos_b200 import _lib, ops
+from ethos_b200 import _lib, functional as EF, ops
 
 
 @pytest.fixture
@@ -75,3 +75,25 @@ def test_balance_backward_refuses():
     with pytest.raises(_lib.EthosError, match="WORKSPACE"):
         ops.balance_backward(one, scratch, (6000, 2, 4), 5, torch.float32)
     assert ops.balance_backward(one, scratch, (6, 2, 4), 5, torch.float32).shape == (6, 2, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("padding", [None, 0, 6, -1, -7])
+def test_embedding_backward_takes_padding_rows_as_the_module_does(padding):
+    """A negative index counts from the end, in the call without autograd as
+    in functional.embedding."""
+    g = torch.Generator().manual_seed(2)
+    ids = torch.randint(0, 7, (50,), generator=g).cuda()
+    W, dy = (torch.randn(n, 8, generator=g).cuda() for n in (7, 50))
+    W.requires_grad_(True)
+    want, = torch.autograd.grad(EF.embedding(ids, W, padding_idx=padding), W, dy)
+    assert torch.equal(ops.embedding_backward(ids, dy, 7, padding_idx=padding), want)
+    assert padding is None or not want[padding].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("padding", [7, -8, 1 << 40])
+def test_embedding_backward_refuses_padding_rows_outside_the_table(padding):
+    ids, dy = torch.zeros(3, dtype=torch.int64, device="cuda"), torch.ones(3, 8, device="cuda")
+    with pytest.raises(ValueError, match="padding_idx"):
+        ops.embedding_backward(ids, dy, 7, padding_idx=padding)
