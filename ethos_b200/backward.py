@@ -54,6 +54,8 @@ def layer_backward(ctx, gy, gw=None):
     them (None: none)."""
     layer = ctx.layer
     sv = ctx.saved
+    if ctx.saved_tensors:  # handed out as well (autograd checks that they are unchanged)
+        sv["weights"], sv["ids"] = ctx.saved_tensors
     pw = sv["pw"]
     if gy is None:  # only the routing weights were used
         gy = torch.zeros_like(sv["xin"])

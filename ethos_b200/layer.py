@@ -206,6 +206,8 @@ class _EthosLayerFunction(torch.autograd.Function):
         w, ids = out["weights"].detach(), out["ids"].detach()
         ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)
+        if need_grad:  # the backward reads them: a change in place raises there
+            ctx.save_for_backward(w, ids)
         return out["y"].to(x2d.dtype), w, ids
 
     @staticmethod
@@ -316,7 +318,8 @@ class EthosExpertLayer(nn.Module):
         """``y [B, S, d_model]``; with ``return_routing`` also the routing
         weights (fp32 ``[B * S, H, k]``, differentiable: a loss on them, such
         as ``functional.balance_loss``, reaches the router) and the expert ids
-        (int32, the same shape)."""
+        (int32, the same shape).  The backward reads both: one that was
+        changed in place makes it raise."""
         ops._require_cuda(x, "x")
         batch_size, seq_len, d_model = x.shape
         x2d = x.reshape(-1, d_model)
