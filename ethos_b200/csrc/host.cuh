@@ -11,6 +11,7 @@
 #include <utility>
 
 #include "ethos_b200.h"
+#include "kernel_table.h"
 
 namespace ethos {
 
@@ -55,18 +56,13 @@ inline int base_device_info(DeviceInfo** out) {
 
 // Sets the dynamic shared-memory limit of a kernel once per device.
 inline int smem_attr_once(const void* fn, int bytes) {
-  int dev = 0;
+  int dev = 0, set = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ETHOS_ERR_NO_DEVICE;
-  static std::mutex mu;
-  static const void* seen[64][32];
-  static int nseen[64];
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < nseen[dev]; ++i)
-    if (seen[dev][i] == fn) return ETHOS_OK;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return ETHOS_ERR_CUDA;
-  if (nseen[dev] < 32) seen[dev][nseen[dev]++] = fn;
-  return ETHOS_OK;
+  static KernelTable<int> table;
+  return table.get(dev, fn, &set, [&](int* v) {
+    *v = bytes;
+    return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+  }) ? ETHOS_OK : ETHOS_ERR_CUDA;
 }
 
 // ------------------------------------------------------------- tensor maps --
@@ -142,36 +138,27 @@ int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
 // Clusters of two that can run at once for a 2-SM GEMM kernel (queried once
 // per kernel and device: the SM-pair topology decides it, not the tile count).
 inline int max_pair_clusters(const void* fn, int threads, int smem, const DeviceInfo& dev) {
-  int d = 0;
-  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= 64) return 0;
-  static std::mutex mu;
-  static const void* seen[64][8];
-  static int val[64][8];
-  static int nseen[64];
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < nseen[d]; ++i)
-    if (seen[d][i] == fn) return val[d][i];
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(dev.sm_count & ~1));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) {
+  int d = 0, pairs = 0;
+  if (cudaGetDevice(&d) != cudaSuccess) return 0;
+  static KernelTable<int> table;
+  table.get(d, fn, &pairs, [&](int* n) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(dev.sm_count & ~1));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(n, fn, &cfg) == cudaSuccess) return true;
     cudaGetLastError();
-    n = 0;
-  }
-  if (nseen[d] < 8) {
-    seen[d][nseen[d]] = fn;
-    val[d][nseen[d]++] = n;
-  }
-  return n;
+    *n = 0;
+    return false;
+  });
+  return pairs;
 }
 
 // ------------------------------------------------------- workspace layout --
