@@ -313,12 +313,21 @@ struct XentBwd {
   __nv_bfloat16* dl;
   float* dh;
   __nv_bfloat16* dwp;  // rows of dW at a pitch of whole 16-byte pieces
+  // bf16: the label's terms, as in the keep way
+  float* label_grad;
+  EmbedScratch sort;
+  float* label_rows;
 };
 void carve_xent_bwd(Carve& c, const XentPlan& p, XentBwd* s) {
   s->wp = p.pack_w ? c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.v_pad * p.ldd)) : nullptr;
   s->dl = c.take<__nv_bfloat16>(static_cast<size_t>(p.planes * p.t_pad * p.piece));
   s->dh = c.take<float>(static_cast<size_t>(p.slots_piece * p.t_pad * p.dh_ld));
   s->dwp = p.pad_dw ? c.take<__nv_bfloat16>(static_cast<size_t>(p.piece * p.ldd)) : nullptr;
+  s->label_grad = s->label_rows = nullptr;
+  if (p.planes != 1) return;
+  s->label_grad = c.take<float>(static_cast<size_t>(p.t_pad));
+  carve_embed(c, p.t_pad, p.V, p.d, &s->sort);
+  s->label_rows = c.take<float>(static_cast<size_t>(p.t_pad * p.d));
 }
 struct XentKeep {
   XentFwd f;
@@ -529,14 +538,27 @@ int64_t xent_grad_units(const XentPlan& p, int64_t n, int slots, const XeArgs& g
   return (g.do_dh ? p.t_pad / XE_TILE * nt * slots : 0) + (g.do_dw ? (n + XE_TILE - 1) / XE_TILE * nt : 0);
 }
 
+// Label rows of dW (bf16): e[t] h[t] summed by label.
+int xent_label_rows(const XentPlan& p, const XentSave& sv, const EmbedScratch& sort, const float* e, float* label_rows,
+                    int* err, cudaStream_t sm, const DeviceInfo& dev) {
+  const int st = embed_sort<int32_t>(sort, sv.rw.yc, p.t_pad, &sv.rw.meta->rows, p.V, -1, err, sm, dev);
+  if (st != ETHOS_OK) return st;
+  const int d = static_cast<int>(p.d);
+  return d % 8 == 0 ? embed_rows<__nv_bfloat16, true, float, true>(sort, sv.hp, p.ldd, e, p.t_pad, p.V, d, 1.0f,
+                                                                   label_rows, sm, dev)
+                    : embed_rows<__nv_bfloat16, false, float, true>(sort, sv.hp, p.ldd, e, p.t_pad, p.V, d, 1.0f,
+                                                                    label_rows, sm, dev);
+}
+
 template <class D>
 int xent_dhidden(const XentPlan& p, const XentSave& sv, const float* acc, int slots, const float* grad, int reduction,
-                 const void* label_rows, int64_t ldw, void* out, cudaStream_t sm, const DeviceInfo& dev) {
+                 const float* f_rows, const float* e_rows, const void* weight, int64_t ldw, void* out,
+                 cudaStream_t sm, const DeviceInfo& dev) {
   int64_t blocks = (p.T * ((p.d + 7) / 8) + 255) / 256;
   if (blocks > 16ll * dev.sm_count) blocks = 16ll * dev.sm_count;
   return launch_pdl(k_xent_dhidden<D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm, acc, slots,
-                    p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad, reduction, static_cast<const D*>(label_rows), ldw, p.T,
-                    static_cast<int>(p.d), static_cast<D*>(out));
+                    p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad, reduction, f_rows, e_rows, static_cast<const D*>(weight), ldw,
+                    p.T, static_cast<int>(p.d), static_cast<D*>(out));
 }
 
 int xent_check(int64_t tokens, int64_t vocab, int64_t dim, int64_t ldh, int64_t ldw, int dtype, int reduction) {
@@ -766,15 +788,7 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
   if ((st = xent_loss(p, sv, ws.f, reduction, loss, sm, 2 * p.runs, true, true, ws.redo_tile, hr)) != ETHOS_OK) return st;
   if (!d_hidden && !d_weight) return ETHOS_OK;
   if (d_weight) {
-    // label rows of dW: (p[y] - 1) h[t] summed by label
-    if ((st = embed_sort<int32_t>(ws.sort, sv.rw.yc, p.t_pad, &sv.rw.meta->rows, vocab, -1, dev_err, sm, *dev)) !=
-        ETHOS_OK)
-      return st;
-    st = D % 8 == 0 ? embed_rows<__nv_bfloat16, true, float, true>(ws.sort, sv.hp, p.ldd, sv.rw.q, p.t_pad, vocab, D,
-                                                                   1.0f, ws.label_rows, sm, *dev)
-                    : embed_rows<__nv_bfloat16, false, float, true>(ws.sort, sv.hp, p.ldd, sv.rw.q, p.t_pad, vocab, D,
-                                                                    1.0f, ws.label_rows, sm, *dev);
-    if (st != ETHOS_OK) return st;
+    if ((st = xent_label_rows(p, sv, ws.sort, sv.rw.q, ws.label_rows, dev_err, sm, *dev)) != ETHOS_OK) return st;
   }
   const void* wptr = p.pack_w ? static_cast<const void*>(ws.f.wp) : weight;
   const int64_t wld = p.pack_w ? p.ldd : ldw;
@@ -805,7 +819,8 @@ int ethos_xent_forward_backward(const void* hidden, int64_t ldh, const void* wei
     return st;
   if (d_weight && p.pad_dw && (st = xent_unpad(ws.dwp, p.ldd, vocab, dim, d_weight, sm, *dev)) != ETHOS_OK) return st;
   if (!d_hidden) return ETHOS_OK;
-  return xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots, nullptr, reduction, weight, ldw, d_hidden, sm, *dev);
+  return xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots, nullptr, reduction, sv.rw.r, sv.rw.q, weight, ldw,
+                                     d_hidden, sm, *dev);
 }
 
 int ethos_xent_scale(const float* factor, void* x, int64_t nx, void* y, int64_t ny, int dtype, void* stream) {
@@ -875,10 +890,14 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     a.dl = ws.dl;
     a.dl_plane_rows = p.t_pad;
     a.ldl = p.piece;
+    a.label_grad = v0 == 0 ? ws.label_grad : nullptr;
     CUtensorMap dc;
     if ((st = make_tmap_bf16(&dc, ws.dl, p.planes * p.t_pad, p.piece, 32, p.piece)) != ETHOS_OK) return st;
     if ((st = launch_xent_planes<XE_DLOGITS>(p.planes, ha, wb, ha, wb, dc, a, num_m * ((n + p.tile_n - 1) / p.tile_n),
                                              dev_err, sm, *dev)) != ETHOS_OK)
+      return st;
+    if (v0 == 0 && d_weight && p.planes == 1 &&
+        (st = xent_label_rows(p, sv, ws.sort, ws.label_grad, ws.label_rows, dev_err, sm, *dev)) != ETHOS_OK)
       return st;
     XeArgs g = {};
     g.rw = sv.rw;
@@ -893,6 +912,8 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     g.dh_ld = p.dh_ld;
     void* dw = d_weight ? static_cast<char*>(d_weight) + v0 * dim * esz : nullptr;
     g.dw_bf16 = dtype == ETHOS_BF16;
+    g.label_rows = ws.label_rows;
+    g.label_span = p.planes == 1 ? ws.sort.span + v0 : nullptr;
     g.do_dh = d_hidden != nullptr;
     CUtensorMap wc;
     if ((st = xent_dw_out(&wc, dk, &g, dw, n, dim, ws.dwp, p.ldd)) != ETHOS_OK) return st;
@@ -902,10 +923,10 @@ int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int
     if (d_weight && p.pad_dw && (st = xent_unpad(ws.dwp, p.ldd, n, dim, dw, sm, *dev)) != ETHOS_OK) return st;
   }
   if (!d_hidden) return ETHOS_OK;
-  return dtype == ETHOS_BF16 ? xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots_piece, grad, reduction, nullptr, 0,
-                                                           d_hidden, sm, *dev)
-                             : xent_dhidden<float>(p, sv, ws.dh, p.slots_piece, grad, reduction, nullptr, 0, d_hidden,
-                                                   sm, *dev);
+  return dtype == ETHOS_BF16 ? xent_dhidden<__nv_bfloat16>(p, sv, ws.dh, p.slots_piece, grad, reduction, nullptr,
+                                                           ws.label_grad, weight, ldw, d_hidden, sm, *dev)
+                             : xent_dhidden<float>(p, sv, ws.dh, p.slots_piece, grad, reduction, nullptr, nullptr,
+                                                   weight, ldw, d_hidden, sm, *dev);
 }
 
 }  // extern "C"

@@ -28,7 +28,10 @@
 //          logits again, one piece of the vocabulary after another; their
 //          gradient goes to a [tokens, piece] bf16 buffer straight from the
 //          accumulators, and one launch computes both products with it.  Four
-//          products.
+//          products.  The label's own entry, the largest of a row, is not
+//          among them for bf16: its terms are added in fp32 as the keep way
+//          adds them (rounded with the rest, the gradients were off by 2.4e-3
+//          in the norm, where the output's rounding alone is 1.7e-3).
 //
 // Both are bounded by the tensor cores.
 //
@@ -539,11 +542,14 @@ __device__ __forceinline__ float xe_scale(const XeRows& rw, const float* grad, i
 }
 
 // d_hidden[t] = scale * (f sum over slots of acc[slot][pos[t]] + e W[y]), zero
-// for an ignored token; KEEP: f = r, e = p[y] - 1, else f = 1, e = 0.
+// for an ignored token.  KEEP: f = r, e = p[y] - 1; pieces: f = 1 (null),
+// e = g (p[y] - 1) for bf16 and 0 (null) for fp32, whose sum has the label's.
 template <class D>
 __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ acc, int slots, int64_t slot_size,
                                                       int64_t lda, XeRows rw, const float* __restrict__ grad,
-                                                      int reduction, const D* __restrict__ label_rows, int64_t ldw,
+                                                      int reduction, const float* __restrict__ f_rows,
+                                                      const float* __restrict__ e_rows,
+                                                      const D* __restrict__ weight, int64_t ldw,
                                                       int64_t tokens, int d, D* __restrict__ out) {
   pdl_launch_dependents();
   pdl_wait();
@@ -551,7 +557,7 @@ __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ 
   const int pieces = (d + 7) / 8;
   const int64_t total = tokens * pieces;
   const bool vec = d % 8 == 0 && rows_vec(out, d);
-  const bool wvec = label_rows != nullptr && rows_vec(label_rows, ldw);
+  const bool wvec = rows_vec(weight, ldw);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t t = i / pieces;
@@ -567,10 +573,10 @@ __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ 
         v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
         v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
       }
-      if (label_rows != nullptr) {
-        const float f = rw.r[r], e = rw.q[r];
+      if (e_rows != nullptr) {
+        const float f = f_rows != nullptr ? f_rows[r] : 1.0f, e = e_rows[r];
         float w[8];
-        load8(label_rows + static_cast<int64_t>(rw.yc[r]) * ldw, c, d, wvec, w);
+        load8(weight + static_cast<int64_t>(rw.yc[r]) * ldw, c, d, wvec, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = fmaf(v[j], f, e * w[j]);
       }
@@ -676,6 +682,7 @@ struct XeArgs {
   __nv_bfloat16* dl;
   int64_t dl_plane_rows;
   int64_t ldl;
+  float* label_grad;   // DLOGITS, bf16: g (p[y] - 1) of each row, by the units of the first column tile
   // GRADS
   int dh_slots;        // K slices of dh, each with a buffer of its own
   int dh_accumulate;   // add to dh_acc (pieces after the first)
@@ -1299,6 +1306,10 @@ __global__ void __launch_bounds__(XE_THREADS, 1)
         c2 = live ? args.rw.lse[row] * XE_LOG2E : 0.0f;
         at_label = live ? args.rw.q[row] : 0.0f;
         g = args.reduction == XE_NONE && live ? args.grad[args.rw.idx[row]] : 1.0f;
+        if (PLANES == 1) {  // the label's entry goes its own way, in fp32
+          if (args.label_grad != nullptr && st.n0 == 0 && ch == 0 && row < rows) args.label_grad[row] = at_label * g;
+          at_label = 0.0f;
+        }
       }
       // GRADS: this row's label row, looked up and on its way before the wait
       // (loads of it afterwards, by one lane of few warps, took 9 of 146 us of

@@ -58,12 +58,16 @@ def balance_loss(weights, ids, num_experts, mask=None):
 
 
 def _keeping_pays(T, V, d):
-    """Whether forming the logits a second time would take longer than the
-    five launches that keeping their exponentials takes on top (about 20 us):
-    its time is that of the products (1.2 PFLOP/s, rows in tiles of 256) or of
-    reading the table (4.5 TB/s)."""
+    """Whether forming the logits a second time would take longer than the two
+    or three launches that keeping their exponentials takes on top (2 to 4 us of
+    host time): its time is that of the products (1.2 PFLOP/s, rows in tiles of
+    256) or of reading the table (4.5 TB/s).  Loss and gradients, formed again
+    against kept, in us: 95 and 99 for 1 token of 32 000 x 64, 104 and 106 for
+    256 of 32 000 x 256 (3.6 us by this rule), 147 and 131 for 1000 of 32 000 x
+    64 (3.5), 109 and 100 for 1000 of 16 000 x 256 (7), 154 and 133 for 256 of
+    32 000 x 1024 (15)."""
     rows = -(-T // 256) * 256
-    return max(2.0 * rows * V * d / 1.2e9, 2.0 * V * d / 4.5e6) > 20.0
+    return max(2.0 * rows * V * d / 1.2e9, 2.0 * V * d / 4.5e6) > 3.0
 
 
 def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="mean"):

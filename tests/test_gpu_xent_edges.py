@@ -88,3 +88,73 @@ def test_workspaces_at_every_accepted_alignment(T, V, d, dtype, monkeypatch):
     for a, b in ((0, 8), (8, 0)):
         assert L.ethos_xent_backward(*args, p(save.data_ptr() + a), save.numel() - a, h.data_ptr(), W.data_ptr(),
                                      p(ws.data_ptr() + b), ws.numel() - b, loss.data_ptr(), None) == 3
+
+
+def _label_only(T, V, d, seed):
+    """A problem whose gradients are the label's terms: word 0, a row of
+    zeros, has logit 0 and all of the probability, every other word a logit
+    of -64 and less, so that with the loss's gradient g
+        dh[t] = -g[t] W[y[t]],   dW[v] = -sum over the tokens of label v of g[t] h[t]
+    (v > 0) up to e^-60."""
+    g = torch.Generator().manual_seed(seed)
+    W = torch.randn(V, d, generator=g) * 0.25
+    h = torch.randn(T, d, generator=g) * 0.25
+    W[:, 0], h[:, 0] = -5.0, 16.0
+    W[0] = 0.0
+    y = torch.randperm(max(T, V - 1), generator=g)[:T] % (V - 1) + 1
+    assert (h @ W[1:].t()).max() < -64
+    return h.bfloat16(), W.bfloat16(), y, torch.rand(T, generator=g) + 0.5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("T,V,d", [(40, 300, 64), (256, 600, 33), (300, 700, 136), (700, 2049, 24), (1000, 3000, 515)])
+def test_the_labels_terms_are_rounded_once(T, V, d, reduction):
+    """bf16, the logits formed again: the label's entry of their gradient,
+    g (p - 1), is the largest of a row and reaches both gradients in fp32.
+    With one token to a label each result is one product of values of 24 bits
+    (p - 1 within 2^-23, one more rounding by g / n and by the product), rounded
+    to bf16 once: the rounding of a value within 2^-21 of the exact one."""
+    h, W, y, g = _label_only(T, V, d, seed=T)
+    ignored = torch.arange(T) % 5 == 3
+    y[ignored] = -100
+    hc, wc, yc = h.cuda(), W.cuda(), y.cuda()
+    loss, save = ops.linear_cross_entropy_forward(hc, wc, yc, reduction=reduction)
+    up = g if reduction == "none" else g[0]
+    dh, dw = ops.linear_cross_entropy_backward(up.cuda(), hc, wc, save, reduction=reduction)
+    coef = {"none": g.double(), "sum": up.double().expand(T),
+            "mean": (up.double() / int((~ignored).sum())).expand(T)}[reduction]
+    want_h = torch.where(ignored[:, None], 0.0, -coef[:, None] * W.double()[y.clamp(min=0)])
+    want_w = torch.zeros(V, d, dtype=torch.float64)
+    want_w[y[~ignored]] = -coef[~ignored, None] * h.double()[~ignored]
+    rest = torch.ones(V, dtype=torch.bool)
+    rest[0] = rest[y[~ignored]] = False
+    for got, want in ((dh, want_h), (dw[~rest.cuda()][1:], want_w[~rest][1:])):
+        got = got.cpu()
+        ok = torch.zeros(got.shape, dtype=torch.bool)
+        for f in (1.0 - 2.0 ** -21, 1.0, 1.0 + 2.0 ** -21):
+            ok |= got == (want * f).float().to(torch.bfloat16)
+        assert ok.all(), f"{int((~ok).sum())} of {ok.numel()}"
+    # words that are no token's label: their probabilities, below e^-60 (1e-26)
+    assert (dw[rest.cuda()].double().cpu().abs() <= 1e-26 * (coef[:, None] * h.double().abs()).sum(0)).all()
+    ops.check_device_error("cuda")
+
+
+@pytest.mark.gpu
+def test_the_labels_terms_over_several_pieces():
+    """The same where the vocabulary takes two pieces and labels repeat: sums
+    of n fp32 terms, n 2^-24 of their magnitudes, and one rounding to bf16
+    (2^-8 of the value at most)."""
+    T, V, d = 70000, 20000, 16
+    h, W, y, g = (t.cuda() for t in _label_only(T, V, d, seed=1))
+    assert ops._size("ethos_xent_backward_workspace_size", T, V, d, 1) < T * V * 2  # not all columns at once
+    loss, save = ops.linear_cross_entropy_forward(h, W, y, reduction="none")
+    dh, dw = ops.linear_cross_entropy_backward(g, h, W, save, reduction="none")
+    want = -g.double()[:, None] * W.double()[y]
+    assert ((dh.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -21) * want.abs()).all()
+    terms = -g.double()[:, None] * h.double()
+    want, mags = (torch.zeros(V, d, dtype=torch.float64, device="cuda").index_add_(0, y, t)
+                  for t in (terms, terms.abs()))
+    n = torch.bincount(y, minlength=V)[:, None].double()
+    bad = (dw.double() - want).abs() > 2.0 ** -8 * want.abs() + (n + 8) * 2.0 ** -24 * mags
+    assert not bad[1:].any(), f"{int(bad[1:].sum())} of {bad.numel()}"
