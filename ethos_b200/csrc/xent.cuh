@@ -474,9 +474,10 @@ __global__ void __launch_bounds__(256) k_xent_loss(XeRows rw, const float2* __re
       // s: sum of exp(l[v] - c) over the other columns; b: the label's own
       if (!keep && m != c) s *= expf(m - c);  // m < c = l (m is -inf when there is no other column)
       const float b = c == l ? 1.0f : expf(l - c);
-      const float v = c == l ? log1pf(s) : (c - l) + logf(s + b);
+      const float above = c == l ? log1pf(s) : logf(s + b);  // logsumexp - c
+      const float v = c == l ? above : (c - l) + above;
       r = live ? 1.0f / (s + b) : 0.0f;
-      rw.lse[row] = l + v;
+      rw.lse[row] = c + above;  // not l + v: two large numbers where the label is hopeless
       rw.q[row] = -s / (s + b);
       rw.r[row] = r;
       if (live) {

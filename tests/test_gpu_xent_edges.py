@@ -158,3 +158,32 @@ def test_the_labels_terms_over_several_pieces():
     n = torch.bincount(y, minlength=V)[:, None].double()
     bad = (dw.double() - want).abs() > 2.0 ** -8 * want.abs() + (n + 8) * 2.0 ** -24 * mags
     assert not bad[1:].any(), f"{int(bad[1:].sum())} of {bad.numel()}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 40, 300])
+@pytest.mark.parametrize("gap", [300.0, 30000.0])
+def test_a_hopeless_label_leaves_the_other_words_exact(gap, T):
+    """fp32: a label whose logit lies far below takes no part in the other
+    words' probabilities, so their error is that of their own logits,
+    e_l = (d / 16 + 8) 2^-23 A with A from their magnitudes alone: p is within
+    2 e_l + 2^-21, and its sums of n terms within n 2^-24 more."""
+    V, d = 700, 16
+    g = torch.Generator().manual_seed(T)
+    h, W = torch.randn(T, d, generator=g), torch.randn(V, d, generator=g)
+    W[:, 0], h[:, 0] = 0.0, gap / 10
+    W[5] = 0.0
+    W[5, 0] = -10.0
+    y = torch.full((T,), 5)
+    hg, wg = h.cuda().requires_grad_(True), W.cuda().requires_grad_(True)
+    rest = torch.arange(V) != 5
+    others = W[rest][:, 1:].double()
+    p = torch.softmax(h[:, 1:].double() @ others.t(), 1)
+    e_l = (d / 16 + 8) * 2.0 ** -23 * (h[:, 1:].double().abs() @ others.abs().t()).max().item()
+    bound = 2 * e_l + 2.0 ** -21 + max(T, V) * 2.0 ** -24
+    for reduction in ("none", "sum"):
+        loss = EF.linear_cross_entropy(hg, wg, y.cuda(), reduction=reduction)
+        dh, dw = torch.autograd.grad(loss.sum(), (hg, wg))
+        mags_h, mags_w = p @ others.abs(), p.t() @ h.double().abs()
+        assert ((dh[:, 1:].double().cpu() - p @ others).abs() <= bound * mags_h).all()
+        assert ((dw[rest.cuda()].double().cpu() - p.t() @ h.double()).abs() <= bound * mags_w).all()
