@@ -187,3 +187,52 @@ def test_a_hopeless_label_leaves_the_other_words_exact(gap, T):
         mags_h, mags_w = p @ others.abs(), p.t() @ h.double().abs()
         assert ((dh[:, 1:].double().cpu() - p @ others).abs() <= bound * mags_h).all()
         assert ((dw[rest.cuda()].double().cpu() - p.t() @ h.double()).abs() <= bound * mags_w).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("keep", [True, False])
+@pytest.mark.parametrize("T", [6, 300])
+def test_a_second_pass_through_one_graph(T, keep, dtype, monkeypatch):
+    """The first pass asks for one gradient, the second, through the same
+    graph with another factor, for both: each within the bounds of the formula
+    (the factor is one more rounding to bf16)."""
+    monkeypatch.setattr(EF, "_keeping_pays", lambda *a: keep)
+    h, W, y = _inputs(T, 900, 40, dtype, seed=T, ignored=0.2)
+    y[0] = 3
+    _, dh_w, dw_w, q = _exact(h, W, y, "mean")
+    hg, wg = h.cuda().requires_grad_(True), W.cuda().requires_grad_(True)
+    loss = EF.linear_cross_entropy(hg, wg, y.cuda())
+    first, = torch.autograd.grad(loss, hg, retain_graph=True)
+    kept = first.clone()
+    dh, dw = torch.autograd.grad(3.0 * loss, (hg, wg), retain_graph=True)
+    again, = torch.autograd.grad(loss, wg)
+    more = 2.0 ** -9 if dtype == torch.bfloat16 else 2.0 ** -23
+    assert _rel(first, dh_w) <= _grad_bound(q, "ch", 900 / 16, dtype) and torch.equal(first, kept)
+    assert _rel(dh, 3.0 * dh_w) <= _grad_bound(q, "ch", 900 / 16, dtype) + more
+    assert _rel(dw, 3.0 * dw_w) <= _grad_bound(q, "cw", T / 16, dtype) + more
+    assert _rel(again, dw_w) <= _grad_bound(q, "cw", T / 16, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [8, 200, 300])
+def test_nan_and_infinity_stay_in_their_rows_by_every_way(T, dtype):
+    """A token whose state holds NaN or infinity: its loss and its row of dh
+    are NaN, every other token's are what they are without it."""
+    h, W, y = _inputs(T, 600, 64, dtype, seed=4)
+    ok = torch.ones(T, dtype=torch.bool)
+    ok[2] = ok[5] = False
+    hb = h.clone()
+    hb[2, 3], hb[5, 0] = float("nan"), float("inf")
+    res = []
+    for x in (h, hb):
+        loss, save = ops.linear_cross_entropy_forward(x.cuda(), W.cuda(), y.cuda(), reduction="none")
+        dh, dw = ops.linear_cross_entropy_backward(torch.ones(T, device="cuda"), x.cuda(), W.cuda(), save, "none")
+        both = ops.linear_cross_entropy_forward_backward(x.cuda(), W.cuda(), y.cuda(), reduction="sum")
+        res.append((loss, dh) if both is None else (loss, dh, both[2]))
+    for clean, bad in zip(*res):
+        bad, clean = bad.cpu(), clean.cpu()
+        assert torch.equal(bad[ok], clean[ok])
+        rows = bad[~ok] if bad.dim() == 1 else bad[~ok].float().isnan().any(1)
+        assert rows.isnan().all() if bad.dim() == 1 else rows.all()
