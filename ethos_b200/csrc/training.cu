@@ -375,9 +375,9 @@ int xent_rows_pass(const XentPlan& p, const XentSave& sv, const void* hidden, in
   return dtype == ETHOS_BF16
              ? launch_pdl(k_xent_rows<__nv_bfloat16, 1>, grid, dim3(256), 0, sm,
                           static_cast<const __nv_bfloat16*>(hidden), ldh, static_cast<const __nv_bfloat16*>(weight),
-                          ldw, d, sv.rw, sv.hp, p.t_pad, ldd)
+                          ldw, p.V, d, sv.rw, sv.hp, p.t_pad, ldd)
              : launch_pdl(k_xent_rows<float, 3>, grid, dim3(256), 0, sm, static_cast<const float*>(hidden), ldh,
-                          static_cast<const float*>(weight), ldw, d, sv.rw, sv.hp, p.t_pad, ldd);
+                          static_cast<const float*>(weight), ldw, p.V, d, sv.rw, sv.hp, p.t_pad, ldd);
 }
 
 int xent_index(const XentPlan& p, const XentSave& sv, const void* labels, int labels_i64, int64_t ignore_index,
@@ -557,8 +557,8 @@ int xent_dhidden(const XentPlan& p, const XentSave& sv, const float* acc, int sl
   int64_t blocks = (p.T * ((p.d + 7) / 8) + 255) / 256;
   if (blocks > 16ll * dev.sm_count) blocks = 16ll * dev.sm_count;
   return launch_pdl(k_xent_dhidden<D>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, sm, acc, slots,
-                    p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad, reduction, f_rows, e_rows, static_cast<const D*>(weight), ldw,
-                    p.T, static_cast<int>(p.d), static_cast<D*>(out));
+                    p.t_pad * p.dh_ld, p.dh_ld, sv.rw, grad, reduction, f_rows, e_rows, static_cast<const D*>(weight),
+                    ldw, p.V, p.T, static_cast<int>(p.d), static_cast<D*>(out));
 }
 
 int xent_check(int64_t tokens, int64_t vocab, int64_t dim, int64_t ldh, int64_t ldw, int dtype, int reduction) {

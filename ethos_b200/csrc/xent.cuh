@@ -216,8 +216,9 @@ __global__ void __launch_bounds__(256) k_xent_pack(const S* __restrict__ src, in
 // zero.
 template <class S, int PLANES>
 __global__ void __launch_bounds__(256) k_xent_rows(const S* __restrict__ hidden, int64_t ldh,
-                                                   const S* __restrict__ weight, int64_t ldw, int d, XeRows rw,
-                                                   __nv_bfloat16* __restrict__ dst, int64_t plane_rows, int ldd) {
+                                                   const S* __restrict__ weight, int64_t ldw, int64_t vocab, int d,
+                                                   XeRows rw, __nv_bfloat16* __restrict__ dst, int64_t plane_rows,
+                                                   int ldd) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -227,7 +228,8 @@ __global__ void __launch_bounds__(256) k_xent_rows(const S* __restrict__ hidden,
   for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < upto; r += gridDim.x * 8) {
     const bool in = r < rows;
     const S* h = hidden + (in ? static_cast<int64_t>(rw.idx[r]) : 0) * ldh;
-    const int y = in ? rw.yc[r] : -1;
+    int y = in ? rw.yc[r] : -1;
+    if (y >= vocab) y = -1;  // a save buffer of a larger table's forward
     const S* w = weight + static_cast<int64_t>(y < 0 ? 0 : y) * ldw;
     float dot = 0.0f;
 #pragma unroll 2
@@ -550,7 +552,7 @@ __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ 
                                                       int64_t lda, XeRows rw, const float* __restrict__ grad,
                                                       int reduction, const float* __restrict__ f_rows,
                                                       const float* __restrict__ e_rows,
-                                                      const D* __restrict__ weight, int64_t ldw,
+                                                      const D* __restrict__ weight, int64_t ldw, int64_t vocab,
                                                       int64_t tokens, int d, D* __restrict__ out) {
   pdl_launch_dependents();
   pdl_wait();
@@ -574,7 +576,7 @@ __global__ void __launch_bounds__(256) k_xent_dhidden(const float* __restrict__ 
         v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
         v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
       }
-      if (e_rows != nullptr) {
+      if (e_rows != nullptr && rw.yc[r] < vocab) {
         const float f = f_rows != nullptr ? f_rows[r] : 1.0f, e = e_rows[r];
         float w[8];
         load8(weight + static_cast<int64_t>(rw.yc[r]) * ldw, c, d, wvec, w);

@@ -828,6 +828,8 @@ def linear_cross_entropy_backward(grad, hidden, weight, save, reduction="mean", 
         return dh, dw.zero_() if dw is not None else None
     _on(dev, save, "save")
     code = _dtype_code(hidden, "hidden")
+    if save.nbytes != _size("ethos_xent_save_size", T, V, d, code):
+        raise ValueError("save: not of a forward of these sizes")
     hidden, weight = _xent_rows(hidden), _xent_weight(weight)
     grad = grad.to(torch.float32).contiguous()
     ws = _bytes(_size("ethos_xent_backward_workspace_size", T, V, d, code), dev)

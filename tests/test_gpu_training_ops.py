@@ -43,6 +43,30 @@ def test_cross_entropy_backward_refuses_operands_that_do_not_belong_together(xen
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 40, 400])
+def test_cross_entropy_backward_with_another_problems_save(T):
+    """Sizes that the save buffer shows are refused; labels of a larger table
+    (whose size it does not hold) are reported and left out instead of read
+    past the smaller one's end; the other tokens keep their label's terms."""
+    g = torch.Generator().manual_seed(T)
+    h, W = (torch.randn(n, 24, generator=g).bfloat16().cuda() for n in (T, 1 << 20))
+    y = torch.full((T,), (1 << 20) - 1).cuda()
+    y[0] = 7
+    loss, save = ops.linear_cross_entropy_forward(h, W, y, reduction="none")
+    one, back = torch.ones(T, device="cuda"), ops.linear_cross_entropy_backward
+    for bad_h, bad_grad in ((h[:T - 4].repeat(65, 1), one[:1].expand(65 * (T - 4))), (h.repeat(1, 9), one)):
+        with pytest.raises(ValueError, match="save"):
+            back(bad_grad, bad_h, W[:, :1].expand(-1, bad_h.shape[1]), save, "none")
+    small = W[:100].clone()
+    dh, dw = back(one, h, small, save, "none")
+    with pytest.raises(_lib.EthosError):
+        ops.check_device_error("cuda")
+    assert torch.isfinite(dh.float()).all() and torch.isfinite(dw.float()).all()
+    want = -small[7].float()  # the other 99 words have next to none of the larger table's probability
+    assert (dh[0].float() - want).norm() <= 0.02 * want.norm()
+
+
+@pytest.mark.gpu
 def test_scale_refuses_and_takes_any_float_factor():
     x = torch.arange(8, device="cuda", dtype=torch.float32)
     two = torch.full((), 2.0, device="cuda")
