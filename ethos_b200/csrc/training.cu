@@ -494,7 +494,7 @@ int xent_unpad(const __nv_bfloat16* dwp, int64_t ldd, int64_t rows, int64_t d, v
                     static_cast<int>(d), rows * d, static_cast<__nv_bfloat16*>(dw));
 }
 
-// The forward of at most XE_FEW tokens.
+// The forward of few tokens (xent_is_few).
 template <class S, bool kVec>
 int xent_few_t(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
                const void* labels, int labels_i64, int64_t ignore, float* loss_rows, const XentFwd& ws, int* err,
@@ -512,11 +512,24 @@ int xent_few_t(const XentPlan& p, const XentSave& sv, const void* hidden, int64_
                       ws.part, p.t_pad, err);
   };
   if (tt == 1) return go(k_xent_few<S, kVec, 1>);
-  if (tt == 2) return go(k_xent_few<S, kVec, 2>);
-  if (tt == 4) return go(k_xent_few<S, kVec, 4>);
-  return go(k_xent_few<S, kVec, 8>);
+  if constexpr (xe_few<S, kVec>() >= 2) {
+    if (tt == 2) return go(k_xent_few<S, kVec, 2>);
+  }
+  if constexpr (xe_few<S, kVec>() >= 4) {
+    if (tt == 4) return go(k_xent_few<S, kVec, 4>);
+  }
+  if constexpr (xe_few<S, kVec>() >= 8) {
+    if (tt == 8) return go(k_xent_few<S, kVec, 8>);
+  }
+  return ETHOS_ERR_UNSUPPORTED_SHAPE;
 }
-bool xent_is_few(const XentPlan& p) { return p.T <= XE_FEW && up(p.T, 8) * up(p.d, 256) * 4 <= XE_FEW_SMEM; }
+// By width, not by address: the backward asks again and has to find the same.
+// (bf16 tables of whole 16-byte rows at other addresses are refused before.)
+bool xent_is_few(const XentPlan& p) {
+  const int most = p.planes == 3 ? xe_few<float, true>()
+                                 : (p.pack_w ? xe_few<__nv_bfloat16, false>() : xe_few<__nv_bfloat16, true>());
+  return p.T <= most && up(p.T, 8) * up(p.d, 256) * 4 <= XE_FEW_SMEM;
+}
 int xent_few(const XentPlan& p, const XentSave& sv, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
              int dtype, const void* labels, int labels_i64, int64_t ignore, float* loss_rows, const XentFwd& ws,
              int* err, cudaStream_t sm) {

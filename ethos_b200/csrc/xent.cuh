@@ -267,16 +267,26 @@ __device__ __forceinline__ void lse_join(float& m, float& s, float m2, float s2)
 }
 
 // ------------------------------------------------------------- few tokens --
-// The forward for at most XE_FEW tokens: one pass over the vocabulary on the
-// fp32 units, bounded by its bytes (the tensor cores' 256-row tiles have
-// nothing to gain, and their copies stream rows of 128-byte pieces at 4.1 TB/s
-// against 5.7 TB/s of whole rows).  A warp takes 32 / TT rows of the vocabulary
+// The forward for few tokens: one pass over the vocabulary on the fp32 units,
+// bounded by its bytes for one token (the table of 100 277 x 1024 bf16, 205 MB,
+// in 46 to 50 us, 4.1 to 4.4 TB/s) and by its products and their reduction for
+// more.  A warp takes 32 / TT rows of the vocabulary
 // at a time, lanes along the columns, TT >= tokens accumulators for each; the
 // 32 sums are transposed and reduced over the lanes so that lane l holds the
 // logit of row l / TT and token l % TT, and keeps a running (maximum, sum)
 // of its token.  The token's label is left out of the sum and its logit kept.
 // Block 0 also writes the row index that k_xent_index writes otherwise.
-constexpr int XE_FEW = 8;
+//
+// Most tokens that take it rather than the matrix units' row tile of 256.  The
+// whole forward in us, caches cold, for 1, 2, 4 and 8 tokens this way and for 9
+// the other: bf16, 100 277 x 1024: 62, 69, 81, 130 and 82; 32 003 x 512: 24, 26,
+// 28, 36 and 35; 32 003 x 515 (one element at a time): 32, 40, 56, 83 and 47.
+// fp32, 100 277 x 1024: 95, 101, 118, 175 and 399; 32 003 x 515: 40, 48, 67, 97
+// and 100.
+template <class S, bool kVec>
+constexpr int xe_few() {
+  return sizeof(S) == 4 ? 8 : (kVec ? 4 : 2);
+}
 constexpr int XE_FEW_BLOCKS = 148;    // pieces of each row's sum
 constexpr int XE_FEW_SMEM = 128 * 1024;  // the tokens' states in fp32
 
