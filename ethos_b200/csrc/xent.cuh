@@ -640,7 +640,9 @@ __global__ void __launch_bounds__(256) k_xent_unpad(const __nv_bfloat16* __restr
 }
 
 // x *= *factor and y *= *factor, unless it is 1 (the gradients of the KEEP way are those of a
-// loss whose own gradient is 1)
+// loss whose own gradient is 1).  They were rounded to D when they were computed
+// and are rounded again here, which a power of two leaves exact: held in fp32
+// until then, dW would take twice its memory between the calls.
 template <class D>
 __global__ void __launch_bounds__(256) k_xent_scale(const float* __restrict__ factor, D* __restrict__ x, int64_t nx,
                                                     D* __restrict__ y, int64_t ny) {

@@ -82,10 +82,11 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, reduction="m
 
     Where gradients are needed, the loss is one number and the problem is not
     a small one, bf16 operands get them in the forward call, which keeps the
-    logits' exponentials (bf16, up to 4 GiB of workspace) for its own length;
-    the backward multiplies them by the loss's gradient.  Otherwise the backward forms the logits again, a
-    piece of the vocabulary at a time.  Neither way keeps anything of size
-    ``T * V`` between the calls."""
+    logits' exponentials (bf16, up to 4 GiB of workspace) for its own
+    length; the backward multiplies them by the loss's gradient, which rounds
+    them once more unless it is 1 or another power of two.  Otherwise the
+    backward forms the logits again, a piece of the vocabulary at a time.
+    Neither way keeps anything of size ``T * V`` between the calls."""
     red = ops.XENT_REDUCTION.get(reduction)
     if red is None:
         raise ValueError(f"reduction: none, sum or mean, not {reduction!r}")

@@ -477,7 +477,8 @@ int ethos_layer_backward_routed_f32(const ethos_dims* dims, int bn_training, flo
  * Operators of a training step around the expert layers: the token embedding
  * (model.py:374), the balance of the routing, and the cross entropy of the
  * output head (model.py:385, train.py:200).  dtype arguments take the codes
- * below; ids and labels are int32 (ids_i64 = 0) or int64 (1). */
+ * below; ids and labels are int32 (ids_i64 = 0) or int64 (1).  Workspaces, scratch
+ * and save buffers are 16-byte aligned (else ETHOS_ERR_ALIGNMENT). */
 #define ETHOS_F32 0
 #define ETHOS_BF16 1
 
@@ -541,8 +542,9 @@ int ethos_xent_forward(const void* hidden, int64_t ldh, const void* weight, int6
  * (dtype, contiguous; either may be NULL: not computed), given grad, the
  * loss's gradient on the device (fp32, [tokens] for NONE, else one).  The
  * logits are formed again, one piece of the vocabulary at a time (a piece's
- * gradient takes about 1 GiB of the workspace, or 8192 columns).  hidden,
- * weight and the sizes are the forward's. */
+ * gradient takes about 1 GiB of the workspace, or 8192 columns); for bf16 the
+ * label's terms are added to both gradients in fp32.  hidden, weight and the
+ * sizes are the forward's. */
 size_t ethos_xent_backward_workspace_size(int64_t tokens, int64_t vocab, int64_t dim, int dtype);
 int ethos_xent_backward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, int dtype, int reduction,
                         int64_t tokens, int64_t vocab, int64_t dim, const float* grad, const void* save,
