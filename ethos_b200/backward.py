@@ -54,8 +54,7 @@ def layer_backward(ctx, gy, gw=None):
     them (None: none)."""
     layer = ctx.layer
     sv = ctx.saved
-    if ctx.saved_tensors:  # handed out as well (autograd checks that they are unchanged)
-        sv["weights"], sv["ids"] = ctx.saved_tensors
+    ctx.saved_tensors  # noqa: B018 -- raises if the weights or ids that were handed out have been changed
     pw = sv["pw"]
     if gy is None:  # only the routing weights were used
         gy = torch.zeros_like(sv["xin"])
