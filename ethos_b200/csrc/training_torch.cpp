@@ -115,6 +115,13 @@ void once(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, ": its gradient cannot be differentiated (create_graph=True)");
 }
 
+// Rows with unit column stride and a pitch of at least their width.
+Tensor as_rows(const Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous();
+}
+// (a single row may carry any stride)
+int64_t pitch(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }
+
 // -------------------------------------------------------------- embedding --
 struct Embedding : torch::autograd::Function<Embedding> {
   static Tensor forward(AutogradContext* ctx, const Tensor& ids_, const Tensor& weight, double scale, int64_t padding) {
@@ -125,11 +132,11 @@ struct Embedding : torch::autograd::Function<Embedding> {
     const int64_t V = weight.size(0), d = weight.size(1);
     const c10::cuda::CUDAGuard guard(weight.device());
     const Tensor ids = ids_.contiguous();
-    const Tensor w = weight.stride(1) == 1 && weight.stride(0) >= d ? weight : weight.contiguous();
+    const Tensor w = as_rows(weight);
     std::vector<int64_t> shape = ids.sizes().vec();
     shape.push_back(d);
     Tensor out = at::empty(shape, weight.options());
-    check(L.ethos_embedding_forward(ids.const_data_ptr(), i64, w.const_data_ptr(), w.stride(0), code, ids.numel(), V, d,
+    check(L.ethos_embedding_forward(ids.const_data_ptr(), i64, w.const_data_ptr(), pitch(w), code, ids.numel(), V, d,
                                   static_cast<float>(scale), out.mutable_data_ptr(), error_word(w), stream_of(w)),
           "ethos_embedding_forward");
     ctx->save_for_backward({ids});
@@ -207,11 +214,6 @@ struct Balance : torch::autograd::Function<Balance> {
 };
 
 // ---------------------------------------------------------- cross entropy --
-// Rows with unit column stride and a pitch of at least their width.
-Tensor as_rows(const Tensor& t) {
-  return t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous();
-}
-int64_t pitch(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }
 // What the products read in place: rows of 16-byte pieces (other widths go
 // through packed copies in the workspace).
 Tensor as_table(const Tensor& t) {

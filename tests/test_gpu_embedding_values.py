@@ -48,3 +48,16 @@ def test_rows_without_a_token_are_zero_whatever_was_there(V, d, monkeypatch):
         want[1] = 1.0
         want[2] = 0.0 if fill else 0.5
         assert torch.equal(dw, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_table_of_one_row_with_any_stride(dtype):
+    """The row pitch of a one-row table means nothing; torch keeps what the
+    view had, here 1."""
+    col = torch.randn(24, 1, device="cuda").to(dtype)
+    W = col.t()
+    assert W.shape == (1, 24) and W.stride(0) == 1 and W.is_contiguous()
+    ids = torch.zeros(5, dtype=torch.int64, device="cuda")
+    assert torch.equal(EF.embedding(ids, W), W.expand(5, 24))
+    assert torch.equal(ops.embedding_forward(ids, W), W.expand(5, 24))
